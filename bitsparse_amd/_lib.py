@@ -17,7 +17,7 @@ LIB_NAME = "libbitsparse_hip.so"
 # BITSPARSE_HIP_LIB points at another build of the same sources (tuning sweeps)
 LIB_PATH = os.environ.get("BITSPARSE_HIP_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 BS_OK = 0
 BS_ERR_INVALID = 1
@@ -92,6 +92,9 @@ _SIGNATURES = {
                          _i64, _vp],
     "bs_col_sum_workspace_bytes": [_i64, _i64],
     "bs_col_sum": [_vp, _i64, _i64, _vp, _vp, _i64, _vp],
+    "bs_join_forward": [_vp, _vp, _vp, _vp],
+    "bs_join_backward_workspace_bytes": [_i64, _i64],
+    "bs_join_backward": [_vp, _vp, _vp, _i64, _vp],
     "bs_launch_timing": [_int],
     "bs_nontemporal_min_bytes": [_i64],
     "bs_launch_timing_read": [_vp, _vp, _int, _vp],
@@ -107,6 +110,7 @@ _RESTYPES = {
     "bs_linear_relu_compress_max_n": _i64,
     "bs_grad_sums_workspace_bytes": _i64,
     "bs_col_sum_workspace_bytes": _i64,
+    "bs_join_backward_workspace_bytes": _i64,
     "bs_nontemporal_min_bytes": _i64,
     "bs_workspace_amax_slot": _vp,
     "bs_workspace_fallback_counter": _vp,

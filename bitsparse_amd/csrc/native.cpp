@@ -33,7 +33,7 @@ using at::Tensor;
     F(bs_col_sum_workspace_bytes) F(bs_col_sum) F(bs_gemm_compressed_b_workspace_bytes) F(bs_gemm_compressed_b)  \
     F(bs_gemm_compressed_b_packed_workspace_bytes) F(bs_gemm_compressed_b_packed)                                \
     F(bs_gemm_compressed_b_fp8_workspace_bytes) F(bs_gemm_compressed_b_fp8) F(bs_gemm_compressed_b_fp8_packed)   \
-    F(bs_workspace_amax_slot)
+    F(bs_workspace_amax_slot) F(bs_join_forward) F(bs_join_backward_workspace_bytes) F(bs_join_backward)
 struct Lib {
 #define F(name) decltype(&::name) name = nullptr;
     BS_FUNCS(F)
@@ -619,6 +619,244 @@ block_backward(const Tensor& g, const Tensor& x, const Tensor& W1, const Tensor&
     return out;
 }
 
+// ---------------------------------------------------------------------------
+// the step between two blocks (residual.py)
+// ---------------------------------------------------------------------------
+// A tensor the kernels can read at its address: on the GPU, with storage of its
+// own, not inside a tracer's or a transform's wrapper.
+void plain_on_gpu(const Tensor& t, const char* what)
+{
+    TORCH_CHECK(t.is_cuda(), what, ": bitsparse_amd runs on a ROCm GPU; got a tensor on ", t.device());
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        t.has_storage() && t.layout() == at::kStrided &&
+            !t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                                      c10::DispatchKey::FuncTorchGradWrapper,
+                                                      c10::DispatchKey::Functionalize, c10::DispatchKey::Conjugate,
+                                                      c10::DispatchKey::Negative})),
+        what, ": takes plain dense tensors, outside tracers and function transforms");
+}
+
+int row_type(const Tensor& t, const char* what)
+{
+    if (t.scalar_type() == at::kBFloat16) return BS_DT_BF16;
+    if (t.scalar_type() == at::kFloat) return BS_DT_F32;
+    TORCH_CHECK_TYPE(false, what, " must be bfloat16 or float32, got ", t.scalar_type());
+}
+
+// [..., D] as rows of D contiguous elements a stride apart
+Tensor as_rows(const Tensor& t, int64_t D)
+{
+    Tensor r = t.dim() == 2 ? t : t.reshape({D ? t.numel() / D : 0, D});
+    if ((D > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < 0)) r = r.contiguous();
+    return r;
+}
+int64_t row_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+using Maybe = std::optional<Tensor>;
+
+// what a step is besides its tensors
+struct JoinKind {
+    int64_t post, pre;          // BS_NORM_*
+    double eps_post, eps_pre, scale_value;
+    at::ScalarType h_type;
+};
+
+struct JoinCall {
+    bs_join a{};
+    Tensor x, y, gate;          // as the kernels read them
+    int64_t rows, cols;
+    std::vector<Tensor> held;   // copies the pointers above point into
+
+    bs_vector vector(const Maybe& v, const char* what, bool whole)
+    {
+        if (!v) return {nullptr, BS_DT_BF16};
+        plain_on_gpu(*v, what);
+        TORCH_CHECK(v->device() == x.device(), what, " is on ", v->device(), ", x on ", x.device());
+        const int type = row_type(*v, what);
+        if (whole) TORCH_CHECK_VALUE(v->dim() == 1 && v->size(0) == cols, what, ": expected shape [", cols, "], got ", v->sizes());
+        if (!v->is_contiguous()) {
+            held.push_back(v->contiguous());
+            return {held.back().data_ptr(), type};
+        }
+        return {v->data_ptr(), type};
+    }
+
+    JoinCall(const Tensor& x_in, const Maybe& y_in, const Maybe& w_post, const Maybe& b_post, const Maybe& gate_in,
+             const Maybe& scale, const Maybe& w_pre, const Maybe& b_pre, const JoinKind& k)
+    {
+        plain_on_gpu(x_in, "x");
+        TORCH_CHECK_VALUE(x_in.dim() >= 1 && x_in.size(-1) > 0, "x: expected rows [..., D] with D > 0, got ", x_in.sizes());
+        cols = x_in.size(-1);
+        a.x_type = row_type(x_in, "x");
+        x = as_rows(x_in, cols);
+        rows = x.size(0);
+        a.rows = rows, a.cols = cols, a.x = x.data_ptr(), a.x_stride = row_stride(x);
+        a.norm_post = (int)k.post, a.norm_pre = (int)k.pre, a.eps_post = (float)k.eps_post, a.eps_pre = (float)k.eps_pre;
+        a.y_type = k.h_type == at::kFloat ? BS_DT_F32 : BS_DT_BF16;
+        if (y_in) {
+            plain_on_gpu(*y_in, "y");
+            a.y_type = row_type(*y_in, "y");
+            TORCH_CHECK(y_in->device() == x_in.device(), "y is on ", y_in->device(), ", x on ", x_in.device());
+            TORCH_CHECK_VALUE(y_in->sizes() == x_in.sizes(), "y: expected x's shape ", x_in.sizes(), ", got ", y_in->sizes());
+            y = as_rows(*y_in, cols);
+            // (no rows: torch gives a null address, the ABI's sign of an absent y)
+            a.y = rows ? y.data_ptr() : &a, a.y_stride = row_stride(y);
+        }
+        TORCH_CHECK_TYPE(a.x_type == BS_DT_F32 || a.y_type == BS_DT_BF16, y_in ? "y" : "dtype",
+                         " float32 needs a float32 x: the residual stream has at least the block's precision");
+        a.weight_post = vector(w_post, "post.weight", true);
+        a.bias_post = vector(b_post, "post.bias", true);
+        a.weight_pre = vector(w_pre, "pre.weight", true);
+        a.bias_pre = vector(b_pre, "pre.bias", true);
+        a.scale_value = (float)k.scale_value;
+        if (scale) {
+            TORCH_CHECK_VALUE((scale->numel() == 1 && scale->dim() <= 1) || (scale->dim() == 1 && scale->size(0) == cols),
+                              "scale: expected one number or shape [", cols, "], got ", scale->sizes());
+            a.scale = vector(scale, "scale", false);
+            a.scale_per = scale->numel() == 1 ? BS_PER_TENSOR : BS_PER_CHANNEL;
+        }
+        if (gate_in) set_gate(*gate_in, x_in.sizes());
+    }
+
+    void set_gate(const Tensor& g, at::IntArrayRef shape)
+    {
+        if (g.numel() == 1 && g.dim() <= 1) {
+            a.gate = vector(g, "gate", false), a.gate_per = BS_PER_TENSOR;
+            return;
+        }
+        if (g.dim() == 1 && g.size(0) == cols) {
+            a.gate = vector(g, "gate", false), a.gate_per = BS_PER_CHANNEL;
+            return;
+        }
+        std::vector<int64_t> per_row(shape.begin(), shape.end());
+        per_row.back() = 1;
+        const bool element = g.sizes() == shape;
+        TORCH_CHECK_VALUE(element || g.sizes() == at::IntArrayRef(per_row), "gate: expected one number, [", cols, "], ",
+                          at::IntArrayRef(per_row), " or ", shape, ", got ", g.sizes());
+        plain_on_gpu(g, "gate");
+        TORCH_CHECK(g.device() == x.device(), "gate is on ", g.device(), ", x on ", x.device());
+        gate = as_rows(g, element ? cols : 1);
+        a.gate = {rows ? gate.data_ptr() : &a, row_type(g, "gate")};
+        a.gate_per = element ? BS_PER_ELEMENT : BS_PER_ROW;
+        a.gate_stride = row_stride(gate);
+    }
+};
+
+// (x', h, statistics), the undefined ones absent
+std::array<Tensor, 3> join_forward(JoinCall& c, at::IntArrayRef shape, bool stats)
+{
+    Tensor x1, h, st;
+    if (c.a.y) x1 = at::empty(shape, c.x.options());
+    if (c.a.norm_pre) h = at::empty(shape, c.x.options().dtype(c.a.y_type == BS_DT_F32 ? at::kFloat : at::kBFloat16));
+    if (stats && c.rows && (c.a.norm_post || c.a.norm_pre)) {
+        st = at::empty({2, c.rows, 2}, c.x.options().dtype(at::kFloat));
+        c.a.stats_post = st.data_ptr<float>();
+        c.a.stats_pre = c.a.stats_post + 2 * c.rows;
+    }
+    if (c.rows) check(L.bs_join_forward(&c.a, raw(x1), raw(h), stream_of(c.x)), "bs_join_forward");
+    return {x1, h, st};
+}
+
+struct Join : torch::autograd::Function<Join> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Maybe& y,
+                                                  const Maybe& w_post, const Maybe& b_post, const Maybe& gate,
+                                                  const Maybe& scale, const Maybe& w_pre, const Maybe& b_pre,
+                                                  const JoinKind& k)
+    {
+        const c10::DeviceGuard guard(x.device());
+        JoinCall c(x, y, w_post, b_post, gate, scale, w_pre, b_pre, k);
+        const auto [x1, h, st] = join_forward(c, x.sizes(), true);
+        auto or_none = [](const Maybe& m) { return m ? *m : Tensor(); };
+        ctx->save_for_backward({x, or_none(y), or_none(w_post), or_none(b_post), or_none(gate), or_none(scale),
+                                or_none(w_pre), or_none(b_pre), x1, st});
+        ctx->saved_data["post"] = k.post;
+        ctx->saved_data["pre"] = k.pre;
+        ctx->saved_data["eps_post"] = k.eps_post;
+        ctx->saved_data["eps_pre"] = k.eps_pre;
+        ctx->saved_data["scale"] = k.scale_value;
+        ctx->saved_data["h"] = (int64_t)k.h_type;
+        ctx->set_materialize_grads(false);
+        if (!c.a.y) return {h};
+        if (!c.a.norm_pre) return {x1};
+        return {x1, h};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   const torch::autograd::variable_list& grads)
+    {
+        TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(),
+                                    "bitsparse_amd: the step between two blocks has no second derivative (create_graph)");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor& x = saved[0];
+        const c10::DeviceGuard guard(x.device());
+        auto maybe = [&](int i) { return saved[i].defined() ? Maybe(saved[i]) : std::nullopt; };
+        const JoinKind k{ctx->saved_data["post"].toInt(), ctx->saved_data["pre"].toInt(),
+                         ctx->saved_data["eps_post"].toDouble(), ctx->saved_data["eps_pre"].toDouble(),
+                         ctx->saved_data["scale"].toDouble(), (at::ScalarType)ctx->saved_data["h"].toInt()};
+        JoinCall c(x, maybe(1), maybe(2), maybe(3), maybe(4), maybe(5), maybe(6), maybe(7), k);
+        // the tensors among the operands, in order, are the node's edges
+        bool wanted[8];
+        for (int i = 0, edge = 0; i < 8; i++) wanted[i] = saved[i].defined() && ctx->needs_input_grad(edge++);
+        torch::autograd::variable_list out(9);
+        const Tensor gx = c.a.y ? grads[0] : Tensor(), gh = c.a.norm_pre ? grads.back() : Tensor();
+        if (!gx.defined() && !gh.defined()) return out;
+        for (int i = 0; i < 8; i++)
+            if (wanted[i]) out[i] = c.rows ? at::empty(saved[i].sizes(), saved[i].options()) : at::zeros_like(saved[i]);
+        if (c.rows == 0) return out;
+
+        bs_join_grads g{};
+        const Tensor st = saved[9];
+        if (st.defined()) {
+            c.a.stats_post = st.data_ptr<float>();
+            c.a.stats_pre = c.a.stats_post + 2 * c.rows;
+        }
+        Tensor x1, gxr, ghr;
+        if (saved[8].defined()) {
+            x1 = saved[8].contiguous();
+            g.x1 = x1.data_ptr();
+        }
+        auto grad_rows = [&](const Tensor& t, int type, const char* what) {
+            plain_on_gpu(t, what);
+            TORCH_CHECK_VALUE(t.sizes() == x.sizes(), what, ": expected ", x.sizes(), ", got ", t.sizes());
+            TORCH_CHECK_TYPE(row_type(t, what) == type, what, ": unexpected dtype ", t.scalar_type());
+            return as_rows(t, c.cols);
+        };
+        if (gx.defined()) {
+            gxr = grad_rows(gx, c.a.x_type, "the gradient of x'");
+            g.grad_x1 = gxr.data_ptr(), g.grad_x1_stride = row_stride(gxr);
+        }
+        if (gh.defined()) {
+            ghr = grad_rows(gh, c.a.y_type, "the gradient of h");
+            g.grad_h = ghr.data_ptr(), g.grad_h_stride = row_stride(ghr);
+        }
+        g.d_x = raw(out[0]), g.d_y = raw(out[1]), g.d_weight_post = raw(out[2]), g.d_bias_post = raw(out[3]);
+        g.d_gate = raw(out[4]), g.d_scale = raw(out[5]), g.d_weight_pre = raw(out[6]), g.d_bias_pre = raw(out[7]);
+        const int64_t need = L.bs_join_backward_workspace_bytes(c.rows, c.cols);
+        const Tensor ws = empty({need}, c.x, at::kByte);
+        check(L.bs_join_backward(&c.a, &g, ws.data_ptr(), need, stream_of(c.x)), "bs_join_backward");
+        return out;
+    }
+};
+
+// x' and h, each where there is one
+std::vector<Tensor> join(const Tensor& x, const Maybe& y, const Maybe& w_post, const Maybe& b_post, const Maybe& gate,
+                         const Maybe& scale, const Maybe& w_pre, const Maybe& b_pre, int64_t post, int64_t pre,
+                         double eps_post, double eps_pre, double scale_value, at::ScalarType h_type)
+{
+    const JoinKind k{post, pre, eps_post, eps_pre, scale_value, h_type};
+    if (at::GradMode::is_enabled()) {
+        bool any = x.requires_grad();
+        for (const Maybe* m : {&y, &w_post, &b_post, &gate, &scale, &w_pre, &b_pre}) any = any || (*m && (*m)->requires_grad());
+        if (any) return Join::apply(x, y, w_post, b_post, gate, scale, w_pre, b_pre, k);
+    }
+    const c10::DeviceGuard guard(x.device());
+    JoinCall c(x, y, w_post, b_post, gate, scale, w_pre, b_pre, k);
+    const auto [x1, h, st] = join_forward(c, x.sizes(), false);
+    if (!c.a.y) return {h};
+    if (!c.a.norm_pre) return {x1};
+    return {x1, h};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -663,6 +901,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
                                optional(a.cols.scale));
     });
     m.def("col_sum", &col_sum);
+    m.def("join", &join);
     m.def("quantize_t", [](const Tensor& x, bool rows) {
         const c10::DeviceGuard guard(x.device());
         Workspace& w = ws_of(x);

@@ -1,0 +1,265 @@
+// What the forward and backward row kernels of the step between two blocks
+// share: how a row lies on the lanes, loads and stores of its 8-element
+// chunks in either type, sums over a row.
+//
+// A row of D elements is D / 8 chunks.  Up to 1024 elements one wave holds a
+// row (one or two chunks a lane) and a workgroup of four waves holds four;
+// above that one workgroup of ceil(D / 512) waves holds one row, a chunk a
+// lane (two or four past 8192).  The whole row then stays in registers
+// between the passes that its statistics take, and it is read once.
+#pragma once
+
+#include "bs_device.h"
+
+namespace bs {
+
+constexpr int kMaxRowCols = 32768;
+constexpr int kRowsPerSmallBlock = 4;
+
+typedef __bf16 bf16;
+
+// 8 elements as loaded
+template <typename T>
+struct Raw {
+    uint32_t w[2 * sizeof(T)];
+};
+
+template <typename T>
+__device__ __forceinline__ float raw_get(const Raw<T>& r, int e)
+{
+    if constexpr (sizeof(T) == 2)
+        return __uint_as_float(e & 1 ? r.w[e >> 1] & 0xffff0000u : r.w[e >> 1] << 16);
+    else
+        return __uint_as_float(r.w[e]);
+}
+
+// 8 elements at any address that their type allows; those from `nv` on are 0 and not read
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p, int nv)
+{
+    Raw<T> r;
+    if (nv >= 8) {
+        __builtin_memcpy(&r, p, sizeof(r));
+        return r;
+    }
+#pragma unroll
+    for (int i = 0; i < (int)(2 * sizeof(T)); i++) r.w[i] = 0;
+    if (nv <= 0) return r;
+#pragma unroll
+    for (int e = 0; e < 7; e++) {
+        if (e >= nv) continue;
+        if constexpr (sizeof(T) == 2)
+            r.w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << (16 * (e & 1));
+        else
+            r.w[e] = __builtin_bit_cast(uint32_t, p[e]);
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ Raw<T> to_raw(const float (&v)[8])
+{
+    Raw<T> r;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = f32_to_bf16(v[2 * i]) | (f32_to_bf16(v[2 * i + 1]) << 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.w[i] = __float_as_uint(v[i]);
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_raw(T* p, const Raw<T>& r, int nv)
+{
+    if (nv >= 8) {
+        __builtin_memcpy(p, &r, sizeof(r));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 7; e++) {
+        if (e >= nv) continue;
+        if constexpr (sizeof(T) == 2)
+            reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(r.w[e >> 1] >> (16 * (e & 1)));
+        else
+            reinterpret_cast<uint32_t*>(p)[e] = r.w[e];
+    }
+}
+
+// A learned vector (or one number for all columns), in either type; null: `other` everywhere.
+struct RowParam {
+    const void* p;
+    int f32;        // fp32, or bf16
+    int one;        // one number
+};
+
+__device__ __forceinline__ float param_one(const RowParam& a, int64_t i)
+{
+    return a.f32 ? static_cast<const float*>(a.p)[i] : (float)static_cast<const bf16*>(a.p)[i];
+}
+__device__ __forceinline__ void param_chunk(const RowParam& a, int64_t col, int nv, float other, float (&v)[8])
+{
+    if (a.p == nullptr || a.one || nv <= 0) {
+        const float s = a.p == nullptr || nv <= 0 ? other : param_one(a, 0);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = s;
+    } else if (a.f32) {
+        const Raw<float> r = load_raw(static_cast<const float*>(a.p) + col, nv);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = raw_get(r, e);
+    } else {
+        const Raw<bf16> r = load_raw(static_cast<const bf16*>(a.p) + col, nv);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = raw_get(r, e);
+    }
+}
+__device__ __forceinline__ void param_store(void* p, int f32, int64_t i, float v)
+{
+    if (f32)
+        static_cast<float*>(p)[i] = v;
+    else
+        static_cast<uint16_t*>(p)[i] = (uint16_t)f32_to_bf16(v);
+}
+
+// Sum over the 64 lanes of a wave, the same value in every lane: four steps
+// inside rows of 16 lanes, two across them, read back from the last lane.
+__device__ __forceinline__ float wave_sum_f32(float v)
+{
+#define BS_DPP_ADD(ctrl, rows)                                                                                     \
+    v += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), ctrl, rows, 0xf, false))
+    BS_DPP_ADD(0xb1, 0xf);      // lane ^ 1
+    BS_DPP_ADD(0x4e, 0xf);      // lane ^ 2
+    BS_DPP_ADD(0x141, 0xf);     // mirror in 8
+    BS_DPP_ADD(0x140, 0xf);     // mirror in 16
+    BS_DPP_ADD(0x142, 0xa);     // last lane of rows 0, 2 into rows 1, 3
+    BS_DPP_ADD(0x143, 0xc);     // last lane of row 1 into rows 2, 3
+#undef BS_DPP_ADD
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+
+// How a thread's chunks lie in its row.
+template <int C>
+struct RowPlace {
+    int waves;              // of a row
+    int wave, lane_in_row;  // this thread's
+    int nv[C];              // elements of its chunks inside the row
+    int64_t col[C];
+    float n_wave;           // elements of the row in this wave
+    float inv_cols;
+    __device__ __forceinline__ RowPlace(int64_t cols, int waves_)
+    {
+        waves = waves_;
+        lane_in_row = (int)threadIdx.x % (64 * waves);
+        wave = __builtin_amdgcn_readfirstlane(lane_in_row >> 6);
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const int c = (k * 64 * waves + lane_in_row) * 8;
+            col[k] = c;
+            nv[k] = max(0, min(8, (int)cols - c));
+            n += max(0, min(512, (int)cols - (k * waves + wave) * 512));
+        }
+        n_wave = (float)n;
+        inv_cols = 1.0f / (float)cols;
+    }
+    // elements of the row in wave i
+    __device__ __forceinline__ float n_of(int i, int64_t cols) const
+    {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < C; k++) n += max(0, min(512, (int)cols - (k * waves + i) * 512));
+        return (float)n;
+    }
+};
+
+// LDS for the sums of a row over its waves: two buffers in turn, so that one
+// barrier a sum is enough (a thread that writes a buffer again has passed the
+// barrier that came after everybody's reads of it).
+struct RowSums {
+    float4 part[2][16];
+};
+
+// Mean (0 for an RMS norm) and mean of squared deviations of a row.  A layer
+// norm's deviations are from each wave's own mean first; the waves' are joined
+// by n (mean_w - mean)^2, so nothing is lost where the mean is large.
+template <int C>
+__device__ __forceinline__ void row_moments(const float (&v)[C][8], const RowPlace<C>& at, int64_t cols, bool layer,
+                                            RowSums& s, int& turn, float& mean, float& var)
+{
+    float mw = 0.f;
+    if (layer) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < C; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) t += v[k][e];
+        mw = wave_sum_f32(t) / fmaxf(at.n_wave, 1.f);
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < C; k++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float d = v[k][e] - mw;
+            q += e < at.nv[k] ? d * d : 0.f;
+        }
+    q = wave_sum_f32(q);
+    if (at.waves > 1) {
+        if ((threadIdx.x & 63) == 0) s.part[turn][at.wave] = float4{mw, q, 0.f, 0.f};
+        __syncthreads();
+        float m = 0.f;
+        if (layer) {
+            for (int i = 0; i < at.waves; i++) m += s.part[turn][i].x * at.n_of(i, cols);
+            m *= at.inv_cols;
+        }
+        q = 0.f;
+        for (int i = 0; i < at.waves; i++) {
+            const float4 p = s.part[turn][i];
+            const float d = p.x - m;
+            q += layer ? p.y + at.n_of(i, cols) * d * d : p.y;
+        }
+        mw = m;
+        turn ^= 1;
+    }
+    mean = mw;
+    var = q * at.inv_cols;
+}
+
+// Sums of up to three values over a row, the same in all its threads.
+template <int N, int C>
+__device__ __forceinline__ void row_sums(float (&v)[N], const RowPlace<C>& at, RowSums& s, int& turn)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = wave_sum_f32(v[i]);
+    if (at.waves > 1) {
+        if ((threadIdx.x & 63) == 0)
+            s.part[turn][at.wave] = float4{v[0], N > 1 ? v[N > 1 ? 1 : 0] : 0.f, N > 2 ? v[N > 2 ? 2 : 0] : 0.f, 0.f};
+        __syncthreads();
+        float t[3] = {0.f, 0.f, 0.f};
+        for (int i = 0; i < at.waves; i++) {
+            const float4 p = s.part[turn][i];
+            t[0] += p.x;
+            t[1] += p.y;
+            t[2] += p.z;
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = t[i];
+        turn ^= 1;
+    }
+}
+
+// Workgroups of a row kernel: waves of a row, rows of a workgroup at a time, threads.
+struct RowLaunch {
+    int chunks, waves, rows, threads;
+};
+inline RowLaunch row_launch(int64_t cols)
+{
+    if (cols <= 512) return {1, 1, kRowsPerSmallBlock, 256};
+    if (cols <= 1024) return {2, 1, kRowsPerSmallBlock, 256};
+    const int c = cols <= 8192 ? 1 : cols <= 16384 ? 2 : 4;
+    const int w = (int)((cols + 512 * c - 1) / (512 * c));
+    return {c, w, 1, 64 * w};
+}
+
+}  // namespace bs

@@ -49,7 +49,7 @@ extern "C" {
 const char* bs_last_error(void);
 
 /* ABI version (bumped when an entry point changes): of this header, and of a built library. */
-#define BS_ABI_VERSION 17
+#define BS_ABI_VERSION 18
 int bs_abi_version(void);
 
 /*
@@ -635,6 +635,80 @@ const uint64_t* bs_workspace_amax_slot(const void* workspace, int64_t workspace_
  * Device pointer to a uint32.
  */
 const uint32_t* bs_workspace_fallback_counter(const void* workspace, int64_t workspace_bytes);
+
+/*
+ * The step from one MLP block to the next (no counterpart in the reference,
+ * whose blocks end at their own output):
+ *   p  = norm_post(y) or y;  x' = scale * x + gate * p;  h = norm_pre(x')
+ * over the rows of x (the residual stream) and y (a block's output), with
+ *   norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps) * weight + bias
+ * (BS_NORM_LAYER) or the same without the mean (BS_NORM_RMS).  Without y
+ * (NULL) it is the norm in front of a block alone, h = norm_pre(x).
+ *
+ * Types: BS_DT_BF16 or BS_DT_F32; x' has x's type, h and y share y_type, a
+ * vector has its own.  x = bf16 with y_type = fp32 is refused.  h is the norm
+ * of x' as stored (rounded to x_type).  Sums and statistics are fp32; every
+ * result is rounded once.
+ * Rows of up to 32768 elements; x, y and the element gate have a row stride
+ * (elements, >= 0) and contiguous rows at any address of their type; results
+ * are contiguous.
+ */
+#define BS_DT_F32 3
+#define BS_NORM_NONE 0
+#define BS_NORM_RMS 1
+#define BS_NORM_LAYER 2
+/* what gate or scale holds one value for */
+#define BS_PER_NOTHING 0   /* absent: 1 */
+#define BS_PER_TENSOR 1
+#define BS_PER_CHANNEL 2
+#define BS_PER_ROW 3       /* gate only */
+#define BS_PER_ELEMENT 4   /* gate only */
+
+typedef struct bs_vector {
+    const void* data;      /* NULL: absent */
+    int type;
+} bs_vector;
+
+typedef struct bs_join {
+    int64_t rows, cols;
+    int x_type, y_type;
+    int norm_post, norm_pre;         /* BS_NORM_*; norm_post needs y, one of y and norm_pre is there */
+    float eps_post, eps_pre;
+    const void* x;
+    const void* y;
+    int64_t x_stride, y_stride;
+    bs_vector weight_post, bias_post, weight_pre, bias_pre;
+    bs_vector gate, scale;
+    int gate_per, scale_per;         /* BS_PER_*; absent vectors have BS_PER_NOTHING */
+    int64_t gate_stride;             /* between the rows of a BS_PER_ROW or BS_PER_ELEMENT gate */
+    float scale_value;               /* scale where it is no vector */
+    float* stats_post;               /* [rows, 2] mean and 1 / deviation; forward: NULL or written, */
+    float* stats_pre;                /* backward: read */
+} bs_join;
+
+/* x1 = x' ([rows, cols], with y), h ([rows, cols], with norm_pre). */
+int bs_join_forward(const bs_join* args, void* x1, void* h, void* stream);
+
+/*
+ * Gradients of that step.  grad_x1 and grad_h (row strides in elements; NULL:
+ * zero) are of x' (x's type) and of h (y_type); x1 is the forward's x' (with
+ * y; row stride cols).  Every result may be NULL; those there are written
+ * whole, in the type of what they are the gradient of: d_x, d_y [rows, cols];
+ * d_gate in the gate's own shape, d_scale, and those of the four vectors.
+ * bs_join.x is read for d_scale (and, without y, for everything).  Sums over
+ * the rows go through `workspace` in a fixed order: the same call gives the
+ * same bits.
+ */
+typedef struct bs_join_grads {
+    const void* x1;
+    const void* grad_x1;
+    const void* grad_h;
+    int64_t grad_x1_stride, grad_h_stride;
+    void *d_x, *d_y, *d_gate, *d_scale, *d_weight_post, *d_bias_post, *d_weight_pre, *d_bias_pre;
+} bs_join_grads;
+int64_t bs_join_backward_workspace_bytes(int64_t rows, int64_t cols);
+int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* workspace, int64_t workspace_bytes,
+                     void* stream);
 
 #ifdef __cplusplus
 }
