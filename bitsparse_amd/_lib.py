@@ -95,6 +95,8 @@ _SIGNATURES = {
     "bs_join_forward": [_vp, _vp, _vp, _vp],
     "bs_join_backward_workspace_bytes": [_i64, _i64],
     "bs_join_backward": [_vp, _vp, _vp, _i64, _vp],
+    "bs_newton_schulz_workspace_bytes": [_i64, _i64, _i64],
+    "bs_newton_schulz": [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp],
     "bs_launch_timing": [_int],
     "bs_nontemporal_min_bytes": [_i64],
     "bs_launch_timing_read": [_vp, _vp, _int, _vp],
@@ -111,6 +113,7 @@ _RESTYPES = {
     "bs_grad_sums_workspace_bytes": _i64,
     "bs_col_sum_workspace_bytes": _i64,
     "bs_join_backward_workspace_bytes": _i64,
+    "bs_newton_schulz_workspace_bytes": _i64,
     "bs_nontemporal_min_bytes": _i64,
     "bs_workspace_amax_slot": _vp,
     "bs_workspace_fallback_counter": _vp,

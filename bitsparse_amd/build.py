@@ -15,7 +15,7 @@ PKG = os.path.join(ROOT, "bitsparse_amd")
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 SOURCES = ["runtime.hip", "fp8.hip", "codec.hip", "dw_gemm.hip", "dw_gemm8.hip", "up_gemm.hip", "colsum.hip",
-           "rownorm_fwd.hip", "rownorm_bwd.hip", "probe.hip"]
+           "rownorm_fwd.hip", "rownorm_bwd.hip", "newton.hip", "probe.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -15,6 +15,7 @@
 
 #include <map>
 #include <memory>
+#include <set>
 
 #include "bitsparse_hip.h"
 
@@ -33,7 +34,8 @@ using at::Tensor;
     F(bs_col_sum_workspace_bytes) F(bs_col_sum) F(bs_gemm_compressed_b_workspace_bytes) F(bs_gemm_compressed_b)  \
     F(bs_gemm_compressed_b_packed_workspace_bytes) F(bs_gemm_compressed_b_packed)                                \
     F(bs_gemm_compressed_b_fp8_workspace_bytes) F(bs_gemm_compressed_b_fp8) F(bs_gemm_compressed_b_fp8_packed)   \
-    F(bs_workspace_amax_slot) F(bs_join_forward) F(bs_join_backward_workspace_bytes) F(bs_join_backward)
+    F(bs_workspace_amax_slot) F(bs_join_forward) F(bs_join_backward_workspace_bytes) F(bs_join_backward) \
+    F(bs_newton_schulz_workspace_bytes) F(bs_newton_schulz)
 struct Lib {
 #define F(name) decltype(&::name) name = nullptr;
     BS_FUNCS(F)
@@ -857,6 +859,128 @@ std::vector<Tensor> join(const Tensor& x, const Maybe& y, const Maybe& w_post, c
     return {x1, h};
 }
 
+// ---------------------------------------------------------------------------
+// orthogonalised updates (muon.py)
+// ---------------------------------------------------------------------------
+struct NewtonRule {
+    int64_t steps;
+    double a, b, c, eps;
+};
+
+// rows of t at their own stride; `what` is written, so its rows are contiguous and apart
+int64_t matrix_stride(const Tensor& t, const char* what)
+{
+    const int64_t R = t.size(0), C = t.size(1);
+    TORCH_CHECK_VALUE((C <= 1 || t.stride(1) == 1) && (R <= 1 || t.stride(0) >= C), what,
+                      ": its rows have to be contiguous and apart (strides ", t.strides(), ")");
+    return R > 1 ? t.stride(0) : C;
+}
+
+// One call for matrices of one shape up to transposition.
+void newton_group(const std::vector<bs_matrix>& mats, int64_t m, int64_t n, const bs_newton_schulz_rule& rule, const Tensor& on)
+{
+    const int64_t count = mats.size(), need = L.bs_newton_schulz_workspace_bytes(m, n, count);
+    const Tensor ws = at::empty({need}, on.options().dtype(at::kByte));
+    check(L.bs_newton_schulz(mats.data(), count, m, n, &rule, ws.data_ptr(), need, stream_of(on)), "bs_newton_schulz");
+}
+
+void check_matrix(const Tensor& t, const char* what)
+{
+    plain_on_gpu(t, what);
+    TORCH_CHECK_VALUE(t.dim() == 2 && t.numel() > 0, what, ": expected a matrix with elements, got ", t.sizes());
+}
+
+Tensor orthogonalize(const Tensor& G, int64_t steps, double a, double b, double c, double eps)
+{
+    plain_on_gpu(G, "G");
+    TORCH_CHECK_VALUE(G.dim() >= 2, "G: expected matrices [..., R, C], got ", G.sizes());
+    const c10::DeviceGuard guard(G.device());
+    bs_newton_schulz_rule rule{};
+    rule.grad_type = row_type(G, "G");
+    rule.out_type = BS_DT_BF16;
+    rule.steps = (int)std::clamp<int64_t>(steps, -1, 1000);
+    rule.a = (float)a, rule.b = (float)b, rule.c = (float)c, rule.eps = (float)eps;
+    Tensor out = at::empty(G.sizes(), G.options().dtype(at::kBFloat16));
+    if (G.numel() == 0) return out;
+    const int64_t R = G.size(-2), C = G.size(-1), count = G.numel() / (R * C);
+    Tensor g = G.dim() == 3 ? G : G.reshape({count, R, C});
+    if (C > 1 && g.stride(2) != 1) g = g.contiguous();
+    std::vector<bs_matrix> mats(count);
+    for (int64_t i = 0; i < count; i++) {
+        mats[i].grad = static_cast<const char*>(g.data_ptr()) + i * g.stride(0) * g.element_size();
+        mats[i].grad_stride = R > 1 ? g.stride(1) : C;
+        mats[i].out = static_cast<char*>(out.data_ptr()) + i * R * C * 2;
+        mats[i].out_stride = C;
+    }
+    newton_group(mats, R, C, rule, G);
+    return out;
+}
+
+// The update of lists of weights: matrices of one shape (up to transposition)
+// and set of types go together.  All are checked before the first is touched.
+void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, const std::vector<Tensor>& M, double lr, double mu,
+                 bool nesterov, double decay, bool by_rms, double scale, int64_t steps, double a, double b, double c, double eps)
+{
+    TORCH_CHECK_VALUE(W.size() == G.size() && W.size() == M.size(), "params, grads and momenta: lists of one length, got ",
+                      W.size(), ", ", G.size(), ", ", M.size());
+    if (W.empty()) return;
+    TORCH_CHECK_VALUE(steps >= 1 && steps <= 100, "steps must be in 1..100, got ", steps);
+    struct Key {
+        int64_t m, n;
+        int g, mt, w, dev;
+        double s;
+        bool operator<(const Key& o) const
+        {
+            return std::tie(m, n, g, mt, w, dev, s) < std::tie(o.m, o.n, o.g, o.mt, o.w, o.dev, o.s);
+        }
+    };
+    std::map<Key, std::vector<bs_matrix>> groups;
+    std::map<int, Tensor> on;
+    std::vector<Tensor> held;
+    std::set<const void*> written;
+    for (size_t i = 0; i < W.size(); i++) {
+        check_matrix(W[i], "a parameter");
+        check_matrix(G[i], "a gradient");
+        check_matrix(M[i], "a momentum");
+        TORCH_CHECK_VALUE(G[i].sizes() == W[i].sizes() && M[i].sizes() == W[i].sizes(), "parameter ", i, " ", W[i].sizes(),
+                          ", its gradient ", G[i].sizes(), " and momentum ", M[i].sizes(), " differ in shape");
+        TORCH_CHECK(G[i].device() == W[i].device() && M[i].device() == W[i].device(), "parameter ", i,
+                    ", its gradient and momentum are on different devices");
+        TORCH_CHECK_VALUE(written.insert(W[i].data_ptr()).second && written.insert(M[i].data_ptr()).second,
+                          "parameter ", i, " or its momentum is in the lists twice");
+        const int64_t R = W[i].size(0), C = W[i].size(1);
+        TORCH_CHECK_VALUE(std::max(R, C) <= 65536 && R * C < (int64_t(1) << 30), "parameter ", i, ": ", W[i].sizes(),
+                          " is past 65536 rows or columns or 2^30 elements");
+        Tensor g = G[i];
+        if (C > 1 && g.stride(1) != 1) held.push_back(g = g.contiguous());
+        bs_matrix t{};
+        t.grad = g.data_ptr(), t.grad_stride = R > 1 ? g.stride(0) : C;
+        t.momentum = M[i].data_ptr(), t.momentum_stride = matrix_stride(M[i], "a momentum");
+        t.out = W[i].data_ptr(), t.out_stride = matrix_stride(W[i], "a parameter");
+        t.transposed = R > C;
+        // 0.2 sqrt(max): updates of the size of Adam's; sqrt(rows / columns) for tall ones
+        const double s = by_rms ? 0.2 * std::sqrt((double)std::max(R, C)) : scale < 0 ? std::sqrt(std::max(1.0, (double)R / (double)C)) : scale;
+        const Key key{std::min(R, C), std::max(R, C), row_type(g, "a gradient"), row_type(M[i], "a momentum"),
+                      row_type(W[i], "a parameter"), W[i].get_device(), s};
+        groups[key].push_back(t);
+        on.emplace(key.dev, W[i]);
+    }
+    for (const auto& [key, mats] : groups) {
+        const Tensor& like = on.at(key.dev);
+        const c10::DeviceGuard guard(like.device());
+        bs_newton_schulz_rule rule{};
+        rule.grad_type = key.g, rule.momentum_type = key.mt, rule.out_type = key.w;
+        rule.momentum = 1, rule.nesterov = nesterov, rule.update = 1;
+        rule.steps = (int)steps;
+        rule.a = (float)a, rule.b = (float)b, rule.c = (float)c, rule.eps = (float)eps, rule.mu = (float)mu;
+        rule.keep = (float)(1.0 - lr * decay), rule.rate = (float)(lr * key.s);
+        newton_group(mats, key.m, key.n, rule, like);
+    }
+    // (autograd's saved copies of the parameters are stale now)
+    for (const auto* list : {&W, &M})
+        for (const Tensor& t : *list) t.unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -902,6 +1026,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     });
     m.def("col_sum", &col_sum);
     m.def("join", &join);
+    m.def("orthogonalize", &orthogonalize);
+    m.def("muon_update", &muon_update, py::call_guard<py::gil_scoped_release>());
     m.def("quantize_t", [](const Tensor& x, bool rows) {
         const c10::DeviceGuard guard(x.device());
         Workspace& w = ws_of(x);

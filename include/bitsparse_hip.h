@@ -710,6 +710,38 @@ int64_t bs_join_backward_workspace_bytes(int64_t rows, int64_t cols);
 int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* workspace, int64_t workspace_bytes,
                      void* stream);
 
+/*
+ * Orthogonalised updates of weight matrices (no counterpart in the reference,
+ * which leaves its weight gradients to torch's optimisers).  For each of
+ * `count` matrices, [rows, cols] or (transposed) [cols, rows]:
+ *   with a momentum: M <- mu M + (1 - mu) G and U = (1 - mu) G + mu M
+ *   (nesterov) or M, of M as stored; without: U = G
+ *   X = U / (||U||_F + eps); `steps` times X <- (a I + b A + c A^2) X with
+ *   A = X X^T (of the transpose, where U has more rows than columns)
+ *   out <- X, or (update) out <- keep * out - rate * X
+ * G, M and out are bf16 or fp32, each type the same for all matrices, with
+ * contiguous rows `*_stride` elements apart.  Products have fp16 operands and
+ * fp32 sums: X comes to 1-3e-3 of the exact result for a gradient of full
+ * rank (directions in which U is 0, and the result too, hold noise of up to
+ * 5e-3 of a unit singular value each).
+ */
+typedef struct bs_matrix {
+    const void* grad;
+    void* momentum;                  /* NULL without one */
+    void* out;
+    int64_t grad_stride, momentum_stride, out_stride;
+    int transposed;
+} bs_matrix;
+typedef struct bs_newton_schulz_rule {
+    int grad_type, momentum_type, out_type;     /* BS_DT_BF16 or BS_DT_F32 */
+    int momentum, nesterov, update;             /* flags */
+    int steps;
+    float a, b, c, eps, mu, keep, rate;
+} bs_newton_schulz_rule;
+int64_t bs_newton_schulz_workspace_bytes(int64_t rows, int64_t cols, int64_t count);
+int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_t rows, int64_t cols,
+                     const bs_newton_schulz_rule* rule, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
