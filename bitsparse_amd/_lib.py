@@ -95,7 +95,7 @@ _SIGNATURES = {
     "bs_join_forward": [_vp, _vp, _vp, _vp],
     "bs_join_backward_workspace_bytes": [_i64, _i64],
     "bs_join_backward": [_vp, _vp, _vp, _i64, _vp],
-    "bs_newton_schulz_workspace_bytes": [_i64, _i64, _i64],
+    "bs_newton_schulz_workspace_bytes": [_i64, _i64, _i64, _int],
     "bs_newton_schulz": [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp],
     "bs_launch_timing": [_int],
     "bs_nontemporal_min_bytes": [_i64],

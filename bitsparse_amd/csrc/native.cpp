@@ -879,7 +879,7 @@ int64_t matrix_stride(const Tensor& t, const char* what)
 // One call for matrices of one shape up to transposition.
 void newton_group(const std::vector<bs_matrix>& mats, int64_t m, int64_t n, const bs_newton_schulz_rule& rule, const Tensor& on)
 {
-    const int64_t count = mats.size(), need = L.bs_newton_schulz_workspace_bytes(m, n, count);
+    const int64_t count = mats.size(), need = L.bs_newton_schulz_workspace_bytes(m, n, count, rule.precise);
     const Tensor ws = at::empty({need}, on.options().dtype(at::kByte));
     check(L.bs_newton_schulz(mats.data(), count, m, n, &rule, ws.data_ptr(), need, stream_of(on)), "bs_newton_schulz");
 }
@@ -890,7 +890,7 @@ void check_matrix(const Tensor& t, const char* what)
     TORCH_CHECK_VALUE(t.dim() == 2 && t.numel() > 0, what, ": expected a matrix with elements, got ", t.sizes());
 }
 
-Tensor orthogonalize(const Tensor& G, int64_t steps, double a, double b, double c, double eps)
+Tensor orthogonalize(const Tensor& G, int64_t steps, double a, double b, double c, double eps, bool precise)
 {
     plain_on_gpu(G, "G");
     TORCH_CHECK_VALUE(G.dim() >= 2, "G: expected matrices [..., R, C], got ", G.sizes());
@@ -898,6 +898,7 @@ Tensor orthogonalize(const Tensor& G, int64_t steps, double a, double b, double 
     bs_newton_schulz_rule rule{};
     rule.grad_type = row_type(G, "G");
     rule.out_type = BS_DT_BF16;
+    rule.precise = precise;
     rule.steps = (int)std::clamp<int64_t>(steps, -1, 1000);
     rule.a = (float)a, rule.b = (float)b, rule.c = (float)c, rule.eps = (float)eps;
     Tensor out = at::empty(G.sizes(), G.options().dtype(at::kBFloat16));
@@ -919,7 +920,8 @@ Tensor orthogonalize(const Tensor& G, int64_t steps, double a, double b, double 
 // The update of lists of weights: matrices of one shape (up to transposition)
 // and set of types go together.  All are checked before the first is touched.
 void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, const std::vector<Tensor>& M, double lr, double mu,
-                 bool nesterov, double decay, bool by_rms, double scale, int64_t steps, double a, double b, double c, double eps)
+                 bool nesterov, double decay, bool by_rms, double scale, int64_t steps, double a, double b, double c, double eps,
+                 const std::optional<bool>& precise)
 {
     TORCH_CHECK_VALUE(W.size() == G.size() && W.size() == M.size(), "params, grads and momenta: lists of one length, got ",
                       W.size(), ", ", G.size(), ", ", M.size());
@@ -949,8 +951,8 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         TORCH_CHECK_VALUE(written.insert(W[i].data_ptr()).second && written.insert(M[i].data_ptr()).second,
                           "parameter ", i, " or its momentum is in the lists twice");
         const int64_t R = W[i].size(0), C = W[i].size(1);
-        TORCH_CHECK_VALUE(std::max(R, C) <= 65536 && R * C < (int64_t(1) << 30), "parameter ", i, ": ", W[i].sizes(),
-                          " is past 65536 rows or columns or 2^30 elements");
+        TORCH_CHECK_VALUE(std::max(R, C) <= 65536 && R * C < (int64_t(1) << 29), "parameter ", i, ": ", W[i].sizes(),
+                          " is past 65536 rows or columns or 2^29 elements");
         Tensor g = G[i];
         if (C > 1 && g.stride(1) != 1) held.push_back(g = g.contiguous());
         bs_matrix t{};
@@ -971,6 +973,7 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         bs_newton_schulz_rule rule{};
         rule.grad_type = key.g, rule.momentum_type = key.mt, rule.out_type = key.w;
         rule.momentum = 1, rule.nesterov = nesterov, rule.update = 1;
+        rule.precise = precise.value_or(key.w == BS_DT_F32);
         rule.steps = (int)steps;
         rule.a = (float)a, rule.b = (float)b, rule.c = (float)c, rule.eps = (float)eps, rule.mu = (float)mu;
         rule.keep = (float)(1.0 - lr * decay), rule.rate = (float)(lr * key.s);

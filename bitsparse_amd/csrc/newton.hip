@@ -17,13 +17,19 @@
 // result on gradients, fp16 ones 1.0-2.4e-3, less than the 1.7e-3 that
 // rounding the result itself to bf16 costs.
 //
+// Where the result goes into fp32 weights that is not enough: there each of X,
+// A and B is held as two fp16 numbers, the value and what is left of it (22
+// bits), and a product is three, high x high + high x low + low x high, one
+// after the other into the same sums: 2e-6 from the exact result, as products
+// of fp32 operands come, at the matrix cores' fp16 rate.
+//
 // All buffers are padded with zeros to whole tiles, which the products keep
 // (B's padding only meets X's zero rows), so the main loop has no bounds.
 #include <algorithm>
-#include <type_traits>
 
 #include "bs_device.h"
 #include "bs_host.h"
+#include "rownorm.h"
 
 namespace bs {
 
@@ -32,12 +38,14 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kHeld = 4096.f;         // fp16 value = true value * kHeld
 constexpr int kStepK = 64;              // K of a main-loop step
 constexpr int kNsBatch = 64;            // matrices of a launch
-constexpr int kNsParts = 64;            // partial sums of squares of a matrix
+constexpr int kNsParts = 256;           // most partial sums of squares of a matrix
+constexpr int kNsCus = 256, kNsXcds = 8;
 
 enum : int { kGram = 0, kPoly, kStep, kLast };
 
@@ -57,43 +65,73 @@ struct NsMatrices {
 // ---------------------------------------------------------------------------
 struct NsPrep {
     int64_t m, n, mp, np;
-    int g_f32, m_f32, momentum, nesterov;
+    int g_f32, m_f32, momentum, nesterov, parts, precise;
     float mu, eps;
-    double* parts;                      // [count][kNsParts]
-    _Float16* x;                        // [count][mp][np]
+    double* parts_at;                   // [count][kNsParts]
+    _Float16* x;                        // [count][mp][np], precise: and the low parts behind all of them
+    int64_t low;                        // elements from a value to its low part
 };
 
-__device__ __forceinline__ float ns_load(const void* p, int f32, int64_t i)
+__device__ __forceinline__ void ns_chunk(const void* p, int f32, int64_t i, int nv, float (&v)[8])
 {
-    return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const __bf16*>(p)[i];
+    if (f32) {
+        const Raw<float> r = load_raw(static_cast<const float*>(p) + i, nv);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = raw_get(r, e);
+    } else {
+        const Raw<bf16> r = load_raw(static_cast<const bf16*>(p) + i, nv);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = raw_get(r, e);
+    }
 }
-__device__ __forceinline__ void ns_store(void* p, int f32, int64_t i, float v)
+
+// 8 elements of U; with a momentum M' comes from (update) M or is read
+__device__ __forceinline__ void ns_u(const NsPrep& a, const NsMatrix& t, int64_t r, int64_t c, int nv, bool update, float (&u)[8])
 {
-    if (f32)
-        static_cast<float*>(p)[i] = v;
-    else
-        static_cast<uint16_t*>(p)[i] = (uint16_t)f32_to_bf16(v);
+    ns_chunk(t.g, a.g_f32, r * t.g_stride + c, nv, u);
+    if (!a.momentum) return;
+    float m[8];
+    ns_chunk(t.m, a.m_f32, r * t.m_stride + c, nv, m);
+    if (update) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) m[e] = a.mu * m[e] + (1.f - a.mu) * u[e];
+        if (a.m_f32) {
+            store_raw(static_cast<float*>(t.m) + r * t.m_stride + c, to_raw<float>(m), nv);
+        } else {
+            const Raw<bf16> o = to_raw<bf16>(m);
+            store_raw(static_cast<bf16*>(t.m) + r * t.m_stride + c, o, nv);
+#pragma unroll
+            for (int e = 0; e < 8; e++) m[e] = raw_get(o, e);       // U is of M' as stored
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) u[e] = a.nesterov ? (1.f - a.mu) * u[e] + a.mu * m[e] : m[e];
 }
-// M' as its type holds it, and U
-__device__ __forceinline__ float ns_update(const NsPrep& a, float g, float m) { return a.nesterov ? (1.f - a.mu) * g + a.mu * m : m; }
 
 // The momentum's update and partial sums of squares of U (in 64 bits: any
-// gradient that fp32 holds has a norm).  blockIdx.y: the matrix.
+// gradient that fp32 holds has a norm).  blockIdx.y: the matrix.  Memory
+// bound: 8 elements a load, four chunks of a thread in flight.
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsPrep a, NsMatrices mats)
 {
     const NsMatrix t = mats.at[blockIdx.y];
-    const int64_t rows = t.tall ? a.n : a.m, cols = t.tall ? a.m : a.n, total = rows * cols;
+    const uint32_t rows = (uint32_t)(t.tall ? a.n : a.m), cols = (uint32_t)(t.tall ? a.m : a.n);
+    const uint32_t per_row = (cols + 7) / 8, total = rows * per_row;    // (< 2^30)
+    const uint32_t step = gridDim.x * 256;
     double s = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
-        float u = ns_load(t.g, a.g_f32, r * t.g_stride + c);
-        if (a.momentum) {
-            const int64_t at = r * t.m_stride + c;
-            const float m = a.mu * ns_load(t.m, a.m_f32, at) + (1.f - a.mu) * u;
-            ns_store(t.m, a.m_f32, at, m);
-            u = ns_update(a, u, a.m_f32 ? m : (float)(__bf16)m);
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += 4 * step) {
+        float u[4][8];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t at = i + k * step, r = at / per_row, c = (at - r * per_row) * 8;
+            const int nv = at < total ? (int)min(8u, cols - c) : 0;
+            ns_u(a, t, r, c, nv, true, u[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) u[k][e] = e < nv ? u[k][e] : 0.f;
         }
-        s += (double)u * (double)u;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) s += (double)u[k][e] * (double)u[k][e];
     }
     __shared__ double s_part[256];
     s_part[threadIdx.x] = s;
@@ -102,34 +140,60 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsPrep a, NsMatrices mats)
         if ((int)threadIdx.x < w) s_part[threadIdx.x] += s_part[threadIdx.x + w];
         __syncthreads();
     }
-    if (threadIdx.x == 0) a.parts[(int64_t)blockIdx.y * kNsParts + blockIdx.x] = s_part[0];
+    if (threadIdx.x == 0) a.parts_at[(int64_t)blockIdx.y * kNsParts + blockIdx.x] = s_part[0];
 }
 
-// X_0 in 64 x 64 tiles of [mp, np], zeros outside [m, n].
-__global__ __launch_bounds__(256) void ns_scale_kernel(NsPrep a, NsMatrices mats, int parts)
+__device__ __forceinline__ f16x8 ns_low(const float (&v)[8], f16x8 high)
+{
+    f16x8 l;
+#pragma unroll
+    for (int e = 0; e < 8; e++) l[e] = (_Float16)(v[e] - (float)high[e]);
+    return l;
+}
+
+// X_0 in 64 x 64 tiles of [mp, np], zeros outside [m, n]; a taller matrix is
+// turned through LDS.  Every workgroup adds the partial sums itself, in order.
+__global__ __launch_bounds__(256) void ns_scale_kernel(NsPrep a, NsMatrices mats)
 {
     const NsMatrix t = mats.at[blockIdx.z];
-    __shared__ float s_t[64][65];
-    double q = 0.0;
-    for (int i = 0; i < parts; i++) q += a.parts[(int64_t)blockIdx.z * kNsParts + i];
-    const float norm = (float)sqrt(q) + a.eps;
+    __shared__ float s_t[64][68];
+    __shared__ double s_q[kNsParts];
     const int64_t i0 = (int64_t)blockIdx.y * 64, j0 = (int64_t)blockIdx.x * 64;
-    const int c = threadIdx.x & 63, r4 = threadIdx.x >> 6;
-    for (int r = r4; r < 64; r += 4) {
+    const int64_t rows = t.tall ? a.n : a.m, cols = t.tall ? a.m : a.n;
+    float u[2][8];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int r = k * 32 + (int)threadIdx.x / 8, c = (int)threadIdx.x % 8 * 8;
         const int64_t gr = (t.tall ? j0 : i0) + r, gc = (t.tall ? i0 : j0) + c;
-        float u = 0.f;
-        if (gr < (t.tall ? a.n : a.m) && gc < (t.tall ? a.m : a.n)) {
-            u = ns_load(t.g, a.g_f32, gr * t.g_stride + gc);
-            if (a.momentum) u = ns_update(a, u, ns_load(t.m, a.m_f32, gr * t.m_stride + gc));
+        const int nv = gr < rows ? (int)max((int64_t)0, min((int64_t)8, cols - gc)) : 0;
+        ns_u(a, t, nv ? gr : 0, nv ? gc : 0, nv, false, u[k]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            u[k][e] = e < nv ? u[k][e] : 0.f;
+            if (t.tall) s_t[c + e][r] = u[k][e];
         }
-        if (t.tall)
-            s_t[c][r] = u;
-        else
-            s_t[r][c] = u;
     }
+    s_q[threadIdx.x] = (int)threadIdx.x < a.parts ? a.parts_at[(int64_t)blockIdx.z * kNsParts + threadIdx.x] : 0.0;
     __syncthreads();
-    for (int r = r4; r < 64; r += 4)
-        a.x[((int64_t)blockIdx.z * a.mp + i0 + r) * a.np + j0 + c] = (_Float16)(s_t[r][c] / norm * kHeld);
+    for (int w = kNsParts / 2; w > 0; w >>= 1) {
+        if ((int)threadIdx.x < w) s_q[threadIdx.x] += s_q[threadIdx.x + w];
+        __syncthreads();
+    }
+    const float norm = (float)sqrt(s_q[0]) + a.eps;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int r = k * 32 + (int)threadIdx.x / 8, c = (int)threadIdx.x % 8 * 8;
+        float v[8];
+        f16x8 h;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[e] = (t.tall ? s_t[r][c + e] : u[k][e]) / norm * kHeld;
+            h[e] = (_Float16)v[e];
+        }
+        _Float16* out = a.x + ((int64_t)blockIdx.z * a.mp + i0 + r) * a.np + j0 + c;
+        *reinterpret_cast<f16x8*>(out) = h;
+        if (a.precise) *reinterpret_cast<f16x8*>(out + a.low) = ns_low(v, h);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -139,10 +203,15 @@ __global__ __launch_bounds__(256) void ns_scale_kernel(NsPrep a, NsMatrices mats
 struct NsGemm {
     const _Float16 *p, *q;              // [count] matrices
     int64_t p_size, q_size, out_size;   // elements of one matrix
+    int64_t p_low, q_low, out_low;      // precise: elements from a value to its low part
     int ldp, ldq, ldo;
-    int k_steps;
-    int tiles_m, tiles_n;               // of the whole product
-    int count;
+    int k_steps;                        // of one pass over K
+    int passes;                         // 1, or 3 (precise)
+    int tiles_m, tiles_n;               // of one matrix's product
+    int tiles;                          // of all matrices, those left out by symmetry not counted
+    int whole;                          // tiles with a workgroup of their own; the others' steps are
+    int sharers;                        // dealt out evenly to this many workgroups
+    float* part;                        // [sharers][2][tile]: their sums
     _Float16* out;
     float a, b, c;                      // poly
     // last
@@ -151,34 +220,156 @@ struct NsGemm {
     float keep, rate;
 };
 
-// WGM x WGN waves, each a block of 32 IM x 32 JN
-template <int WGM_, int WGN_, int IM_, int JN_>
+// WGM x WGN waves, each a block of 32 IM x 32 JN; STAGES of the K loop in LDS
+template <int WGM_, int WGN_, int IM_, int JN_, int STAGES_>
 struct NsCfg {
-    static constexpr int WGM = WGM_, WGN = WGN_, IM = IM_, JN = JN_;
-    static constexpr int THREADS = 64 * WGM * WGN;
+    static constexpr int WGM = WGM_, WGN = WGN_, IM = IM_, JN = JN_, STAGES = STAGES_;
+    static constexpr int WAVES = WGM * WGN, THREADS = 64 * WAVES;
     static constexpr int TM = 32 * IM * WGM, TN = 32 * JN * WGN;
     static constexpr int P_BYTES = TM * kStepK * 2, Q_BYTES = TN * kStepK * 2;
     static constexpr int STAGE = P_BYTES + Q_BYTES;
+    static constexpr int LOADS = STAGE / 1024 / WAVES;          // of a wave for a stage
     static constexpr int PITCH = TN + 8;                        // of the result's tile in LDS
-    static constexpr int LDS = 2 * STAGE > TM * PITCH * 2 ? 2 * STAGE : TM * PITCH * 2;
+    static constexpr int LDS = STAGES * STAGE > TM * PITCH * 2 ? STAGES * STAGE : TM * PITCH * 2;
+    static_assert(TM == TN, "square tiles: half of a symmetric product is its lower triangle of tiles");
     static_assert(LDS <= 160 * 1024, "LDS budget");
-    static_assert(P_BYTES / 1024 % (WGM * WGN) == 0 && Q_BYTES / 1024 % (WGM * WGN) == 0, "whole loads for every wave");
+    static_assert(P_BYTES / 1024 % WAVES == 0 && Q_BYTES / 1024 % WAVES == 0, "whole loads for every wave");
 };
-using NsLarge = NsCfg<2, 4, 4, 2>;      // 256 x 256
-using NsMiddle = NsCfg<2, 2, 2, 2>;     // 128 x 128
-using NsSmall = NsCfg<2, 2, 1, 1>;      // 64 x 64
+using NsLarge = NsCfg<2, 4, 4, 2, 2>;       // 256 x 256
+using NsMiddle = NsCfg<2, 2, 2, 2, 2>;      // 128 x 128
+using NsSmall = NsCfg<2, 2, 1, 1, 4>;       // 64 x 64
 
 // 16 bytes a lane from `rsrc` at voff + soff straight into LDS at `lds` + 16 lane
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t lds, uint32_t voff, uint32_t soff)
 {
     // (one wait state between the write of m0 and its use)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform_u32(lds)), "v"(voff), "s"(rsrc), "s"(soff)
+                 : "memory");
 }
 __device__ __forceinline__ i32x4 ns_rsrc(const void* p, uint32_t bytes)
 {
     const uint64_t a = (uint64_t)p;
     return i32x4{(int)uniform_u32((uint32_t)a), (int)uniform_u32((uint32_t)(a >> 32) & 0xffffu), (int)bytes, 0x00020000};
+}
+template <int N>
+__device__ __forceinline__ void wait_loads()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+struct NsTile {
+    int batch, ti, tj;
+};
+template <bool SYM>
+__device__ __forceinline__ NsTile ns_tile(const NsGemm& g, int tile)
+{
+    const int per = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
+    NsTile t;
+    t.batch = tile / per;
+    tile -= t.batch * per;
+    if constexpr (SYM) {        // those with tj <= ti
+        t.ti = (int)((sqrtf(8.f * (float)tile + 1.f) - 1.f) * 0.5f);
+        while ((t.ti + 1) * (t.ti + 2) / 2 <= tile) t.ti++;
+        while (t.ti * (t.ti + 1) / 2 > tile) t.ti--;
+        t.tj = tile - t.ti * (t.ti + 1) / 2;
+    } else {                    // four rows of tiles at a time: neighbours share rows of P and columns of Q
+        const int group = tile / (4 * g.tiles_n), first = 4 * group, rows = min(4, g.tiles_m - first);
+        tile -= group * 4 * g.tiles_n;
+        t.ti = first + tile % rows;
+        t.tj = tile / rows;
+    }
+    return t;
+}
+
+// Results of a tile.  A lane holds row i = lane % 32 of a block, columns
+// 8 q + 4 (lane / 32) + e in register 4 q + e.
+template <class Cfg, int KIND>
+__device__ __forceinline__ void ns_finish(const NsGemm& g, const NsMatrices& mats, const NsTile t, f32x16 (&acc)[Cfg::IM][Cfg::JN],
+                                          char* s_mem)
+{
+    constexpr bool kSym = KIND == kGram || KIND == kPoly;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wm = wave / Cfg::WGN, wn = wave % Cfg::WGN;
+    const bool precise = g.passes > 1;
+    if constexpr (KIND == kLast) {      // straight to the weights, in their own orientation
+        const NsMatrix mat = mats.at[t.batch];
+#pragma unroll
+        for (int i = 0; i < Cfg::IM; i++)
+#pragma unroll
+            for (int j = 0; j < Cfg::JN; j++)
+#pragma unroll
+                for (int qd = 0; qd < 4; qd++) {
+                    const int64_t r = (int64_t)t.ti * Cfg::TM + (wm * Cfg::IM + i) * 32 + (lane & 31);
+                    const int64_t c = (int64_t)t.tj * Cfg::TN + (wn * Cfg::JN + j) * 32 + 8 * qd + 4 * (lane >> 5);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (r >= g.m || c + e >= g.n) continue;
+                        const float o = acc[i][j][4 * qd + e] * (1.f / (kHeld * kHeld));
+                        const int64_t at = mat.tall ? (c + e) * mat.w_stride + r : r * mat.w_stride + c + e;
+                        const float v = g.update ? g.keep * param_one(RowParam{mat.w, g.w_f32, 0}, at) - g.rate * o : o;
+                        param_store(mat.w, g.w_f32, at, v);
+                    }
+                }
+    } else {
+        // through LDS as a row-major tile, the high parts and (precise) then the low ones
+        _Float16* tile_s = reinterpret_cast<_Float16*>(s_mem);
+        for (int part = 0; part < (precise ? 2 : 1); part++) {
+            // (made anew for the second time round: kept, the 128 products would not fit the registers)
+            float scale = (KIND == kPoly ? g.c : 1.f) / kHeld;
+            asm volatile("" : "+v"(scale)::"memory");
+#pragma unroll
+            for (int i = 0; i < Cfg::IM; i++)
+#pragma unroll
+                for (int j = 0; j < Cfg::JN; j++) {
+                    const int r = (wm * Cfg::IM + i) * 32 + (lane & 31);
+#pragma unroll
+                    for (int qd = 0; qd < 4; qd++) {
+                        const int c = (wn * Cfg::JN + j) * 32 + 8 * qd + 4 * (lane >> 5);
+                        f16x4 v, old = {}, old_low = {};
+                        const int gi = t.ti * Cfg::TM + r, gj = t.tj * Cfg::TN + c;
+                        if constexpr (KIND == kPoly) {      // p is A
+                            const _Float16* at = g.p + t.batch * g.p_size + (int64_t)gi * g.ldp + gj;
+                            old = *reinterpret_cast<const f16x4*>(at);
+                            if (precise) old_low = *reinterpret_cast<const f16x4*>(at + g.p_low);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float x = acc[i][j][4 * qd + e] * scale;
+                            if constexpr (KIND == kPoly)
+                                x += g.b * ((float)old[e] + (float)old_low[e]) + (gi == gj + e ? g.a * kHeld : 0.f);
+                            v[e] = (_Float16)x;
+                            if (part) v[e] = (_Float16)(x - (float)v[e]);
+                        }
+                        *reinterpret_cast<f16x4*>(tile_s + r * Cfg::PITCH + c) = v;
+                    }
+                }
+            __syncthreads();
+            _Float16* out = g.out + t.batch * g.out_size + (part ? g.out_low : 0);
+            for (int k = threadIdx.x; k < Cfg::TM * Cfg::TN / 8; k += Cfg::THREADS) {
+                const int r = k / (Cfg::TN / 8), c = k % (Cfg::TN / 8) * 8;
+                *reinterpret_cast<f16x8*>(out + (int64_t)(t.ti * Cfg::TM + r) * g.ldo + t.tj * Cfg::TN + c) =
+                    *reinterpret_cast<const f16x8*>(tile_s + r * Cfg::PITCH + c);
+            }
+            if (kSym && t.ti != t.tj) {
+                for (int k = threadIdx.x; k < Cfg::TM * Cfg::TN / 8; k += Cfg::THREADS) {
+                    const int r = k / (Cfg::TM / 8), c = k % (Cfg::TM / 8) * 8;     // row r, columns c on of the transpose
+                    f16x8 v;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = tile_s[(c + e) * Cfg::PITCH + r];
+                    *reinterpret_cast<f16x8*>(out + (int64_t)(t.tj * Cfg::TN + r) * g.ldo + t.ti * Cfg::TM + c) = v;
+                }
+            }
+            if (precise) __syncthreads();
+        }
+    }
+}
+
+// where a sharer's sums of its first (0) or second tile lie: 16 bytes a lane, block after block of its wave
+template <class Cfg>
+__device__ __forceinline__ float* ns_part(const NsGemm& g, int sharer, int second)
+{
+    return g.part + ((int64_t)(2 * sharer + second) * Cfg::WAVES + ((int)threadIdx.x >> 6)) * (Cfg::IM * Cfg::JN * 1024) +
+           ((int)threadIdx.x & 63) * 4;
 }
 
 template <class Cfg, int KIND>
@@ -186,67 +377,32 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
 {
     __shared__ __attribute__((aligned(16))) char s_mem[Cfg::LDS];
     constexpr bool kSym = KIND == kGram || KIND == kPoly;
-    constexpr int kWaves = Cfg::WGM * Cfg::WGN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave / Cfg::WGN, wn = wave % Cfg::WGN;
-
-    // the tile: of a symmetric product only those with tj <= ti
-    const int per = kSym ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
-    const int batch = (int)blockIdx.x / per, tile = (int)blockIdx.x % per;
-    int ti, tj;
-    if constexpr (kSym) {
-        ti = (int)((sqrtf(8.f * (float)tile + 1.f) - 1.f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
-        while (ti * (ti + 1) / 2 > tile) ti--;
-        tj = tile - ti * (ti + 1) / 2;
-    } else {
-        ti = tile % g.tiles_m;
-        tj = tile / g.tiles_m;
-    }
-
-    const _Float16* p = g.p + batch * g.p_size + (int64_t)ti * Cfg::TM * g.ldp;
-    const _Float16* q = g.q + batch * g.q_size + (kSym ? (int64_t)tj * Cfg::TN * g.ldq : (int64_t)tj * Cfg::TN);
-    const i32x4 rp = ns_rsrc(p, (uint32_t)(Cfg::TM * (int64_t)g.ldp * 2));
-    // (rows of Q: the tile's, or all K up to the tile's last column)
-    const i32x4 rq = ns_rsrc(q, kSym ? (uint32_t)(Cfg::TN * (int64_t)g.ldq * 2)
-                                     : (uint32_t)(((int64_t)(g.k_steps * kStepK - 1) * g.ldq + Cfg::TN) * 2));
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem;
 
-    // Loads.  An [R, 64] tile with K along the row: rows of 128 bytes, the 16-byte chunk c of row r at c ^ (r & 7), so
-    // that eight lanes reading one chunk of eight rows meet all banks.  A [64, TN] tile with K down the rows: chunk c of
-    // row k at c ^ 2 (k & 3), so that the four rows a transposing read takes lie in different bank groups.
-    auto load_rows = [&](i32x4 rsrc, uint32_t lds, int rows, int ld, int k0) {
-        for (int s = 0; s < rows / 8 / kWaves; s++) {
-            const int slot = s * kWaves + wave;                     // 1 KiB: 8 rows
-            const int r = slot * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
-            load_to_lds(rsrc, lds + slot * 1024, (uint32_t)(r * ld + c * 8) * 2u, (uint32_t)k0 * 2u);
-        }
-    };
-    auto load_cols = [&](i32x4 rsrc, uint32_t lds, int ld, int k0) {
-        constexpr int kChunks = Cfg::TN / 8;                        // of a row
-        for (int s = 0; s < Cfg::Q_BYTES / 1024 / kWaves; s++) {
-            const int at = (s * kWaves + wave) * 64 + lane;
-            const int k = at / kChunks, c = (at % kChunks) ^ (2 * (k & 3));
-            load_to_lds(rsrc, lds + (s * kWaves + wave) * 1024, (uint32_t)(k * ld + c * 8) * 2u, (uint32_t)k0 * (uint32_t)ld * 2u);
-        }
-    };
-    auto load = [&](int step) {
-        const uint32_t at = lds0 + (step & 1) * Cfg::STAGE;
-        load_rows(rp, at, Cfg::TM, g.ldp, step * kStepK);
-        if constexpr (kSym)
-            load_rows(rq, at + Cfg::P_BYTES, Cfg::TN, g.ldq, step * kStepK);
-        else
-            load_cols(rq, at + Cfg::P_BYTES, g.ldq, step * kStepK);
-    };
+    // Workgroups go round the XCDs in turn: each XCD takes a contiguous part of every 256.
+    int id = (int)blockIdx.x;
+    {
+        const int group = id / kNsCus * kNsCus, here = min(kNsCus, (int)gridDim.x - group);
+        if (here == kNsCus) id = group + (id - group) % kNsXcds * (kNsCus / kNsXcds) + (id - group) / kNsXcds;
+    }
+    const int k_total = g.k_steps * g.passes;
+    // this workgroup's steps: of one tile, or its share of the others' (at most two tiles)
+    int64_t from, to;
+    const bool shares = id >= g.whole;
+    if (!shares) {
+        from = (int64_t)id * k_total;
+        to = from + k_total;
+    } else {
+        const int64_t all = (int64_t)(g.tiles - g.whole) * k_total, w = id - g.whole;
+        from = (int64_t)g.whole * k_total + all * w / g.sharers;
+        to = (int64_t)g.whole * k_total + all * (w + 1) / g.sharers;
+    }
 
-    f32x16 acc[Cfg::IM][Cfg::JN];
-#pragma unroll
-    for (int i = 0; i < Cfg::IM; i++)
-#pragma unroll
-        for (int j = 0; j < Cfg::JN; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
-
+    // Fragment addresses.  An [R, 64] tile with K along the row: rows of 128 bytes, the 16-byte chunk c of row r at
+    // c ^ (r & 7), so that eight lanes reading one chunk of eight rows meet all banks.  A [64, TN] tile with K down the
+    // rows: chunk c of row k at c ^ 2 (k & 3), so that the four rows a transposing read takes lie in different banks.
     auto row_frag = [&](const char* t, int r0, int slice) -> f16x8 {
         const int r = r0 + (lane & 31), c = (2 * slice + (lane >> 5)) ^ (r & 7);
         return *reinterpret_cast<const f16x8*>(t + r * 128 + c * 16);
@@ -265,169 +421,290 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
         return __builtin_bit_cast(f16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
-    load(0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    for (int step = 0; step < g.k_steps; step++) {
-        if (step + 1 < g.k_steps) load(step + 1);
-        const char* tp = s_mem + (step & 1) * Cfg::STAGE;
-        const char* tq = tp + Cfg::P_BYTES;
+    for (int second = 0; from < to; second++) {
+        // (the division leaves its uniform result in vector registers)
+        const int tile = (int)uniform_u32((uint32_t)(from / k_total));
+        const int k_from = (int)uniform_u32((uint32_t)(from - (int64_t)tile * k_total));
+        const int k_to = (int)uniform_u32((uint32_t)min((int64_t)k_total, to - (int64_t)tile * k_total));
+        from += k_to - k_from;
+        const NsTile t = ns_tile<kSym>(g, tile);
+        const _Float16* p = g.p + t.batch * g.p_size + (int64_t)t.ti * Cfg::TM * g.ldp;
+        const _Float16* q = g.q + t.batch * g.q_size + (kSym ? (int64_t)t.tj * Cfg::TN * g.ldq : (int64_t)t.tj * Cfg::TN);
+        // (rows of Q: the tile's, or all K up to the tile's last column)
+        const int64_t p_room = Cfg::TM * (int64_t)g.ldp;
+        const int64_t q_room = kSym ? Cfg::TN * (int64_t)g.ldq : (int64_t)(g.k_steps * kStepK - 1) * g.ldq + Cfg::TN;
+        const bool low = g.passes > 1;
+        const i32x4 rp = ns_rsrc(p, (uint32_t)((p_room + (low ? g.p_low : 0)) * 2));
+        const i32x4 rq = ns_rsrc(q, (uint32_t)((q_room + (low ? g.q_low : 0)) * 2));
+        auto load = [&](int step, int stage) {
+            const uint32_t at = lds0 + stage * Cfg::STAGE;
+            const int pass = step < g.k_steps ? 0 : step < 2 * g.k_steps ? 1 : 2;       // high high, high low, low high
+            const uint32_t k0 = (uint32_t)(step - pass * g.k_steps) * kStepK;
+            const uint32_t p_off = (k0 + (pass == 2 ? (uint32_t)g.p_low : 0u)) * 2u;
+            const uint32_t q_off = ((kSym ? k0 : k0 * (uint32_t)g.ldq) + (pass == 1 ? (uint32_t)g.q_low : 0u)) * 2u;
+            auto rows = [&](i32x4 rsrc, uint32_t lds, int bytes, int ld, uint32_t off) {
+                for (int s = 0; s < bytes / 1024 / Cfg::WAVES; s++) {
+                    const int slot = s * Cfg::WAVES + wave;                             // 1 KiB: 8 rows
+                    const int r = slot * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
+                    load_to_lds(rsrc, lds + slot * 1024, (uint32_t)(r * ld + c * 8) * 2u, uniform_u32(off));
+                }
+            };
+            rows(rp, at, Cfg::P_BYTES, g.ldp, p_off);
+            if constexpr (kSym) {
+                rows(rq, at + Cfg::P_BYTES, Cfg::Q_BYTES, g.ldq, q_off);
+            } else {
+                constexpr int kChunks = Cfg::TN / 8;                                    // of a row
+                for (int s = 0; s < Cfg::Q_BYTES / 1024 / Cfg::WAVES; s++) {
+                    const int slot = s * Cfg::WAVES + wave, n = slot * 64 + lane;
+                    const int k = n / kChunks, c = (n % kChunks) ^ (2 * (k & 3));
+                    load_to_lds(rq, at + Cfg::P_BYTES + slot * 1024, (uint32_t)(k * g.ldq + c * 8) * 2u, uniform_u32(q_off));
+                }
+            }
+        };
+
+        f32x16 acc[Cfg::IM][Cfg::JN];
 #pragma unroll
-        for (int s = 0; s < kStepK / 16; s++) {
-            f16x8 fp[Cfg::IM], fq[Cfg::JN];
-#pragma unroll
-            for (int i = 0; i < Cfg::IM; i++) fp[i] = row_frag(tp, wm * 32 * Cfg::IM + 32 * i, s);
+        for (int i = 0; i < Cfg::IM; i++)
 #pragma unroll
             for (int j = 0; j < Cfg::JN; j++)
-                fq[j] = kSym ? row_frag(tq, wn * 32 * Cfg::JN + 32 * j, s) : col_frag(tq, wn * 32 * Cfg::JN + 32 * j, s);
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+
+        constexpr int kAhead = Cfg::STAGES - 1;
+        if (second) __builtin_amdgcn_s_barrier();       // (the first tile's last reads, see below)
+#pragma unroll
+        for (int s = 0; s < kAhead; s++)
+            if (k_from + s < k_to) load(k_from + s, s);
+        int stage = 0;
+        for (int step = k_from; step < k_to; step++) {
+            // this step's tiles are there and the stage that is loaded next has been read, in every wave
+            if (step + kAhead <= k_to)
+                wait_loads<(kAhead - 1) * Cfg::LOADS>();
+            else
+                wait_loads<0>();
+            __builtin_amdgcn_s_barrier();
+            if (step + kAhead < k_to) load(step + kAhead, stage == 0 ? kAhead : stage - 1);
+            const char* tp = s_mem + stage * Cfg::STAGE;
+            const char* tq = tp + Cfg::P_BYTES;
+            stage = stage == kAhead ? 0 : stage + 1;
+#pragma unroll
+            for (int s = 0; s < kStepK / 16; s++) {
+                f16x8 fp[Cfg::IM], fq[Cfg::JN];
+#pragma unroll
+                for (int i = 0; i < Cfg::IM; i++) fp[i] = row_frag(tp, wm * 32 * Cfg::IM + 32 * i, s);
+#pragma unroll
+                for (int j = 0; j < Cfg::JN; j++)
+                    fq[j] = kSym ? row_frag(tq, wn * 32 * Cfg::JN + 32 * j, s) : col_frag(tq, wn * 32 * Cfg::JN + 32 * j, s);
+#pragma unroll
+                for (int i = 0; i < Cfg::IM; i++)
+#pragma unroll
+                    for (int j = 0; j < Cfg::JN; j++)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[j], fp[i], acc[i][j], 0, 0, 0);
+            }
+        }
+        if (shares) {
+            float* part = ns_part<Cfg>(g, id - g.whole, second);
 #pragma unroll
             for (int i = 0; i < Cfg::IM; i++)
 #pragma unroll
-                for (int j = 0; j < Cfg::JN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[j], fp[i], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < Cfg::JN; j++)
+#pragma unroll
+                    for (int qd = 0; qd < 4; qd++)
+                        *reinterpret_cast<f32x4*>(part + ((i * Cfg::JN + j) * 4 + qd) * 256) =
+                            f32x4{acc[i][j][4 * qd], acc[i][j][4 * qd + 1], acc[i][j][4 * qd + 2], acc[i][j][4 * qd + 3]};
+            wait_loads<0>();        // (this wave's reads of LDS are done before the barrier at the next tile)
+        } else {
+            wait_loads<0>();
+            __builtin_amdgcn_s_barrier();
+            ns_finish<Cfg, KIND>(g, mats, t, acc, s_mem);
         }
-        // this step's reads are done and the next step's tiles are there, in every wave
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
     }
+}
 
-    // Results: lane holds row i = lane % 32 of a block, columns 8 q + 4 (lane / 32) + e in register 4 q + e.  Through LDS
-    // as a row-major tile (the main loop's last barrier has passed).
-    _Float16* tile_s = reinterpret_cast<_Float16*>(s_mem);
-    const float scale = KIND == kLast ? 1.f / kHeld : KIND == kPoly ? g.c / kHeld : 1.f / kHeld;
+// The shared tiles: their sharers' sums added in order, then as a tile with a workgroup of its own.
+template <class Cfg, int KIND>
+__global__ __launch_bounds__(Cfg::THREADS) void ns_join_kernel(NsGemm g, NsMatrices mats)
+{
+    __shared__ __attribute__((aligned(16))) char s_mem[Cfg::TM * Cfg::PITCH * 2];
+    constexpr bool kSym = KIND == kGram || KIND == kPoly;
+    const int64_t k_total = (int64_t)g.k_steps * g.passes, all = (g.tiles - g.whole) * k_total;
+    const int64_t from = (int64_t)blockIdx.x * k_total, to = from + k_total;      // of the shared steps
+    // the sharer of step s is the last w with all w / sharers <= s
+    auto sharer = [&](int64_t s) { return (int)(((s + 1) * g.sharers - 1) / all); };
+    f32x16 acc[Cfg::IM][Cfg::JN];
 #pragma unroll
     for (int i = 0; i < Cfg::IM; i++)
 #pragma unroll
-        for (int j = 0; j < Cfg::JN; j++) {
-            const int r = (wm * Cfg::IM + i) * 32 + (lane & 31);
+        for (int j = 0; j < Cfg::JN; j++)
 #pragma unroll
-            for (int qd = 0; qd < 4; qd++) {
-                const int c = (wn * Cfg::JN + j) * 32 + 8 * qd + 4 * (lane >> 5);
-                f16x4 v;
-                f16x4 old = {};
-                const int gi = ti * Cfg::TM + r, gj = tj * Cfg::TN + c;
-                if constexpr (KIND == kPoly)        // p is A
-                    old = *reinterpret_cast<const f16x4*>(g.p + batch * g.p_size + (int64_t)gi * g.ldp + gj);
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+    for (int w = sharer(from); w <= sharer(to - 1); w++) {
+        const int second = all * w / g.sharers < from;          // it began with the tile before
+        const float* part = ns_part<Cfg>(g, w, second);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float x = acc[i][j][4 * qd + e] * scale;
-                    if constexpr (KIND == kPoly) x += g.b * (float)old[e] + (gi == gj + e ? g.a * kHeld : 0.f);
-                    v[e] = (_Float16)x;
+        for (int i = 0; i < Cfg::IM; i++)
+#pragma unroll
+            for (int j = 0; j < Cfg::JN; j++)
+#pragma unroll
+                for (int qd = 0; qd < 4; qd++) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(part + ((i * Cfg::JN + j) * 4 + qd) * 256);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][4 * qd + e] += v[e];
                 }
-                *reinterpret_cast<f16x4*>(tile_s + r * Cfg::PITCH + c) = v;
-            }
-        }
-    __syncthreads();
-
-    if constexpr (KIND != kLast) {
-        _Float16* out = g.out + batch * g.out_size;
-        for (int t = threadIdx.x; t < Cfg::TM * Cfg::TN / 8; t += Cfg::THREADS) {
-            const int r = t / (Cfg::TN / 8), c = t % (Cfg::TN / 8) * 8;
-            *reinterpret_cast<f16x8*>(out + (int64_t)(ti * Cfg::TM + r) * g.ldo + tj * Cfg::TN + c) =
-                *reinterpret_cast<const f16x8*>(tile_s + r * Cfg::PITCH + c);
-        }
-        if (kSym && ti != tj) {
-            for (int t = threadIdx.x; t < Cfg::TM * Cfg::TN / 8; t += Cfg::THREADS) {
-                const int r = t / (Cfg::TM / 8), c = t % (Cfg::TM / 8) * 8;     // row r, columns c on of the transpose
-                f16x8 v;
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = tile_s[(c + e) * Cfg::PITCH + r];
-                *reinterpret_cast<f16x8*>(out + (int64_t)(tj * Cfg::TN + r) * g.ldo + ti * Cfg::TM + c) = v;
-            }
-        }
-    } else {
-        const NsMatrix mat = mats.at[batch];
-        const int64_t rows = mat.tall ? g.n : g.m, cols = mat.tall ? g.m : g.n;
-        const int64_t r0 = mat.tall ? (int64_t)tj * Cfg::TN : (int64_t)ti * Cfg::TM;
-        const int64_t c0 = mat.tall ? (int64_t)ti * Cfg::TM : (int64_t)tj * Cfg::TN;
-        const int width = mat.tall ? Cfg::TM : Cfg::TN;
-        for (int t = threadIdx.x; t < Cfg::TM * Cfg::TN; t += Cfg::THREADS) {
-            const int r = t / width, c = t % width;
-            if (r0 + r >= rows || c0 + c >= cols) continue;
-            const float o = (float)(mat.tall ? tile_s[c * Cfg::PITCH + r] : tile_s[r * Cfg::PITCH + c]) * (1.f / kHeld);
-            const int64_t at = (r0 + r) * mat.w_stride + c0 + c;
-            ns_store(mat.w, g.w_f32, at, g.update ? g.keep * ns_load(mat.w, g.w_f32, at) - g.rate * o : o);
-        }
     }
+    ns_finish<Cfg, KIND>(g, mats, ns_tile<kSym>(g, g.whole + (int)blockIdx.x), acc, s_mem);
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+// One product of all matrices on tiles of one size: how many of them get a
+// workgroup of their own, and its time in microseconds as the choice sees it.
+struct NsProduct {
+    int tile;
+    int64_t tiles, whole, sharers;
+    double time;
+};
 struct NsPlan {
-    int tile;                   // 256, 128 or 64
+    NsProduct gram, poly, step;
     int64_t mp, np;
-    int64_t x_bytes, a_bytes, parts_bytes, total;   // of `count` matrices
+    int64_t x_bytes, a_bytes, parts_bytes, share_bytes, total;
 };
 
-// The largest tile whose products still give every CU work, and of those whose
-// padding does not undo the gain.
-static NsPlan ns_plan(int64_t m, int64_t n, int64_t count)
+// Time of a K step of one workgroup when every CU has its fill of them, and
+// how many a CU holds.
+struct NsTileRate {
+    int tile, per_cu;
+    double step;
+};
+constexpr NsTileRate kNsRates[] = {{256, 1, 1.75}, {128, 2, 1.15}, {64, 2, 0.45}};
+
+static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, bool sym, int64_t k, int64_t count, int passes)
 {
-    NsPlan p{};
-    auto up = [](int64_t v, int64_t t) { return (v + t - 1) / t * t; };
-    double best = 0;
-    for (const int t : {256, 128, 64}) {
-        const int64_t mp = up(m, t), np = up(n, t), tm = mp / t, tn = np / t;
-        // time of the three products in tile steps over the CUs: a tile step of 256, 128, 64 takes about 1, 0.34, 0.13
-        const double cost = t == 256 ? 1.0 : t == 128 ? 0.34 : 0.13;
-        const int64_t slots = t == 256 ? 256 : t == 128 ? 512 : 1024;
-        auto rounds = [&](int64_t tiles) { return (double)((tiles * count + slots - 1) / slots) * (double)slots / 256.0; };
-        const double time = cost * (rounds(tm * (tm + 1) / 2) * (double)(np + mp) + rounds(tm * tn) * (double)mp);
-        if (p.tile == 0 || time < best) p.tile = t, p.mp = mp, p.np = np, best = time;
+    NsProduct p{};
+    const int64_t tm = rows / r.tile, tn = cols / r.tile, steps = k / kStepK * passes, slots = (int64_t)kNsCus * r.per_cu;
+    p.tile = r.tile;
+    p.tiles = (sym ? tm * (tm + 1) / 2 : tm * tn) * count;
+    p.whole = p.tiles;
+    const int64_t rounds = (p.tiles + slots - 1) / slots, rest = p.tiles % slots;
+    p.time = 3.0 + r.step * (double)(rounds * steps);
+    // A last round that does not fill the chip is dealt out in shares of its steps instead, where the steps saved are
+    // worth the sums' way through memory (written and read once at about 4 TB/s) and one more kernel.
+    if (sym && rest > 0) {
+        const int64_t sharers = std::min(slots, rest * steps);
+        const double bytes = 8.0 * r.tile * r.tile * (double)(sharers + rest);
+        const double shared = 3.0 + r.step * (double)((rounds - 1) * steps + (rest * steps + sharers - 1) / sharers) + 5.0 + bytes / 4e6;
+        if (shared < p.time) p.whole = p.tiles - rest, p.sharers = sharers, p.time = shared;
     }
-    p.x_bytes = p.mp * p.np * 2 * count;
-    p.a_bytes = p.mp * p.mp * 2 * count;
+    return p;
+}
+
+// The tile of each product that its estimate is shortest on.  Padding: whole
+// tiles of the largest size used.
+static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
+{
+    NsPlan best{};
+    auto up = [](int64_t v, int64_t t) { return (v + t - 1) / t * t; };
+    const int passes = precise ? 3 : 1;
+    double best_time = 0;
+    for (const NsTileRate& most : kNsRates) {
+        NsPlan p{};
+        p.mp = up(m, most.tile), p.np = up(n, most.tile);
+        auto pick = [&](int64_t rows, int64_t cols, bool sym, int64_t k) {
+            NsProduct b{};
+            for (const NsTileRate& r : kNsRates) {
+                if (r.tile > most.tile) continue;
+                const NsProduct q = ns_product(r, rows, cols, sym, k, count, passes);
+                if (b.tile == 0 || q.time < b.time) b = q;
+            }
+            return b;
+        };
+        p.gram = pick(p.mp, p.mp, true, p.np);
+        p.poly = pick(p.mp, p.mp, true, p.mp);
+        p.step = pick(p.mp, p.np, false, p.mp);
+        const double time = p.gram.time + p.poly.time + p.step.time;
+        if (best.mp == 0 || time < best_time) best = p, best_time = time;
+    }
+    NsPlan& p = best;
+    p.x_bytes = p.mp * p.np * 2 * count * (precise ? 2 : 1);
+    p.a_bytes = p.mp * p.mp * 2 * count * (precise ? 2 : 1);
     p.parts_bytes = (kNsParts * 8 * count + 255) / 256 * 256;
-    p.total = 2 * p.x_bytes + 2 * p.a_bytes + p.parts_bytes;
+    for (const NsProduct& q : {p.gram, p.poly}) p.share_bytes = std::max(p.share_bytes, q.sharers * 2 * q.tile * q.tile * 4);
+    p.total = 2 * p.x_bytes + 2 * p.a_bytes + p.parts_bytes + p.share_bytes;
     return p;
 }
 
 template <class Cfg, int KIND>
-static hipError_t ns_launch(const NsGemm& g, const NsMatrices& mats, hipStream_t st)
+static void ns_launch(NsGemm g, const NsProduct& p, const NsMatrices& mats, hipStream_t st)
 {
-    const int per = KIND == kGram || KIND == kPoly ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_gemm_kernel<Cfg, KIND>), dim3((uint32_t)(per * g.count)), dim3(Cfg::THREADS), 0, st, g, mats);
-    return hipGetLastError();
+    g.tiles = (int)p.tiles, g.whole = (int)p.whole, g.sharers = (int)p.sharers;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_gemm_kernel<Cfg, KIND>), dim3((uint32_t)(p.whole + p.sharers)), dim3(Cfg::THREADS), 0, st, g, mats);
+    if constexpr (KIND == kGram || KIND == kPoly)
+        if (p.sharers)
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_join_kernel<Cfg, KIND>), dim3((uint32_t)(p.tiles - p.whole)), dim3(Cfg::THREADS), 0, st, g, mats);
+}
+
+template <int KIND>
+static void ns_launch(NsGemm g, const NsPlan& plan, const NsProduct& p, const NsMatrices& mats, hipStream_t st)
+{
+    g.tiles_m = (int)(plan.mp / p.tile);
+    g.tiles_n = (int)((KIND == kGram || KIND == kPoly ? plan.mp : plan.np) / p.tile);
+    if (p.tile == 256)
+        ns_launch<NsLarge, KIND>(g, p, mats, st);
+    else if (p.tile == 128)
+        ns_launch<NsMiddle, KIND>(g, p, mats, st);
+    else
+        ns_launch<NsSmall, KIND>(g, p, mats, st);
 }
 
 struct NsWork {
     _Float16 *x[2], *a, *b;
 };
 
-template <class Cfg>
-static hipError_t ns_products(const NsPlan& p, const NsWork& w, NsGemm g, const NsMatrices& mats, int steps, hipStream_t st)
+static void ns_products(const NsPlan& p, const NsWork& w, NsGemm g, const NsMatrices& mats, int64_t count, int steps, hipStream_t st)
 {
-    g.tiles_m = (int)(p.mp / Cfg::TM);
-    g.tiles_n = (int)(p.np / Cfg::TN);
-    hipError_t e = hipSuccess;
-    for (int k = 0; k < steps && e == hipSuccess; k++) {
+    const int64_t x_size = p.mp * p.np, a_size = p.mp * p.mp;
+    for (int k = 0; k < steps; k++) {
         _Float16 *x = w.x[k & 1], *y = w.x[(k + 1) & 1];
         NsGemm gram = g;
-        gram.p = gram.q = x, gram.p_size = gram.q_size = p.mp * p.np, gram.ldp = gram.ldq = (int)p.np;
-        gram.out = w.a, gram.out_size = p.mp * p.mp, gram.ldo = (int)p.mp, gram.k_steps = (int)(p.np / kStepK);
-        e = ns_launch<Cfg, kGram>(gram, mats, st);
-        if (e != hipSuccess) break;
+        gram.p = gram.q = x, gram.p_size = gram.q_size = x_size, gram.p_low = gram.q_low = x_size * count;
+        gram.ldp = gram.ldq = (int)p.np, gram.k_steps = (int)(p.np / kStepK);
+        gram.out = w.a, gram.out_size = a_size, gram.out_low = a_size * count, gram.ldo = (int)p.mp;
+        ns_launch<kGram>(gram, p, p.gram, mats, st);
         NsGemm poly = gram;
-        poly.p = poly.q = w.a, poly.p_size = poly.q_size = p.mp * p.mp, poly.ldp = poly.ldq = (int)p.mp;
-        poly.out = w.b, poly.k_steps = (int)(p.mp / kStepK);
-        e = ns_launch<Cfg, kPoly>(poly, mats, st);
-        if (e != hipSuccess) break;
+        poly.p = poly.q = w.a, poly.p_size = poly.q_size = a_size, poly.p_low = poly.q_low = a_size * count;
+        poly.ldp = poly.ldq = (int)p.mp, poly.k_steps = (int)(p.mp / kStepK);
+        poly.out = w.b;
+        ns_launch<kPoly>(poly, p, p.poly, mats, st);
         NsGemm step = poly;
-        step.p = w.b, step.q = x, step.q_size = p.mp * p.np, step.ldq = (int)p.np;
-        step.out = y, step.out_size = p.mp * p.np, step.ldo = (int)p.np;
-        e = k + 1 < steps ? ns_launch<Cfg, kStep>(step, mats, st) : ns_launch<Cfg, kLast>(step, mats, st);
+        step.p = w.b, step.q = x, step.q_size = x_size, step.q_low = x_size * count, step.ldq = (int)p.np;
+        step.out = y, step.out_size = x_size, step.out_low = x_size * count, step.ldo = (int)p.np;
+        if (k + 1 < steps)
+            ns_launch<kStep>(step, p, p.step, mats, st);
+        else
+            ns_launch<kLast>(step, p, p.step, mats, st);
     }
-    return e;
+}
+
+// Matrices that go through the products together: as many as keep every
+// offset inside a buffer under 2^32 bytes.
+static int64_t ns_together(int64_t m, int64_t n, int64_t count, bool precise)
+{
+    int64_t most = std::min<int64_t>(count, kNsBatch);
+    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    while (most > 1 && precise && (most + 1) * up(m) * up(n) * 2 >= (int64_t(1) << 32)) most--;
+    return most;
 }
 
 }  // namespace bs
 
 using namespace bs;
 
-extern "C" int64_t bs_newton_schulz_workspace_bytes(int64_t rows, int64_t cols, int64_t count)
+extern "C" int64_t bs_newton_schulz_workspace_bytes(int64_t rows, int64_t cols, int64_t count, int precise)
 {
     if (rows <= 0 || cols <= 0 || count <= 0 || rows > 65536 || cols > 65536) return 0;
-    return ns_plan(std::min(rows, cols), std::max(rows, cols), std::min<int64_t>(count, kNsBatch)).total;
+    const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+    return ns_plan(m, n, ns_together(m, n, count, precise != 0), precise != 0).total;
 }
 
 extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_t rows, int64_t cols,
@@ -439,7 +716,7 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         return set_error(BS_ERR_INVALID, "%s: null arguments or a negative count", what);
     const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
     if (m <= 0 || n > 65536) return set_error(BS_ERR_INVALID, "%s: matrices of 1..65536 rows and columns, got %lld x %lld", what, (long long)rows, (long long)cols);
-    if (m * n >= (int64_t(1) << 30)) return set_error(BS_ERR_INVALID, "%s: rows*cols must be < 2^30", what);
+    if (m * n >= (int64_t(1) << 29)) return set_error(BS_ERR_INVALID, "%s: rows*cols must be < 2^29", what);
     const bs_newton_schulz_rule& r = *rule;
     if (r.steps < 1 || r.steps > 100) return set_error(BS_ERR_INVALID, "%s: steps must be in 1..100, got %d", what, r.steps);
     auto known = [](int t) { return t == BS_DT_BF16 || t == BS_DT_F32; };
@@ -458,12 +735,22 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
             return set_error(BS_ERR_INVALID, "%s: rows of a matrix that is written overlap", what);
     }
     if (count == 0) return BS_OK;
-    if (workspace == nullptr || ((uintptr_t)workspace & 255u) || workspace_bytes < bs_newton_schulz_workspace_bytes(rows, cols, count))
+    const bool precise = r.precise != 0;
+    if (workspace == nullptr || ((uintptr_t)workspace & 255u) || workspace_bytes < bs_newton_schulz_workspace_bytes(rows, cols, count, precise))
         return set_error(BS_ERR_INVALID, "%s: workspace too small or misaligned", what);
     const hipStream_t st = (hipStream_t)stream;
-    for (int64_t first = 0; first < count; first += kNsBatch) {
-        const int64_t here = std::min<int64_t>(count - first, kNsBatch);
-        const NsPlan p = ns_plan(m, n, std::min<int64_t>(count, kNsBatch));
+    const int64_t together = ns_together(m, n, count, precise);
+    const NsPlan full = ns_plan(m, n, together, precise);
+    for (int64_t first = 0; first < count; first += together) {
+        const int64_t here = std::min<int64_t>(count - first, together);
+        // (a last group with fewer matrices: its plan may want more workspace than the full one's, so its tiles have workgroups of their own)
+        NsPlan p = full;
+        if (here < together) {
+            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = 0; };
+            fewer(p.gram);
+            fewer(p.poly);
+            fewer(p.step);
+        }
         NsMatrices mats{};
         for (int64_t i = 0; i < here; i++) {
             const bs_matrix& t = matrices[first + i];
@@ -474,26 +761,25 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         NsPrep a{};
         a.m = m, a.n = n, a.mp = p.mp, a.np = p.np;
         a.g_f32 = r.grad_type == BS_DT_F32, a.m_f32 = r.momentum_type == BS_DT_F32, a.momentum = r.momentum, a.nesterov = r.nesterov;
-        a.mu = r.mu, a.eps = r.eps;
-        a.parts = reinterpret_cast<double*>(ws);
+        a.mu = r.mu, a.eps = r.eps, a.precise = precise, a.low = p.mp * p.np * here;
+        // about 4096 elements or more to a workgroup, and no more of them than 8 a CU over all matrices
+        a.parts = (int)std::max<int64_t>(1, std::min({(int64_t)kNsParts, (m * n + 8191) / 8192, (8 * kNsCus + here - 1) / here}));
+        a.parts_at = reinterpret_cast<double*>(ws);
         NsWork w;
-        w.x[0] = reinterpret_cast<_Float16*>(ws + p.parts_bytes);
-        w.x[1] = reinterpret_cast<_Float16*>(ws + p.parts_bytes + p.x_bytes);
-        w.a = reinterpret_cast<_Float16*>(ws + p.parts_bytes + 2 * p.x_bytes);
-        w.b = reinterpret_cast<_Float16*>(ws + p.parts_bytes + 2 * p.x_bytes + p.a_bytes);
+        char* at = ws + p.parts_bytes;
+        w.x[0] = reinterpret_cast<_Float16*>(at);
+        w.x[1] = reinterpret_cast<_Float16*>(at + p.x_bytes);
+        w.a = reinterpret_cast<_Float16*>(at + 2 * p.x_bytes);
+        w.b = reinterpret_cast<_Float16*>(at + 2 * p.x_bytes + p.a_bytes);
         a.x = w.x[0];
-        const int parts = (int)std::min<int64_t>(kNsParts, (m * n + 4095) / 4096);
-        hipLaunchKernelGGL(ns_norm_kernel, dim3(parts, (uint32_t)here), dim3(256), 0, st, a, mats);
-        hipLaunchKernelGGL(ns_scale_kernel, dim3((uint32_t)(p.np / 64), (uint32_t)(p.mp / 64), (uint32_t)here), dim3(256), 0, st, a, mats, parts);
-        hipError_t e = hipGetLastError();
-        if (e == hipSuccess) {
-            NsGemm g{};
-            g.count = (int)here, g.a = r.a, g.b = r.b, g.c = r.c;
-            g.m = m, g.n = n, g.w_f32 = r.out_type == BS_DT_F32, g.update = r.update, g.keep = r.keep, g.rate = r.rate;
-            e = p.tile == 256 ? ns_products<NsLarge>(p, w, g, mats, r.steps, st)
-                : p.tile == 128 ? ns_products<NsMiddle>(p, w, g, mats, r.steps, st)
-                                : ns_products<NsSmall>(p, w, g, mats, r.steps, st);
-        }
+        hipLaunchKernelGGL(ns_norm_kernel, dim3(a.parts, (uint32_t)here), dim3(256), 0, st, a, mats);
+        hipLaunchKernelGGL(ns_scale_kernel, dim3((uint32_t)(p.np / 64), (uint32_t)(p.mp / 64), (uint32_t)here), dim3(256), 0, st, a, mats);
+        NsGemm g{};
+        g.passes = precise ? 3 : 1, g.a = r.a, g.b = r.b, g.c = r.c;
+        g.part = reinterpret_cast<float*>(at + 2 * p.x_bytes + 2 * p.a_bytes);
+        g.m = m, g.n = n, g.w_f32 = r.out_type == BS_DT_F32, g.update = r.update, g.keep = r.keep, g.rate = r.rate;
+        ns_products(p, w, g, mats, here, r.steps, st);
+        const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
     }
     return BS_OK;

@@ -14,8 +14,10 @@ optimiser around it.
 Precision: products of fp16 operands summed in fp32.  For gradients of full
 rank the result is within 1-3e-3 (2-norm) of the exact iteration's, of which
 1.7e-3 is the rounding to bf16.  Where a gradient has directions of no
-gradient at all (fewer tokens than rows), the iteration raises rounding noise
-there to at most 5e-3 of a full singular value each.
+gradient at all (fewer tokens than rows), the iteration raises the operands'
+rounding noise there.  ``precise`` holds every operand as two fp16 numbers and
+multiplies three times: 2e-6 before the result's own rounding, at a third of
+the speed; updates of float32 weights do so unless told otherwise.
 """
 from __future__ import annotations
 
@@ -30,20 +32,22 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
 def orthogonalize(G: Tensor, *, steps: int = 5, coefficients: tuple[float, float, float] = COEFFICIENTS,
-                  eps: float = 1e-7) -> Tensor:
+                  eps: float = 1e-7, precise: bool = False) -> Tensor:
     """The orthogonalised matrices of G [..., R, C] (bfloat16 or float32, up to
-    65536 rows and columns and 2^30 elements each), in bfloat16, contiguous.
+    65536 rows and columns and fewer than 2^29 elements each), in bfloat16, contiguous.
 
-    No gradient flows through it (an optimiser's operator)."""
+    ``precise``: products of 22-bit operands (see above).  No gradient flows
+    through it (an optimiser's operator)."""
     a, b, c = coefficients
     with torch.no_grad():
-        return native().orthogonalize(G, steps, a, b, c, eps)
+        return native().orthogonalize(G, steps, a, b, c, eps, precise)
 
 
 def muon_update_(params: Sequence[Tensor], grads: Sequence[Tensor], momenta: Sequence[Tensor], *, lr: float,
                  momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  adjust: str | float = "shape", steps: int = 5,
-                 coefficients: tuple[float, float, float] = COEFFICIENTS, eps: float = 1e-7) -> None:
+                 coefficients: tuple[float, float, float] = COEFFICIENTS, eps: float = 1e-7,
+                 precise: bool | None = None) -> None:
     """For each matrix W [R, C] with its gradient G and momentum M, in place:
 
         M <- momentum M + (1 - momentum) G
@@ -52,6 +56,7 @@ def muon_update_(params: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seq
 
     s: sqrt(max(1, R / C)) (``adjust="shape"``), 0.2 sqrt(max(R, C))
     (``"rms"``: updates of the size that Adam's have) or the number given.
+    precise: products of 22-bit operands, by default for float32 weights.
     Each of the three lists is bfloat16 or float32; W and M have contiguous
     rows, their own memory, and are updated on the current stream."""
     if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0:
@@ -68,7 +73,7 @@ def muon_update_(params: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seq
     a, b, c = coefficients
     with torch.no_grad():
         native().muon_update(list(params), list(grads), list(momenta), lr, momentum, nesterov, weight_decay, by_rms,
-                             scale, steps, a, b, c, eps)
+                             scale, steps, a, b, c, eps, precise)
 
 
 class Muon(torch.optim.Optimizer):
@@ -82,12 +87,12 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  adjust: str | float = "shape", steps: int = 5, coefficients: tuple[float, float, float] = COEFFICIENTS,
-                 eps: float = 1e-7, momentum_dtype: torch.dtype = torch.float32):
+                 eps: float = 1e-7, momentum_dtype: torch.dtype = torch.float32, precise: bool | None = None):
         if momentum_dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"momentum_dtype must be float32 or bfloat16, got {momentum_dtype}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       adjust=adjust, steps=steps, coefficients=coefficients, eps=eps,
-                                      momentum_dtype=momentum_dtype))
+                                      momentum_dtype=momentum_dtype, precise=precise))
         for group in self.param_groups:
             for p in group["params"]:
                 if p.dim() != 2:
@@ -115,5 +120,5 @@ class Muon(torch.optim.Optimizer):
                     self.state[p]["momentum"] = torch.zeros(p.shape, dtype=group["momentum_dtype"], device=p.device)
             muon_update_(params, [p.grad for p in params], [self.state[p]["momentum"] for p in params],
                          **{k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "adjust", "steps",
-                                                  "coefficients", "eps")})
+                                                  "coefficients", "eps", "precise")})
         return loss

@@ -722,8 +722,8 @@ int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* work
  * G, M and out are bf16 or fp32, each type the same for all matrices, with
  * contiguous rows `*_stride` elements apart.  Products have fp16 operands and
  * fp32 sums: X comes to 1-3e-3 of the exact result for a gradient of full
- * rank (directions in which U is 0, and the result too, hold noise of up to
- * 5e-3 of a unit singular value each).
+ * rank.  With `precise` every operand is two fp16 numbers and a product three:
+ * 2e-6, at a third of the speed.
  */
 typedef struct bs_matrix {
     const void* grad;
@@ -735,10 +735,11 @@ typedef struct bs_matrix {
 typedef struct bs_newton_schulz_rule {
     int grad_type, momentum_type, out_type;     /* BS_DT_BF16 or BS_DT_F32 */
     int momentum, nesterov, update;             /* flags */
+    int precise;                     /* flag: operands of 22 bits */
     int steps;
     float a, b, c, eps, mu, keep, rate;
 } bs_newton_schulz_rule;
-int64_t bs_newton_schulz_workspace_bytes(int64_t rows, int64_t cols, int64_t count);
+int64_t bs_newton_schulz_workspace_bytes(int64_t rows, int64_t cols, int64_t count, int precise);
 int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_t rows, int64_t cols,
                      const bs_newton_schulz_rule* rule, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -278,3 +278,75 @@ def test_refusals():
     M.muon_update_([], [], [], lr=0.1)
     with pytest.raises(ValueError):
         M.Muon([torch.nn.Parameter(torch.zeros(3, device="cuda"))])
+
+
+# ---------------------------------------------------------------------------
+# operands of 22 bits
+# ---------------------------------------------------------------------------
+def _model22(U, steps=5):
+    """The iteration with the roundings of the precise form: each operand a sum of two fp16 numbers, products exact to
+    fp32's sums but for low x low"""
+    def h(t):
+        hi = (t * 4096.0).half().float()
+        return hi / 4096.0, (t * 4096.0 - hi).half().float() / 4096.0
+
+    def mul(p, q):
+        return p[0] @ q[0] + p[0] @ q[1] + p[1] @ q[0]
+    X = U.double()
+    X = h((X / (X.square().sum((-2, -1), keepdim=True).sqrt() + EPS)).float())
+    a, b, c = COEF
+    eye = torch.eye(U.shape[-2], device=U.device)
+    for _ in range(steps):
+        A = h(mul(X, tuple(x.mT.contiguous() for x in X)))
+        B = h(a * eye + b * (A[0] + A[1]) + c * mul(A, A))
+        Y = mul(B, X)
+        X = h(Y)
+    return Y
+
+
+@pytest.mark.parametrize("kind", ["normal", "low", "one", "decay"])
+@pytest.mark.parametrize("R,C", [(1, 3), (33, 100), (130, 260), (700, 500), (513, 2050)])
+def test_precise(kind, R, C):
+    """Into fp32 weights of 0: all that is left of them is the orthogonalised gradient.  The model's own sums are fp32 in
+    another order than the kernels', and what they lose (some 2^-24 of a sum's terms) is raised like the operands'
+    roundings: bar twice the model's distance, plus 2^-20."""
+    G = _grads(1, R, C, 12, kind)[0]
+    W, m = torch.zeros(R, C, device="cuda"), torch.zeros(R, C, device="cuda")
+    _mod().muon_update_([W], [G], [m], lr=1.0, momentum=0.0, adjust=1.0)
+    wide = G if R <= C else G.T.contiguous()
+    want = _exact(wide[None])
+    model = _err(_model22(wide[None]), want)
+    got = -(W if R <= C else W.T)
+    err = _err(got[None], want)
+    assert err <= 2 * model + 2.0 ** -20, (err, model)
+    # in bf16: nothing but the result's own rounding is left, half a unit
+    O = _mod().orthogonalize(wide, precise=True)
+    tol = 2.0 ** -8 * want[0].abs() + 2 * (2 * model + 2.0 ** -20) * want[0].norm()
+    assert ((O.double() - want[0]).abs() <= tol).all()
+
+
+def test_precise_or_not():
+    """fp32 weights are precise unless told otherwise, bf16 ones the other way round; either may choose."""
+    G, m = _grads(1, 200, 300, 13)[0], torch.zeros(200, 300, device="cuda")
+    want = _exact(G[None])
+    errs = {}
+    for dtype in (F32, BF):
+        for precise in (None, True, False):
+            W = torch.zeros(200, 300, device="cuda", dtype=dtype)
+            _mod().muon_update_([W], [G], [m.clone()], lr=1.0, momentum=0.0, adjust=1.0, precise=precise)
+            errs[dtype, precise] = _err(-W[None], want)
+    assert errs[F32, None] == errs[F32, True] < 1e-5 and 5e-4 < errs[F32, False] < 3e-3
+    assert errs[BF, None] == errs[BF, False] > errs[BF, True]
+
+
+@pytest.mark.parametrize("B,R,C", [(1, 2304, 4700), (3, 1000, 3100), (2, 1024, 4100), (65, 200, 70)])
+@pytest.mark.parametrize("precise", [False, True])
+def test_shared_tiles(B, R, C, precise):
+    """Counts of tiles that leave a last round to be dealt out in shares, several matrices of them; more matrices than
+    go together."""
+    G = _grads(B, R, C, 14).to(BF)
+    got = _mod().orthogonalize(G, precise=precise)
+    if precise:
+        assert _err(got, _exact(G)) < 2.0e-3
+    else:
+        _check(G, got)
