@@ -24,7 +24,11 @@
 // of fp32 operands come, at the matrix cores' fp16 rate.
 //
 // All buffers are padded with zeros to whole tiles, which the products keep
-// (B's padding only meets X's zero rows), so the main loop has no bounds.
+// (B's padding only meets X's zero rows), so the main loop has no bounds.  A
+// matrix [R, C] lies as C / 32 panels of R rows (and 32 more, see NsPlan): every tile that a product loads
+// for 32 steps of K is then one run of memory (P's and gram's) or runs of 2 KiB
+// (X's columns in step), where rows of 64 bytes out of a row-major matrix cost
+// half of each cache line.
 #include <algorithm>
 
 #include "bs_device.h"
@@ -42,7 +46,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kHeld = 4096.f;         // fp16 value = true value * kHeld
-constexpr int kStepK = 64;              // K of a main-loop step
+constexpr int kPanel = 32;              // columns of a panel; K of a main-loop step
 constexpr int kNsBatch = 64;            // matrices of a launch
 constexpr int kNsParts = 256;           // most partial sums of squares of a matrix
 constexpr int kNsCus = 256, kNsXcds = 8;
@@ -64,11 +68,11 @@ struct NsMatrices {
 // U, its norm and X_0
 // ---------------------------------------------------------------------------
 struct NsPrep {
-    int64_t m, n, mp, np;
+    int64_t m, n, pitch, np;
     int g_f32, m_f32, momentum, nesterov, parts, precise;
     float mu, eps;
     double* parts_at;                   // [count][kNsParts]
-    _Float16* x;                        // [count][mp][np], precise: and the low parts behind all of them
+    _Float16* x;                        // [count] matrices, precise: and the low parts behind all of them
     int64_t low;                        // elements from a value to its low part
 };
 
@@ -143,6 +147,12 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsPrep a, NsMatrices mats)
     if (threadIdx.x == 0) a.parts_at[(int64_t)blockIdx.y * kNsParts + blockIdx.x] = s_part[0];
 }
 
+// where element (r, c) of a matrix lies
+__device__ __forceinline__ int64_t panel_at(int64_t pitch, int64_t r, int64_t c)
+{
+    return ((c / kPanel) * pitch + r) * kPanel + c % kPanel;
+}
+
 __device__ __forceinline__ f16x8 ns_low(const float (&v)[8], f16x8 high)
 {
     f16x8 l;
@@ -190,7 +200,7 @@ __global__ __launch_bounds__(256) void ns_scale_kernel(NsPrep a, NsMatrices mats
             v[e] = (t.tall ? s_t[r][c + e] : u[k][e]) / norm * kHeld;
             h[e] = (_Float16)v[e];
         }
-        _Float16* out = a.x + ((int64_t)blockIdx.z * a.mp + i0 + r) * a.np + j0 + c;
+        _Float16* out = a.x + (int64_t)blockIdx.z * a.pitch * a.np + panel_at(a.pitch, i0 + r, j0 + c);
         *reinterpret_cast<f16x8*>(out) = h;
         if (a.precise) *reinterpret_cast<f16x8*>(out + a.low) = ns_low(v, h);
     }
@@ -204,13 +214,14 @@ struct NsGemm {
     const _Float16 *p, *q;              // [count] matrices
     int64_t p_size, q_size, out_size;   // elements of one matrix
     int64_t p_low, q_low, out_low;      // precise: elements from a value to its low part
-    int ldp, ldq, ldo;
+    int pitch;                          // rows from panel to panel
     int k_steps;                        // of one pass over K
     int passes;                         // 1, or 3 (precise)
     int tiles_m, tiles_n;               // of one matrix's product
     int tiles;                          // of all matrices, those left out by symmetry not counted
     int whole;                          // tiles with a workgroup of their own; the others' steps are
-    int sharers;                        // dealt out evenly to this many workgroups
+    int sharers;                        // dealt out evenly to this many workgroups,
+    int lanes;                          // a group of tiles to each of this many sets of them
     float* part;                        // [sharers][2][tile]: their sums
     _Float16* out;
     float a, b, c;                      // poly
@@ -226,30 +237,34 @@ struct NsCfg {
     static constexpr int WGM = WGM_, WGN = WGN_, IM = IM_, JN = JN_, STAGES = STAGES_;
     static constexpr int WAVES = WGM * WGN, THREADS = 64 * WAVES;
     static constexpr int TM = 32 * IM * WGM, TN = 32 * JN * WGN;
-    static constexpr int P_BYTES = TM * kStepK * 2, Q_BYTES = TN * kStepK * 2;
+    static constexpr int P_BYTES = TM * kPanel * 2, Q_BYTES = TN * kPanel * 2;
     static constexpr int STAGE = P_BYTES + Q_BYTES;
-    static constexpr int LOADS = STAGE / 1024 / WAVES;          // of a wave for a stage
-    static constexpr int PITCH = TN + 8;                        // of the result's tile in LDS
-    static constexpr int LDS = STAGES * STAGE > TM * PITCH * 2 ? STAGES * STAGE : TM * PITCH * 2;
+    static constexpr int P_LOADS = P_BYTES / 1024 / WAVES, LOADS = STAGE / 1024 / WAVES;   // of a wave for a stage
+    static constexpr int LDS = STAGES * STAGE;
     static_assert(TM == TN, "square tiles: half of a symmetric product is its lower triangle of tiles");
-    static_assert(LDS <= 160 * 1024, "LDS budget");
+    static_assert(LDS <= 160 * 1024 && LDS >= WAVES * 32 * 36 * 4, "LDS budget");
     static_assert(P_BYTES / 1024 % WAVES == 0 && Q_BYTES / 1024 % WAVES == 0, "whole loads for every wave");
+    static_assert(STAGES >= 3, "a stage that is read, the one whose first fragments are read ahead, one that is loaded");
 };
-using NsLarge = NsCfg<2, 4, 4, 2, 2>;       // 256 x 256
-using NsMiddle = NsCfg<2, 2, 2, 2, 2>;      // 128 x 128
-using NsSmall = NsCfg<2, 2, 1, 1, 4>;       // 64 x 64
+#ifndef NS_L
+#define NS_L 4
+#define NS_M 4
+#define NS_S 6
+#endif
+using NsLarge = NsCfg<2, 4, 4, 2, NS_L>;       // 256 x 256
+using NsMiddle = NsCfg<2, 2, 2, 2, NS_M>;      // 128 x 128
+using NsSmall = NsCfg<2, 2, 1, 1, NS_S>;       // 64 x 64
 
 // 16 bytes a lane from `rsrc` at voff + soff straight into LDS at `lds` + 16 lane
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t lds, uint32_t voff, uint32_t soff)
 {
     // (one wait state between the write of m0 and its use)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform_u32(lds)), "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform_u32(lds)), "v"(voff), "s"(rsrc), "s"(uniform_u32(soff)));
 }
 __device__ __forceinline__ i32x4 ns_rsrc(const void* p, uint32_t bytes)
 {
     const uint64_t a = (uint64_t)p;
-    return i32x4{(int)uniform_u32((uint32_t)a), (int)uniform_u32((uint32_t)(a >> 32) & 0xffffu), (int)bytes, 0x00020000};
+    return i32x4{(int)uniform_u32((uint32_t)a), (int)uniform_u32((uint32_t)(a >> 32) & 0xffffu), (int)uniform_u32(bytes), 0x00020000};
 }
 template <int N>
 __device__ __forceinline__ void wait_loads()
@@ -267,11 +282,22 @@ __device__ __forceinline__ NsTile ns_tile(const NsGemm& g, int tile)
     NsTile t;
     t.batch = tile / per;
     tile -= t.batch * per;
-    if constexpr (SYM) {        // those with tj <= ti
-        t.ti = (int)((sqrtf(8.f * (float)tile + 1.f) - 1.f) * 0.5f);
-        while ((t.ti + 1) * (t.ti + 2) / 2 <= tile) t.ti++;
-        while (t.ti * (t.ti + 1) / 2 > tile) t.ti--;
-        t.tj = tile - t.ti * (t.ti + 1) / 2;
+    if constexpr (SYM) {        // those with tj <= ti: 8 A^2 + 2 A in the first A groups of four rows, column by column
+        int a = (int)sqrtf((float)tile * 0.125f);
+        while (8 * (a + 1) * (a + 1) + 2 * (a + 1) <= tile) a++;
+        while (8 * a * a + 2 * a > tile) a--;
+        tile -= 8 * a * a + 2 * a;
+        const int rows = min(4, g.tiles_m - 4 * a), whole = rows * (4 * a + 1);       // columns 0 .. 4 a have all rows
+        if (tile < whole) {
+            t.ti = 4 * a + tile % rows;
+            t.tj = tile / rows;
+        } else {
+            tile -= whole;
+            int c = 1;
+            for (; tile >= rows - c; c++) tile -= rows - c;
+            t.tj = 4 * a + c;
+            t.ti = t.tj + tile;
+        }
     } else {                    // four rows of tiles at a time: neighbours share rows of P and columns of Q
         const int group = tile / (4 * g.tiles_n), first = 4 * group, rows = min(4, g.tiles_m - first);
         tile -= group * 4 * g.tiles_n;
@@ -281,85 +307,79 @@ __device__ __forceinline__ NsTile ns_tile(const NsGemm& g, int tile)
     return t;
 }
 
-// Results of a tile.  A lane holds row i = lane % 32 of a block, columns
-// 8 q + 4 (lane / 32) + e in register 4 q + e.
-template <class Cfg, int KIND>
-__device__ __forceinline__ void ns_finish(const NsGemm& g, const NsMatrices& mats, const NsTile t, f32x16 (&acc)[Cfg::IM][Cfg::JN],
-                                          char* s_mem)
+// Results of a 32 x 32 block at (r0, c0) of matrix `batch`, whose lane holds
+// row lane % 32, columns 8 q + 4 (lane / 32) + e in register 4 q + e.
+// `scratch`: 4608 bytes of LDS of this wave's own.  `mirror`: also as the
+// block at (c0, r0) of a symmetric result, turned by transposing reads.
+template <int KIND>
+__device__ __forceinline__ void ns_finish(const NsGemm& g, const NsMatrices& mats, int batch, int r0, int c0, bool mirror,
+                                          const f32x16& acc, char* scratch)
 {
-    constexpr bool kSym = KIND == kGram || KIND == kPoly;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wm = wave / Cfg::WGN, wn = wave % Cfg::WGN;
-    const bool precise = g.passes > 1;
-    if constexpr (KIND == kLast) {      // straight to the weights, in their own orientation
-        const NsMatrix mat = mats.at[t.batch];
+    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+    if constexpr (KIND == kLast) {      // the weights, in their own orientation: 8 elements of a row a lane
+        const NsMatrix mat = mats.at[batch];
+        float* s = reinterpret_cast<float*>(scratch);
 #pragma unroll
-        for (int i = 0; i < Cfg::IM; i++)
+        for (int q = 0; q < 4; q++)
+            *reinterpret_cast<f32x4*>(s + row * 36 + 8 * q + 4 * half) = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+        const int64_t rows = mat.tall ? g.n : g.m, cols = mat.tall ? g.m : g.n, wr = mat.tall ? c0 : r0, wc = mat.tall ? r0 : c0;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-            for (int j = 0; j < Cfg::JN; j++)
+        for (int u = 0; u < 2; u++) {
+            const int r = 16 * u + (lane >> 2), c = 8 * (lane & 3);
+            const int nv = wr + r < rows ? (int)max((int64_t)0, min((int64_t)8, cols - (wc + c))) : 0;
+            const int64_t at = nv ? (wr + r) * mat.w_stride + wc + c : 0;
+            float o[8], w[8];
+            if (g.update) ns_chunk(mat.w, g.w_f32, at, nv, w);
 #pragma unroll
-                for (int qd = 0; qd < 4; qd++) {
-                    const int64_t r = (int64_t)t.ti * Cfg::TM + (wm * Cfg::IM + i) * 32 + (lane & 31);
-                    const int64_t c = (int64_t)t.tj * Cfg::TN + (wn * Cfg::JN + j) * 32 + 8 * qd + 4 * (lane >> 5);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (r >= g.m || c + e >= g.n) continue;
-                        const float o = acc[i][j][4 * qd + e] * (1.f / (kHeld * kHeld));
-                        const int64_t at = mat.tall ? (c + e) * mat.w_stride + r : r * mat.w_stride + c + e;
-                        const float v = g.update ? g.keep * param_one(RowParam{mat.w, g.w_f32, 0}, at) - g.rate * o : o;
-                        param_store(mat.w, g.w_f32, at, v);
-                    }
-                }
+            for (int e = 0; e < 8; e++) {
+                o[e] = (mat.tall ? s[(c + e) * 36 + r] : s[r * 36 + c + e]) * (1.f / (kHeld * kHeld));
+                if (g.update) o[e] = g.keep * w[e] - g.rate * o[e];
+            }
+            if (g.w_f32)
+                store_raw(static_cast<float*>(mat.w) + at, to_raw<float>(o), nv);
+            else
+                store_raw(static_cast<bf16*>(mat.w) + at, to_raw<bf16>(o), nv);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else {
-        // through LDS as a row-major tile, the high parts and (precise) then the low ones
-        _Float16* tile_s = reinterpret_cast<_Float16*>(s_mem);
+        _Float16* out = g.out + batch * g.out_size;
+        const int64_t at = ((int64_t)(c0 / kPanel) * g.pitch + r0) * kPanel, turned = ((int64_t)(r0 / kPanel) * g.pitch + c0) * kPanel;
+        const bool precise = g.passes > 1;
+        f16x4 high[4], low[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int in = row * kPanel + 8 * q + 4 * half;
+            f16x4 old = {}, old_low = {};
+            if constexpr (KIND == kPoly) {      // p is A
+                old = *reinterpret_cast<const f16x4*>(g.p + batch * g.p_size + at + in);
+                if (precise) old_low = *reinterpret_cast<const f16x4*>(g.p + batch * g.p_size + g.p_low + at + in);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float x = acc[4 * q + e] * ((KIND == kPoly ? g.c : 1.f) / kHeld);
+                if constexpr (KIND == kPoly)
+                    x += g.b * ((float)old[e] + (float)old_low[e]) + (r0 + row == c0 + 8 * q + 4 * half + e ? g.a * kHeld : 0.f);
+                high[q][e] = (_Float16)x;
+                low[q][e] = (_Float16)(x - (float)high[q][e]);
+            }
+            *reinterpret_cast<f16x4*>(out + at + in) = high[q];
+            if (precise) *reinterpret_cast<f16x4*>(out + g.out_low + at + in) = low[q];
+        }
+        if (!mirror) return;
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
         for (int part = 0; part < (precise ? 2 : 1); part++) {
-            // (made anew for the second time round: kept, the 128 products would not fit the registers)
-            float scale = (KIND == kPoly ? g.c : 1.f) / kHeld;
-            asm volatile("" : "+v"(scale)::"memory");
 #pragma unroll
-            for (int i = 0; i < Cfg::IM; i++)
+            for (int q = 0; q < 4; q++)
+                *reinterpret_cast<f16x4*>(scratch + row * 64 + (8 * q + 4 * half) * 2) = part ? low[q] : high[q];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-                for (int j = 0; j < Cfg::JN; j++) {
-                    const int r = (wm * Cfg::IM + i) * 32 + (lane & 31);
-#pragma unroll
-                    for (int qd = 0; qd < 4; qd++) {
-                        const int c = (wn * Cfg::JN + j) * 32 + 8 * qd + 4 * (lane >> 5);
-                        f16x4 v, old = {}, old_low = {};
-                        const int gi = t.ti * Cfg::TM + r, gj = t.tj * Cfg::TN + c;
-                        if constexpr (KIND == kPoly) {      // p is A
-                            const _Float16* at = g.p + t.batch * g.p_size + (int64_t)gi * g.ldp + gj;
-                            old = *reinterpret_cast<const f16x4*>(at);
-                            if (precise) old_low = *reinterpret_cast<const f16x4*>(at + g.p_low);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float x = acc[i][j][4 * qd + e] * scale;
-                            if constexpr (KIND == kPoly)
-                                x += g.b * ((float)old[e] + (float)old_low[e]) + (gi == gj + e ? g.a * kHeld : 0.f);
-                            v[e] = (_Float16)x;
-                            if (part) v[e] = (_Float16)(x - (float)v[e]);
-                        }
-                        *reinterpret_cast<f16x4*>(tile_s + r * Cfg::PITCH + c) = v;
-                    }
-                }
-            __syncthreads();
-            _Float16* out = g.out + t.batch * g.out_size + (part ? g.out_low : 0);
-            for (int k = threadIdx.x; k < Cfg::TM * Cfg::TN / 8; k += Cfg::THREADS) {
-                const int r = k / (Cfg::TN / 8), c = k % (Cfg::TN / 8) * 8;
-                *reinterpret_cast<f16x8*>(out + (int64_t)(t.ti * Cfg::TM + r) * g.ldo + t.tj * Cfg::TN + c) =
-                    *reinterpret_cast<const f16x8*>(tile_s + r * Cfg::PITCH + c);
+            for (int q = 0; q < 4; q++) {       // rows 8 q + 4 half on of the block, this lane's column of it
+                const int j = lane & 15;
+                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(scratch + (8 * q + 4 * half + (j >> 2)) * 64 + ((lane & 16) + 4 * (j & 3)) * 2));
+                *reinterpret_cast<s16x4*>(out + (part ? g.out_low : 0) + turned + row * kPanel + 8 * q + 4 * half) = v;
             }
-            if (kSym && t.ti != t.tj) {
-                for (int k = threadIdx.x; k < Cfg::TM * Cfg::TN / 8; k += Cfg::THREADS) {
-                    const int r = k / (Cfg::TM / 8), c = k % (Cfg::TM / 8) * 8;     // row r, columns c on of the transpose
-                    f16x8 v;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = tile_s[(c + e) * Cfg::PITCH + r];
-                    *reinterpret_cast<f16x8*>(out + (int64_t)(t.tj * Cfg::TN + r) * g.ldo + t.ti * Cfg::TM + c) = v;
-                }
-            }
-            if (precise) __syncthreads();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
     }
 }
@@ -395,30 +415,29 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
         from = (int64_t)id * k_total;
         to = from + k_total;
     } else {
-        const int64_t all = (int64_t)(g.tiles - g.whole) * k_total, w = id - g.whole;
-        from = (int64_t)g.whole * k_total + all * w / g.sharers;
-        to = (int64_t)g.whole * k_total + all * (w + 1) / g.sharers;
+        // Lane l has the tiles l, l + lanes, ... behind the whole ones, its sharers' steps one after the other in them:
+        // those at one place in every lane are at the same K of neighbouring tiles at the same time and share what they load.
+        const int64_t all = (int64_t)(g.tiles - g.whole) / g.lanes * k_total, w = (id - g.whole) / g.lanes, sharers = g.sharers / g.lanes;
+        from = all * w / sharers;
+        to = all * (w + 1) / sharers;
     }
 
-    // Fragment addresses.  An [R, 64] tile with K along the row: rows of 128 bytes, the 16-byte chunk c of row r at
-    // c ^ (r & 7), so that eight lanes reading one chunk of eight rows meet all banks.  A [64, TN] tile with K down the
-    // rows: chunk c of row k at c ^ 2 (k & 3), so that the four rows a transposing read takes lie in different banks.
+    // A stage's tiles in LDS: rows of 64 bytes, of P (and a symmetric Q) K along them, 16-byte chunk c of row r at
+    // c ^ (r / 4 & 3): the 16 lanes that a fragment read serves at a time (0-3, 12-15, 20-23, 24-27 and so on) then meet
+    // all 64 banks.  Of step's Q panels of 32 columns, K down the rows: 32 lanes of a transposing read take four whole rows.
+    const uint32_t voff_rows = (uint32_t)((lane & ~3) | ((lane & 3) ^ (lane >> 4 & 3))) * 16u, voff_cols = (uint32_t)lane * 16u;
     auto row_frag = [&](const char* t, int r0, int slice) -> f16x8 {
-        const int r = r0 + (lane & 31), c = (2 * slice + (lane >> 5)) ^ (r & 7);
-        return *reinterpret_cast<const f16x8*>(t + r * 128 + c * 16);
+        const int r = r0 + (lane & 31), c = (2 * slice + (lane >> 5)) ^ (r >> 2 & 3);
+        return *reinterpret_cast<const f16x8*>(t + r * 64 + c * 16);
     };
     // within 16 lanes lane j points at row k0 + j / 4, columns 4 (j % 4) on, and gets column j of four rows
     auto col_frag = [&](const char* t, int c0, int slice) -> f16x8 {
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const int j = lane & 15, col = c0 + (lane & 16) + 4 * (j & 3);
-        s16x4 h[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int k = 16 * slice + 8 * (lane >> 5) + 4 * u + (j >> 2);
-            const int chunk = (col >> 3) ^ (2 * (k & 3));
-            h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t + k * (Cfg::TN * 2) + chunk * 16 + (col & 7) * 2));
-        }
-        return __builtin_bit_cast(f16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        const int j = lane & 15, k = 16 * slice + 8 * (lane >> 5) + (j >> 2);
+        const char* at = t + c0 * 64 + k * 64 + ((lane & 16) + 4 * (j & 3)) * 2;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 256));
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
     for (int second = 0; from < to; second++) {
@@ -427,37 +446,31 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
         const int k_from = (int)uniform_u32((uint32_t)(from - (int64_t)tile * k_total));
         const int k_to = (int)uniform_u32((uint32_t)min((int64_t)k_total, to - (int64_t)tile * k_total));
         from += k_to - k_from;
-        const NsTile t = ns_tile<kSym>(g, tile);
-        const _Float16* p = g.p + t.batch * g.p_size + (int64_t)t.ti * Cfg::TM * g.ldp;
-        const _Float16* q = g.q + t.batch * g.q_size + (kSym ? (int64_t)t.tj * Cfg::TN * g.ldq : (int64_t)t.tj * Cfg::TN);
-        // (rows of Q: the tile's, or all K up to the tile's last column)
-        const int64_t p_room = Cfg::TM * (int64_t)g.ldp;
-        const int64_t q_room = kSym ? Cfg::TN * (int64_t)g.ldq : (int64_t)(g.k_steps * kStepK - 1) * g.ldq + Cfg::TN;
+        const NsTile t = ns_tile<kSym>(g, shares ? g.whole + tile * g.lanes + (id - g.whole) % g.lanes : tile);
+        const _Float16* p = g.p + t.batch * g.p_size + (int64_t)t.ti * Cfg::TM * kPanel;
+        const _Float16* q = g.q + t.batch * g.q_size + (kSym ? (int64_t)t.tj * Cfg::TN * kPanel : (int64_t)t.tj * Cfg::TN * g.pitch);
+        // (from the tile's first element to its last: of P and a symmetric Q over all panels, of step's Q over its own)
+        const int64_t p_room = ((int64_t)(g.k_steps - 1) * g.pitch + Cfg::TM) * kPanel;
+        const int64_t q_room = kSym ? ((int64_t)(g.k_steps - 1) * g.pitch + Cfg::TN) * kPanel : (int64_t)Cfg::TN * g.pitch;
         const bool low = g.passes > 1;
         const i32x4 rp = ns_rsrc(p, (uint32_t)((p_room + (low ? g.p_low : 0)) * 2));
         const i32x4 rq = ns_rsrc(q, (uint32_t)((q_room + (low ? g.q_low : 0)) * 2));
-        auto load = [&](int step, int stage) {
+        // this wave's loads s0 .. s1 - 1 for a step
+        auto load = [&](int step, int stage, int s0, int s1) {
             const uint32_t at = lds0 + stage * Cfg::STAGE;
             const int pass = step < g.k_steps ? 0 : step < 2 * g.k_steps ? 1 : 2;       // high high, high low, low high
-            const uint32_t k0 = (uint32_t)(step - pass * g.k_steps) * kStepK;
-            const uint32_t p_off = (k0 + (pass == 2 ? (uint32_t)g.p_low : 0u)) * 2u;
-            const uint32_t q_off = ((kSym ? k0 : k0 * (uint32_t)g.ldq) + (pass == 1 ? (uint32_t)g.q_low : 0u)) * 2u;
-            auto rows = [&](i32x4 rsrc, uint32_t lds, int bytes, int ld, uint32_t off) {
-                for (int s = 0; s < bytes / 1024 / Cfg::WAVES; s++) {
-                    const int slot = s * Cfg::WAVES + wave;                             // 1 KiB: 8 rows
-                    const int r = slot * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
-                    load_to_lds(rsrc, lds + slot * 1024, (uint32_t)(r * ld + c * 8) * 2u, uniform_u32(off));
-                }
-            };
-            rows(rp, at, Cfg::P_BYTES, g.ldp, p_off);
-            if constexpr (kSym) {
-                rows(rq, at + Cfg::P_BYTES, Cfg::Q_BYTES, g.ldq, q_off);
-            } else {
-                constexpr int kChunks = Cfg::TN / 8;                                    // of a row
-                for (int s = 0; s < Cfg::Q_BYTES / 1024 / Cfg::WAVES; s++) {
-                    const int slot = s * Cfg::WAVES + wave, n = slot * 64 + lane;
-                    const int k = n / kChunks, c = (n % kChunks) ^ (2 * (k & 3));
-                    load_to_lds(rq, at + Cfg::P_BYTES + slot * 1024, (uint32_t)(k * g.ldq + c * 8) * 2u, uniform_u32(q_off));
+            const uint32_t k = (uint32_t)(step - pass * g.k_steps);
+            const uint32_t p_off = k * (uint32_t)g.pitch * 64u + (pass == 2 ? (uint32_t)g.p_low * 2u : 0u);
+            const uint32_t q_off = k * (kSym ? (uint32_t)g.pitch * 64u : 2048u) + (pass == 1 ? (uint32_t)g.q_low * 2u : 0u);
+#pragma unroll
+            for (int s = s0; s < s1; s++) {
+                if (s < Cfg::P_LOADS) {
+                    const int slot = s * Cfg::WAVES + wave;                             // 1 KiB
+                    load_to_lds(rp, at + slot * 1024, voff_rows, p_off + slot * 1024);
+                } else {
+                    const int slot = (s - Cfg::P_LOADS) * Cfg::WAVES + wave;
+                    const uint32_t off = kSym ? slot * 1024u : (slot >> 1) * (uint32_t)g.pitch * 64u + (slot & 1) * 1024u;
+                    load_to_lds(rq, at + Cfg::P_BYTES + slot * 1024, kSym ? voff_rows : voff_cols, q_off + off);
                 }
             }
         };
@@ -470,38 +483,63 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
 
-        constexpr int kAhead = Cfg::STAGES - 1;
-        if (second) __builtin_amdgcn_s_barrier();       // (the first tile's last reads, see below)
+        // The fragments of a step's first slice are read in the step before, ahead of the barrier between, so that the
+        // products go on through it: a barrier vouches for the stage after the one that begins.
+        f16x8 fp[2][Cfg::IM], fq[2][Cfg::JN];
+        auto read_p = [&](int stage, int s, int i) { fp[s & 1][i] = row_frag(s_mem + stage * Cfg::STAGE, (wm * Cfg::IM + i) * 32, s); };
+        auto read_q = [&](int stage, int s, int j) {
+            const char* t = s_mem + stage * Cfg::STAGE + Cfg::P_BYTES;
+            fq[s & 1][j] = kSym ? row_frag(t, (wn * Cfg::JN + j) * 32, s) : col_frag(t, (wn * Cfg::JN + j) * 32, s);
+        };
+        constexpr int kAhead = Cfg::STAGES - 1, kSlices = kPanel / 16;
+        if (second) __builtin_amdgcn_s_barrier();       // (the first tile's last reads)
 #pragma unroll
         for (int s = 0; s < kAhead; s++)
-            if (k_from + s < k_to) load(k_from + s, s);
+            if (k_from + s < k_to) load(k_from + s, s, 0, Cfg::LOADS);
+        if (k_from + kAhead <= k_to)
+            wait_loads<(kAhead - 1) * Cfg::LOADS>();
+        else
+            wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+#pragma unroll
+        for (int j = 0; j < Cfg::JN; j++) read_q(0, 0, j);
+#pragma unroll
+        for (int i = 0; i < Cfg::IM; i++) read_p(0, 0, i);
         int stage = 0;
         for (int step = k_from; step < k_to; step++) {
-            // this step's tiles are there and the stage that is loaded next has been read, in every wave
+            // the next step's tiles are there and the stage that is loaded now has been read, in every wave
             if (step + kAhead <= k_to)
-                wait_loads<(kAhead - 1) * Cfg::LOADS>();
+                wait_loads<(kAhead - 2) * Cfg::LOADS>();
             else
                 wait_loads<0>();
             __builtin_amdgcn_s_barrier();
-            if (step + kAhead < k_to) load(step + kAhead, stage == 0 ? kAhead : stage - 1);
-            const char* tp = s_mem + stage * Cfg::STAGE;
-            const char* tq = tp + Cfg::P_BYTES;
-            stage = stage == kAhead ? 0 : stage + 1;
+            const bool more = step + kAhead < k_to;
+            const int into = stage == 0 ? kAhead : stage - 1, next = stage == kAhead ? 0 : stage + 1;
 #pragma unroll
-            for (int s = 0; s < kStepK / 16; s++) {
-                f16x8 fp[Cfg::IM], fq[Cfg::JN];
+            for (int s = 0; s < kSlices; s++) {
+                // Reads, products and loads in turn: eight waves that all read first would wait for one another.
+                // (behind the last step the next stage holds what it held: read, not used)
+                const int from_stage = s + 1 < kSlices ? stage : next, of = s + 1 < kSlices ? s + 1 : 0;
 #pragma unroll
-                for (int i = 0; i < Cfg::IM; i++) fp[i] = row_frag(tp, wm * 32 * Cfg::IM + 32 * i, s);
+                for (int i = 0; i < Cfg::IM; i++) {
+                    if (i == 0) {
 #pragma unroll
-                for (int j = 0; j < Cfg::JN; j++)
-                    fq[j] = kSym ? row_frag(tq, wn * 32 * Cfg::JN + 32 * j, s) : col_frag(tq, wn * 32 * Cfg::JN + 32 * j, s);
-#pragma unroll
-                for (int i = 0; i < Cfg::IM; i++)
+                        for (int j = 0; j < Cfg::JN; j++) read_q(from_stage, of, j);
+                    }
+                    read_p(from_stage, of, i);
 #pragma unroll
                     for (int j = 0; j < Cfg::JN; j++)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[j], fp[i], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s & 1][j], fp[s & 1][i], acc[i][j], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    constexpr int kAll = Cfg::IM * kSlices;
+                    const int at = s * Cfg::IM + i;
+                    if (more) load(step + kAhead, into, at * Cfg::LOADS / kAll, (at + 1) * Cfg::LOADS / kAll);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
+            stage = next;
         }
+        wait_loads<0>();
         if (shares) {
             float* part = ns_part<Cfg>(g, id - g.whole, second);
 #pragma unroll
@@ -512,47 +550,51 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
                     for (int qd = 0; qd < 4; qd++)
                         *reinterpret_cast<f32x4*>(part + ((i * Cfg::JN + j) * 4 + qd) * 256) =
                             f32x4{acc[i][j][4 * qd], acc[i][j][4 * qd + 1], acc[i][j][4 * qd + 2], acc[i][j][4 * qd + 3]};
-            wait_loads<0>();        // (this wave's reads of LDS are done before the barrier at the next tile)
         } else {
-            wait_loads<0>();
-            __builtin_amdgcn_s_barrier();
-            ns_finish<Cfg, KIND>(g, mats, t, acc, s_mem);
+            __builtin_amdgcn_s_barrier();       // (every wave's reads are done: the LDS is scratch now)
+#pragma unroll
+            for (int i = 0; i < Cfg::IM; i++)
+#pragma unroll
+                for (int j = 0; j < Cfg::JN; j++)
+                    ns_finish<KIND>(g, mats, t.batch, t.ti * Cfg::TM + (wm * Cfg::IM + i) * 32, t.tj * Cfg::TN + (wn * Cfg::JN + j) * 32,
+                                    kSym && t.ti != t.tj, acc[i][j], s_mem + wave * 4608);
         }
     }
 }
 
-// The shared tiles: their sharers' sums added in order, then as a tile with a workgroup of its own.
+// The shared tiles: their sharers' sums added in order, then as a tile with a
+// workgroup of its own.  A wave a block of 32 x 32.
 template <class Cfg, int KIND>
-__global__ __launch_bounds__(Cfg::THREADS) void ns_join_kernel(NsGemm g, NsMatrices mats)
+__global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsMatrices mats)
 {
-    __shared__ __attribute__((aligned(16))) char s_mem[Cfg::TM * Cfg::PITCH * 2];
-    constexpr bool kSym = KIND == kGram || KIND == kPoly;
-    const int64_t k_total = (int64_t)g.k_steps * g.passes, all = (g.tiles - g.whole) * k_total;
-    const int64_t from = (int64_t)blockIdx.x * k_total, to = from + k_total;      // of the shared steps
+    __shared__ __attribute__((aligned(16))) char s_mem[4 * 4608];
+    constexpr int kBlocks = Cfg::WAVES * Cfg::IM * Cfg::JN;
+    static_assert(kBlocks % 4 == 0, "four blocks of a tile to a workgroup");
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int shared = (int)blockIdx.x / (kBlocks / 4), block = (int)blockIdx.x % (kBlocks / 4) * 4 + wave;
+    const int of_wave = block / (Cfg::IM * Cfg::JN), i = block % (Cfg::IM * Cfg::JN) / Cfg::JN, j = block % Cfg::JN;
+    const int64_t k_total = (int64_t)g.k_steps * g.passes, all = (g.tiles - g.whole) / g.lanes * k_total;
+    const int64_t from = shared / g.lanes * k_total, to = from + k_total;      // of its lane's steps
+    const int sharers = g.sharers / g.lanes;
     // the sharer of step s is the last w with all w / sharers <= s
-    auto sharer = [&](int64_t s) { return (int)(((s + 1) * g.sharers - 1) / all); };
-    f32x16 acc[Cfg::IM][Cfg::JN];
+    auto sharer = [&](int64_t s) { return (int)(((s + 1) * sharers - 1) / all); };
+    f32x16 acc;
 #pragma unroll
-    for (int i = 0; i < Cfg::IM; i++)
+    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    const int last = sharer(to - 1);
+    for (int w = sharer(from); w <= last; w++) {
+        const int second = all * w / sharers < from;            // it began with the tile before
+        const float* part = g.part + ((int64_t)(2 * (w * g.lanes + shared % g.lanes) + second) * Cfg::WAVES + of_wave) * (Cfg::IM * Cfg::JN * 1024) + (i * Cfg::JN + j) * 1024 + lane * 4;
 #pragma unroll
-        for (int j = 0; j < Cfg::JN; j++)
+        for (int q = 0; q < 4; q++) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(part + q * 256);
 #pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
-    for (int w = sharer(from); w <= sharer(to - 1); w++) {
-        const int second = all * w / g.sharers < from;          // it began with the tile before
-        const float* part = ns_part<Cfg>(g, w, second);
-#pragma unroll
-        for (int i = 0; i < Cfg::IM; i++)
-#pragma unroll
-            for (int j = 0; j < Cfg::JN; j++)
-#pragma unroll
-                for (int qd = 0; qd < 4; qd++) {
-                    const f32x4 v = *reinterpret_cast<const f32x4*>(part + ((i * Cfg::JN + j) * 4 + qd) * 256);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][j][4 * qd + e] += v[e];
-                }
+            for (int e = 0; e < 4; e++) acc[4 * q + e] += v[e];
+        }
     }
-    ns_finish<Cfg, KIND>(g, mats, ns_tile<kSym>(g, g.whole + (int)blockIdx.x), acc, s_mem);
+    const NsTile t = ns_tile<KIND == kGram || KIND == kPoly>(g, g.whole + shared);
+    ns_finish<KIND>(g, mats, t.batch, t.ti * Cfg::TM + (of_wave / Cfg::WGN * Cfg::IM + i) * 32,
+                    t.tj * Cfg::TN + (of_wave % Cfg::WGN * Cfg::JN + j) * 32, t.ti != t.tj, acc, s_mem + wave * 4608);
 }
 
 // ---------------------------------------------------------------------------
@@ -562,12 +604,16 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_join_kernel(NsGemm g, NsMatri
 // workgroup of their own, and its time in microseconds as the choice sees it.
 struct NsProduct {
     int tile;
-    int64_t tiles, whole, sharers;
+    int64_t tiles, whole, sharers, lanes;
     double time;
 };
 struct NsPlan {
     NsProduct gram, poly, step;
     int64_t mp, np;
+    // Panels are 2 KiB further apart than their rows need: at one step of step all workgroups load the same 32 rows of
+    // their panels, which a power of two would put on the same few memory channels.
+    int64_t pitch() const { return mp + kPanel; }
+    int64_t size(int64_t cols) const { return pitch() * cols; }     // elements of a matrix with so many columns
     int64_t x_bytes, a_bytes, parts_bytes, share_bytes, total;
 };
 
@@ -577,12 +623,12 @@ struct NsTileRate {
     int tile, per_cu;
     double step;
 };
-constexpr NsTileRate kNsRates[] = {{256, 1, 1.75}, {128, 2, 1.15}, {64, 2, 0.45}};
+constexpr NsTileRate kNsRates[] = {{256, 1, 0.88}, {128, 2, 0.58}, {64, 2, 0.23}};
 
 static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, bool sym, int64_t k, int64_t count, int passes)
 {
     NsProduct p{};
-    const int64_t tm = rows / r.tile, tn = cols / r.tile, steps = k / kStepK * passes, slots = (int64_t)kNsCus * r.per_cu;
+    const int64_t tm = rows / r.tile, tn = cols / r.tile, steps = k / kPanel * passes, slots = (int64_t)kNsCus * r.per_cu;
     p.tile = r.tile;
     p.tiles = (sym ? tm * (tm + 1) / 2 : tm * tn) * count;
     p.whole = p.tiles;
@@ -591,10 +637,12 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
     // A last round that does not fill the chip is dealt out in shares of its steps instead, where the steps saved are
     // worth the sums' way through memory (written and read once at about 4 TB/s) and one more kernel.
     if (sym && rest > 0) {
-        const int64_t sharers = std::min(slots, rest * steps);
+        int64_t lanes = 8;
+        while (rest % lanes) lanes /= 2;
+        const int64_t sharers = std::min(slots, rest * steps);      // (slots and rest: multiples of lanes)
         const double bytes = 8.0 * r.tile * r.tile * (double)(sharers + rest);
         const double shared = 3.0 + r.step * (double)((rounds - 1) * steps + (rest * steps + sharers - 1) / sharers) + 5.0 + bytes / 4e6;
-        if (shared < p.time) p.whole = p.tiles - rest, p.sharers = sharers, p.time = shared;
+        if (shared < p.time) p.whole = p.tiles - rest, p.sharers = sharers, p.lanes = lanes, p.time = shared;
     }
     return p;
 }
@@ -626,8 +674,8 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
         if (best.mp == 0 || time < best_time) best = p, best_time = time;
     }
     NsPlan& p = best;
-    p.x_bytes = p.mp * p.np * 2 * count * (precise ? 2 : 1);
-    p.a_bytes = p.mp * p.mp * 2 * count * (precise ? 2 : 1);
+    p.x_bytes = p.size(p.np) * 2 * count * (precise ? 2 : 1);
+    p.a_bytes = p.size(p.mp) * 2 * count * (precise ? 2 : 1);
     p.parts_bytes = (kNsParts * 8 * count + 255) / 256 * 256;
     for (const NsProduct& q : {p.gram, p.poly}) p.share_bytes = std::max(p.share_bytes, q.sharers * 2 * q.tile * q.tile * 4);
     p.total = 2 * p.x_bytes + 2 * p.a_bytes + p.parts_bytes + p.share_bytes;
@@ -637,11 +685,11 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
 template <class Cfg, int KIND>
 static void ns_launch(NsGemm g, const NsProduct& p, const NsMatrices& mats, hipStream_t st)
 {
-    g.tiles = (int)p.tiles, g.whole = (int)p.whole, g.sharers = (int)p.sharers;
+    g.tiles = (int)p.tiles, g.whole = (int)p.whole, g.sharers = (int)p.sharers, g.lanes = (int)p.lanes;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_gemm_kernel<Cfg, KIND>), dim3((uint32_t)(p.whole + p.sharers)), dim3(Cfg::THREADS), 0, st, g, mats);
     if constexpr (KIND == kGram || KIND == kPoly)
         if (p.sharers)
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_join_kernel<Cfg, KIND>), dim3((uint32_t)(p.tiles - p.whole)), dim3(Cfg::THREADS), 0, st, g, mats);
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_join_kernel<Cfg, KIND>), dim3((uint32_t)(p.tiles - p.whole) * (Cfg::WAVES * Cfg::IM * Cfg::JN / 4)), dim3(256), 0, st, g, mats);
 }
 
 template <int KIND>
@@ -663,22 +711,22 @@ struct NsWork {
 
 static void ns_products(const NsPlan& p, const NsWork& w, NsGemm g, const NsMatrices& mats, int64_t count, int steps, hipStream_t st)
 {
-    const int64_t x_size = p.mp * p.np, a_size = p.mp * p.mp;
+    const int64_t x_size = p.size(p.np), a_size = p.size(p.mp);
     for (int k = 0; k < steps; k++) {
         _Float16 *x = w.x[k & 1], *y = w.x[(k + 1) & 1];
         NsGemm gram = g;
         gram.p = gram.q = x, gram.p_size = gram.q_size = x_size, gram.p_low = gram.q_low = x_size * count;
-        gram.ldp = gram.ldq = (int)p.np, gram.k_steps = (int)(p.np / kStepK);
-        gram.out = w.a, gram.out_size = a_size, gram.out_low = a_size * count, gram.ldo = (int)p.mp;
+        gram.pitch = (int)p.pitch(), gram.k_steps = (int)(p.np / kPanel);
+        gram.out = w.a, gram.out_size = a_size, gram.out_low = a_size * count;
         ns_launch<kGram>(gram, p, p.gram, mats, st);
         NsGemm poly = gram;
         poly.p = poly.q = w.a, poly.p_size = poly.q_size = a_size, poly.p_low = poly.q_low = a_size * count;
-        poly.ldp = poly.ldq = (int)p.mp, poly.k_steps = (int)(p.mp / kStepK);
+        poly.k_steps = (int)(p.mp / kPanel);
         poly.out = w.b;
         ns_launch<kPoly>(poly, p, p.poly, mats, st);
         NsGemm step = poly;
-        step.p = w.b, step.q = x, step.q_size = x_size, step.q_low = x_size * count, step.ldq = (int)p.np;
-        step.out = y, step.out_size = x_size, step.out_low = x_size * count, step.ldo = (int)p.np;
+        step.p = w.b, step.q = x, step.q_size = x_size, step.q_low = x_size * count;
+        step.out = y, step.out_size = x_size, step.out_low = x_size * count;
         if (k + 1 < steps)
             ns_launch<kStep>(step, p, p.step, mats, st);
         else
@@ -692,7 +740,7 @@ static int64_t ns_together(int64_t m, int64_t n, int64_t count, bool precise)
 {
     int64_t most = std::min<int64_t>(count, kNsBatch);
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-    while (most > 1 && precise && (most + 1) * up(m) * up(n) * 2 >= (int64_t(1) << 32)) most--;
+    while (most > 1 && precise && (most + 1) * (up(m) + kPanel) * up(n) * 2 >= (int64_t(1) << 32)) most--;
     return most;
 }
 
@@ -759,9 +807,9 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         }
         char* ws = static_cast<char*>(workspace);
         NsPrep a{};
-        a.m = m, a.n = n, a.mp = p.mp, a.np = p.np;
+        a.m = m, a.n = n, a.np = p.np;
         a.g_f32 = r.grad_type == BS_DT_F32, a.m_f32 = r.momentum_type == BS_DT_F32, a.momentum = r.momentum, a.nesterov = r.nesterov;
-        a.mu = r.mu, a.eps = r.eps, a.precise = precise, a.low = p.mp * p.np * here;
+        a.mu = r.mu, a.eps = r.eps, a.precise = precise, a.low = p.size(p.np) * here, a.pitch = p.pitch();
         // about 4096 elements or more to a workgroup, and no more of them than 8 a CU over all matrices
         a.parts = (int)std::max<int64_t>(1, std::min({(int64_t)kNsParts, (m * n + 8191) / 8192, (8 * kNsCus + here - 1) / here}));
         a.parts_at = reinterpret_cast<double*>(ws);
