@@ -219,7 +219,7 @@ struct NsGemm {
     int passes;                         // 1, or 3 (precise)
     int tiles_m, tiles_n;               // of one matrix's product
     int tiles;                          // of all matrices, those left out by symmetry not counted
-    int whole;                          // tiles with a workgroup of their own; the others' steps are
+    int whole;                          // tiles that one workgroup does; the others' steps are
     int sharers;                        // dealt out evenly to this many workgroups,
     int lanes;                          // a group of tiles to each of this many sets of them
     float* part;                        // [sharers][2][tile]: their sums
@@ -231,6 +231,8 @@ struct NsGemm {
     float keep, rate;
 };
 
+constexpr int kScratch = 16 * 36 * 4;  // bytes of LDS for a wave's results on their way out
+
 // WGM x WGN waves, each a block of 32 IM x 32 JN; STAGES of the K loop in LDS
 template <int WGM_, int WGN_, int IM_, int JN_, int STAGES_>
 struct NsCfg {
@@ -239,11 +241,11 @@ struct NsCfg {
     static constexpr int TM = 32 * IM * WGM, TN = 32 * JN * WGN;
     static constexpr int P_BYTES = TM * kPanel * 2, Q_BYTES = TN * kPanel * 2;
     static constexpr int STAGE = P_BYTES + Q_BYTES;
-    static constexpr int P_LOADS = P_BYTES / 1024 / WAVES, LOADS = STAGE / 1024 / WAVES;   // of a wave for a stage
-    static constexpr int LDS = STAGES * STAGE;
+    static constexpr int HALF = P_BYTES / 1024 / WAVES, LOADS = 2 * HALF;       // of a wave for a stage: of P, of both
+    static constexpr int LDS = STAGES * STAGE + WAVES * kScratch;
     static_assert(TM == TN, "square tiles: half of a symmetric product is its lower triangle of tiles");
-    static_assert(LDS <= 160 * 1024 && LDS >= WAVES * 32 * 36 * 4, "LDS budget");
-    static_assert(P_BYTES / 1024 % WAVES == 0 && Q_BYTES / 1024 % WAVES == 0, "whole loads for every wave");
+    static_assert(LDS <= 160 * 1024, "LDS budget");
+    static_assert(P_BYTES / 1024 % WAVES == 0 && (HALF == 1 || HALF == 2), "whole loads for every wave");
     static_assert(STAGES >= 3, "a stage that is read, the one whose first fragments are read ahead, one that is loaded");
 };
 #ifndef NS_L
@@ -255,11 +257,17 @@ using NsLarge = NsCfg<2, 4, 4, 2, NS_L>;       // 256 x 256
 using NsMiddle = NsCfg<2, 2, 2, 2, NS_M>;      // 128 x 128
 using NsSmall = NsCfg<2, 2, 1, 1, NS_S>;       // 64 x 64
 
-// 16 bytes a lane from `rsrc` at voff + soff straight into LDS at `lds` + 16 lane
+// N runs of 1 KiB, one behind the other, from `rsrc` at voff + soff (16 bytes a
+// lane) straight into LDS at `lds`
+template <int N>
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t lds, uint32_t voff, uint32_t soff)
 {
-    // (one wait state between the write of m0 and its use)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform_u32(lds)), "v"(voff), "s"(rsrc), "s"(uniform_u32(soff)));
+    // (one wait state between the write of m0 and its use; the offset counts on both sides)
+    if constexpr (N == 1)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
+                     "buffer_load_dwordx4 %1, %2, %3 offen offset:1024 lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
 }
 __device__ __forceinline__ i32x4 ns_rsrc(const void* p, uint32_t bytes)
 {
@@ -269,8 +277,9 @@ __device__ __forceinline__ i32x4 ns_rsrc(const void* p, uint32_t bytes)
 template <int N>
 __device__ __forceinline__ void wait_loads()
 {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 struct NsTile {
     int batch, ti, tj;
@@ -309,7 +318,7 @@ __device__ __forceinline__ NsTile ns_tile(const NsGemm& g, int tile)
 
 // Results of a 32 x 32 block at (r0, c0) of matrix `batch`, whose lane holds
 // row lane % 32, columns 8 q + 4 (lane / 32) + e in register 4 q + e.
-// `scratch`: 4608 bytes of LDS of this wave's own.  `mirror`: also as the
+// `scratch`: kScratch bytes of LDS of this wave's own.  `mirror`: also as the
 // block at (c0, r0) of a symmetric result, turned by transposing reads.
 template <int KIND>
 __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsMatrices& mats, int batch, int r0, int c0, bool mirror,
@@ -319,29 +328,36 @@ __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsMatrices& mat
     if constexpr (KIND == kLast) {      // the weights, in their own orientation: 8 elements of a row a lane
         const NsMatrix mat = mats.at[batch];
         float* s = reinterpret_cast<float*>(scratch);
+        const int64_t rows = mat.tall ? g.n : g.m, cols = mat.tall ? g.m : g.n;
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-            *reinterpret_cast<f32x4*>(s + row * 36 + 8 * q + 4 * half) = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-        const int64_t rows = mat.tall ? g.n : g.m, cols = mat.tall ? g.m : g.n, wr = mat.tall ? c0 : r0, wc = mat.tall ? r0 : c0;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int u = 0; u < 2; u++) {   // 16 rows of the block, or (tall) 16 columns
+            if (mat.tall) {             // columns 16 u on: registers 8 u on
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int r = 16 * u + (lane >> 2), c = 8 * (lane & 3);
-            const int nv = wr + r < rows ? (int)max((int64_t)0, min((int64_t)8, cols - (wc + c))) : 0;
-            const int64_t at = nv ? (wr + r) * mat.w_stride + wc + c : 0;
+                for (int q = 0; q < 2; q++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[(8 * q + 4 * half + e) * 36 + row] = acc[8 * u + 4 * q + e];
+            } else if (row / 16 == u) {
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    *reinterpret_cast<f32x4*>(s + row % 16 * 36 + 8 * q + 4 * half) = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const int64_t wr = (mat.tall ? c0 : r0) + 16 * u + (lane >> 2), wc = (mat.tall ? r0 : c0) + 8 * (lane & 3);
+            const int nv = wr < rows ? (int)max((int64_t)0, min((int64_t)8, cols - wc)) : 0;
+            const int64_t at = nv ? wr * mat.w_stride + wc : 0;
             float o[8], w[8];
             if (g.update) ns_chunk(mat.w, g.w_f32, at, nv, w);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                o[e] = (mat.tall ? s[(c + e) * 36 + r] : s[r * 36 + c + e]) * (1.f / (kHeld * kHeld));
+                o[e] = s[(lane >> 2) * 36 + 8 * (lane & 3) + e] * (1.f / (kHeld * kHeld));
                 if (g.update) o[e] = g.keep * w[e] - g.rate * o[e];
             }
             if (g.w_f32)
                 store_raw(static_cast<float*>(mat.w) + at, to_raw<float>(o), nv);
             else
                 store_raw(static_cast<bf16*>(mat.w) + at, to_raw<bf16>(o), nv);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else {
         _Float16* out = g.out + batch * g.out_size;
         const int64_t at = ((int64_t)(c0 / kPanel) * g.pitch + r0) * kPanel, turned = ((int64_t)(r0 / kPanel) * g.pitch + c0) * kPanel;
@@ -363,21 +379,33 @@ __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsMatrices& mat
                 high[q][e] = (_Float16)x;
                 low[q][e] = (_Float16)(x - (float)high[q][e]);
             }
-            *reinterpret_cast<f16x4*>(out + at + in) = high[q];
-            if (precise) *reinterpret_cast<f16x4*>(out + g.out_low + at + in) = low[q];
         }
-        if (!mirror) return;
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        for (int part = 0; part < (precise ? 2 : 1); part++) {
+        // Out as whole rows, 1 KiB a store, through LDS: 16-byte chunk q of row r lies at q ^ (r / 4 & 3).  (Stored from the
+        // lanes that hold them, 8 bytes of a row each, the results take four times the requests to L2.)
+        auto emit = [&](const f16x4 (&v)[4], _Float16* to) {
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-                *reinterpret_cast<f16x4*>(scratch + row * 64 + (8 * q + 4 * half) * 2) = part ? low[q] : high[q];
+            for (int q = 0; q < 4; q++) *reinterpret_cast<f16x4*>(scratch + row * 64 + (q ^ (row >> 2 & 3)) * 16 + 8 * half) = v[q];
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-            for (int q = 0; q < 4; q++) {       // rows 8 q + 4 half on of the block, this lane's column of it
-                const int j = lane & 15;
-                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(scratch + (8 * q + 4 * half + (j >> 2)) * 64 + ((lane & 16) + 4 * (j & 3)) * 2));
-                *reinterpret_cast<s16x4*>(out + (part ? g.out_low : 0) + turned + row * kPanel + 8 * q + 4 * half) = v;
+            for (int u = 0; u < 2; u++) {
+                const int r = 16 * u + (lane >> 2);
+                *reinterpret_cast<f16x8*>(to + u * 512 + lane * 8) = *reinterpret_cast<const f16x8*>(scratch + r * 64 + ((lane & 3) ^ (r >> 2 & 3)) * 16);
+            }
+        };
+        for (int part = 0; part < (precise ? 2 : 1); part++) {
+            _Float16* to = out + (part ? g.out_low : 0);
+            emit(part ? low : high, to + at);
+            if (mirror) {       // turned by transposing reads: rows 8 q + 4 half on of this lane's column
+                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                f16x4 v[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int j = lane & 15, r = 8 * q + 4 * half + (j >> 2), c = (lane & 16) + 4 * (j & 3);
+                    v[q] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(scratch + r * 64 + (c / 8 ^ (r >> 2 & 3)) * 16 + c % 8 * 2)));
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                emit(v, to + turned);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
@@ -392,6 +420,10 @@ __device__ __forceinline__ float* ns_part(const NsGemm& g, int sharer, int secon
            ((int)threadIdx.x & 63) * 4;
 }
 
+// Each workgroup goes through whole tiles and then through its share of the
+// others', one unbroken sequence of K steps: the loads run STAGES - 1 steps
+// ahead, over the ends of tiles too, so that only a tile's results interrupt
+// the products.
 template <class Cfg, int KIND>
 __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatrices mats)
 {
@@ -400,6 +432,7 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave / Cfg::WGN, wn = wave % Cfg::WGN;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem;
+    char* scratch = s_mem + Cfg::STAGES * Cfg::STAGE + wave * kScratch;
 
     // Workgroups go round the XCDs in turn: each XCD takes a contiguous part of every 256.
     int id = (int)blockIdx.x;
@@ -408,19 +441,34 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
         if (here == kNsCus) id = group + (id - group) % kNsXcds * (kNsCus / kNsXcds) + (id - group) / kNsXcds;
     }
     const int k_total = g.k_steps * g.passes;
-    // this workgroup's steps: of one tile, or its share of the others' (at most two tiles)
-    int64_t from, to;
-    const bool shares = id >= g.whole;
-    if (!shares) {
-        from = (int64_t)id * k_total;
-        to = from + k_total;
-    } else {
-        // Lane l has the tiles l, l + lanes, ... behind the whole ones, its sharers' steps one after the other in them:
-        // those at one place in every lane are at the same K of neighbouring tiles at the same time and share what they load.
-        const int64_t all = (int64_t)(g.tiles - g.whole) / g.lanes * k_total, w = (id - g.whole) / g.lanes, sharers = g.sharers / g.lanes;
-        from = all * w / sharers;
-        to = all * (w + 1) / sharers;
+    const int wholes = id < g.whole ? (g.whole - id - 1) / (int)gridDim.x + 1 : 0;
+    // Its share of the rest.  Lane l has the tiles l, l + lanes, ... behind the whole ones, its sharers' steps one after the
+    // other in them: those at one place in every lane are at the same K of neighbouring tiles at the same time and share
+    // what they load.  (The divisions leave their uniform results in vector registers.)
+    int share_from = 0, share_to = 0, share_tile = 0;           // steps of the tiles from share_tile on
+    if (id < g.sharers) {
+        const int64_t all = (int64_t)(g.tiles - g.whole) / g.lanes * k_total, w = id / g.lanes, sharers = g.sharers / g.lanes;
+        const int64_t from = all * w / sharers, to = all * (w + 1) / sharers, first = from / k_total;
+        share_tile = (int)uniform_u32((uint32_t)first);
+        share_from = (int)uniform_u32((uint32_t)(from - first * k_total));
+        share_to = (int)uniform_u32((uint32_t)(to - first * k_total));
     }
+    const int pieces = wholes + (share_to > share_from) + (share_to > k_total);
+    const int64_t steps = (int64_t)wholes * k_total + (share_to - share_from);
+    struct Piece {
+        NsTile t;
+        int from, to;
+    };
+    auto piece = [&](int i) {
+        Piece p;
+        const bool whole = i < wholes;
+        const int second = i - wholes;
+        p.t = ns_tile<kSym>(g, whole ? id + i * (int)gridDim.x : g.whole + (share_tile + second) * g.lanes + id % g.lanes);
+        p.t = {(int)uniform_u32((uint32_t)p.t.batch), (int)uniform_u32((uint32_t)p.t.ti), (int)uniform_u32((uint32_t)p.t.tj)};
+        p.from = whole || second ? 0 : share_from;
+        p.to = whole ? k_total : second ? share_to - k_total : min(share_to, k_total);
+        return p;
+    };
 
     // A stage's tiles in LDS: rows of 64 bytes, of P (and a symmetric Q) K along them, 16-byte chunk c of row r at
     // c ^ (r / 4 & 3): the 16 lanes that a fragment read serves at a time (0-3, 12-15, 20-23, 24-27 and so on) then meet
@@ -440,41 +488,80 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
         return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
-    for (int second = 0; from < to; second++) {
-        // (the division leaves its uniform result in vector registers)
-        const int tile = (int)uniform_u32((uint32_t)(from / k_total));
-        const int k_from = (int)uniform_u32((uint32_t)(from - (int64_t)tile * k_total));
-        const int k_to = (int)uniform_u32((uint32_t)min((int64_t)k_total, to - (int64_t)tile * k_total));
-        from += k_to - k_from;
-        const NsTile t = ns_tile<kSym>(g, shares ? g.whole + tile * g.lanes + (id - g.whole) % g.lanes : tile);
-        const _Float16* p = g.p + t.batch * g.p_size + (int64_t)t.ti * Cfg::TM * kPanel;
-        const _Float16* q = g.q + t.batch * g.q_size + (kSym ? (int64_t)t.tj * Cfg::TN * kPanel : (int64_t)t.tj * Cfg::TN * g.pitch);
-        // (from the tile's first element to its last: of P and a symmetric Q over all panels, of step's Q over its own)
-        const int64_t p_room = ((int64_t)(g.k_steps - 1) * g.pitch + Cfg::TM) * kPanel;
-        const int64_t q_room = kSym ? ((int64_t)(g.k_steps - 1) * g.pitch + Cfg::TN) * kPanel : (int64_t)Cfg::TN * g.pitch;
-        const bool low = g.passes > 1;
-        const i32x4 rp = ns_rsrc(p, (uint32_t)((p_room + (low ? g.p_low : 0)) * 2));
-        const i32x4 rq = ns_rsrc(q, (uint32_t)((q_room + (low ? g.q_low : 0)) * 2));
-        // this wave's loads s0 .. s1 - 1 for a step
-        auto load = [&](int step, int stage, int s0, int s1) {
-            const uint32_t at = lds0 + stage * Cfg::STAGE;
-            const int pass = step < g.k_steps ? 0 : step < 2 * g.k_steps ? 1 : 2;       // high high, high low, low high
-            const uint32_t k = (uint32_t)(step - pass * g.k_steps);
-            const uint32_t p_off = k * (uint32_t)g.pitch * 64u + (pass == 2 ? (uint32_t)g.p_low * 2u : 0u);
-            const uint32_t q_off = k * (kSym ? (uint32_t)g.pitch * 64u : 2048u) + (pass == 1 ? (uint32_t)g.q_low * 2u : 0u);
-#pragma unroll
-            for (int s = s0; s < s1; s++) {
-                if (s < Cfg::P_LOADS) {
-                    const int slot = s * Cfg::WAVES + wave;                             // 1 KiB
-                    load_to_lds(rp, at + slot * 1024, voff_rows, p_off + slot * 1024);
-                } else {
-                    const int slot = (s - Cfg::P_LOADS) * Cfg::WAVES + wave;
-                    const uint32_t off = kSym ? slot * 1024u : (slot >> 1) * (uint32_t)g.pitch * 64u + (slot & 1) * 1024u;
-                    load_to_lds(rq, at + Cfg::P_BYTES + slot * 1024, kSym ? voff_rows : voff_cols, q_off + off);
-                }
+    // This wave's loads, step by step: HALF KiB of P, then of Q.  Passes (precise): high high, high low, low high.
+    const uint32_t p_wave = (uint32_t)wave * (Cfg::HALF * 1024u);
+    const uint32_t q_wave = kSym ? p_wave : (uint32_t)(wave * Cfg::HALF >> 1) * (uint32_t)g.pitch * 64u + (uint32_t)(wave * Cfg::HALF & 1) * 1024u;
+    const uint32_t p_step = (uint32_t)g.pitch * 64u, q_step = kSym ? p_step : 2048u;
+    // (what lies between a tile's first element and its last: of P and a symmetric Q over all panels, of step's Q over its own)
+    const bool low = g.passes > 1;
+    const int64_t p_room = ((int64_t)(g.k_steps - 1) * g.pitch + Cfg::TM) * kPanel + (low ? g.p_low : 0);
+    const int64_t q_room = (kSym ? ((int64_t)(g.k_steps - 1) * g.pitch + Cfg::TN) * kPanel : (int64_t)Cfg::TN * g.pitch) + (low ? g.q_low : 0);
+    i32x4 rp, rq;
+    int next_piece = 0, left_in_piece = 0, left_in_pass = 0, pass = 0;
+    uint32_t p_off = 0, q_off = 0, lds_at = lds0 + p_wave;
+    auto start_pass = [&](int k) {
+        left_in_pass = g.k_steps - k;
+        p_off = (uint32_t)k * p_step + p_wave + (pass == 2 ? (uint32_t)g.p_low * 2u : 0u);
+        q_off = (uint32_t)k * q_step + q_wave + (pass == 1 ? (uint32_t)g.q_low * 2u : 0u);
+    };
+    auto start_piece = [&] {
+        const Piece i = piece(next_piece++);
+        const _Float16* p = g.p + i.t.batch * g.p_size + (int64_t)i.t.ti * Cfg::TM * kPanel;
+        const _Float16* q = g.q + i.t.batch * g.q_size + (kSym ? (int64_t)i.t.tj * Cfg::TN * kPanel : (int64_t)i.t.tj * Cfg::TN * g.pitch);
+        rp = ns_rsrc(p, (uint32_t)(p_room * 2));
+        rq = ns_rsrc(q, (uint32_t)(q_room * 2));
+        left_in_piece = i.to - i.from;
+        pass = i.from >= 2 * g.k_steps ? 2 : i.from >= g.k_steps ? 1 : 0;
+        start_pass(i.from - pass * g.k_steps);
+    };
+    auto load_p = [&] { load_to_lds<Cfg::HALF>(rp, lds_at, voff_rows, p_off); };
+    auto load_q = [&] {
+        load_to_lds<Cfg::HALF>(rq, lds_at + Cfg::P_BYTES, kSym ? voff_rows : voff_cols, q_off);
+        lds_at = lds_at == lds0 + p_wave + (Cfg::STAGES - 1) * Cfg::STAGE ? lds0 + p_wave : lds_at + Cfg::STAGE;
+        p_off += p_step;
+        q_off += q_step;
+        left_in_piece--;
+        if (--left_in_pass == 0 || left_in_piece == 0) {
+            if (left_in_piece) {
+                pass++;
+                start_pass(0);
+            } else if (next_piece < pieces) {
+                start_piece();
             }
-        };
+        }
+    };
 
+    // The fragments of a step's first slice are read in the step before, ahead of the barrier between, so that the
+    // products go on through it: a barrier vouches for the stage after the one that begins.
+    f16x8 fp[2][Cfg::IM], fq[2][Cfg::JN];
+    auto read_p = [&](int stage, int s, int i) { fp[s & 1][i] = row_frag(s_mem + stage * Cfg::STAGE, (wm * Cfg::IM + i) * 32, s); };
+    auto read_q = [&](int stage, int s, int j) {
+        const char* t = s_mem + stage * Cfg::STAGE + Cfg::P_BYTES;
+        fq[s & 1][j] = kSym ? row_frag(t, (wn * Cfg::JN + j) * 32, s) : col_frag(t, (wn * Cfg::JN + j) * 32, s);
+    };
+    constexpr int kAhead = Cfg::STAGES - 1, kSlices = kPanel / 16;
+    if (pieces == 0) return;
+    start_piece();
+#pragma unroll
+    for (int s = 0; s < kAhead; s++)
+        if (s < steps) {
+            load_p();
+            load_q();
+        }
+    if (kAhead <= steps)
+        wait_loads<(kAhead - 1) * Cfg::LOADS>();
+    else
+        wait_loads<0>();
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int j = 0; j < Cfg::JN; j++) read_q(0, 0, j);
+#pragma unroll
+    for (int i = 0; i < Cfg::IM; i++) read_p(0, 0, i);
+
+    int stage = 0;
+    int64_t to_load = steps - kAhead;               // steps whose loads are not issued yet (or less than none)
+    for (int n = 0; n < pieces; n++) {
+        const Piece here = piece(n);
         f32x16 acc[Cfg::IM][Cfg::JN];
 #pragma unroll
         for (int i = 0; i < Cfg::IM; i++)
@@ -482,39 +569,15 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
             for (int j = 0; j < Cfg::JN; j++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
-
-        // The fragments of a step's first slice are read in the step before, ahead of the barrier between, so that the
-        // products go on through it: a barrier vouches for the stage after the one that begins.
-        f16x8 fp[2][Cfg::IM], fq[2][Cfg::JN];
-        auto read_p = [&](int stage, int s, int i) { fp[s & 1][i] = row_frag(s_mem + stage * Cfg::STAGE, (wm * Cfg::IM + i) * 32, s); };
-        auto read_q = [&](int stage, int s, int j) {
-            const char* t = s_mem + stage * Cfg::STAGE + Cfg::P_BYTES;
-            fq[s & 1][j] = kSym ? row_frag(t, (wn * Cfg::JN + j) * 32, s) : col_frag(t, (wn * Cfg::JN + j) * 32, s);
-        };
-        constexpr int kAhead = Cfg::STAGES - 1, kSlices = kPanel / 16;
-        if (second) __builtin_amdgcn_s_barrier();       // (the first tile's last reads)
-#pragma unroll
-        for (int s = 0; s < kAhead; s++)
-            if (k_from + s < k_to) load(k_from + s, s, 0, Cfg::LOADS);
-        if (k_from + kAhead <= k_to)
-            wait_loads<(kAhead - 1) * Cfg::LOADS>();
-        else
-            wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-#pragma unroll
-        for (int j = 0; j < Cfg::JN; j++) read_q(0, 0, j);
-#pragma unroll
-        for (int i = 0; i < Cfg::IM; i++) read_p(0, 0, i);
-        int stage = 0;
-        for (int step = k_from; step < k_to; step++) {
-            // the next step's tiles are there and the stage that is loaded now has been read, in every wave
-            if (step + kAhead <= k_to)
+        for (int step = here.from; step < here.to; step++, to_load--) {
+            // The next step's tiles are there, and the stage that is loaded now has been read, in every wave (its last
+            // fragments went into products before this; those under way are of this step's stage).
+            if (to_load >= 0)
                 wait_loads<(kAhead - 2) * Cfg::LOADS>();
             else
                 wait_loads<0>();
             __builtin_amdgcn_s_barrier();
-            const bool more = step + kAhead < k_to;
-            const int into = stage == 0 ? kAhead : stage - 1, next = stage == kAhead ? 0 : stage + 1;
+            const int next = stage == kAhead ? 0 : stage + 1;
 #pragma unroll
             for (int s = 0; s < kSlices; s++) {
                 // Reads, products and loads in turn: eight waves that all read first would wait for one another.
@@ -525,23 +588,24 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
                     if (i == 0) {
 #pragma unroll
                         for (int j = 0; j < Cfg::JN; j++) read_q(from_stage, of, j);
+                        read_p(from_stage, of, 0);
                     }
-                    read_p(from_stage, of, i);
+                    if (i + 1 < Cfg::IM) read_p(from_stage, of, i + 1);
 #pragma unroll
                     for (int j = 0; j < Cfg::JN; j++)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s & 1][j], fp[s & 1][i], acc[i][j], 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
-                    constexpr int kAll = Cfg::IM * kSlices;
-                    const int at = s * Cfg::IM + i;
-                    if (more) load(step + kAhead, into, at * Cfg::LOADS / kAll, (at + 1) * Cfg::LOADS / kAll);
+                    if (to_load > 0 && i == (Cfg::IM - 1) / 2) {
+                        if (s == 0) load_p();
+                        if (s == kSlices - 1) load_q();
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
             stage = next;
         }
-        wait_loads<0>();
-        if (shares) {
-            float* part = ns_part<Cfg>(g, id - g.whole, second);
+        if (n >= wholes) {
+            float* part = ns_part<Cfg>(g, id, n - wholes);
 #pragma unroll
             for (int i = 0; i < Cfg::IM; i++)
 #pragma unroll
@@ -551,13 +615,12 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
                         *reinterpret_cast<f32x4*>(part + ((i * Cfg::JN + j) * 4 + qd) * 256) =
                             f32x4{acc[i][j][4 * qd], acc[i][j][4 * qd + 1], acc[i][j][4 * qd + 2], acc[i][j][4 * qd + 3]};
         } else {
-            __builtin_amdgcn_s_barrier();       // (every wave's reads are done: the LDS is scratch now)
 #pragma unroll
             for (int i = 0; i < Cfg::IM; i++)
 #pragma unroll
                 for (int j = 0; j < Cfg::JN; j++)
-                    ns_finish<KIND>(g, mats, t.batch, t.ti * Cfg::TM + (wm * Cfg::IM + i) * 32, t.tj * Cfg::TN + (wn * Cfg::JN + j) * 32,
-                                    kSym && t.ti != t.tj, acc[i][j], s_mem + wave * 4608);
+                    ns_finish<KIND>(g, mats, here.t.batch, here.t.ti * Cfg::TM + (wm * Cfg::IM + i) * 32,
+                                    here.t.tj * Cfg::TN + (wn * Cfg::JN + j) * 32, kSym && here.t.ti != here.t.tj, acc[i][j], scratch);
         }
     }
 }
@@ -567,7 +630,7 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
 template <class Cfg, int KIND>
 __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsMatrices mats)
 {
-    __shared__ __attribute__((aligned(16))) char s_mem[4 * 4608];
+    __shared__ __attribute__((aligned(16))) char s_mem[4 * kScratch];
     constexpr int kBlocks = Cfg::WAVES * Cfg::IM * Cfg::JN;
     static_assert(kBlocks % 4 == 0, "four blocks of a tile to a workgroup");
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -594,7 +657,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsMatrices mats)
     }
     const NsTile t = ns_tile<KIND == kGram || KIND == kPoly>(g, g.whole + shared);
     ns_finish<KIND>(g, mats, t.batch, t.ti * Cfg::TM + (of_wave / Cfg::WGN * Cfg::IM + i) * 32,
-                    t.tj * Cfg::TN + (of_wave % Cfg::WGN * Cfg::JN + j) * 32, t.ti != t.tj, acc, s_mem + wave * 4608);
+                    t.tj * Cfg::TN + (of_wave % Cfg::WGN * Cfg::JN + j) * 32, t.ti != t.tj, acc, s_mem + wave * kScratch);
 }
 
 // ---------------------------------------------------------------------------
@@ -604,7 +667,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsMatrices mats)
 // workgroup of their own, and its time in microseconds as the choice sees it.
 struct NsProduct {
     int tile;
-    int64_t tiles, whole, sharers, lanes;
+    int64_t tiles, whole, sharers, lanes, groups;
     double time;
 };
 struct NsPlan {
@@ -632,6 +695,7 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
     p.tile = r.tile;
     p.tiles = (sym ? tm * (tm + 1) / 2 : tm * tn) * count;
     p.whole = p.tiles;
+    p.groups = std::min(p.tiles, slots);
     const int64_t rounds = (p.tiles + slots - 1) / slots, rest = p.tiles % slots;
     p.time = 3.0 + r.step * (double)(rounds * steps);
     // A last round that does not fill the chip is dealt out in shares of its steps instead, where the steps saved are
@@ -642,7 +706,7 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
         const int64_t sharers = std::min(slots, rest * steps);      // (slots and rest: multiples of lanes)
         const double bytes = 8.0 * r.tile * r.tile * (double)(sharers + rest);
         const double shared = 3.0 + r.step * (double)((rounds - 1) * steps + (rest * steps + sharers - 1) / sharers) + 5.0 + bytes / 4e6;
-        if (shared < p.time) p.whole = p.tiles - rest, p.sharers = sharers, p.lanes = lanes, p.time = shared;
+        if (shared < p.time) p.whole = p.tiles - rest, p.sharers = sharers, p.lanes = lanes, p.groups = p.whole ? slots : sharers, p.time = shared;
     }
     return p;
 }
@@ -686,7 +750,7 @@ template <class Cfg, int KIND>
 static void ns_launch(NsGemm g, const NsProduct& p, const NsMatrices& mats, hipStream_t st)
 {
     g.tiles = (int)p.tiles, g.whole = (int)p.whole, g.sharers = (int)p.sharers, g.lanes = (int)p.lanes;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_gemm_kernel<Cfg, KIND>), dim3((uint32_t)(p.whole + p.sharers)), dim3(Cfg::THREADS), 0, st, g, mats);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_gemm_kernel<Cfg, KIND>), dim3((uint32_t)p.groups), dim3(Cfg::THREADS), 0, st, g, mats);
     if constexpr (KIND == kGram || KIND == kPoly)
         if (p.sharers)
             hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_join_kernel<Cfg, KIND>), dim3((uint32_t)(p.tiles - p.whole) * (Cfg::WAVES * Cfg::IM * Cfg::JN / 4)), dim3(256), 0, st, g, mats);
@@ -794,7 +858,7 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         // (a last group with fewer matrices: its plan may want more workspace than the full one's, so its tiles have workgroups of their own)
         NsPlan p = full;
         if (here < together) {
-            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = 0; };
+            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = 0, q.groups = std::min(q.tiles, q.groups); };
             fewer(p.gram);
             fewer(p.poly);
             fewer(p.step);
