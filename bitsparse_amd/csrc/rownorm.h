@@ -2,11 +2,11 @@
 // share: how a row lies on the lanes, loads and stores of its 8-element
 // chunks in either type, sums over a row.
 //
-// A row of D elements is D / 8 chunks.  Up to 1024 elements one wave holds a
-// row (one or two chunks a lane) and a workgroup of four waves holds four;
-// above that one workgroup of ceil(D / 512) waves holds one row, a chunk a
-// lane (two or four past 8192).  The whole row then stays in registers
-// between the passes that its statistics take, and it is read once.
+// A row of D elements is D / 8 chunks.  ceil(D / 512) waves hold a row, a
+// chunk a lane, and a workgroup holds as many rows as its eight waves make
+// (longer rows: 16 waves, and two or four chunks a lane).  The whole row then
+// stays in registers between the passes that its statistics take, and it is
+// read once.
 #pragma once
 
 #include "bs_device.h"
@@ -14,7 +14,6 @@
 namespace bs {
 
 constexpr int kMaxRowCols = 32768;
-constexpr int kRowsPerSmallBlock = 4;
 
 typedef __bf16 bf16;
 
@@ -142,26 +141,27 @@ __device__ __forceinline__ float wave_sum_f32(float v)
 template <int C>
 struct RowPlace {
     int waves;              // of a row
+    int sub;                // which of the workgroup's rows
     int wave, lane_in_row;  // this thread's
-    int nv[C];              // elements of its chunks inside the row
+    int in_row[C];          // elements of its chunks inside the row
     int64_t col[C];
     float n_wave;           // elements of the row in this wave
     float inv_cols;
     __device__ __forceinline__ RowPlace(int64_t cols, int waves_)
     {
         waves = waves_;
-        lane_in_row = (int)threadIdx.x % (64 * waves);
-        wave = __builtin_amdgcn_readfirstlane(lane_in_row >> 6);
-        int n = 0;
+        const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        sub = w / waves;
+        wave = w - sub * waves;
+        lane_in_row = wave * 64 + ((int)threadIdx.x & 63);
+        n_wave = n_of(wave, cols);
+        inv_cols = 1.0f / (float)cols;
 #pragma unroll
         for (int k = 0; k < C; k++) {
             const int c = (k * 64 * waves + lane_in_row) * 8;
             col[k] = c;
-            nv[k] = max(0, min(8, (int)cols - c));
-            n += max(0, min(512, (int)cols - (k * waves + wave) * 512));
+            in_row[k] = max(0, min(8, (int)cols - c));
         }
-        n_wave = (float)n;
-        inv_cols = 1.0f / (float)cols;
     }
     // elements of the row in wave i
     __device__ __forceinline__ float n_of(int i, int64_t cols) const
@@ -173,7 +173,7 @@ struct RowPlace {
     }
 };
 
-// LDS for the sums of a row over its waves: two buffers in turn, so that one
+// LDS for the sums of rows over their waves: two buffers in turn, so that one
 // barrier a sum is enough (a thread that writes a buffer again has passed the
 // barrier that came after everybody's reads of it).
 struct RowSums {
@@ -184,7 +184,7 @@ struct RowSums {
 // norm's deviations are from each wave's own mean first; the waves' are joined
 // by n (mean_w - mean)^2, so nothing is lost where the mean is large.
 template <int C>
-__device__ __forceinline__ void row_moments(const float (&v)[C][8], const RowPlace<C>& at, int64_t cols, bool layer,
+__device__ __forceinline__ void row_moments(const float (&v)[C][8], const int (&nv)[C], const RowPlace<C>& at, int64_t cols, bool layer,
                                             RowSums& s, int& turn, float& mean, float& var)
 {
     float mw = 0.f;
@@ -202,20 +202,21 @@ __device__ __forceinline__ void row_moments(const float (&v)[C][8], const RowPla
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float d = v[k][e] - mw;
-            q += e < at.nv[k] ? d * d : 0.f;
+            q += e < nv[k] ? d * d : 0.f;
         }
     q = wave_sum_f32(q);
     if (at.waves > 1) {
-        if ((threadIdx.x & 63) == 0) s.part[turn][at.wave] = float4{mw, q, 0.f, 0.f};
+        const float4* part = s.part[turn] + at.sub * at.waves;
+        if ((threadIdx.x & 63) == 0) s.part[turn][at.sub * at.waves + at.wave] = float4{mw, q, 0.f, 0.f};
         __syncthreads();
         float m = 0.f;
         if (layer) {
-            for (int i = 0; i < at.waves; i++) m += s.part[turn][i].x * at.n_of(i, cols);
+            for (int i = 0; i < at.waves; i++) m += part[i].x * at.n_of(i, cols);
             m *= at.inv_cols;
         }
         q = 0.f;
         for (int i = 0; i < at.waves; i++) {
-            const float4 p = s.part[turn][i];
+            const float4 p = part[i];
             const float d = p.x - m;
             q += layer ? p.y + at.n_of(i, cols) * d * d : p.y;
         }
@@ -233,12 +234,13 @@ __device__ __forceinline__ void row_sums(float (&v)[N], const RowPlace<C>& at, R
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = wave_sum_f32(v[i]);
     if (at.waves > 1) {
+        const float4* part = s.part[turn] + at.sub * at.waves;
         if ((threadIdx.x & 63) == 0)
-            s.part[turn][at.wave] = float4{v[0], N > 1 ? v[N > 1 ? 1 : 0] : 0.f, N > 2 ? v[N > 2 ? 2 : 0] : 0.f, 0.f};
+            s.part[turn][at.sub * at.waves + at.wave] = float4{v[0], N > 1 ? v[N > 1 ? 1 : 0] : 0.f, N > 2 ? v[N > 2 ? 2 : 0] : 0.f, 0.f};
         __syncthreads();
         float t[3] = {0.f, 0.f, 0.f};
         for (int i = 0; i < at.waves; i++) {
-            const float4 p = s.part[turn][i];
+            const float4 p = part[i];
             t[0] += p.x;
             t[1] += p.y;
             t[2] += p.z;
@@ -249,17 +251,18 @@ __device__ __forceinline__ void row_sums(float (&v)[N], const RowPlace<C>& at, R
     }
 }
 
-// Workgroups of a row kernel: waves of a row, rows of a workgroup at a time, threads.
+// Workgroups of a row kernel: chunks of a lane, waves of a row, rows of a
+// workgroup at a time, threads.  `wide`: the longest rows of one chunk a lane.
 struct RowLaunch {
     int chunks, waves, rows, threads;
 };
-inline RowLaunch row_launch(int64_t cols)
+inline RowLaunch row_launch(int64_t cols, int64_t wide)
 {
-    if (cols <= 512) return {1, 1, kRowsPerSmallBlock, 256};
-    if (cols <= 1024) return {2, 1, kRowsPerSmallBlock, 256};
-    const int c = cols <= 8192 ? 1 : cols <= 16384 ? 2 : 4;
+    const int most = wide > 4096 ? 16 : 8;
+    const int c = cols <= wide ? 1 : cols <= 2 * wide ? 2 : 4;
     const int w = (int)((cols + 512 * c - 1) / (512 * c));
-    return {c, w, 1, 64 * w};
+    const int r = w <= most / 2 ? 8 / w > 0 ? 8 / w : 1 : 1;
+    return {c, w, r, 64 * w * r};
 }
 
 }  // namespace bs

@@ -24,6 +24,11 @@
 #include "rownorm.h"
 #include "rownorm_host.h"
 
+#ifndef BS_BWD_THREADS
+#define BS_BWD_THREADS 512
+#define BS_BWD_ROUNDS 4
+#endif
+
 namespace bs {
 
 enum : int { kSumA = 0, kSumB, kSumW2, kSumB2, kSumScale, kColSums };
@@ -44,21 +49,46 @@ struct JoinBwd {
     int one_scale, one_gate;    // gradients of a scale or gate that is one number
     float* part;            // [blocks, sums wanted, cols]
     float* part_one;        // [blocks, 2]
-    int waves;
+    int waves, rows_here;       // of a row, of a workgroup at a time
 };
 
-template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD>
+// JOIN: there is a y.  C chunks a lane; HOLD: the vectors fit the registers; AHEAD: and the next row's loads.
+template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD, bool AHEAD>
 __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
 {
     __shared__ RowSums s_sums;
-    __shared__ float s_join[C <= 2 && MAXT == 256 ? kRowsPerSmallBlock : 1][C <= 2 && MAXT == 256 ? 64 * C * 8 : 1];
+    __shared__ float s_join[C == 1 ? 4096 : 1];         // a sum of every row of the workgroup
     const RowPlace<C> at(a.cols, a.waves);
     int turn = 0;
-    constexpr bool kSmall = MAXT == 256;
-    const int rows_here = kSmall ? kRowsPerSmallBlock : 1;
-    const int sub = kSmall ? (int)threadIdx.x >> 6 : 0;
     const bool per_row = a.gate_per == BS_PER_ROW, per_element = a.gate_per == BS_PER_ELEMENT;
     const bool layer_post = a.post == BS_NORM_LAYER, layer_pre = a.pre == BS_NORM_LAYER;
+
+    // the next row's loads are in flight while this row's sums meet
+    struct Row {
+        Raw<XT> gx[C], x1[C], x[C];
+        Raw<YT> gh[C], y[C];
+        float2 st_pre, st_post;
+    };
+    Row next;
+    auto load = [&](Row& o, int64_t row) {
+        const bool mine = row < a.rows;
+        o.st_pre = a.gh && mine ? *reinterpret_cast<const float2*>(a.stats_pre + 2 * row) : float2{0.f, 1.f};
+        if constexpr (JOIN) o.st_post = a.post && mine ? *reinterpret_cast<const float2*>(a.stats_post + 2 * row) : float2{0.f, 1.f};
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const int nv = mine ? at.in_row[k] : 0, nv_gx = a.gx ? nv : 0, nv_gh = a.gh ? nv : 0;
+            o.gx[k] = load_raw(static_cast<const XT*>(a.gx) + row * a.gx_stride + at.col[k], nv_gx);
+            o.gh[k] = load_raw(static_cast<const YT*>(a.gh) + row * a.gh_stride + at.col[k], nv_gh);
+            o.x1[k] = load_raw(static_cast<const XT*>(a.x1) + row * a.x1_stride + at.col[k], nv_gh);
+            if constexpr (JOIN) {
+                o.y[k] = load_raw(static_cast<const YT*>(a.y) + row * a.y_stride + at.col[k], nv);
+                o.x[k] = load_raw(static_cast<const XT*>(a.x) + row * a.x_stride + at.col[k], a.x ? nv : 0);
+            }
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * a.rows_here;
+    int64_t row = (int64_t)blockIdx.x * a.rows_here + at.sub;
+    load(next, row);
 
     float acc[kColSums][C][8];
 #pragma unroll
@@ -68,11 +98,11 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[i][k][e] = 0.f;
     float sc[C][8], gate[C][8], w1[C][8], w2[C][8];
-    auto vectors_pre = [&](int k) { param_chunk(a.w_pre, at.col[k], at.nv[k], 1.f, w2[k]); };
+    auto vectors_pre = [&](int k) { param_chunk(a.w_pre, at.col[k], at.in_row[k], 1.f, w2[k]); };
     auto vectors_post = [&](int k) {
-        param_chunk(a.scale, at.col[k], at.nv[k], a.scale_value, sc[k]);
-        param_chunk(a.gate, at.col[k], at.nv[k], 1.f, gate[k]);
-        param_chunk(a.w_post, at.col[k], at.nv[k], 1.f, w1[k]);
+        param_chunk(a.scale, at.col[k], at.in_row[k], a.scale_value, sc[k]);
+        param_chunk(a.gate, at.col[k], at.in_row[k], 1.f, gate[k]);
+        param_chunk(a.w_post, at.col[k], at.in_row[k], 1.f, w1[k]);
     };
     if constexpr (HOLD) {
 #pragma unroll
@@ -82,32 +112,27 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
         }
     }
 
-    const int64_t step = (int64_t)gridDim.x * rows_here;
-    for (int64_t row = (int64_t)blockIdx.x * rows_here + sub; row < a.rows; row += step) {
-        Raw<XT> gxr[C], x1r[C], xr[C];
-        Raw<YT> ghr[C], yr[C];
+    // (as many rounds for every row of a workgroup: they meet at barriers)
+    for (int64_t first = (int64_t)blockIdx.x * a.rows_here; first < a.rows; first += step, row += step) {
+        const bool mine = row < a.rows;
+        int nv[C];
 #pragma unroll
-        for (int k = 0; k < C; k++) {
-            const int nv_gx = a.gx ? at.nv[k] : 0, nv_gh = a.gh ? at.nv[k] : 0;
-            gxr[k] = load_raw(static_cast<const XT*>(a.gx) + row * a.gx_stride + at.col[k], nv_gx);
-            ghr[k] = load_raw(static_cast<const YT*>(a.gh) + row * a.gh_stride + at.col[k], nv_gh);
-            x1r[k] = load_raw(static_cast<const XT*>(a.x1) + row * a.x1_stride + at.col[k], nv_gh);
-            if constexpr (JOIN) {
-                yr[k] = load_raw(static_cast<const YT*>(a.y) + row * a.y_stride + at.col[k], a.y ? at.nv[k] : 0);
-                xr[k] = load_raw(static_cast<const XT*>(a.x) + row * a.x_stride + at.col[k], a.x ? at.nv[k] : 0);
-            }
+        for (int k = 0; k < C; k++) nv[k] = mine ? at.in_row[k] : 0;
+        Row now = next;
+        if constexpr (AHEAD) {
+            load(next, row + step);
         }
         float G[C][8];
         if (a.gh) {
-            const float2 st = *reinterpret_cast<const float2*>(a.stats_pre + 2 * row);
+            const float2 st = now.st_pre;
             float dn[C][8], n[C][8], s[2] = {0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < C; k++) {
                 if constexpr (!HOLD) vectors_pre(k);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float gh = raw_get(ghr[k], e);
-                    n[k][e] = (raw_get(x1r[k], e) - st.x) * st.y;
+                    const float gh = raw_get(now.gh[k], e);
+                    n[k][e] = (raw_get(now.x1[k], e) - st.x) * st.y;
                     dn[k][e] = gh * w2[k][e];
                     s[0] += dn[k][e];
                     s[1] += dn[k][e] * n[k][e];
@@ -120,36 +145,36 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
 #pragma unroll
             for (int k = 0; k < C; k++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) G[k][e] = raw_get(gxr[k], e) + st.y * (dn[k][e] - m0 - n[k][e] * m1);
+                for (int e = 0; e < 8; e++) G[k][e] = raw_get(now.gx[k], e) + st.y * (dn[k][e] - m0 - n[k][e] * m1);
         } else {
 #pragma unroll
             for (int k = 0; k < C; k++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) G[k][e] = raw_get(gxr[k], e);
+                for (int e = 0; e < 8; e++) G[k][e] = raw_get(now.gx[k], e);
         }
         if constexpr (!JOIN) {
             if (a.dx)
 #pragma unroll
                 for (int k = 0; k < C; k++)
-                    store_raw(static_cast<XT*>(a.dx) + row * a.cols + at.col[k], to_raw<XT>(G[k]), at.nv[k]);
+                    store_raw(static_cast<XT*>(a.dx) + row * a.cols + at.col[k], to_raw<XT>(G[k]), nv[k]);
         } else {
-            const float2 st = a.post && a.stats_post ? *reinterpret_cast<const float2*>(a.stats_post + 2 * row) : float2{0.f, 1.f};
-            const float rg = per_row ? param_one(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride) : 1.f;
+            const float2 st = now.st_post;
+            const float rg = per_row && mine ? param_one(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride) : 1.f;
             float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < C; k++) {
                 if constexpr (!HOLD) vectors_post(k);
                 float o[8], ge[8], b1[8];
                 if (per_element)
-                    param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], at.nv[k], 0.f, ge);
-                if (a.d_row_gate) param_chunk(a.b_post, at.col[k], at.nv[k], 0.f, b1);
+                    param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, ge);
+                if (a.d_row_gate) param_chunk(a.b_post, at.col[k], nv[k], 0.f, b1);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     // (elements past the row: x' and the gradients are 0 there and so is G but for a layer norm's mean)
-                    const float g0 = e < at.nv[k] ? G[k][e] : 0.f;
+                    const float g0 = e < nv[k] ? G[k][e] : 0.f;
                     o[e] = sc[k][e] * g0;
-                    acc[kSumScale][k][e] += g0 * raw_get(xr[k], e);
-                    const float n = (raw_get(yr[k], e) - st.x) * st.y;
+                    acc[kSumScale][k][e] += g0 * raw_get(now.x[k], e);
+                    const float n = (raw_get(now.y[k], e) - st.x) * st.y;
                     const float gg = per_element ? g0 * ge[e] : rg * g0;    // G of the gate's part that is not a vector
                     acc[kSumA][k][e] += gg * n;
                     acc[kSumB][k][e] += gg;
@@ -162,16 +187,16 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                         s[2] += ge[e];
                     }
                 }
-                if (a.dx) store_raw(static_cast<XT*>(a.dx) + row * a.cols + at.col[k], to_raw<XT>(o), at.nv[k]);
+                if (a.dx) store_raw(static_cast<XT*>(a.dx) + row * a.cols + at.col[k], to_raw<XT>(o), nv[k]);
                 if (a.d_row_gate && per_element) {
                     if (a.row_gate_f32)
-                        store_raw(static_cast<float*>(a.d_row_gate) + row * a.cols + at.col[k], to_raw<float>(ge), at.nv[k]);
+                        store_raw(static_cast<float*>(a.d_row_gate) + row * a.cols + at.col[k], to_raw<float>(ge), nv[k]);
                     else
-                        store_raw(static_cast<bf16*>(a.d_row_gate) + row * a.cols + at.col[k], to_raw<bf16>(ge), at.nv[k]);
+                        store_raw(static_cast<bf16*>(a.d_row_gate) + row * a.cols + at.col[k], to_raw<bf16>(ge), nv[k]);
                 }
             }
             if (a.post || (per_row && a.d_row_gate)) row_sums(s, at, s_sums, turn);
-            if (per_row && a.d_row_gate && at.lane_in_row == 0) param_store(a.d_row_gate, a.row_gate_f32, row, s[2]);
+            if (per_row && a.d_row_gate && mine && at.lane_in_row == 0) param_store(a.d_row_gate, a.row_gate_f32, row, s[2]);
             if (a.dy) {
                 const float m0 = layer_post ? s[0] * at.inv_cols : 0.f, m1 = a.post ? s[1] * at.inv_cols : 0.f;
 #pragma unroll
@@ -179,13 +204,14 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                     float o[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float n = (raw_get(yr[k], e) - st.x) * st.y;
+                        const float n = (raw_get(now.y[k], e) - st.x) * st.y;
                         o[e] = st.y * (G[k][e] - m0 - n * m1);
                     }
-                    store_raw(static_cast<YT*>(a.dy) + row * a.cols + at.col[k], to_raw<YT>(o), at.nv[k]);
+                    store_raw(static_cast<YT*>(a.dy) + row * a.cols + at.col[k], to_raw<YT>(o), nv[k]);
                 }
             }
         }
+        if constexpr (!AHEAD) load(next, row + step);
     }
 
     // one number for all columns: this workgroup's part of its gradient
@@ -194,11 +220,11 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
 #pragma unroll
         for (int k = 0; k < C; k++) {
             float b1[8];
-            param_chunk(a.b_post, at.col[k], at.nv[k], 0.f, b1);
+            param_chunk(a.b_post, at.col[k], at.in_row[k], 0.f, b1);
             if constexpr (!HOLD) vectors_post(k);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                if (e >= at.nv[k]) continue;
+                if (e >= at.in_row[k]) continue;
                 t[0] += acc[kSumScale][k][e];
                 t[1] += w1[k][e] * acc[kSumA][k][e] + b1[e] * acc[kSumB][k][e];
             }
@@ -221,24 +247,21 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
     for (int i = 0; i < kColSums; i++) {
         if (!(a.want >> i & 1)) continue;
         float* out = a.part + ((int64_t)blockIdx.x * n_sums + slot++) * a.cols;
-        if constexpr (kSmall) {
+        if (C == 1 && a.rows_here > 1) {
             // the workgroup's rows into one
             __syncthreads();
+            const int pitch = 512 * a.waves;
 #pragma unroll
-            for (int k = 0; k < C; k++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) s_join[sub][(k * 8 + e) * 64 + at.lane_in_row] = acc[i][k][e];
+            for (int e = 0; e < 8; e++) s_join[at.sub * pitch + e * (pitch / 8) + at.lane_in_row] = acc[i][0][e];
             __syncthreads();
-            for (int c = threadIdx.x; c < a.cols; c += 256) {
-                const int q = (c / 512 * 8 + c % 8) * 64 + c / 8 % 64;
+            for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
                 float t = 0.f;
-#pragma unroll
-                for (int r = 0; r < kRowsPerSmallBlock; r++) t += s_join[r][q];
+                for (int r = 0; r < a.rows_here; r++) t += s_join[r * pitch + c % 8 * (pitch / 8) + c / 8];
                 out[c] = t;
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < C; k++) store_raw(out + at.col[k], to_raw<float>(acc[i][k]), at.nv[k]);
+            for (int k = 0; k < C; k++) store_raw(out + at.col[k], to_raw<float>(acc[i][k]), at.in_row[k]);
         }
     }
 }
@@ -328,29 +351,26 @@ __global__ __launch_bounds__(kFinishThreads) void join_finish_kernel(JoinFinish 
     if (a.d_scale && !a.one_scale) param_store(a.d_scale, a.f32_scale, c, s[kSumScale]);
 }
 
-// Workgroups of the first kernel: all that are resident at once (two of eight
-// waves a CU), and no fewer than four rows to each of a workgroup's row slots,
-// so that the partial sums stay a small part of the bytes moved.
+// Workgroups of the first kernel: all that are resident at once (8 waves a
+// CU), and no fewer than four rounds of rows to each, so that the partial sums
+// stay a small part of the bytes moved.
 static int64_t backward_blocks(int64_t rows, const RowLaunch& l)
 {
-    const int64_t most = 256ll * std::max(1, 1024 / l.threads);
-    return std::max<int64_t>(1, std::min((rows + 4 * l.rows - 1) / (4 * l.rows), most));
+    const int64_t most = 256ll * std::max(1, BS_BWD_THREADS / l.threads);
+    return std::max<int64_t>(1, std::min((rows + BS_BWD_ROUNDS * l.rows - 1) / (BS_BWD_ROUNDS * l.rows), most));
 }
+// Sixteen waves would leave 128 registers a lane, fewer than the sums take: rows past 4096 have two chunks a lane.
+static RowLaunch backward_launch(int64_t cols) { return row_launch(cols, cols <= 16384 ? 4096 : 8192); }
 
 template <typename XT, typename YT, bool JOIN>
 static void launch_backward(const JoinBwd& a, const RowLaunch& l, int64_t blocks, hipStream_t st)
 {
     const dim3 grid((uint32_t)blocks), block(l.threads);
-    if (l.rows > 1) {
-        auto* kernel = l.chunks == 1 ? join_backward_kernel<XT, YT, JOIN, 1, 256, true> : join_backward_kernel<XT, YT, JOIN, 2, 256, true>;
-        hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
-    } else if (l.chunks == 1) {
-        auto* kernel = l.threads <= 512 ? join_backward_kernel<XT, YT, JOIN, 1, 512, true> : join_backward_kernel<XT, YT, JOIN, 1, 1024, true>;
-        hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
-    } else {
-        auto* kernel = l.chunks == 2 ? join_backward_kernel<XT, YT, JOIN, 2, 1024, false> : join_backward_kernel<XT, YT, JOIN, 4, 1024, false>;
-        hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
-    }
+    auto* kernel = l.chunks == 1 ? join_backward_kernel<XT, YT, JOIN, 1, 512, true, true>
+                   : l.chunks == 2 ? join_backward_kernel<XT, YT, JOIN, 2, 512, false, false>
+                   : l.threads <= 512 ? join_backward_kernel<XT, YT, JOIN, 4, 512, false, false>
+                                      : join_backward_kernel<XT, YT, JOIN, 4, 1024, false, false>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
 }
 
 }  // namespace bs
@@ -360,7 +380,7 @@ using namespace bs;
 extern "C" int64_t bs_join_backward_workspace_bytes(int64_t rows, int64_t cols)
 {
     if (rows <= 0 || cols <= 0 || cols > kMaxRowCols) return 0;
-    return backward_blocks(rows, row_launch(cols)) * (kColSums * cols + 2) * 4;
+    return backward_blocks(rows, backward_launch(cols)) * (kColSums * cols + 2) * 4;
 }
 
 extern "C" int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* workspace,
@@ -398,7 +418,7 @@ extern "C" int bs_join_backward(const bs_join* args, const bs_join_grads* grads,
     if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15u))
         return set_error(BS_ERR_INVALID, "%s: workspace too small or misaligned", what);
 
-    const RowLaunch l = row_launch(j.cols);
+    const RowLaunch l = backward_launch(j.cols);
     const int64_t blocks = backward_blocks(j.rows, l);
     JoinBwd a{};
     a.rows = j.rows, a.cols = j.cols;
@@ -423,7 +443,7 @@ extern "C" int bs_join_backward(const bs_join* args, const bs_join_grads* grads,
     if (g.d_scale && !a.one_scale) a.want |= 1 << kSumScale;
     a.part = static_cast<float*>(workspace);
     a.part_one = a.part + blocks * kColSums * j.cols;
-    a.waves = l.waves;
+    a.waves = l.waves, a.rows_here = l.rows;
     const hipStream_t st = (hipStream_t)stream;
     const bool xb = j.x_type == BS_DT_BF16, yb = j.y_type == BS_DT_BF16;
     if (join)

@@ -14,6 +14,10 @@
 #include "rownorm.h"
 #include "rownorm_host.h"
 
+#ifndef BS_FWD_THREADS
+#define BS_FWD_THREADS 1024
+#endif
+
 namespace bs {
 
 struct JoinFwd {
@@ -29,7 +33,7 @@ struct JoinFwd {
     float eps_post, eps_pre;
     float *stats_post, *stats_pre;
     void *x1, *h;
-    int waves;
+    int waves, rows_here;       // of a row, of a workgroup at a time
 };
 
 // JOIN: there is a y.  C chunks a lane; HOLD: the vectors fit the registers.
@@ -39,18 +43,31 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
     __shared__ RowSums s_sums;
     const RowPlace<C> at(a.cols, a.waves);
     int turn = 0;
-    const int rows_here = MAXT == 256 && a.waves == 1 ? kRowsPerSmallBlock : 1;
-    const int sub = rows_here > 1 ? (int)threadIdx.x >> 6 : 0;
     const bool per_row = a.gate_per == BS_PER_ROW, per_element = a.gate_per == BS_PER_ELEMENT;
+
+    const int64_t step = (int64_t)gridDim.x * a.rows_here;
+    int64_t row = (int64_t)blockIdx.x * a.rows_here + at.sub;
+    Raw<XT> xr[C];
+    Raw<YT> yr[C];
+    int nv[C], nv_next[C];
+    auto load = [&](int64_t r) {
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            nv_next[k] = r < a.rows ? at.in_row[k] : 0;
+            xr[k] = load_raw(static_cast<const XT*>(a.x) + r * a.x_stride + at.col[k], nv_next[k]);
+            if constexpr (JOIN) yr[k] = load_raw(static_cast<const YT*>(a.y) + r * a.y_stride + at.col[k], nv_next[k]);
+        }
+    };
+    load(row);
 
     float sc[C][8], gw[C][8], gb[C][8], w2[C][8], b2[C][8];
     auto vectors = [&](int k) {
         if constexpr (JOIN) {
-            param_chunk(a.scale, at.col[k], at.nv[k], a.scale_value, sc[k]);
+            param_chunk(a.scale, at.col[k], at.in_row[k], a.scale_value, sc[k]);
             float g[8];
-            param_chunk(a.gate, at.col[k], at.nv[k], 1.f, g);
-            param_chunk(a.w_post, at.col[k], at.nv[k], 1.f, gw[k]);
-            param_chunk(a.b_post, at.col[k], at.nv[k], 0.f, gb[k]);
+            param_chunk(a.gate, at.col[k], at.in_row[k], 1.f, g);
+            param_chunk(a.w_post, at.col[k], at.in_row[k], 1.f, gw[k]);
+            param_chunk(a.b_post, at.col[k], at.in_row[k], 0.f, gb[k]);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 gw[k][e] *= g[e];
@@ -58,8 +75,8 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
             }
         }
         if (a.pre) {
-            param_chunk(a.w_pre, at.col[k], at.nv[k], 1.f, w2[k]);
-            param_chunk(a.b_pre, at.col[k], at.nv[k], 0.f, b2[k]);
+            param_chunk(a.w_pre, at.col[k], at.in_row[k], 1.f, w2[k]);
+            param_chunk(a.b_pre, at.col[k], at.in_row[k], 0.f, b2[k]);
         }
     };
     if constexpr (HOLD) {
@@ -67,46 +84,37 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
         for (int k = 0; k < C; k++) vectors(k);
     }
 
-    const int64_t step = (int64_t)gridDim.x * rows_here;
-    int64_t row = (int64_t)blockIdx.x * rows_here + sub;
-    Raw<XT> xr[C];
-    Raw<YT> yr[C];
-    auto load = [&](int64_t r) {
-#pragma unroll
-        for (int k = 0; k < C; k++) {
-            xr[k] = load_raw(static_cast<const XT*>(a.x) + r * a.x_stride + at.col[k], at.nv[k]);
-            if constexpr (JOIN) yr[k] = load_raw(static_cast<const YT*>(a.y) + r * a.y_stride + at.col[k], at.nv[k]);
-        }
-    };
-    // (a workgroup of several rows has one wave to a row and no barrier: each leaves by itself)
-    if (row < a.rows) load(row);
-    for (; row < a.rows; row += step) {
+    // (as many rounds for every row of a workgroup: they meet at barriers)
+    for (int64_t first = (int64_t)blockIdx.x * a.rows_here; first < a.rows; first += step, row += step) {
         float v[C][8], y[C][8];
 #pragma unroll
-        for (int k = 0; k < C; k++)
+        for (int k = 0; k < C; k++) {
+            nv[k] = nv_next[k];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 v[k][e] = raw_get(xr[k], e);
                 if constexpr (JOIN) y[k][e] = raw_get(yr[k], e);
             }
-        if (row + step < a.rows) load(row + step);
+        }
+        const bool mine = row < a.rows;
+        load(row + step);
 
         if constexpr (JOIN) {
             float mean = 0.f, rstd = 1.f;
             if (a.post) {
                 float var;
-                row_moments(y, at, a.cols, a.post == BS_NORM_LAYER, s_sums, turn, mean, var);
+                row_moments(y, nv, at, a.cols, a.post == BS_NORM_LAYER, s_sums, turn, mean, var);
                 rstd = 1.0f / sqrtf(var + a.eps_post);
-                if (a.stats_post && at.lane_in_row == 0)
+                if (a.stats_post && mine && at.lane_in_row == 0)
                     *reinterpret_cast<float2*>(a.stats_post + 2 * row) = float2{mean, rstd};
             }
-            const float rg = per_row ? param_one(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride) : 1.f;
+            const float rg = per_row && mine ? param_one(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride) : 1.f;
 #pragma unroll
             for (int k = 0; k < C; k++) {
                 if constexpr (!HOLD) vectors(k);
                 float g[8];
                 if (per_element)
-                    param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], at.nv[k], 0.f, g);
+                    param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, g);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     float p = (y[k][e] - mean) * rstd * gw[k][e] + gb[k][e];
@@ -114,16 +122,16 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                     v[k][e] = sc[k][e] * v[k][e] + rg * p;
                 }
                 const Raw<XT> o = to_raw<XT>(v[k]);
-                store_raw(static_cast<XT*>(a.x1) + row * a.cols + at.col[k], o, at.nv[k]);
+                store_raw(static_cast<XT*>(a.x1) + row * a.cols + at.col[k], o, nv[k]);
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[k][e] = e < at.nv[k] ? raw_get(o, e) : 0.f;   // as stored
+                for (int e = 0; e < 8; e++) v[k][e] = e < nv[k] ? raw_get(o, e) : 0.f;   // as stored
             }
         }
         if (a.pre) {
             float mean, var;
-            row_moments(v, at, a.cols, a.pre == BS_NORM_LAYER, s_sums, turn, mean, var);
+            row_moments(v, nv, at, a.cols, a.pre == BS_NORM_LAYER, s_sums, turn, mean, var);
             const float rstd = 1.0f / sqrtf(var + a.eps_pre);
-            if (a.stats_pre && at.lane_in_row == 0)
+            if (a.stats_pre && mine && at.lane_in_row == 0)
                 *reinterpret_cast<float2*>(a.stats_pre + 2 * row) = float2{mean, rstd};
 #pragma unroll
             for (int k = 0; k < C; k++) {
@@ -131,7 +139,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                 float h[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) h[e] = (v[k][e] - mean) * rstd * w2[k][e] + b2[k][e];
-                store_raw(static_cast<YT*>(a.h) + row * a.cols + at.col[k], to_raw<YT>(h), at.nv[k]);
+                store_raw(static_cast<YT*>(a.h) + row * a.cols + at.col[k], to_raw<YT>(h), nv[k]);
             }
         }
     }
@@ -140,20 +148,13 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
 template <typename XT, typename YT, bool JOIN>
 static int launch_forward(const JoinFwd& a, const RowLaunch& l, hipStream_t st)
 {
-    // as many workgroups as are resident at once (8 waves a SIMD at most), each taking every so manieth row
+    // as many workgroups as are resident at once (about 16 waves a CU), each taking every so manieth row
     const int64_t need = (a.rows + l.rows - 1) / l.rows;
-    const int64_t most = 256ll * std::max(1, 2048 / l.threads);
+    const int64_t most = 256ll * std::max(1, BS_FWD_THREADS / l.threads);
     const dim3 grid((uint32_t)std::min(need, most)), block(l.threads);
-    if (l.rows > 1) {
-        auto* kernel = l.chunks == 1 ? join_forward_kernel<XT, YT, JOIN, 1, 256, true> : join_forward_kernel<XT, YT, JOIN, 2, 256, true>;
-        hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
-    } else if (l.chunks == 1) {
-        auto* kernel = l.threads <= 512 ? join_forward_kernel<XT, YT, JOIN, 1, 512, true> : join_forward_kernel<XT, YT, JOIN, 1, 1024, true>;
-        hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
-    } else {
-        auto* kernel = l.chunks == 2 ? join_forward_kernel<XT, YT, JOIN, 2, 1024, false> : join_forward_kernel<XT, YT, JOIN, 4, 1024, false>;
-        hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
-    }
+    auto* kernel = l.chunks == 1 ? l.threads <= 512 ? join_forward_kernel<XT, YT, JOIN, 1, 512, true> : join_forward_kernel<XT, YT, JOIN, 1, 1024, true>
+                   : l.chunks == 2 ? join_forward_kernel<XT, YT, JOIN, 2, 1024, false> : join_forward_kernel<XT, YT, JOIN, 4, 1024, false>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "bs_join_forward launch: %s", hipGetErrorString(e));
 }
@@ -218,7 +219,7 @@ extern "C" int bs_join_forward(const bs_join* args, void* x1, void* h, void* str
         return set_error(BS_ERR_INVALID, "bs_join_forward: null result");
     if (!aligned_to_type(x1, j.x_type) || !aligned_to_type(h, j.y_type))
         return set_error(BS_ERR_INVALID, "bs_join_forward: result misaligned for its type");
-    const RowLaunch l = row_launch(j.cols);
+    const RowLaunch l = row_launch(j.cols, 8192);
     const bool whole = j.gate_per == BS_PER_TENSOR || j.gate_per == BS_PER_CHANNEL;
     JoinFwd a{};
     a.rows = j.rows, a.cols = j.cols, a.x = j.x, a.y = j.y, a.x_stride = j.x_stride, a.y_stride = j.y_stride;
@@ -229,7 +230,7 @@ extern "C" int bs_join_forward(const bs_join* args, void* x1, void* h, void* str
     a.row_gate = whole ? nullptr : j.gate.data, a.row_gate_f32 = j.gate.type == BS_DT_F32;
     a.gate_per = j.gate_per, a.gate_stride = j.gate_stride, a.scale_value = j.scale_value;
     a.post = j.norm_post, a.pre = j.norm_pre, a.eps_post = j.eps_post, a.eps_pre = j.eps_pre;
-    a.stats_post = j.stats_post, a.stats_pre = j.stats_pre, a.x1 = x1, a.h = h, a.waves = l.waves;
+    a.stats_post = j.stats_post, a.stats_pre = j.stats_pre, a.x1 = x1, a.h = h, a.waves = l.waves, a.rows_here = l.rows;
     const hipStream_t st = (hipStream_t)stream;
     if (j.y == nullptr) {
         if (j.x_type == BS_DT_BF16) return launch_forward<bf16, bf16, false>(a, l, st);
