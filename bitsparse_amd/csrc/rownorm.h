@@ -32,8 +32,10 @@ __device__ __forceinline__ float raw_get(const Raw<T>& r, int e)
         return __uint_as_float(r.w[e]);
 }
 
-// 8 elements at any address that their type allows; those from `nv` on are 0 and not read
-template <typename T>
+// 8 elements at any address that their type allows; those from `nv` on are 0
+// and not read.  WHOLE: nv is 0 or 8 everywhere (rows of a multiple of 8).
+// The last chunk of another row moves as 4, 2 and 1 elements.
+template <bool WHOLE = false, typename T>
 __device__ __forceinline__ Raw<T> load_raw(const T* p, int nv)
 {
     Raw<T> r;
@@ -41,17 +43,37 @@ __device__ __forceinline__ Raw<T> load_raw(const T* p, int nv)
         __builtin_memcpy(&r, p, sizeof(r));
         return r;
     }
-#pragma unroll
-    for (int i = 0; i < (int)(2 * sizeof(T)); i++) r.w[i] = 0;
-    if (nv <= 0) return r;
-#pragma unroll
-    for (int e = 0; e < 7; e++) {
-        if (e >= nv) continue;
-        if constexpr (sizeof(T) == 2)
-            r.w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << (16 * (e & 1));
-        else
-            r.w[e] = __builtin_bit_cast(uint32_t, p[e]);
+    constexpr int W = 2 * (int)sizeof(T);       // words
+    typedef uint32_t half_t __attribute__((ext_vector_type(W / 2), aligned(2)));
+    typedef uint32_t quarter_t __attribute__((ext_vector_type(W / 4), aligned(2)));
+    half_t four = 0;
+    quarter_t two = 0;
+    uint32_t one = 0;
+    if (!WHOLE && nv > 0) {
+        if (nv & 4) {
+            four = *reinterpret_cast<const half_t*>(p);
+            p += 4;
+        }
+        if (nv & 2) {
+            two = *reinterpret_cast<const quarter_t*>(p);
+            p += 2;
+        }
+        if (nv & 1) one = sizeof(T) == 2 ? *reinterpret_cast<const uint16_t*>(p) : *reinterpret_cast<const uint32_t*>(p);
     }
+#pragma unroll
+    for (int i = 0; i < W / 2; i++) r.w[i] = four[i];
+#pragma unroll
+    for (int i = 0; i < W / 4; i++) {           // behind the four, or first
+        r.w[W / 2 + i] = nv & 4 ? two[i] : 0u;
+        r.w[i] = nv & 4 ? r.w[i] : two[i];
+        r.w[W - W / 4 + i] = 0u;
+    }
+    constexpr int S = W / 4;                    // words of two elements
+    const int pairs = nv >> 1;
+    r.w[0] |= pairs == 0 ? one : 0u;
+    r.w[S] |= pairs == 1 ? one : 0u;
+    r.w[2 * S] |= pairs == 2 ? one : 0u;
+    r.w[3 * S] |= pairs == 3 ? one : 0u;
     return r;
 }
 
@@ -69,20 +91,39 @@ __device__ __forceinline__ Raw<T> to_raw(const float (&v)[8])
     return r;
 }
 
-template <typename T>
+template <bool WHOLE = false, typename T>
 __device__ __forceinline__ void store_raw(T* p, const Raw<T>& r, int nv)
 {
     if (nv >= 8) {
         __builtin_memcpy(p, &r, sizeof(r));
         return;
     }
+    if (WHOLE || nv <= 0) return;
+    constexpr int W = 2 * (int)sizeof(T);
+    typedef uint32_t half_t __attribute__((ext_vector_type(W / 2), aligned(2)));
+    typedef uint32_t quarter_t __attribute__((ext_vector_type(W / 4), aligned(2)));
+    half_t four;
+    quarter_t two;
 #pragma unroll
-    for (int e = 0; e < 7; e++) {
-        if (e >= nv) continue;
+    for (int i = 0; i < W / 2; i++) four[i] = r.w[i];
+    // (masks, not selections: those between elements of an array become its address)
+    const uint32_t far = nv & 4 ? ~0u : 0u, mid = nv & 2 ? ~0u : 0u;
+#pragma unroll
+    for (int i = 0; i < W / 4; i++) two[i] = (r.w[W / 2 + i] & far) | (r.w[i] & ~far);
+    const uint32_t one = (((r.w[W - W / 4] & far) | (r.w[W / 4] & ~far)) & mid) | (two[0] & ~mid);
+    if (nv & 4) {
+        *reinterpret_cast<half_t*>(p) = four;
+        p += 4;
+    }
+    if (nv & 2) {
+        *reinterpret_cast<quarter_t*>(p) = two;
+        p += 2;
+    }
+    if (nv & 1) {
         if constexpr (sizeof(T) == 2)
-            reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(r.w[e >> 1] >> (16 * (e & 1)));
+            *reinterpret_cast<uint16_t*>(p) = (uint16_t)one;
         else
-            reinterpret_cast<uint32_t*>(p)[e] = r.w[e];
+            *reinterpret_cast<uint32_t*>(p) = one;
     }
 }
 

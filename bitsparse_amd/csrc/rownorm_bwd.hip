@@ -53,15 +53,19 @@ struct JoinBwd {
 };
 
 // JOIN: there is a y.  C chunks a lane; HOLD: the vectors fit the registers; AHEAD: and the next row's loads.
-template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD, bool AHEAD>
+// WHOLE: rows of a multiple of 8 elements.
+// PLAIN: RMS norms (or none), no gate that differs from row to row, no sums for biases: a third fewer instructions, which
+// two waves a SIMD do not hide behind the loads (16384 x 4096: BS_T1 against BS_T0 us).
+template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD, bool AHEAD, bool PLAIN, bool WHOLE>
 __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
 {
     __shared__ RowSums s_sums;
     __shared__ float s_join[C == 1 ? 4096 : 1];         // a sum of every row of the workgroup
     const RowPlace<C> at(a.cols, a.waves);
     int turn = 0;
-    const bool per_row = a.gate_per == BS_PER_ROW, per_element = a.gate_per == BS_PER_ELEMENT;
-    const bool layer_post = a.post == BS_NORM_LAYER, layer_pre = a.pre == BS_NORM_LAYER;
+    const bool per_row = !PLAIN && a.gate_per == BS_PER_ROW, per_element = !PLAIN && a.gate_per == BS_PER_ELEMENT;
+    const bool layer_post = !PLAIN && a.post == BS_NORM_LAYER, layer_pre = !PLAIN && a.pre == BS_NORM_LAYER;
+    void* const d_row_gate = PLAIN ? nullptr : a.d_row_gate;
 
     // the next row's loads are in flight while this row's sums meet
     struct Row {
@@ -77,12 +81,12 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
 #pragma unroll
         for (int k = 0; k < C; k++) {
             const int nv = mine ? at.in_row[k] : 0, nv_gx = a.gx ? nv : 0, nv_gh = a.gh ? nv : 0;
-            o.gx[k] = load_raw(static_cast<const XT*>(a.gx) + row * a.gx_stride + at.col[k], nv_gx);
-            o.gh[k] = load_raw(static_cast<const YT*>(a.gh) + row * a.gh_stride + at.col[k], nv_gh);
-            o.x1[k] = load_raw(static_cast<const XT*>(a.x1) + row * a.x1_stride + at.col[k], nv_gh);
+            o.gx[k] = load_raw<WHOLE>(static_cast<const XT*>(a.gx) + row * a.gx_stride + at.col[k], nv_gx);
+            o.gh[k] = load_raw<WHOLE>(static_cast<const YT*>(a.gh) + row * a.gh_stride + at.col[k], nv_gh);
+            o.x1[k] = load_raw<WHOLE>(static_cast<const XT*>(a.x1) + row * a.x1_stride + at.col[k], nv_gh);
             if constexpr (JOIN) {
-                o.y[k] = load_raw(static_cast<const YT*>(a.y) + row * a.y_stride + at.col[k], nv);
-                o.x[k] = load_raw(static_cast<const XT*>(a.x) + row * a.x_stride + at.col[k], a.x ? nv : 0);
+                o.y[k] = load_raw<WHOLE>(static_cast<const YT*>(a.y) + row * a.y_stride + at.col[k], nv);
+                o.x[k] = load_raw<WHOLE>(static_cast<const XT*>(a.x) + row * a.x_stride + at.col[k], a.x ? nv : 0);
             }
         }
     };
@@ -97,12 +101,15 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
         for (int k = 0; k < C; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[i][k][e] = 0.f;
-    float sc[C][8], gate[C][8], w1[C][8], w2[C][8];
+    float sc[C][8], gw[C][8], w2[C][8];       // scale, gate * weight_post, weight_pre
     auto vectors_pre = [&](int k) { param_chunk(a.w_pre, at.col[k], at.in_row[k], 1.f, w2[k]); };
     auto vectors_post = [&](int k) {
         param_chunk(a.scale, at.col[k], at.in_row[k], a.scale_value, sc[k]);
-        param_chunk(a.gate, at.col[k], at.in_row[k], 1.f, gate[k]);
-        param_chunk(a.w_post, at.col[k], at.in_row[k], 1.f, w1[k]);
+        float g[8];
+        param_chunk(a.gate, at.col[k], at.in_row[k], 1.f, g);
+        param_chunk(a.w_post, at.col[k], at.in_row[k], 1.f, gw[k]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) gw[k][e] *= g[e];
     };
     if constexpr (HOLD) {
 #pragma unroll
@@ -124,7 +131,7 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
         }
         float G[C][8];
         if (a.gh) {
-            const float2 st = now.st_pre;
+            const float2 st = {PLAIN ? 0.f : now.st_pre.x, now.st_pre.y};
             float dn[C][8], n[C][8], s[2] = {0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < C; k++) {
@@ -134,10 +141,10 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                     const float gh = raw_get(now.gh[k], e);
                     n[k][e] = (raw_get(now.x1[k], e) - st.x) * st.y;
                     dn[k][e] = gh * w2[k][e];
-                    s[0] += dn[k][e];
+                    if (!PLAIN) s[0] += dn[k][e];
                     s[1] += dn[k][e] * n[k][e];
                     acc[kSumW2][k][e] += gh * n[k][e];
-                    acc[kSumB2][k][e] += gh;
+                    if (!PLAIN) acc[kSumB2][k][e] += gh;
                 }
             }
             row_sums(s, at, s_sums, turn);
@@ -156,9 +163,9 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
             if (a.dx)
 #pragma unroll
                 for (int k = 0; k < C; k++)
-                    store_raw(static_cast<XT*>(a.dx) + row * a.cols + at.col[k], to_raw<XT>(G[k]), nv[k]);
+                    store_raw<WHOLE>(static_cast<XT*>(a.dx) + row * a.cols + at.col[k], to_raw<XT>(G[k]), nv[k]);
         } else {
-            const float2 st = now.st_post;
+            const float2 st = {PLAIN ? 0.f : now.st_post.x, now.st_post.y};
             const float rg = per_row && mine ? param_one(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride) : 1.f;
             float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
@@ -167,36 +174,36 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                 float o[8], ge[8], b1[8];
                 if (per_element)
                     param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, ge);
-                if (a.d_row_gate) param_chunk(a.b_post, at.col[k], nv[k], 0.f, b1);
+                if (d_row_gate) param_chunk(a.b_post, at.col[k], nv[k], 0.f, b1);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    // (elements past the row: x' and the gradients are 0 there and so is G but for a layer norm's mean)
-                    const float g0 = e < nv[k] ? G[k][e] : 0.f;
+                    // (past the row's end x' and the gradients are 0, and so is G but for a layer norm's mean)
+                    const float g0 = PLAIN || e < nv[k] ? G[k][e] : 0.f;
                     o[e] = sc[k][e] * g0;
                     acc[kSumScale][k][e] += g0 * raw_get(now.x[k], e);
                     const float n = (raw_get(now.y[k], e) - st.x) * st.y;
-                    const float gg = per_element ? g0 * ge[e] : rg * g0;    // G of the gate's part that is not a vector
+                    const float gg = PLAIN ? g0 : per_element ? g0 * ge[e] : rg * g0;    // G of the gate's part that is not a vector
                     acc[kSumA][k][e] += gg * n;
-                    acc[kSumB][k][e] += gg;
-                    const float dm = gate[k][e] * gg * w1[k][e];
-                    s[0] += dm;
+                    if (!PLAIN) acc[kSumB][k][e] += gg;
+                    const float dm = gg * gw[k][e];
+                    if (!PLAIN) s[0] += dm;
                     s[1] += dm * n;
                     G[k][e] = dm;
-                    if (a.d_row_gate) {
-                        ge[e] = g0 * (n * w1[k][e] + b1[e]);
+                    if (d_row_gate) {
+                        ge[e] = g0 * (n * gw[k][e] + b1[e]);      // (such a gate is no vector: gw is weight_post)
                         s[2] += ge[e];
                     }
                 }
-                if (a.dx) store_raw(static_cast<XT*>(a.dx) + row * a.cols + at.col[k], to_raw<XT>(o), nv[k]);
-                if (a.d_row_gate && per_element) {
+                if (a.dx) store_raw<WHOLE>(static_cast<XT*>(a.dx) + row * a.cols + at.col[k], to_raw<XT>(o), nv[k]);
+                if (d_row_gate && per_element) {
                     if (a.row_gate_f32)
-                        store_raw(static_cast<float*>(a.d_row_gate) + row * a.cols + at.col[k], to_raw<float>(ge), nv[k]);
+                        store_raw<WHOLE>(static_cast<float*>(d_row_gate) + row * a.cols + at.col[k], to_raw<float>(ge), nv[k]);
                     else
-                        store_raw(static_cast<bf16*>(a.d_row_gate) + row * a.cols + at.col[k], to_raw<bf16>(ge), nv[k]);
+                        store_raw<WHOLE>(static_cast<bf16*>(d_row_gate) + row * a.cols + at.col[k], to_raw<bf16>(ge), nv[k]);
                 }
             }
-            if (a.post || (per_row && a.d_row_gate)) row_sums(s, at, s_sums, turn);
-            if (per_row && a.d_row_gate && mine && at.lane_in_row == 0) param_store(a.d_row_gate, a.row_gate_f32, row, s[2]);
+            if (a.post || (per_row && d_row_gate)) row_sums(s, at, s_sums, turn);
+            if (per_row && d_row_gate && mine && at.lane_in_row == 0) param_store(d_row_gate, a.row_gate_f32, row, s[2]);
             if (a.dy) {
                 const float m0 = layer_post ? s[0] * at.inv_cols : 0.f, m1 = a.post ? s[1] * at.inv_cols : 0.f;
 #pragma unroll
@@ -207,7 +214,7 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                         const float n = (raw_get(now.y[k], e) - st.x) * st.y;
                         o[e] = st.y * (G[k][e] - m0 - n * m1);
                     }
-                    store_raw(static_cast<YT*>(a.dy) + row * a.cols + at.col[k], to_raw<YT>(o), nv[k]);
+                    store_raw<WHOLE>(static_cast<YT*>(a.dy) + row * a.cols + at.col[k], to_raw<YT>(o), nv[k]);
                 }
             }
         }
@@ -219,14 +226,14 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
         float t[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < C; k++) {
-            float b1[8];
+            float b1[8], w1[8];
             param_chunk(a.b_post, at.col[k], at.in_row[k], 0.f, b1);
-            if constexpr (!HOLD) vectors_post(k);
+            param_chunk(a.w_post, at.col[k], at.in_row[k], 1.f, w1);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 if (e >= at.in_row[k]) continue;
                 t[0] += acc[kSumScale][k][e];
-                t[1] += w1[k][e] * acc[kSumA][k][e] + b1[e] * acc[kSumB][k][e];
+                t[1] += w1[e] * acc[kSumA][k][e] + b1[e] * acc[kSumB][k][e];
             }
         }
         const int wave = (int)threadIdx.x >> 6, waves = (int)blockDim.x >> 6;
@@ -366,10 +373,17 @@ template <typename XT, typename YT, bool JOIN>
 static void launch_backward(const JoinBwd& a, const RowLaunch& l, int64_t blocks, hipStream_t st)
 {
     const dim3 grid((uint32_t)blocks), block(l.threads);
-    auto* kernel = l.chunks == 1 ? join_backward_kernel<XT, YT, JOIN, 1, 512, true, true>
-                   : l.chunks == 2 ? join_backward_kernel<XT, YT, JOIN, 2, 512, false, false>
-                   : l.threads <= 512 ? join_backward_kernel<XT, YT, JOIN, 4, 512, false, false>
-                                      : join_backward_kernel<XT, YT, JOIN, 4, 1024, false, false>;
+    // (the gradient of a gate that is one number takes the bias's sum where there is a bias)
+    const bool plain = a.post != BS_NORM_LAYER && a.pre != BS_NORM_LAYER && a.gate_per <= BS_PER_CHANNEL &&
+                       !(a.want & (1 << kSumB | 1 << kSumB2)) && !(a.one_gate && a.b_post.p);
+    const bool whole = a.cols % 8 == 0;
+    auto* kernel = l.chunks == 1 ? (plain ? whole ? join_backward_kernel<XT, YT, JOIN, 1, 512, true, true, true, true>
+                                                  : join_backward_kernel<XT, YT, JOIN, 1, 512, true, true, true, false>
+                                          : whole ? join_backward_kernel<XT, YT, JOIN, 1, 512, true, true, false, true>
+                                                  : join_backward_kernel<XT, YT, JOIN, 1, 512, true, true, false, false>)
+                   : l.chunks == 2    ? join_backward_kernel<XT, YT, JOIN, 2, 512, false, false, false, false>
+                   : l.threads <= 512 ? join_backward_kernel<XT, YT, JOIN, 4, 512, false, false, false, false>
+                                      : join_backward_kernel<XT, YT, JOIN, 4, 1024, false, false, false, false>;
     hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
 }
 

@@ -36,8 +36,9 @@ struct JoinFwd {
     int waves, rows_here;       // of a row, of a workgroup at a time
 };
 
-// JOIN: there is a y.  C chunks a lane; HOLD: the vectors fit the registers.
-template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD>
+// JOIN: there is a y.  C chunks a lane; HOLD: the vectors fit the registers;
+// WHOLE: rows of a multiple of 8 elements.
+template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD, bool WHOLE>
 __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
 {
     __shared__ RowSums s_sums;
@@ -54,8 +55,8 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
 #pragma unroll
         for (int k = 0; k < C; k++) {
             nv_next[k] = r < a.rows ? at.in_row[k] : 0;
-            xr[k] = load_raw(static_cast<const XT*>(a.x) + r * a.x_stride + at.col[k], nv_next[k]);
-            if constexpr (JOIN) yr[k] = load_raw(static_cast<const YT*>(a.y) + r * a.y_stride + at.col[k], nv_next[k]);
+            xr[k] = load_raw<WHOLE>(static_cast<const XT*>(a.x) + r * a.x_stride + at.col[k], nv_next[k]);
+            if constexpr (JOIN) yr[k] = load_raw<WHOLE>(static_cast<const YT*>(a.y) + r * a.y_stride + at.col[k], nv_next[k]);
         }
     };
     load(row);
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                     v[k][e] = sc[k][e] * v[k][e] + rg * p;
                 }
                 const Raw<XT> o = to_raw<XT>(v[k]);
-                store_raw(static_cast<XT*>(a.x1) + row * a.cols + at.col[k], o, nv[k]);
+                store_raw<WHOLE>(static_cast<XT*>(a.x1) + row * a.cols + at.col[k], o, nv[k]);
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[k][e] = e < nv[k] ? raw_get(o, e) : 0.f;   // as stored
             }
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                 float h[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) h[e] = (v[k][e] - mean) * rstd * w2[k][e] + b2[k][e];
-                store_raw(static_cast<YT*>(a.h) + row * a.cols + at.col[k], to_raw<YT>(h), nv[k]);
+                store_raw<WHOLE>(static_cast<YT*>(a.h) + row * a.cols + at.col[k], to_raw<YT>(h), nv[k]);
             }
         }
     }
@@ -152,8 +153,12 @@ static int launch_forward(const JoinFwd& a, const RowLaunch& l, hipStream_t st)
     const int64_t need = (a.rows + l.rows - 1) / l.rows;
     const int64_t most = 256ll * std::max(1, BS_FWD_THREADS / l.threads);
     const dim3 grid((uint32_t)std::min(need, most)), block(l.threads);
-    auto* kernel = l.chunks == 1 ? l.threads <= 512 ? join_forward_kernel<XT, YT, JOIN, 1, 512, true> : join_forward_kernel<XT, YT, JOIN, 1, 1024, true>
-                   : l.chunks == 2 ? join_forward_kernel<XT, YT, JOIN, 2, 1024, false> : join_forward_kernel<XT, YT, JOIN, 4, 1024, false>;
+    const bool whole = a.cols % 8 == 0;
+    auto* kernel = l.chunks == 1 ? (l.threads <= 512 ? whole ? join_forward_kernel<XT, YT, JOIN, 1, 512, true, true>
+                                                             : join_forward_kernel<XT, YT, JOIN, 1, 512, true, false>
+                                                     : join_forward_kernel<XT, YT, JOIN, 1, 1024, true, false>)
+                   : l.chunks == 2 ? join_forward_kernel<XT, YT, JOIN, 2, 1024, false, false>
+                                   : join_forward_kernel<XT, YT, JOIN, 4, 1024, false, false>;
     hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "bs_join_forward launch: %s", hipGetErrorString(e));
