@@ -30,6 +30,7 @@
 // (X's columns in step), where rows of 64 bytes out of a row-major matrix cost
 // half of each cache line.
 #include <algorithm>
+#include <type_traits>
 
 #include "bs_device.h"
 #include "bs_host.h"
@@ -51,7 +52,8 @@ constexpr int kNsBatch = 64;            // matrices of a launch
 constexpr int kNsParts = 256;           // most partial sums of squares of a matrix
 constexpr int kNsCus = 256, kNsXcds = 8;
 
-enum : int { kGram = 0, kPoly, kStep, kLast };
+// (constants of a plain type: an unnamed one in a kernel's name differs between its host and device sides)
+constexpr int kGram = 0, kPoly = 1, kStep = 2, kLast = 3;
 
 struct NsMatrix {
     const void* g;
@@ -63,6 +65,11 @@ struct NsMatrix {
 struct NsMatrices {
     NsMatrix at[kNsBatch];
 };
+// what a product's kernel is given of them: 4 KiB that only the last one reads
+struct NsNone {
+};
+template <int KIND>
+using NsGiven = std::conditional_t<KIND == kLast, NsMatrices, NsNone>;
 
 // ---------------------------------------------------------------------------
 // U, its norm and X_0
@@ -245,17 +252,11 @@ struct NsCfg {
     static constexpr int LDS = STAGES * STAGE + WAVES * kScratch;
     static_assert(TM == TN, "square tiles: half of a symmetric product is its lower triangle of tiles");
     static_assert(LDS <= 160 * 1024, "LDS budget");
-    static_assert(P_BYTES / 1024 % WAVES == 0 && (HALF == 1 || HALF == 2), "whole loads for every wave");
+    static_assert(P_BYTES / 1024 % WAVES == 0 && HALF == 2, "whole loads for every wave");
     static_assert(STAGES >= 3, "a stage that is read, the one whose first fragments are read ahead, one that is loaded");
 };
-#ifndef NS_L
-#define NS_L 4
-#define NS_M 4
-#define NS_S 6
-#endif
-using NsLarge = NsCfg<2, 4, 4, 2, NS_L>;       // 256 x 256
-using NsMiddle = NsCfg<2, 2, 2, 2, NS_M>;      // 128 x 128
-using NsSmall = NsCfg<2, 2, 1, 1, NS_S>;       // 64 x 64
+using NsLarge = NsCfg<2, 4, 4, 2, 4>;       // 256 x 256
+using NsMiddle = NsCfg<2, 2, 2, 2, 4>;      // 128 x 128
 
 // N runs of 1 KiB, one behind the other, from `rsrc` at voff + soff (16 bytes a
 // lane) straight into LDS at `lds`
@@ -265,9 +266,14 @@ __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t lds, uint32_t v
     // (one wait state between the write of m0 and its use; the offset counts on both sides)
     if constexpr (N == 1)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
-    else
+    else if constexpr (N == 2)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
                      "buffer_load_dwordx4 %1, %2, %3 offen offset:1024 lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
+                     "buffer_load_dwordx4 %1, %2, %3 offen offset:1024 lds\n\t"
+                     "buffer_load_dwordx4 %1, %2, %3 offen offset:2048 lds\n\t"
+                     "buffer_load_dwordx4 %1, %2, %3 offen offset:3072 lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
 }
 __device__ __forceinline__ i32x4 ns_rsrc(const void* p, uint32_t bytes)
 {
@@ -321,7 +327,7 @@ __device__ __forceinline__ NsTile ns_tile(const NsGemm& g, int tile)
 // `scratch`: kScratch bytes of LDS of this wave's own.  `mirror`: also as the
 // block at (c0, r0) of a symmetric result, turned by transposing reads.
 template <int KIND>
-__device__ __forceinline__ void ns_finish(const NsGemm& g, const NsMatrices& mats, int batch, int r0, int c0, bool mirror,
+__device__ __forceinline__ void ns_finish(const NsGemm& g, const NsGiven<KIND>& mats, int batch, int r0, int c0, bool mirror,
                                           const f32x16& acc, char* scratch)
 {
     const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
@@ -420,12 +426,151 @@ __device__ __forceinline__ float* ns_part(const NsGemm& g, int sharer, int secon
            ((int)threadIdx.x & 63) * 4;
 }
 
+// A stage's tiles in LDS: rows of 64 bytes, of P (and a symmetric Q) K along
+// them, 16-byte chunk c of row r at c ^ (r / 4 & 3): the 16 lanes that a
+// fragment read serves at a time (0-3, 12-15, 20-23, 24-27 and so on) then meet
+// all 64 banks.  Of step's Q panels of 32 columns, K down the rows: 32 lanes of
+// a transposing read take four whole rows.
+__device__ __forceinline__ uint32_t ns_voff_rows(int lane) { return (uint32_t)((lane & ~3) | ((lane & 3) ^ (lane >> 4 & 3))) * 16u; }
+__device__ __forceinline__ f16x8 ns_row_frag(const char* t, int r0, int slice, int lane)
+{
+    const int r = r0 + (lane & 31), c = (2 * slice + (lane >> 5)) ^ (r >> 2 & 3);
+    return *reinterpret_cast<const f16x8*>(t + r * 64 + c * 16);
+}
+// within 16 lanes lane j points at row k0 + j / 4, columns 4 (j % 4) on, and gets column j of four rows
+__device__ __forceinline__ f16x8 ns_col_frag(const char* t, int c0, int slice, int lane)
+{
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const int j = lane & 15, k = 16 * slice + 8 * (lane >> 5) + (j >> 2);
+    const char* at = t + c0 * 64 + k * 64 + ((lane & 16) + 4 * (j & 3)) * 2;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 256));
+    return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Few tiles: 64 x 64 a workgroup, each of its four waves the whole tile over a
+// quarter of K, with loads of its own and no barrier until their sums meet.
+// Such a product is bound by latency: a wave has five steps of loads in flight
+// (with all of a CU's LDS, as much as its share of L2 delivers), and the
+// products take a quarter of the steps one after the other that they take in
+// workgroups that split the tile instead (36 tiles of 256 x 1024: BS_T2 us
+// against 9.9; 136 of 1024 x 2752: BS_T3 against 18).
+constexpr int kFewTile = 64, kFewStages = 5, kFewStage = 2 * kFewTile * kPanel * 2;
+template <int KIND>
+__global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mats)
+{
+    __shared__ __attribute__((aligned(16))) char s_mem[4 * kFewStages * kFewStage];
+    static_assert(sizeof(s_mem) <= 160 * 1024 && 12 * 4096 + 4 * kScratch <= (int)sizeof(s_mem), "LDS budget");
+    constexpr bool kSym = KIND == kGram || KIND == kPoly;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    int id = (int)blockIdx.x;
+    {
+        const int group = id / kNsCus * kNsCus, here = min(kNsCus, (int)gridDim.x - group);
+        if (here == kNsCus) id = group + (id - group) % kNsXcds * (kNsCus / kNsXcds) + (id - group) / kNsXcds;
+    }
+    NsTile t = ns_tile<kSym>(g, id);
+    t = {(int)uniform_u32((uint32_t)t.batch), (int)uniform_u32((uint32_t)t.ti), (int)uniform_u32((uint32_t)t.tj)};
+    const int k_total = g.k_steps * g.passes, from = k_total * wave / 4, to = k_total * (wave + 1) / 4;
+    const _Float16* p = g.p + t.batch * g.p_size + (int64_t)t.ti * kFewTile * kPanel;
+    const _Float16* q = g.q + t.batch * g.q_size + (kSym ? (int64_t)t.tj * kFewTile * kPanel : (int64_t)t.tj * kFewTile * g.pitch);
+    const bool low = g.passes > 1;
+    const int64_t p_room = ((int64_t)(g.k_steps - 1) * g.pitch + kFewTile) * kPanel + (low ? g.p_low : 0);
+    const int64_t q_room = (kSym ? ((int64_t)(g.k_steps - 1) * g.pitch + kFewTile) * kPanel : (int64_t)kFewTile * g.pitch) + (low ? g.q_low : 0);
+    const i32x4 rp = ns_rsrc(p, (uint32_t)(p_room * 2)), rq = ns_rsrc(q, (uint32_t)(q_room * 2));
+    char* const ring = s_mem + wave * (kFewStages * kFewStage);
+    const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem + (uint32_t)wave * (kFewStages * kFewStage);
+    const uint32_t voff_rows = ns_voff_rows(lane), voff_cols = (uint32_t)lane * 16u;
+    auto load = [&](int step, int stage) {
+        const int pass = step < g.k_steps ? 0 : step < 2 * g.k_steps ? 1 : 2;
+        const uint32_t k = (uint32_t)(step - pass * g.k_steps), lds = ring0 + stage * kFewStage;
+        load_to_lds<4>(rp, lds, voff_rows, k * (uint32_t)g.pitch * 64u + (pass == 2 ? (uint32_t)g.p_low * 2u : 0u));
+        const uint32_t q_off = k * (kSym ? (uint32_t)g.pitch * 64u : 2048u) + (pass == 1 ? (uint32_t)g.q_low * 2u : 0u);
+        if constexpr (kSym) {
+            load_to_lds<4>(rq, lds + kFewStage / 2, voff_rows, q_off);
+        } else {
+            load_to_lds<2>(rq, lds + kFewStage / 2, voff_cols, q_off);
+            load_to_lds<2>(rq, lds + kFewStage / 2 + 2048, voff_cols, q_off + (uint32_t)g.pitch * 64u);
+        }
+    };
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+    f16x8 fp[2][2], fq[2][2];           // [slice][block]
+    auto read = [&](int stage) {
+        const char* tp = ring + stage * kFewStage;
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                fp[s][i] = ns_row_frag(tp, 32 * i, s, lane);
+                fq[s][i] = kSym ? ns_row_frag(tp + kFewStage / 2, 32 * i, s, lane) : ns_col_frag(tp + kFewStage / 2, 32 * i, s, lane);
+            }
+    };
+#pragma unroll
+    for (int s = 0; s < kFewStages; s++)
+        if (from + s < to) load(from + s, s);
+    int stage = 0;
+    for (int step = from; step < to; step++) {
+        // this step's tiles are there (eight loads a step; the last steps wait for all)
+        if (step + kFewStages <= to)
+            wait_loads<8 * (kFewStages - 1)>();
+        else
+            wait_loads<0>();
+        read(stage);
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s][j], fp[s][i], acc[i][j], 0, 0, 0);
+        // (the fragments are in registers: the stage may be loaded again)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (step + kFewStages < to) load(step + kFewStages, stage);
+        stage = stage == kFewStages - 1 ? 0 : stage + 1;
+    }
+    // The waves' sums: block w of the tile to wave w, added in the waves' order.
+    wait_all();
+    __syncthreads();
+    f32x4* const meet = reinterpret_cast<f32x4*>(s_mem);      // [block][the other waves][4][64]
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int block = 2 * i + j;
+            if (block == wave) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                meet[((block * 3 + (wave < block ? wave : wave - 1)) * 4 + e) * 64 + lane] =
+                    f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+        }
+    __syncthreads();
+    const f32x16 mine = wave == 0 ? acc[0][0] : wave == 1 ? acc[0][1] : wave == 2 ? acc[1][0] : acc[1][1];
+    f32x16 sum;
+#pragma unroll
+    for (int e = 0; e < 16; e++) sum[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const f32x4 v = w == wave ? f32x4{mine[4 * e], mine[4 * e + 1], mine[4 * e + 2], mine[4 * e + 3]}
+                                      : meet[((wave * 3 + (w < wave ? w : w - 1)) * 4 + e) * 64 + lane];
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum[4 * e + k] += v[k];
+        }
+    ns_finish<KIND>(g, mats, t.batch, t.ti * kFewTile + 32 * (wave >> 1), t.tj * kFewTile + 32 * (wave & 1), kSym && t.ti != t.tj, sum,
+                    s_mem + 12 * 4096 + wave * kScratch);
+}
+
 // Each workgroup goes through whole tiles and then through its share of the
 // others', one unbroken sequence of K steps: the loads run STAGES - 1 steps
 // ahead, over the ends of tiles too, so that only a tile's results interrupt
 // the products.
 template <class Cfg, int KIND>
-__global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatrices mats)
+__global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven<KIND> mats)
 {
     __shared__ __attribute__((aligned(16))) char s_mem[Cfg::LDS];
     constexpr bool kSym = KIND == kGram || KIND == kPoly;
@@ -470,23 +615,7 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
         return p;
     };
 
-    // A stage's tiles in LDS: rows of 64 bytes, of P (and a symmetric Q) K along them, 16-byte chunk c of row r at
-    // c ^ (r / 4 & 3): the 16 lanes that a fragment read serves at a time (0-3, 12-15, 20-23, 24-27 and so on) then meet
-    // all 64 banks.  Of step's Q panels of 32 columns, K down the rows: 32 lanes of a transposing read take four whole rows.
-    const uint32_t voff_rows = (uint32_t)((lane & ~3) | ((lane & 3) ^ (lane >> 4 & 3))) * 16u, voff_cols = (uint32_t)lane * 16u;
-    auto row_frag = [&](const char* t, int r0, int slice) -> f16x8 {
-        const int r = r0 + (lane & 31), c = (2 * slice + (lane >> 5)) ^ (r >> 2 & 3);
-        return *reinterpret_cast<const f16x8*>(t + r * 64 + c * 16);
-    };
-    // within 16 lanes lane j points at row k0 + j / 4, columns 4 (j % 4) on, and gets column j of four rows
-    auto col_frag = [&](const char* t, int c0, int slice) -> f16x8 {
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const int j = lane & 15, k = 16 * slice + 8 * (lane >> 5) + (j >> 2);
-        const char* at = t + c0 * 64 + k * 64 + ((lane & 16) + 4 * (j & 3)) * 2;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 256));
-        return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
+    const uint32_t voff_rows = ns_voff_rows(lane), voff_cols = (uint32_t)lane * 16u;
 
     // This wave's loads, step by step: HALF KiB of P, then of Q.  Passes (precise): high high, high low, low high.
     const uint32_t p_wave = (uint32_t)wave * (Cfg::HALF * 1024u);
@@ -534,10 +663,10 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
     // The fragments of a step's first slice are read in the step before, ahead of the barrier between, so that the
     // products go on through it: a barrier vouches for the stage after the one that begins.
     f16x8 fp[2][Cfg::IM], fq[2][Cfg::JN];
-    auto read_p = [&](int stage, int s, int i) { fp[s & 1][i] = row_frag(s_mem + stage * Cfg::STAGE, (wm * Cfg::IM + i) * 32, s); };
+    auto read_p = [&](int stage, int s, int i) { fp[s & 1][i] = ns_row_frag(s_mem + stage * Cfg::STAGE, (wm * Cfg::IM + i) * 32, s, lane); };
     auto read_q = [&](int stage, int s, int j) {
         const char* t = s_mem + stage * Cfg::STAGE + Cfg::P_BYTES;
-        fq[s & 1][j] = kSym ? row_frag(t, (wn * Cfg::JN + j) * 32, s) : col_frag(t, (wn * Cfg::JN + j) * 32, s);
+        fq[s & 1][j] = kSym ? ns_row_frag(t, (wn * Cfg::JN + j) * 32, s, lane) : ns_col_frag(t, (wn * Cfg::JN + j) * 32, s, lane);
     };
     constexpr int kAhead = Cfg::STAGES - 1, kSlices = kPanel / 16;
     if (pieces == 0) return;
@@ -628,7 +757,7 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsMatri
 // The shared tiles: their sharers' sums added in order, then as a tile with a
 // workgroup of its own.  A wave a block of 32 x 32.
 template <class Cfg, int KIND>
-__global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsMatrices mats)
+__global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsGiven<KIND> mats)
 {
     __shared__ __attribute__((aligned(16))) char s_mem[4 * kScratch];
     constexpr int kBlocks = Cfg::WAVES * Cfg::IM * Cfg::JN;
@@ -680,13 +809,15 @@ struct NsPlan {
     int64_t x_bytes, a_bytes, parts_bytes, share_bytes, total;
 };
 
-// Time of a K step of one workgroup when every CU has its fill of them, and
-// how many a CU holds.
+// What a product takes on tiles of a size, in microseconds: a K step of 32 of
+// a workgroup alone on its CU and of one among `per_cu` of them, and what comes
+// with every round of tiles (first loads, results).
 struct NsTileRate {
     int tile, per_cu;
-    double step;
+    double alone, full, round;
 };
-constexpr NsTileRate kNsRates[] = {{256, 1, 0.88}, {128, 2, 0.58}, {64, 2, 0.23}};
+constexpr NsTileRate kNsRates[] = {{256, 1, 0.85, 0.85, 5.0}, {128, 2, 0.32, 0.70, 3.0}, {kFewTile, 1, 0.075, 0.075, 1.5}};
+constexpr double kNsLaunch = 4.0;
 
 static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, bool sym, int64_t k, int64_t count, int passes)
 {
@@ -695,18 +826,25 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
     p.tile = r.tile;
     p.tiles = (sym ? tm * (tm + 1) / 2 : tm * tn) * count;
     p.whole = p.tiles;
-    p.groups = std::min(p.tiles, slots);
+    p.groups = r.tile == kFewTile ? p.tiles : std::min(p.tiles, slots);
     const int64_t rounds = (p.tiles + slots - 1) / slots, rest = p.tiles % slots;
-    p.time = 3.0 + r.step * (double)(rounds * steps);
+    auto time = [&](int64_t tiles, double k_steps) { return (tiles > kNsCus ? r.full : r.alone) * k_steps + r.round; };
+    p.time = kNsLaunch + (double)(rounds - 1) * time(slots, (double)steps) + time(rounds > 1 ? slots : p.tiles, (double)steps);
     // A last round that does not fill the chip is dealt out in shares of its steps instead, where the steps saved are
-    // worth the sums' way through memory (written and read once at about 4 TB/s) and one more kernel.
-    if (sym && rest > 0) {
+    // worth the sums' way through memory (written and read once at about 4 TB/s, one after the other for a tile) and
+    // one more kernel.
+    if (sym && rest > 0 && r.tile != kFewTile) {
         int64_t lanes = 8;
         while (rest % lanes) lanes /= 2;
-        const int64_t sharers = std::min(slots, rest * steps);      // (slots and rest: multiples of lanes)
-        const double bytes = 8.0 * r.tile * r.tile * (double)(sharers + rest);
-        const double shared = 3.0 + r.step * (double)((rounds - 1) * steps + (rest * steps + sharers - 1) / sharers) + 5.0 + bytes / 4e6;
-        if (shared < p.time) p.whole = p.tiles - rest, p.sharers = sharers, p.lanes = lanes, p.groups = p.whole ? slots : sharers, p.time = shared;
+        for (const int64_t most : {slots, 4 * rest, 2 * rest}) {
+            const int64_t sharers = std::min({slots, rest * steps, most});      // (all multiples of lanes)
+            const double share = (double)(rest * steps) / (double)sharers, parts = (double)sharers / (double)rest + 1.0;
+            const double bytes = 8.0 * r.tile * r.tile * (double)(sharers + rest);
+            const double shared = kNsLaunch + (double)(rounds - 1) * time(slots, (double)steps) + time(sharers, share) + kNsLaunch +
+                                  0.8 * parts + bytes / 4e6;
+            if (shared < p.time)
+                p.whole = p.tiles - rest, p.sharers = sharers, p.lanes = lanes, p.groups = p.whole ? slots : sharers, p.time = shared;
+        }
     }
     return p;
 }
@@ -725,7 +863,7 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
         auto pick = [&](int64_t rows, int64_t cols, bool sym, int64_t k) {
             NsProduct b{};
             for (const NsTileRate& r : kNsRates) {
-                if (r.tile > most.tile) continue;
+                if (r.tile > most.tile) continue;       // (the sizes divide one another)
                 const NsProduct q = ns_product(r, rows, cols, sym, k, count, passes);
                 if (b.tile == 0 || q.time < b.time) b = q;
             }
@@ -746,27 +884,37 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
     return p;
 }
 
-template <class Cfg, int KIND>
-static void ns_launch(NsGemm g, const NsProduct& p, const NsMatrices& mats, hipStream_t st)
+template <int KIND>
+static NsGiven<KIND> ns_given(const NsMatrices& mats)
 {
-    g.tiles = (int)p.tiles, g.whole = (int)p.whole, g.sharers = (int)p.sharers, g.lanes = (int)p.lanes;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_gemm_kernel<Cfg, KIND>), dim3((uint32_t)p.groups), dim3(Cfg::THREADS), 0, st, g, mats);
+    if constexpr (KIND == kLast)
+        return mats;
+    else
+        return {};
+}
+
+template <class Cfg, int KIND>
+static void ns_launch_cfg(const NsGemm& g, const NsProduct& p, const NsMatrices& mats, hipStream_t st)
+{
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_gemm_kernel<Cfg, KIND>), dim3((uint32_t)p.groups), dim3(Cfg::THREADS), 0, st, g, ns_given<KIND>(mats));
     if constexpr (KIND == kGram || KIND == kPoly)
         if (p.sharers)
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_join_kernel<Cfg, KIND>), dim3((uint32_t)(p.tiles - p.whole) * (Cfg::WAVES * Cfg::IM * Cfg::JN / 4)), dim3(256), 0, st, g, mats);
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_join_kernel<Cfg, KIND>), dim3((uint32_t)(p.tiles - p.whole) * (Cfg::WAVES * Cfg::IM * Cfg::JN / 4)),
+                               dim3(256), 0, st, g, ns_given<KIND>(mats));
 }
 
 template <int KIND>
 static void ns_launch(NsGemm g, const NsPlan& plan, const NsProduct& p, const NsMatrices& mats, hipStream_t st)
 {
+    g.tiles = (int)p.tiles, g.whole = (int)p.whole, g.sharers = (int)p.sharers, g.lanes = (int)p.lanes;
     g.tiles_m = (int)(plan.mp / p.tile);
     g.tiles_n = (int)((KIND == kGram || KIND == kPoly ? plan.mp : plan.np) / p.tile);
     if (p.tile == 256)
-        ns_launch<NsLarge, KIND>(g, p, mats, st);
+        ns_launch_cfg<NsLarge, KIND>(g, p, mats, st);
     else if (p.tile == 128)
-        ns_launch<NsMiddle, KIND>(g, p, mats, st);
+        ns_launch_cfg<NsMiddle, KIND>(g, p, mats, st);
     else
-        ns_launch<NsSmall, KIND>(g, p, mats, st);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_few_kernel<KIND>), dim3((uint32_t)p.tiles), dim3(256), 0, st, g, ns_given<KIND>(mats));
 }
 
 struct NsWork {
@@ -858,7 +1006,7 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         // (a last group with fewer matrices: its plan may want more workspace than the full one's, so its tiles have workgroups of their own)
         NsPlan p = full;
         if (here < together) {
-            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = 0, q.groups = std::min(q.tiles, q.groups); };
+            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = 0, q.groups = std::min(q.tiles, q.groups); };       // (a few-tiles product: as many groups as tiles)
             fewer(p.gram);
             fewer(p.poly);
             fewer(p.step);
