@@ -49,7 +49,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr float kHeld = 4096.f;         // fp16 value = true value * kHeld
 constexpr int kPanel = 32;              // columns of a panel; K of a main-loop step
 constexpr int kNsBatch = 64;            // matrices of a launch
-constexpr int kNsParts = 256;           // most partial sums of squares of a matrix
+constexpr int kNsParts = 1024;          // most partial sums of squares of a matrix
 constexpr int kNsCus = 256, kNsXcds = 8;
 
 // (constants of a plain type: an unnamed one in a kernel's name differs between its host and device sides)
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(256) void ns_scale_kernel(NsPrep a, NsMatrices mats
 {
     const NsMatrix t = mats.at[blockIdx.z];
     __shared__ float s_t[64][68];
-    __shared__ double s_q[kNsParts];
+    __shared__ double s_q[256];
     const int64_t i0 = (int64_t)blockIdx.y * 64, j0 = (int64_t)blockIdx.x * 64;
     const int64_t rows = t.tall ? a.n : a.m, cols = t.tall ? a.m : a.n;
     float u[2][8];
@@ -190,9 +190,11 @@ __global__ __launch_bounds__(256) void ns_scale_kernel(NsPrep a, NsMatrices mats
             if (t.tall) s_t[c + e][r] = u[k][e];
         }
     }
-    s_q[threadIdx.x] = (int)threadIdx.x < a.parts ? a.parts_at[(int64_t)blockIdx.z * kNsParts + threadIdx.x] : 0.0;
+    double sq = 0.0;
+    for (int i = threadIdx.x; i < a.parts; i += 256) sq += a.parts_at[(int64_t)blockIdx.z * kNsParts + i];
+    s_q[threadIdx.x] = sq;
     __syncthreads();
-    for (int w = kNsParts / 2; w > 0; w >>= 1) {
+    for (int w = 128; w > 0; w >>= 1) {
         if ((int)threadIdx.x < w) s_q[threadIdx.x] += s_q[threadIdx.x + w];
         __syncthreads();
     }
@@ -322,13 +324,30 @@ __device__ __forceinline__ NsTile ns_tile(const NsGemm& g, int tile)
     return t;
 }
 
+// A's values where poly's results of a block go (p is A).
+struct NsOld {
+    f16x4 high[4], low[4];
+};
+__device__ __forceinline__ NsOld ns_old(const NsGemm& g, int batch, int r0, int c0)
+{
+    const int lane = threadIdx.x & 63;
+    const _Float16* at = g.p + batch * g.p_size + ((int64_t)(c0 / kPanel) * g.pitch + r0 + (lane & 31)) * kPanel + 4 * (lane >> 5);
+    NsOld o = {};
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        o.high[q] = *reinterpret_cast<const f16x4*>(at + 8 * q);
+        if (g.passes > 1) o.low[q] = *reinterpret_cast<const f16x4*>(at + g.p_low + 8 * q);
+    }
+    return o;
+}
+
 // Results of a 32 x 32 block at (r0, c0) of matrix `batch`, whose lane holds
 // row lane % 32, columns 8 q + 4 (lane / 32) + e in register 4 q + e.
 // `scratch`: kScratch bytes of LDS of this wave's own.  `mirror`: also as the
 // block at (c0, r0) of a symmetric result, turned by transposing reads.
 template <int KIND>
 __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsGiven<KIND>& mats, int batch, int r0, int c0, bool mirror,
-                                          const f32x16& acc, char* scratch)
+                                          const f32x16& acc, char* scratch, const NsOld& old)
 {
     const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
     if constexpr (KIND == kLast) {      // the weights, in their own orientation: 8 elements of a row a lane
@@ -371,17 +390,11 @@ __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsGiven<KIND>& 
         f16x4 high[4], low[4];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            const int in = row * kPanel + 8 * q + 4 * half;
-            f16x4 old = {}, old_low = {};
-            if constexpr (KIND == kPoly) {      // p is A
-                old = *reinterpret_cast<const f16x4*>(g.p + batch * g.p_size + at + in);
-                if (precise) old_low = *reinterpret_cast<const f16x4*>(g.p + batch * g.p_size + g.p_low + at + in);
-            }
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 float x = acc[4 * q + e] * ((KIND == kPoly ? g.c : 1.f) / kHeld);
                 if constexpr (KIND == kPoly)
-                    x += g.b * ((float)old[e] + (float)old_low[e]) + (r0 + row == c0 + 8 * q + 4 * half + e ? g.a * kHeld : 0.f);
+                    x += g.b * ((float)old.high[q][e] + (float)old.low[q][e]) + (r0 + row == c0 + 8 * q + 4 * half + e ? g.a * kHeld : 0.f);
                 high[q][e] = (_Float16)x;
                 low[q][e] = (_Float16)(x - (float)high[q][e]);
             }
@@ -499,6 +512,10 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+    // this wave's block of the result; what poly adds to it comes with the first loads
+    const int r0 = t.ti * kFewTile + 32 * (wave >> 1), c0 = t.tj * kFewTile + 32 * (wave & 1);
+    NsOld old;
+    if constexpr (KIND == kPoly) old = ns_old(g, t.batch, r0, c0);
     f16x8 fp[2][2], fq[2][2];           // [slice][block]
     auto read = [&](int stage) {
         const char* tp = ring + stage * kFewStage;
@@ -561,8 +578,7 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
 #pragma unroll
             for (int k = 0; k < 4; k++) sum[4 * e + k] += v[k];
         }
-    ns_finish<KIND>(g, mats, t.batch, t.ti * kFewTile + 32 * (wave >> 1), t.tj * kFewTile + 32 * (wave & 1), kSym && t.ti != t.tj, sum,
-                    s_mem + 12 * 4096 + wave * kScratch);
+    ns_finish<KIND>(g, mats, t.batch, r0, c0, kSym && t.ti != t.tj, sum, s_mem + 12 * 4096 + wave * kScratch, old);
 }
 
 // Each workgroup goes through whole tiles and then through its share of the
@@ -748,8 +764,12 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven
             for (int i = 0; i < Cfg::IM; i++)
 #pragma unroll
                 for (int j = 0; j < Cfg::JN; j++)
-                    ns_finish<KIND>(g, mats, here.t.batch, here.t.ti * Cfg::TM + (wm * Cfg::IM + i) * 32,
-                                    here.t.tj * Cfg::TN + (wn * Cfg::JN + j) * 32, kSym && here.t.ti != here.t.tj, acc[i][j], scratch);
+                {
+                    const int r0 = here.t.ti * Cfg::TM + (wm * Cfg::IM + i) * 32, c0 = here.t.tj * Cfg::TN + (wn * Cfg::JN + j) * 32;
+                    NsOld old;
+                    if constexpr (KIND == kPoly) old = ns_old(g, here.t.batch, r0, c0);
+                    ns_finish<KIND>(g, mats, here.t.batch, r0, c0, kSym && here.t.ti != here.t.tj, acc[i][j], scratch, old);
+                }
         }
     }
 }
@@ -765,6 +785,10 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsGiven<KIND> ma
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int shared = (int)blockIdx.x / (kBlocks / 4), block = (int)blockIdx.x % (kBlocks / 4) * 4 + wave;
     const int of_wave = block / (Cfg::IM * Cfg::JN), i = block % (Cfg::IM * Cfg::JN) / Cfg::JN, j = block % Cfg::JN;
+    const NsTile t = ns_tile<KIND == kGram || KIND == kPoly>(g, g.whole + shared);
+    const int r0 = t.ti * Cfg::TM + (of_wave / Cfg::WGN * Cfg::IM + i) * 32, c0 = t.tj * Cfg::TN + (of_wave % Cfg::WGN * Cfg::JN + j) * 32;
+    NsOld old;
+    if constexpr (KIND == kPoly) old = ns_old(g, t.batch, r0, c0);
     const int64_t k_total = (int64_t)g.k_steps * g.passes, all = (g.tiles - g.whole) / g.lanes * k_total;
     const int64_t from = shared / g.lanes * k_total, to = from + k_total;      // of its lane's steps
     const int sharers = g.sharers / g.lanes;
@@ -784,9 +808,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsGiven<KIND> ma
             for (int e = 0; e < 4; e++) acc[4 * q + e] += v[e];
         }
     }
-    const NsTile t = ns_tile<KIND == kGram || KIND == kPoly>(g, g.whole + shared);
-    ns_finish<KIND>(g, mats, t.batch, t.ti * Cfg::TM + (of_wave / Cfg::WGN * Cfg::IM + i) * 32,
-                    t.tj * Cfg::TN + (of_wave % Cfg::WGN * Cfg::JN + j) * 32, t.ti != t.tj, acc, s_mem + wave * kScratch);
+    ns_finish<KIND>(g, mats, t.batch, r0, c0, t.ti != t.tj, acc, s_mem + wave * kScratch, old);
 }
 
 // ---------------------------------------------------------------------------
@@ -809,14 +831,15 @@ struct NsPlan {
     int64_t x_bytes, a_bytes, parts_bytes, share_bytes, total;
 };
 
-// What a product takes on tiles of a size, in microseconds: a K step of 32 of
-// a workgroup alone on its CU and of one among `per_cu` of them, and what comes
-// with every round of tiles (first loads, results).
+// What a product takes on tiles of a size, in microseconds: a K step of 32 with
+// few workgroups on the chip and with `per_cu` on every CU, and what comes with
+// every round of tiles (first loads, results).  Measured with each size alone on
+// products of 256 x 1024 to 4096 x 16384 and batches of them.
 struct NsTileRate {
     int tile, per_cu;
     double alone, full, round;
 };
-constexpr NsTileRate kNsRates[] = {{256, 1, 0.85, 0.85, 5.0}, {128, 2, 0.32, 0.70, 3.0}, {kFewTile, 1, 0.075, 0.075, 1.5}};
+constexpr NsTileRate kNsRates[] = {{256, 1, 0.6, 0.85, 5.0}, {128, 2, 0.25, 0.70, 3.0}, {kFewTile, 1, 0.08, 0.145, 1.7}};
 constexpr double kNsLaunch = 4.0;
 
 static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, bool sym, int64_t k, int64_t count, int passes)
@@ -828,20 +851,21 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
     p.whole = p.tiles;
     p.groups = r.tile == kFewTile ? p.tiles : std::min(p.tiles, slots);
     const int64_t rounds = (p.tiles + slots - 1) / slots, rest = p.tiles % slots;
-    auto time = [&](int64_t tiles, double k_steps) { return (tiles > kNsCus ? r.full : r.alone) * k_steps + r.round; };
+    auto time = [&](int64_t tiles, double k_steps) {
+        return (r.alone + (r.full - r.alone) * std::min(1.0, (double)tiles / (double)slots)) * k_steps + r.round;
+    };
     p.time = kNsLaunch + (double)(rounds - 1) * time(slots, (double)steps) + time(rounds > 1 ? slots : p.tiles, (double)steps);
     // A last round that does not fill the chip is dealt out in shares of its steps instead, where the steps saved are
-    // worth the sums' way through memory (written and read once at about 4 TB/s, one after the other for a tile) and
-    // one more kernel.
+    // worth the sums' way through memory (at about 4 TB/s, one after the other for a tile) and one more kernel.
     if (sym && rest > 0 && r.tile != kFewTile) {
         int64_t lanes = 8;
         while (rest % lanes) lanes /= 2;
         for (const int64_t most : {slots, 4 * rest, 2 * rest}) {
             const int64_t sharers = std::min({slots, rest * steps, most});      // (all multiples of lanes)
             const double share = (double)(rest * steps) / (double)sharers, parts = (double)sharers / (double)rest + 1.0;
-            const double bytes = 8.0 * r.tile * r.tile * (double)(sharers + rest);
-            const double shared = kNsLaunch + (double)(rounds - 1) * time(slots, (double)steps) + time(sharers, share) + kNsLaunch +
-                                  0.8 * parts + bytes / 4e6;
+            const double bytes = 5.0 * r.tile * r.tile * (double)(sharers + rest);     // read, and a part of the writing
+            const double shared = kNsLaunch + (double)(rounds - 1) * time(slots, (double)steps) + time(sharers, share) + 3.0 +
+                                  0.5 * parts + bytes / 4e6;
             if (shared < p.time)
                 p.whole = p.tiles - rest, p.sharers = sharers, p.lanes = lanes, p.groups = p.whole ? slots : sharers, p.time = shared;
         }
