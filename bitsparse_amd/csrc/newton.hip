@@ -466,8 +466,8 @@ __device__ __forceinline__ f16x8 ns_col_frag(const char* t, int c0, int slice, i
 // Such a product is bound by latency: a wave has five steps of loads in flight
 // (with all of a CU's LDS, as much as its share of L2 delivers), and the
 // products take a quarter of the steps one after the other that they take in
-// workgroups that split the tile instead (36 tiles of 256 x 1024: BS_T2 us
-// against 9.9; 136 of 1024 x 2752: BS_T3 against 18).
+// workgroups that split the tile instead (gram of 256 x 1024, 10 tiles: 7.5 us
+// against 9.9; of 1001 x 2731, 136 tiles: 12.8 against 18.2 with its shares).
 constexpr int kFewTile = 64, kFewStages = 5, kFewStage = 2 * kFewTile * kPanel * 2;
 template <int KIND>
 __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mats)

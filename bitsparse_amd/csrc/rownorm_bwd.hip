@@ -17,17 +17,13 @@
 // written once, a row in registers throughout.  Each workgroup keeps its
 // column sums in registers over all its rows and writes one row of partial
 // sums; the second kernel adds those in order.  No atomics: the same bits at
-// every call.
+// every call.  16384 x 4096 in bf16: 182 us, 5.2 TB/s (a copy reaches 5.15);
+// 8192 x 768, which stays in the last level cache: 23 us, 3.8 TB/s.
 #include <algorithm>
 
 #include "bs_host.h"
 #include "rownorm.h"
 #include "rownorm_host.h"
-
-#ifndef BS_BWD_THREADS
-#define BS_BWD_THREADS 512
-#define BS_BWD_ROUNDS 4
-#endif
 
 namespace bs {
 
@@ -55,7 +51,7 @@ struct JoinBwd {
 // JOIN: there is a y.  C chunks a lane; HOLD: the vectors fit the registers; AHEAD: and the next row's loads.
 // WHOLE: rows of a multiple of 8 elements.
 // PLAIN: RMS norms (or none), no gate that differs from row to row, no sums for biases: a third fewer instructions, which
-// two waves a SIMD do not hide behind the loads (16384 x 4096: BS_T1 against BS_T0 us).
+// two waves a SIMD do not hide behind the loads (16384 x 4096: 182 against 232 us).
 template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD, bool AHEAD, bool PLAIN, bool WHOLE>
 __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
 {
@@ -360,11 +356,13 @@ __global__ __launch_bounds__(kFinishThreads) void join_finish_kernel(JoinFinish 
 
 // Workgroups of the first kernel: all that are resident at once (8 waves a
 // CU), and no fewer than four rounds of rows to each, so that the partial sums
-// stay a small part of the bytes moved.
+// stay a small part of the bytes moved.  Twice as many take 40 us instead of 34
+// at 8192 x 768 and 85 instead of 72 at 3005 x 2501; two or eight rounds as long.
+constexpr int kBwdThreads = 512, kBwdRounds = 4;        // threads of a CU
 static int64_t backward_blocks(int64_t rows, const RowLaunch& l)
 {
-    const int64_t most = 256ll * std::max(1, BS_BWD_THREADS / l.threads);
-    return std::max<int64_t>(1, std::min((rows + BS_BWD_ROUNDS * l.rows - 1) / (BS_BWD_ROUNDS * l.rows), most));
+    const int64_t most = 256ll * std::max(1, kBwdThreads / l.threads);
+    return std::max<int64_t>(1, std::min((rows + kBwdRounds * l.rows - 1) / (kBwdRounds * l.rows), most));
 }
 // Sixteen waves would leave 128 registers a lane, fewer than the sums take: rows past 4096 have two chunks a lane.
 static RowLaunch backward_launch(int64_t cols) { return row_launch(cols, cols <= 16384 ? 4096 : 8192); }
