@@ -42,7 +42,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -287,6 +286,12 @@ __device__ __forceinline__ void wait_loads()
 {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+// (the builtin alone orders no memory access of the compiler's)
+__device__ __forceinline__ void ns_barrier()
+{
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 __device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 struct NsTile {
@@ -324,6 +329,14 @@ __device__ __forceinline__ NsTile ns_tile(const NsGemm& g, int tile)
     return t;
 }
 
+// A block of 32 x 32 results: four 16 x 16 products, q = 2 (row half) + column
+// half, a lane holding row lane % 16, columns 4 (lane / 16) + e of each.
+struct NsBlock {
+    f32x4 q[4];
+};
+__device__ __forceinline__ int ns_row(int q, int lane) { return 16 * (q >> 1) + (lane & 15); }
+__device__ __forceinline__ int ns_col(int q, int lane) { return 16 * (q & 1) + 4 * (lane >> 4); }
+
 // A's values where poly's results of a block go (p is A).
 struct NsOld {
     f16x4 high[4], low[4];
@@ -331,40 +344,39 @@ struct NsOld {
 __device__ __forceinline__ NsOld ns_old(const NsGemm& g, int batch, int r0, int c0)
 {
     const int lane = threadIdx.x & 63;
-    const _Float16* at = g.p + batch * g.p_size + ((int64_t)(c0 / kPanel) * g.pitch + r0 + (lane & 31)) * kPanel + 4 * (lane >> 5);
+    const _Float16* at = g.p + batch * g.p_size + ((int64_t)(c0 / kPanel) * g.pitch + r0) * kPanel;
     NsOld o = {};
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-        o.high[q] = *reinterpret_cast<const f16x4*>(at + 8 * q);
-        if (g.passes > 1) o.low[q] = *reinterpret_cast<const f16x4*>(at + g.p_low + 8 * q);
+        const int in = ns_row(q, lane) * kPanel + ns_col(q, lane);
+        o.high[q] = *reinterpret_cast<const f16x4*>(at + in);
+        if (g.passes > 1) o.low[q] = *reinterpret_cast<const f16x4*>(at + g.p_low + in);
     }
     return o;
 }
 
-// Results of a 32 x 32 block at (r0, c0) of matrix `batch`, whose lane holds
-// row lane % 32, columns 8 q + 4 (lane / 32) + e in register 4 q + e.
-// `scratch`: kScratch bytes of LDS of this wave's own.  `mirror`: also as the
-// block at (c0, r0) of a symmetric result, turned by transposing reads.
+// Results of a block at (r0, c0) of matrix `batch`.  `scratch`: kScratch bytes
+// of LDS of this wave's own.  `mirror`: also as the block at (c0, r0) of a
+// symmetric result, turned by transposing reads.
 template <int KIND>
 __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsGiven<KIND>& mats, int batch, int r0, int c0, bool mirror,
-                                          const f32x16& acc, char* scratch, const NsOld& old)
+                                          const NsBlock& acc, char* scratch, const NsOld& old)
 {
-    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+    const int lane = threadIdx.x & 63;
     if constexpr (KIND == kLast) {      // the weights, in their own orientation: 8 elements of a row a lane
         const NsMatrix mat = mats.at[batch];
         float* s = reinterpret_cast<float*>(scratch);
         const int64_t rows = mat.tall ? g.n : g.m, cols = mat.tall ? g.m : g.n;
 #pragma unroll
         for (int u = 0; u < 2; u++) {   // 16 rows of the block, or (tall) 16 columns
-            if (mat.tall) {             // columns 16 u on: registers 8 u on
 #pragma unroll
-                for (int q = 0; q < 2; q++)
+            for (int v = 0; v < 2; v++) {
+                if (mat.tall) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[(8 * q + 4 * half + e) * 36 + row] = acc[8 * u + 4 * q + e];
-            } else if (row / 16 == u) {
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                    *reinterpret_cast<f32x4*>(s + row % 16 * 36 + 8 * q + 4 * half) = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+                    for (int e = 0; e < 4; e++) s[(4 * (lane >> 4) + e) * 36 + 16 * v + (lane & 15)] = acc.q[2 * v + u][e];
+                } else {
+                    *reinterpret_cast<f32x4*>(s + (lane & 15) * 36 + 16 * v + 4 * (lane >> 4)) = acc.q[2 * u + v];
+                }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             const int64_t wr = (mat.tall ? c0 : r0) + 16 * u + (lane >> 2), wc = (mat.tall ? r0 : c0) + 8 * (lane & 3);
@@ -389,21 +401,23 @@ __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsGiven<KIND>& 
         const bool precise = g.passes > 1;
         f16x4 high[4], low[4];
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
+        for (int q = 0; q < 4; q++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                float x = acc[4 * q + e] * ((KIND == kPoly ? g.c : 1.f) / kHeld);
+                float x = acc.q[q][e] * ((KIND == kPoly ? g.c : 1.f) / kHeld);
                 if constexpr (KIND == kPoly)
-                    x += g.b * ((float)old.high[q][e] + (float)old.low[q][e]) + (r0 + row == c0 + 8 * q + 4 * half + e ? g.a * kHeld : 0.f);
+                    x += g.b * ((float)old.high[q][e] + (float)old.low[q][e]) + (r0 + ns_row(q, lane) == c0 + ns_col(q, lane) + e ? g.a * kHeld : 0.f);
                 high[q][e] = (_Float16)x;
                 low[q][e] = (_Float16)(x - (float)high[q][e]);
             }
-        }
-        // Out as whole rows, 1 KiB a store, through LDS: 16-byte chunk q of row r lies at q ^ (r / 4 & 3).  (Stored from the
+        // Out as whole rows, 1 KiB a store, through LDS: 16-byte chunk c of row r lies at c ^ (r / 4 & 3).  (Stored from the
         // lanes that hold them, 8 bytes of a row each, the results take four times the requests to L2.)
         auto emit = [&](const f16x4 (&v)[4], _Float16* to) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) *reinterpret_cast<f16x4*>(scratch + row * 64 + (q ^ (row >> 2 & 3)) * 16 + 8 * half) = v[q];
+            for (int q = 0; q < 4; q++) {
+                const int r = ns_row(q, lane), c = ns_col(q, lane);
+                *reinterpret_cast<f16x4*>(scratch + r * 64 + (c / 8 ^ (r >> 2 & 3)) * 16 + c % 8 * 2) = v[q];
+            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
             for (int u = 0; u < 2; u++) {
@@ -414,12 +428,12 @@ __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsGiven<KIND>& 
         for (int part = 0; part < (precise ? 2 : 1); part++) {
             _Float16* to = out + (part ? g.out_low : 0);
             emit(part ? low : high, to + at);
-            if (mirror) {       // turned by transposing reads: rows 8 q + 4 half on of this lane's column
+            if (mirror) {       // row by column: a transposing read gives 16 lanes a column each of four rows
                 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
                 f16x4 v[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    const int j = lane & 15, r = 8 * q + 4 * half + (j >> 2), c = (lane & 16) + 4 * (j & 3);
+                    const int j = lane & 15, r = ns_col(q, lane) + (j >> 2), c = 16 * (q >> 1) + 4 * (j & 3);
                     v[q] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                         (lds_s16x4*)(scratch + r * 64 + (c / 8 ^ (r >> 2 & 3)) * 16 + c % 8 * 2)));
                 }
@@ -440,22 +454,26 @@ __device__ __forceinline__ float* ns_part(const NsGemm& g, int sharer, int secon
 }
 
 // A stage's tiles in LDS: rows of 64 bytes, of P (and a symmetric Q) K along
-// them, 16-byte chunk c of row r at c ^ (r / 4 & 3): the 16 lanes that a
-// fragment read serves at a time (0-3, 12-15, 20-23, 24-27 and so on) then meet
-// all 64 banks.  Of step's Q panels of 32 columns, K down the rows: 32 lanes of
-// a transposing read take four whole rows.
-__device__ __forceinline__ uint32_t ns_voff_rows(int lane) { return (uint32_t)((lane & ~3) | ((lane & 3) ^ (lane >> 4 & 3))) * 16u; }
-__device__ __forceinline__ f16x8 ns_row_frag(const char* t, int r0, int slice, int lane)
+// them, the 16-byte chunk c of row r at c ^ t(r / 4 & 3) with t = 0, 2, 3, 1:
+// the 16 lanes that a fragment read serves at a time (0-3, 12-15, 20-23, 24-27
+// and so on) then meet all 64 banks.  Of step's Q panels of 32 columns, K down
+// the rows, the halves of rows 8-15 and 24-31 changed over: 32 lanes of a
+// transposing read take half of eight rows.
+__device__ __forceinline__ int ns_turn(int r) { return 0x78 >> (2 * (r >> 2 & 3)) & 3; }
+__device__ __forceinline__ uint32_t ns_voff_rows(int lane) { return (uint32_t)((lane & ~3) | ((lane & 3) ^ ns_turn(lane >> 2))) * 16u; }
+__device__ __forceinline__ uint32_t ns_voff_cols(int lane) { return (uint32_t)((lane & ~3) | ((lane & 3) ^ 2 * (lane >> 5))) * 16u; }
+// 16 rows from r0 on, 32 of K: a lane has row lane % 16, 8 of K from 8 (lane / 16) on
+__device__ __forceinline__ f16x8 ns_row_frag(const char* t, int r0, int lane)
 {
-    const int r = r0 + (lane & 31), c = (2 * slice + (lane >> 5)) ^ (r >> 2 & 3);
-    return *reinterpret_cast<const f16x8*>(t + r * 64 + c * 16);
+    const int r = r0 + (lane & 15);
+    return *reinterpret_cast<const f16x8*>(t + r * 64 + ((lane >> 4) ^ ns_turn(r)) * 16);
 }
-// within 16 lanes lane j points at row k0 + j / 4, columns 4 (j % 4) on, and gets column j of four rows
-__device__ __forceinline__ f16x8 ns_col_frag(const char* t, int c0, int slice, int lane)
+// the same of 16 columns; within 16 lanes lane j points at row k0 + j / 4, columns 4 (j % 4) on, and gets column j of four rows
+__device__ __forceinline__ f16x8 ns_col_frag(const char* t, int c0, int lane)
 {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const int j = lane & 15, k = 16 * slice + 8 * (lane >> 5) + (j >> 2);
-    const char* at = t + c0 * 64 + k * 64 + ((lane & 16) + 4 * (j & 3)) * 2;
+    const int j = lane & 15, k = 8 * (lane >> 4) + (j >> 2), half = (c0 >> 4 & 1) ^ (lane >> 4 & 1);
+    const char* at = t + (c0 & ~31) * 64 + k * 64 + half * 32 + (j & 3) * 8;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 256));
     return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -492,7 +510,7 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
     const i32x4 rp = ns_rsrc(p, (uint32_t)(p_room * 2)), rq = ns_rsrc(q, (uint32_t)(q_room * 2));
     char* const ring = s_mem + wave * (kFewStages * kFewStage);
     const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem + (uint32_t)wave * (kFewStages * kFewStage);
-    const uint32_t voff_rows = ns_voff_rows(lane), voff_cols = (uint32_t)lane * 16u;
+    const uint32_t voff_rows = ns_voff_rows(lane), voff_cols = ns_voff_cols(lane);
     auto load = [&](int step, int stage) {
         const int pass = step < g.k_steps ? 0 : step < 2 * g.k_steps ? 1 : 2;
         const uint32_t k = (uint32_t)(step - pass * g.k_steps), lds = ring0 + stage * kFewStage;
@@ -505,27 +523,23 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
             load_to_lds<2>(rq, lds + kFewStage / 2 + 2048, voff_cols, q_off + (uint32_t)g.pitch * 64u);
         }
     };
-    f32x16 acc[2][2];
+    f32x4 acc[4][4];
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+        for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     // this wave's block of the result; what poly adds to it comes with the first loads
     const int r0 = t.ti * kFewTile + 32 * (wave >> 1), c0 = t.tj * kFewTile + 32 * (wave & 1);
     NsOld old;
     if constexpr (KIND == kPoly) old = ns_old(g, t.batch, r0, c0);
-    f16x8 fp[2][2], fq[2][2];           // [slice][block]
+    f16x8 fp[4], fq[4];
     auto read = [&](int stage) {
         const char* tp = ring + stage * kFewStage;
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                fp[s][i] = ns_row_frag(tp, 32 * i, s, lane);
-                fq[s][i] = kSym ? ns_row_frag(tp + kFewStage / 2, 32 * i, s, lane) : ns_col_frag(tp + kFewStage / 2, 32 * i, s, lane);
-            }
+        for (int i = 0; i < 4; i++) {
+            fp[i] = ns_row_frag(tp, 16 * i, lane);
+            fq[i] = kSym ? ns_row_frag(tp + kFewStage / 2, 16 * i, lane) : ns_col_frag(tp + kFewStage / 2, 16 * i, lane);
+        }
     };
 #pragma unroll
     for (int s = 0; s < kFewStages; s++)
@@ -539,11 +553,9 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
             wait_loads<0>();
         read(stage);
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s][j], fp[s][i], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < 4; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fq[j], fp[i], acc[i][j], 0, 0, 0);
         // (the fragments are in registers: the stage may be loaded again)
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (step + kFewStages < to) load(step + kFewStages, stage);
@@ -560,24 +572,19 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
             const int block = 2 * i + j;
             if (block == wave) continue;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                meet[((block * 3 + (wave < block ? wave : wave - 1)) * 4 + e) * 64 + lane] =
-                    f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+            for (int q = 0; q < 4; q++)
+                meet[((block * 3 + (wave < block ? wave : wave - 1)) * 4 + q) * 64 + lane] = acc[2 * i + (q >> 1)][2 * j + (q & 1)];
         }
     __syncthreads();
-    const f32x16 mine = wave == 0 ? acc[0][0] : wave == 1 ? acc[0][1] : wave == 2 ? acc[1][0] : acc[1][1];
-    f32x16 sum;
+    NsBlock sum;
 #pragma unroll
-    for (int e = 0; e < 16; e++) sum[e] = 0.f;
+    for (int q = 0; q < 4; q++) {
+        const int a = q >> 1, b = q & 1;
+        const f32x4 mine = wave == 0 ? acc[a][b] : wave == 1 ? acc[a][2 + b] : wave == 2 ? acc[2 + a][b] : acc[2 + a][2 + b];
+        sum.q[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; w++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const f32x4 v = w == wave ? f32x4{mine[4 * e], mine[4 * e + 1], mine[4 * e + 2], mine[4 * e + 3]}
-                                      : meet[((wave * 3 + (w < wave ? w : w - 1)) * 4 + e) * 64 + lane];
-#pragma unroll
-            for (int k = 0; k < 4; k++) sum[4 * e + k] += v[k];
-        }
+        for (int w = 0; w < 4; w++) sum.q[q] += w == wave ? mine : meet[((wave * 3 + (w < wave ? w : w - 1)) * 4 + q) * 64 + lane];
+    }
     ns_finish<KIND>(g, mats, t.batch, r0, c0, kSym && t.ti != t.tj, sum, s_mem + 12 * 4096 + wave * kScratch, old);
 }
 
@@ -631,7 +638,7 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven
         return p;
     };
 
-    const uint32_t voff_rows = ns_voff_rows(lane), voff_cols = (uint32_t)lane * 16u;
+    const uint32_t voff_rows = ns_voff_rows(lane), voff_cols = ns_voff_cols(lane);
 
     // This wave's loads, step by step: HALF KiB of P, then of Q.  Passes (precise): high high, high low, low high.
     const uint32_t p_wave = (uint32_t)wave * (Cfg::HALF * 1024u);
@@ -676,15 +683,19 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven
         }
     };
 
-    // The fragments of a step's first slice are read in the step before, ahead of the barrier between, so that the
-    // products go on through it: a barrier vouches for the stage after the one that begins.
-    f16x8 fp[2][Cfg::IM], fq[2][Cfg::JN];
-    auto read_p = [&](int stage, int s, int i) { fp[s & 1][i] = ns_row_frag(s_mem + stage * Cfg::STAGE, (wm * Cfg::IM + i) * 32, s, lane); };
-    auto read_q = [&](int stage, int s, int j) {
+    // A step's products go over the first half of its columns and then over the second.  A fragment is read again for the
+    // next time as soon as its last product is under way, half a step to a whole one ahead: the next step's rows and first
+    // columns during the second half, ahead of the barrier between the steps, so that the products go on through it.  A
+    // barrier so vouches for the stage after the one that begins.
+    constexpr int NI = 2 * Cfg::IM, NJ = 2 * Cfg::JN;
+    f16x8 fp[NI], fq[NJ];
+    auto read_p = [&](int stage, int i) { fp[i] = ns_row_frag(s_mem + stage * Cfg::STAGE, wm * 32 * Cfg::IM + 16 * i, lane); };
+    auto read_q = [&](int stage, int j) {
         const char* t = s_mem + stage * Cfg::STAGE + Cfg::P_BYTES;
-        fq[s & 1][j] = kSym ? ns_row_frag(t, (wn * Cfg::JN + j) * 32, s, lane) : ns_col_frag(t, (wn * Cfg::JN + j) * 32, s, lane);
+        const int c0 = wn * 32 * Cfg::JN + 16 * j;
+        fq[j] = kSym ? ns_row_frag(t, c0, lane) : ns_col_frag(t, c0, lane);
     };
-    constexpr int kAhead = Cfg::STAGES - 1, kSlices = kPanel / 16;
+    constexpr int kAhead = Cfg::STAGES - 1;
     if (pieces == 0) return;
     start_piece();
 #pragma unroll
@@ -697,23 +708,21 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven
         wait_loads<(kAhead - 1) * Cfg::LOADS>();
     else
         wait_loads<0>();
-    __builtin_amdgcn_s_barrier();
+    ns_barrier();
 #pragma unroll
-    for (int j = 0; j < Cfg::JN; j++) read_q(0, 0, j);
+    for (int j = 0; j < NJ / 2; j++) read_q(0, j);
 #pragma unroll
-    for (int i = 0; i < Cfg::IM; i++) read_p(0, 0, i);
+    for (int i = 0; i < NI; i++) read_p(0, i);
 
     int stage = 0;
     int64_t to_load = steps - kAhead;               // steps whose loads are not issued yet (or less than none)
     for (int n = 0; n < pieces; n++) {
         const Piece here = piece(n);
-        f32x16 acc[Cfg::IM][Cfg::JN];
+        f32x4 acc[NI][NJ];
 #pragma unroll
-        for (int i = 0; i < Cfg::IM; i++)
+        for (int i = 0; i < NI; i++)
 #pragma unroll
-            for (int j = 0; j < Cfg::JN; j++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+            for (int j = 0; j < NJ; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int step = here.from; step < here.to; step++, to_load--) {
             // The next step's tiles are there, and the stage that is loaded now has been read, in every wave (its last
             // fragments went into products before this; those under way are of this step's stage).
@@ -721,32 +730,29 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven
                 wait_loads<(kAhead - 2) * Cfg::LOADS>();
             else
                 wait_loads<0>();
-            __builtin_amdgcn_s_barrier();
+            ns_barrier();
             const int next = stage == kAhead ? 0 : stage + 1;
+            // Reads, products and loads in turn: eight waves that all read first would wait for one another.
+            // (behind the last step the next stage holds what it held: read, not used)
 #pragma unroll
-            for (int s = 0; s < kSlices; s++) {
-                // Reads, products and loads in turn: eight waves that all read first would wait for one another.
-                // (behind the last step the next stage holds what it held: read, not used)
-                const int from_stage = s + 1 < kSlices ? stage : next, of = s + 1 < kSlices ? s + 1 : 0;
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < Cfg::IM; i++) {
-                    if (i == 0) {
+                for (int i = 0; i < NI; i++) {
+                    // first half: the columns of the second; second half: the next step's first columns
+                    if (i < NJ / 2) read_q(h ? next : stage, h ? i : NJ / 2 + i);
 #pragma unroll
-                        for (int j = 0; j < Cfg::JN; j++) read_q(from_stage, of, j);
-                        read_p(from_stage, of, 0);
-                    }
-                    if (i + 1 < Cfg::IM) read_p(from_stage, of, i + 1);
-#pragma unroll
-                    for (int j = 0; j < Cfg::JN; j++)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fq[s & 1][j], fp[s & 1][i], acc[i][j], 0, 0, 0);
+                    for (int j = h * NJ / 2; j < (h + 1) * NJ / 2; j++)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fq[j], fp[i], acc[i][j], 0, 0, 0);
+                    if (h) read_p(next, i);
                     __builtin_amdgcn_sched_barrier(0);
-                    if (to_load > 0 && i == (Cfg::IM - 1) / 2) {
-                        if (s == 0) load_p();
-                        if (s == kSlices - 1) load_q();
+                    if (to_load > 0 && i == NI / 2 - 1) {
+                        if (h)
+                            load_q();
+                        else
+                            load_p();
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            }
             stage = next;
         }
         if (n >= wholes) {
@@ -756,19 +762,18 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven
 #pragma unroll
                 for (int j = 0; j < Cfg::JN; j++)
 #pragma unroll
-                    for (int qd = 0; qd < 4; qd++)
-                        *reinterpret_cast<f32x4*>(part + ((i * Cfg::JN + j) * 4 + qd) * 256) =
-                            f32x4{acc[i][j][4 * qd], acc[i][j][4 * qd + 1], acc[i][j][4 * qd + 2], acc[i][j][4 * qd + 3]};
+                    for (int q = 0; q < 4; q++)
+                        *reinterpret_cast<f32x4*>(part + ((i * Cfg::JN + j) * 4 + q) * 256) = acc[2 * i + (q >> 1)][2 * j + (q & 1)];
         } else {
 #pragma unroll
             for (int i = 0; i < Cfg::IM; i++)
 #pragma unroll
-                for (int j = 0; j < Cfg::JN; j++)
-                {
+                for (int j = 0; j < Cfg::JN; j++) {
                     const int r0 = here.t.ti * Cfg::TM + (wm * Cfg::IM + i) * 32, c0 = here.t.tj * Cfg::TN + (wn * Cfg::JN + j) * 32;
                     NsOld old;
                     if constexpr (KIND == kPoly) old = ns_old(g, here.t.batch, r0, c0);
-                    ns_finish<KIND>(g, mats, here.t.batch, r0, c0, kSym && here.t.ti != here.t.tj, acc[i][j], scratch, old);
+                    ns_finish<KIND>(g, mats, here.t.batch, r0, c0, kSym && here.t.ti != here.t.tj,
+                                    NsBlock{{acc[2 * i][2 * j], acc[2 * i][2 * j + 1], acc[2 * i + 1][2 * j], acc[2 * i + 1][2 * j + 1]}}, scratch, old);
                 }
         }
     }
@@ -794,19 +799,13 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsGiven<KIND> ma
     const int sharers = g.sharers / g.lanes;
     // the sharer of step s is the last w with all w / sharers <= s
     auto sharer = [&](int64_t s) { return (int)(((s + 1) * sharers - 1) / all); };
-    f32x16 acc;
-#pragma unroll
-    for (int e = 0; e < 16; e++) acc[e] = 0.f;
+    NsBlock acc = {};
     const int last = sharer(to - 1);
     for (int w = sharer(from); w <= last; w++) {
         const int second = all * w / sharers < from;            // it began with the tile before
         const float* part = g.part + ((int64_t)(2 * (w * g.lanes + shared % g.lanes) + second) * Cfg::WAVES + of_wave) * (Cfg::IM * Cfg::JN * 1024) + (i * Cfg::JN + j) * 1024 + lane * 4;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(part + q * 256);
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[4 * q + e] += v[e];
-        }
+        for (int q = 0; q < 4; q++) acc.q[q] += *reinterpret_cast<const f32x4*>(part + q * 256);
     }
     ns_finish<KIND>(g, mats, t.batch, r0, c0, t.ti != t.tj, acc, s_mem + wave * kScratch, old);
 }
