@@ -13,9 +13,8 @@
 // A and B are held as fp16 times 2^12: ||X_0|| <= 1 keeps every singular
 // value of the iteration below 1.21 and so every element of X, A and B below
 // 3.5, far inside fp16's range, and elements down to 2^-26 keep all 11 bits.
-// bf16 operands, three bits shorter, measure 1.0-2.0e-2 from the exact
-// result on gradients, fp16 ones 1.0-2.4e-3, less than the 1.7e-3 that
-// rounding the result itself to bf16 costs.
+// On gradients the result is 1.0-2.4e-3 from the exact one so (bf16 operands,
+// three bits shorter: 1.0-2.0e-2), where rounding it to bf16 costs 1.7e-3.
 //
 // Where the result goes into fp32 weights that is not enough: there each of X,
 // A and B is held as two fp16 numbers, the value and what is left of it (22
@@ -25,10 +24,10 @@
 //
 // All buffers are padded with zeros to whole tiles, which the products keep
 // (B's padding only meets X's zero rows), so the main loop has no bounds.  A
-// matrix [R, C] lies as C / 32 panels of R rows (and 32 more, see NsPlan): every tile that a product loads
-// for 32 steps of K is then one run of memory (P's and gram's) or runs of 2 KiB
-// (X's columns in step), where rows of 64 bytes out of a row-major matrix cost
-// half of each cache line.
+// matrix [R, C] lies as C / 32 panels of R rows: every tile that a product
+// loads for a step of 32 of K is then one run of memory (P's and gram's) or
+// runs of 2 KiB (X's columns in step), where rows of 64 bytes out of a row-major
+// matrix cost half of each cache line (4096 x 16384: gram 318 us instead of 355).
 #include <algorithm>
 #include <type_traits>
 
@@ -41,7 +40,6 @@ namespace bs {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -249,11 +247,11 @@ struct NsCfg {
     static constexpr int TM = 32 * IM * WGM, TN = 32 * JN * WGN;
     static constexpr int P_BYTES = TM * kPanel * 2, Q_BYTES = TN * kPanel * 2;
     static constexpr int STAGE = P_BYTES + Q_BYTES;
-    static constexpr int HALF = P_BYTES / 1024 / WAVES, LOADS = 2 * HALF;       // of a wave for a stage: of P, of both
+    static constexpr int LOADS = 4;                             // of a wave for a stage: 2 KiB of P, 2 of Q
     static constexpr int LDS = STAGES * STAGE + WAVES * kScratch;
     static_assert(TM == TN, "square tiles: half of a symmetric product is its lower triangle of tiles");
     static_assert(LDS <= 160 * 1024, "LDS budget");
-    static_assert(P_BYTES / 1024 % WAVES == 0 && HALF == 2, "whole loads for every wave");
+    static_assert(P_BYTES == WAVES * 2048, "a stage is one pair of loads of P and one of Q of every wave");
     static_assert(STAGES >= 3, "a stage that is read, the one whose first fragments are read ahead, one that is loaded");
 };
 using NsLarge = NsCfg<2, 4, 4, 2, 4>;       // 256 x 256
@@ -265,9 +263,8 @@ template <int N>
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t lds, uint32_t voff, uint32_t soff)
 {
     // (one wait state between the write of m0 and its use; the offset counts on both sides)
-    if constexpr (N == 1)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
-    else if constexpr (N == 2)
+    static_assert(N == 2 || N == 4, "pairs of runs");
+    if constexpr (N == 2)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
                      "buffer_load_dwordx4 %1, %2, %3 offen offset:1024 lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
     else
@@ -591,7 +588,10 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
 // Each workgroup goes through whole tiles and then through its share of the
 // others', one unbroken sequence of K steps: the loads run STAGES - 1 steps
 // ahead, over the ends of tiles too, so that only a tile's results interrupt
-// the products.
+// the products.  Bound by power: with random values the chip runs these
+// products at about 1.8 GHz, with zeros at 2.3, and the matrix pipes are busy
+// for 63 to 65% of the cycles; step of 4096 x 16384 takes 490 us, 1.12
+// PFLOP/s (the library's product of that shape 505 us).
 template <class Cfg, int KIND>
 __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven<KIND> mats)
 {
@@ -640,9 +640,9 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven
 
     const uint32_t voff_rows = ns_voff_rows(lane), voff_cols = ns_voff_cols(lane);
 
-    // This wave's loads, step by step: HALF KiB of P, then of Q.  Passes (precise): high high, high low, low high.
-    const uint32_t p_wave = (uint32_t)wave * (Cfg::HALF * 1024u);
-    const uint32_t q_wave = kSym ? p_wave : (uint32_t)(wave * Cfg::HALF >> 1) * (uint32_t)g.pitch * 64u + (uint32_t)(wave * Cfg::HALF & 1) * 1024u;
+    // This wave's loads, step by step: 2 KiB of P, then of Q (of step's, a panel).  Passes (precise): high high, high low, low high.
+    const uint32_t p_wave = (uint32_t)wave * 2048u;
+    const uint32_t q_wave = kSym ? p_wave : (uint32_t)wave * (uint32_t)g.pitch * 64u;
     const uint32_t p_step = (uint32_t)g.pitch * 64u, q_step = kSym ? p_step : 2048u;
     // (what lies between a tile's first element and its last: of P and a symmetric Q over all panels, of step's Q over its own)
     const bool low = g.passes > 1;
@@ -666,9 +666,9 @@ __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven
         pass = i.from >= 2 * g.k_steps ? 2 : i.from >= g.k_steps ? 1 : 0;
         start_pass(i.from - pass * g.k_steps);
     };
-    auto load_p = [&] { load_to_lds<Cfg::HALF>(rp, lds_at, voff_rows, p_off); };
+    auto load_p = [&] { load_to_lds<2>(rp, lds_at, voff_rows, p_off); };
     auto load_q = [&] {
-        load_to_lds<Cfg::HALF>(rq, lds_at + Cfg::P_BYTES, kSym ? voff_rows : voff_cols, q_off);
+        load_to_lds<2>(rq, lds_at + Cfg::P_BYTES, kSym ? voff_rows : voff_cols, q_off);
         lds_at = lds_at == lds0 + p_wave + (Cfg::STAGES - 1) * Cfg::STAGE ? lds0 + p_wave : lds_at + Cfg::STAGE;
         p_off += p_step;
         q_off += q_step;
@@ -790,7 +790,8 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsGiven<KIND> ma
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int shared = (int)blockIdx.x / (kBlocks / 4), block = (int)blockIdx.x % (kBlocks / 4) * 4 + wave;
     const int of_wave = block / (Cfg::IM * Cfg::JN), i = block % (Cfg::IM * Cfg::JN) / Cfg::JN, j = block % Cfg::JN;
-    const NsTile t = ns_tile<KIND == kGram || KIND == kPoly>(g, g.whole + shared);
+    constexpr bool kSym = KIND == kGram || KIND == kPoly;
+    const NsTile t = ns_tile<kSym>(g, g.whole + shared);
     const int r0 = t.ti * Cfg::TM + (of_wave / Cfg::WGN * Cfg::IM + i) * 32, c0 = t.tj * Cfg::TN + (of_wave % Cfg::WGN * Cfg::JN + j) * 32;
     NsOld old;
     if constexpr (KIND == kPoly) old = ns_old(g, t.batch, r0, c0);
@@ -807,7 +808,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsGiven<KIND> ma
 #pragma unroll
         for (int q = 0; q < 4; q++) acc.q[q] += *reinterpret_cast<const f32x4*>(part + q * 256);
     }
-    ns_finish<KIND>(g, mats, t.batch, r0, c0, t.ti != t.tj, acc, s_mem + wave * kScratch, old);
+    ns_finish<KIND>(g, mats, t.batch, r0, c0, kSym && t.ti != t.tj, acc, s_mem + wave * kScratch, old);
 }
 
 // ---------------------------------------------------------------------------
@@ -855,8 +856,9 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
     };
     p.time = kNsLaunch + (double)(rounds - 1) * time(slots, (double)steps) + time(rounds > 1 ? slots : p.tiles, (double)steps);
     // A last round that does not fill the chip is dealt out in shares of its steps instead, where the steps saved are
-    // worth the sums' way through memory (at about 4 TB/s, one after the other for a tile) and one more kernel.
-    if (sym && rest > 0 && r.tile != kFewTile) {
+    // worth the sums' way through memory (at about 4 TB/s, one after the other for a tile) and one more kernel (step of
+    // two matrices of 2048 x 5500 in 22 bits, 352 tiles for 256 CUs: 340 us in two rounds, 251 + 19 with shares).
+    if (rest > 0 && r.tile != kFewTile) {
         int64_t lanes = 8;
         while (rest % lanes) lanes /= 2;
         for (const int64_t most : {slots, 4 * rest, 2 * rest}) {
@@ -902,7 +904,7 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
     p.x_bytes = p.size(p.np) * 2 * count * (precise ? 2 : 1);
     p.a_bytes = p.size(p.mp) * 2 * count * (precise ? 2 : 1);
     p.parts_bytes = (kNsParts * 8 * count + 255) / 256 * 256;
-    for (const NsProduct& q : {p.gram, p.poly}) p.share_bytes = std::max(p.share_bytes, q.sharers * 2 * q.tile * q.tile * 4);
+    for (const NsProduct& q : {p.gram, p.poly, p.step}) p.share_bytes = std::max(p.share_bytes, q.sharers * 2 * q.tile * q.tile * 4);
     p.total = 2 * p.x_bytes + 2 * p.a_bytes + p.parts_bytes + p.share_bytes;
     return p;
 }
@@ -920,10 +922,9 @@ template <class Cfg, int KIND>
 static void ns_launch_cfg(const NsGemm& g, const NsProduct& p, const NsMatrices& mats, hipStream_t st)
 {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_gemm_kernel<Cfg, KIND>), dim3((uint32_t)p.groups), dim3(Cfg::THREADS), 0, st, g, ns_given<KIND>(mats));
-    if constexpr (KIND == kGram || KIND == kPoly)
-        if (p.sharers)
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_join_kernel<Cfg, KIND>), dim3((uint32_t)(p.tiles - p.whole) * (Cfg::WAVES * Cfg::IM * Cfg::JN / 4)),
-                               dim3(256), 0, st, g, ns_given<KIND>(mats));
+    if (p.sharers)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_join_kernel<Cfg, KIND>), dim3((uint32_t)(p.tiles - p.whole) * (Cfg::WAVES * Cfg::IM * Cfg::JN / 4)),
+                           dim3(256), 0, st, g, ns_given<KIND>(mats));
 }
 
 template <int KIND>
