@@ -214,6 +214,17 @@ struct RowPlace {
     }
 };
 
+// 1 / sqrt(v) within about half a unit of the last place: one Newton step on
+// the instruction's value, whose residual 1 - v r^2 is exact to its last bit
+// by fused products (the correctly rounded root and division cost more and
+// round twice).  0 and infinity have no residual and keep inf and 0.
+__device__ __forceinline__ float row_rstd(float v)
+{
+    const float r = rsqrtf(v), h = v * r;
+    const float e = fmaf(-h, r, 1.f) - fmaf(v, r, -h) * r;
+    return fabsf(e) < 0.5f ? fmaf(0.5f * r, e, r) : r;
+}
+
 // LDS for the sums of rows over their waves: two buffers in turn, so that one
 // barrier a sum is enough (a thread that writes a buffer again has passed the
 // barrier that came after everybody's reads of it).

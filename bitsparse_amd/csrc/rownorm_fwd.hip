@@ -102,7 +102,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
             if (a.post) {
                 float var;
                 row_moments(y, nv, at, a.cols, a.post == BS_NORM_LAYER, s_sums, turn, mean, var);
-                rstd = 1.0f / sqrtf(var + a.eps_post);
+                rstd = row_rstd(var + a.eps_post);
                 if (a.stats_post && mine && at.lane_in_row == 0)
                     *reinterpret_cast<float2*>(a.stats_post + 2 * row) = float2{mean, rstd};
             }
@@ -115,9 +115,11 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                     param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, g);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    float p = (y[k][e] - mean) * rstd * gw[k][e] + gb[k][e];
-                    if (per_element) p *= g[e];
-                    v[k][e] = sc[k][e] * v[k][e] + rg * p;
+                    // (rstd last: with RMS norms of 16-bit x, y and vectors every product before is exact, and the
+                    // sum the only rounding in 32 bits)
+                    const float gate = per_element ? g[e] : rg;
+                    const float t = (y[k][e] - mean) * gw[k][e] * gate;
+                    v[k][e] = fmaf(t, rstd, fmaf(sc[k][e], v[k][e], gb[k][e] * gate));
                 }
                 const Raw<XT> o = to_raw<XT>(v[k]);
                 store_raw<WHOLE>(static_cast<XT*>(a.x1) + row * a.cols + at.col[k], o, nv[k]);
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
         if (a.pre) {
             float mean, var;
             row_moments(v, nv, at, a.cols, a.pre == BS_NORM_LAYER, s_sums, turn, mean, var);
-            const float rstd = 1.0f / sqrtf(var + a.eps_pre);
+            const float rstd = row_rstd(var + a.eps_pre);
             if (a.stats_pre && mine && at.lane_in_row == 0)
                 *reinterpret_cast<float2*>(a.stats_pre + 2 * row) = float2{mean, rstd};
 #pragma unroll
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                 if constexpr (!HOLD) vectors(k);
                 float h[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) h[e] = (v[k][e] - mean) * rstd * w2[k][e] + b2[k][e];
+                for (int e = 0; e < 8; e++) h[e] = fmaf((v[k][e] - mean) * w2[k][e], rstd, b2[k][e]);
                 store_raw<WHOLE>(static_cast<YT*>(a.h) + row * a.cols + at.col[k], to_raw<YT>(h), nv[k]);
             }
         }
