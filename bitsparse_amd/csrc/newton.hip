@@ -12,7 +12,7 @@
 // The products run on the matrix cores with fp16 operands and fp32 sums.  X,
 // A and B are held as fp16 times 2^12: ||X_0|| <= 1 keeps every singular
 // value of the iteration below 1.21 and so every element of X, A and B below
-// 3.5, far inside fp16's range, and elements down to 2^-26 keep all 11 bits.
+// 3.5 (other coefficients: refused where they leave fp16's range), and elements down to 2^-26 keep all 11 bits.
 // On gradients the result is 1.0-2.4e-3 from the exact one so (bf16 operands,
 // three bits shorter: 1.0-2.0e-2), where rounding it to bf16 costs 1.7e-3.
 //
@@ -29,6 +29,7 @@
 // runs of 2 KiB (X's columns in step), where rows of 64 bytes out of a row-major
 // matrix cost half of each cache line (4096 x 16384: gram 318 us instead of 355).
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "bs_device.h"
@@ -590,8 +591,9 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
 // ahead, over the ends of tiles too, so that only a tile's results interrupt
 // the products.  Bound by power: with random values the chip runs these
 // products at about 1.8 GHz, with zeros at 2.3, and the matrix pipes are busy
-// for 63 to 65% of the cycles; step of 4096 x 16384 takes 490 us, 1.12
-// PFLOP/s (the library's product of that shape 505 us).
+// for 63 to 65% of the cycles; step of 4096 x 16384 takes 420 us with a
+// gradient's values and 490 with normal ones, 1.1 to 1.3 PFLOP/s (the library's
+// product of that shape 505 us with normal ones).
 template <class Cfg, int KIND>
 __global__ __launch_bounds__(Cfg::THREADS) void ns_gemm_kernel(NsGemm g, NsGiven<KIND> mats)
 {
@@ -980,6 +982,29 @@ static int64_t ns_together(int64_t m, int64_t n, int64_t count, bool precise)
     return most;
 }
 
+// Whether all X but the last, and all A and B, stay where fp16 holds them.  Their elements are no larger than their
+// largest singular values: from s <= 1 on, q(s^2) of B and s q(s^2) of the next X with q(t) = a + b t + c t^2, whose
+// extremes lie at the ends or where a derivative is 0.
+static bool ns_in_range(double a, double b, double c, int steps)
+{
+    constexpr double kMost = 15.0;      // (65504 / kHeld = 15.99, less the products' own errors)
+    if (!std::isfinite(a + b + c)) return false;
+    double s = 1.0;
+    for (int k = 0; k < steps; k++) {
+        const double end = s * s, root = std::sqrt(std::max(0.0, 9.0 * b * b - 20.0 * a * c));
+        double most_b = 0.0, most_x = 0.0;
+        for (double t : {0.0, end, -b / (2.0 * c), (-3.0 * b + root) / (10.0 * c), (-3.0 * b - root) / (10.0 * c), -a / (3.0 * b)}) {
+            if (!(t >= 0.0 && t <= end)) continue;      // (nor where a divisor is 0)
+            const double q = std::fabs(a + b * t + c * t * t);
+            most_b = std::max(most_b, q);
+            most_x = std::max(most_x, std::sqrt(t) * q);
+        }
+        if (end > kMost || most_b > kMost || (k + 1 < steps && most_x > kMost)) return false;
+        s = most_x;
+    }
+    return true;
+}
+
 }  // namespace bs
 
 using namespace bs;
@@ -1003,6 +1028,8 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
     if (m * n >= (int64_t(1) << 29)) return set_error(BS_ERR_INVALID, "%s: rows*cols must be < 2^29", what);
     const bs_newton_schulz_rule& r = *rule;
     if (r.steps < 1 || r.steps > 100) return set_error(BS_ERR_INVALID, "%s: steps must be in 1..100, got %d", what, r.steps);
+    if (!ns_in_range(r.a, r.b, r.c, r.steps))
+        return set_error(BS_ERR_INVALID, "%s: the coefficients %g, %g, %g take values past 15, out of the operands' range", what, r.a, r.b, r.c);
     auto known = [](int t) { return t == BS_DT_BF16 || t == BS_DT_F32; };
     if (!known(r.grad_type) || !known(r.out_type) || (r.momentum && !known(r.momentum_type)))
         return set_error(BS_ERR_INVALID, "%s: dtypes must be bf16 or fp32", what);

@@ -36,7 +36,8 @@ def orthogonalize(G: Tensor, *, steps: int = 5, coefficients: tuple[float, float
     """The orthogonalised matrices of G [..., R, C] (bfloat16 or float32, up to
     65536 rows and columns and fewer than 2^29 elements each), in bfloat16, contiguous.
 
-    ``precise``: products of 22-bit operands (see above).  No gradient flows
+    ``precise``: products of 22-bit operands (see above).  Coefficients that
+    could take X, A or B past 15 raise ValueError.  No gradient flows
     through it (an optimiser's operator)."""
     a, b, c = coefficients
     with torch.no_grad():

@@ -113,6 +113,18 @@ def test_newton_schulz_refusals(kw, word):
     _refused(_schulz(**kw), word)
 
 
+@pytest.mark.parametrize("a,b,c,steps,ok", [
+    (3.4445, -4.7750, 2.0315, 100, True), (1.5, -0.5, 0.0, 100, True), (2.0, -1.5, 0.5, 5, True),
+    (3.0, 0.0, 0.0, 2, True), (3.0, 0.0, 0.0, 3, False),            # X of 1, 3 and 9, A of 1, 9 and 81
+    (4.5, 0.0, 0.0, 1, True), (4.5, 0.0, 0.0, 2, False),            # the last X is no operand; A of 1 and 20.25
+    (14.9, 0.0, 0.0, 1, True), (15.1, 0.0, 0.0, 1, False), (-15.1, 0.0, 0.0, 1, False), (0.0, 0.0, 16.0, 1, False),
+    (0.0, 70.0, -70.0, 1, False),                                   # B is largest inside the range, 17.5 at t = 0.5
+    (float("nan"), 0.0, 0.0, 1, False), (0.0, float("inf"), 0.0, 1, False)])
+def test_newton_schulz_range(a, b, c, steps, ok):
+    """Coefficients whose operands fp16 does not hold; what is held gets as far as the workspace."""
+    _refused(_schulz(rule=dict(a=a, b=b, c=c, steps=steps), ws=None), "workspace" if ok else "range")
+
+
 def test_newton_schulz_workspace():
     L = _lib.load()
     assert _schulz(count=0) == _lib.BS_OK
