@@ -5,6 +5,7 @@
 //   A_k     = X_k X_k^T                        gram      m^2 n   operations (half of a symmetric product)
 //   B_k     = a I + b A_k + c A_k^2            poly      m^3
 //   X_{k+1} = B_k X_k                          step      2 m^2 n
+// (up to 256 rows X_{k+1} = a X_k + A_k (b X_k + c A_k X_k) instead: ns_narrow_kernel)
 // and of the last X either itself in bf16 or, for an optimiser, the update of
 // the weights.  U is the gradient or, with a momentum, M' = mu M + (1 - mu) G
 // and U = (1 - mu) G + mu M' (Nesterov) or M'.
@@ -484,6 +485,9 @@ __device__ __forceinline__ f16x8 ns_col_frag(const char* t, int c0, int lane)
 // products take a quarter of the steps one after the other that they take in
 // workgroups that split the tile instead (gram of 256 x 1024, 10 tiles: 7.5 us
 // against 9.9; of 1001 x 2731, 136 tiles: 12.8 against 18.2 with its shares).
+// A gram of few tiles and long K has g.sharers workgroups a tile, whose sums
+// ns_few_join_kernel adds (256 x 16384: 8.8 + 5.4 us; 128 x 128 tiles with
+// shares 41 + 5).
 constexpr int kFewTile = 64, kFewStages = 5, kFewStage = 2 * kFewTile * kPanel * 2;
 template <int KIND>
 __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mats)
@@ -497,9 +501,10 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
         const int group = id / kNsCus * kNsCus, here = min(kNsCus, (int)gridDim.x - group);
         if (here == kNsCus) id = group + (id - group) % kNsXcds * (kNsCus / kNsXcds) + (id - group) / kNsXcds;
     }
-    NsTile t = ns_tile<kSym>(g, id);
+    const int split = KIND == kGram ? g.sharers : 1, quarter = 4 * (id % split) + wave;
+    NsTile t = ns_tile<kSym>(g, id / split);
     t = {(int)uniform_u32((uint32_t)t.batch), (int)uniform_u32((uint32_t)t.ti), (int)uniform_u32((uint32_t)t.tj)};
-    const int k_total = g.k_steps * g.passes, from = k_total * wave / 4, to = k_total * (wave + 1) / 4;
+    const int k_total = g.k_steps * g.passes, from = (int)((int64_t)k_total * quarter / (4 * split)), to = (int)((int64_t)k_total * (quarter + 1) / (4 * split));
     const _Float16* p = g.p + t.batch * g.p_size + (int64_t)t.ti * kFewTile * kPanel;
     const _Float16* q = g.q + t.batch * g.q_size + (kSym ? (int64_t)t.tj * kFewTile * kPanel : (int64_t)t.tj * kFewTile * g.pitch);
     const bool low = g.passes > 1;
@@ -583,7 +588,110 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
 #pragma unroll
         for (int w = 0; w < 4; w++) sum.q[q] += w == wave ? mine : meet[((wave * 3 + (w < wave ? w : w - 1)) * 4 + q) * 64 + lane];
     }
+    if (split > 1) {
+        float* const part = g.part + ((int64_t)id * 4 + wave) * 1024 + lane * 4;
+#pragma unroll
+        for (int q = 0; q < 4; q++) *reinterpret_cast<f32x4*>(part + q * 256) = sum.q[q];
+        return;
+    }
     ns_finish<KIND>(g, mats, t.batch, r0, c0, kSym && t.ti != t.tj, sum, s_mem + 12 * 4096 + wave * kScratch, old);
+}
+
+// The tiles of a gram whose K is split over workgroups too: their sums added
+// in order, a wave a block of 32 x 32.
+__global__ __launch_bounds__(256) void ns_few_join_kernel(NsGemm g)
+{
+    __shared__ __attribute__((aligned(16))) char s_mem[4 * kScratch];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const NsTile t = ns_tile<true>(g, (int)blockIdx.x);
+    const float* part = g.part + ((int64_t)blockIdx.x * g.sharers * 4 + wave) * 1024 + lane * 4;
+    NsBlock sum;
+#pragma unroll
+    for (int q = 0; q < 4; q++) sum.q[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < g.sharers; i++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) sum.q[q] += *reinterpret_cast<const f32x4*>(part + (int64_t)i * 4096 + q * 256);
+    ns_finish<kGram>(g, {}, t.batch, t.ti * kFewTile + 32 * (wave >> 1), t.tj * kFewTile + 32 * (wave & 1), t.ti != t.tj, sum,
+                     s_mem + wave * kScratch, NsOld{});
+}
+
+// Matrices of up to 256 rows: X' = a X + A (b X + c A X), so poly and step are
+// two products with the same A and need no B.  A workgroup has 32 columns and
+// all rows, a wave 32 of those.  Its rows of A come from memory into registers
+// in the matrix instructions' own order, all at once, and serve both products;
+// X and then Z = b X + c A X are in LDS for all waves.  Z always has its low
+// part: near a singular value of 1, a X + A Z = 3.4 - 2.7 loses two bits.
+// 256 x 1024: 7 us where the kernels poly and step take 5.2 each, 64 x 1024: 3.6;
+// both bound by the chain of one load, two products and a barrier between.
+template <int KIND, int GROUPS, bool LOW>
+__global__ __launch_bounds__(128 * GROUPS) void ns_narrow_kernel(NsGemm g, NsGiven<KIND> mats)
+{
+    constexpr int kWaves = 2 * GROUPS, kSteps = 2 * GROUPS, kParts = LOW ? 2 : 1, kPart = kSteps * 2048;
+    __shared__ __attribute__((aligned(16))) char s_x[kParts * kPart], s_z[2 * kPart], s_out[kWaves * kScratch];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int batch = (int)blockIdx.x / g.tiles_n, r0 = 32 * wave, c0 = (int)blockIdx.x % g.tiles_n * kPanel;
+    // a step of X, 32 rows of this panel, to each wave; the low part behind it
+    const _Float16* q = g.q + batch * g.q_size + (int64_t)c0 * g.pitch;
+    const i32x4 rq = ns_rsrc(q, (uint32_t)(((int64_t)kPanel * g.pitch + (LOW ? g.q_low : 0)) * 2));
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_x + (uint32_t)wave * 2048u;
+#pragma unroll
+    for (int part = 0; part < kParts; part++)
+        load_to_lds<2>(rq, lds + part * kPart, ns_voff_cols(lane), (uint32_t)wave * 2048u + (part ? (uint32_t)g.q_low * 2u : 0u));
+    f16x8 rows[kParts][kSteps][2];
+    {
+        const _Float16* const a = g.p + batch * g.p_size + (r0 + (lane & 15)) * kPanel + (lane >> 4) * 8;
+#pragma unroll
+        for (int k = 0; k < kSteps; k++)
+#pragma unroll
+            for (int part = 0; part < kParts; part++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    rows[part][k][i] = *reinterpret_cast<const f16x8*>(a + (part ? g.p_low : 0) + ((int64_t)k * g.pitch + 16 * i) * kPanel);
+    }
+    auto product = [&](const char* with, auto passes, f32x4 (&acc)[2][2]) {     // high high, high low, low high
+#pragma unroll
+        for (int pass = 0; pass < decltype(passes)::value; pass++)
+#pragma unroll
+            for (int k = 0; k < kSteps; k++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const f16x8 x = ns_col_frag(with + (pass == 1 ? kPart : 0) + k * 2048, 16 * j, lane);
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, rows[pass / 2][k][i], acc[i][j], 0, 0, 0);
+                }
+    };
+    wait_all();
+    __syncthreads();
+    f32x4 acc[2][2], sum[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    product(s_x, std::integral_constant<int, LOW ? 3 : 1>{}, acc);
+    // where a lane's results lie in a step's rows, their halves changed over as ns_voff_cols puts them
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int r = 16 * i + (lane & 15), at = wave * 2048 + r * 64 + (j ^ (r >> 3 & 1)) * 32 + (lane >> 4) * 8;
+            const f16x4 x = *reinterpret_cast<const f16x4*>(s_x + at);
+            f16x4 x_low = {}, z, z_low;
+            if constexpr (LOW) x_low = *reinterpret_cast<const f16x4*>(s_x + kPart + at);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float held = (float)x[e] + (float)x_low[e], to = g.b * held + g.c * (1.f / kHeld) * acc[i][j][e];
+                z[e] = (_Float16)to;
+                z_low[e] = (_Float16)(to - (float)z[e]);
+                sum[i][j][e] = g.a * kHeld * held;
+            }
+            *reinterpret_cast<f16x4*>(s_z + at) = z;
+            *reinterpret_cast<f16x4*>(s_z + kPart + at) = z_low;
+        }
+    __syncthreads();
+    product(s_z, std::integral_constant<int, LOW ? 3 : 2>{}, sum);
+    ns_finish<KIND>(g, mats, batch, r0, c0, false, NsBlock{{sum[0][0], sum[0][1], sum[1][0], sum[1][1]}}, s_out + wave * kScratch, NsOld{});
 }
 
 // Each workgroup goes through whole tiles and then through its share of the
@@ -820,11 +928,12 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsGemm g, NsGiven<KIND> ma
 // workgroup of their own, and its time in microseconds as the choice sees it.
 struct NsProduct {
     int tile;
-    int64_t tiles, whole, sharers, lanes, groups;
+    int64_t tiles, whole, sharers, lanes, groups;     // (sharers: workgroups in all; of a split gram, a tile's)
     double time;
 };
 struct NsPlan {
     NsProduct gram, poly, step;
+    bool narrow;                        // poly inside of step
     int64_t mp, np;
     // Panels are 2 KiB further apart than their rows need: at one step of step all workgroups load the same 32 rows of
     // their panels, which a power of two would put on the same few memory channels.
@@ -842,10 +951,11 @@ struct NsTileRate {
     double alone, full, round;
 };
 constexpr NsTileRate kNsRates[] = {{256, 1, 0.6, 0.85, 5.0}, {128, 2, 0.25, 0.70, 3.0}, {kFewTile, 1, 0.08, 0.145, 1.7}};
-constexpr double kNsLaunch = 4.0;
+constexpr double kNsLaunch = 4.0, kNsSplitJoin = 0.5, kNsSplitPart = 0.05;
 
-static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, bool sym, int64_t k, int64_t count, int passes)
+static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, int kind, int64_t k, int64_t count, int passes)
 {
+    const bool gram = kind == kGram, sym = gram || kind == kPoly;
     NsProduct p{};
     const int64_t tm = rows / r.tile, tn = cols / r.tile, steps = k / kPanel * passes, slots = (int64_t)kNsCus * r.per_cu;
     p.tile = r.tile;
@@ -857,6 +967,15 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
         return (r.alone + (r.full - r.alone) * std::min(1.0, (double)tiles / (double)slots)) * k_steps + r.round;
     };
     p.time = kNsLaunch + (double)(rounds - 1) * time(slots, (double)steps) + time(rounds > 1 ? slots : p.tiles, (double)steps);
+    if (r.tile == kFewTile) {
+        // a gram's K split over workgroups: their sums lie where the next X will
+        const int64_t room = (rows + kPanel) * k * 2 * count * (passes > 1 ? 2 : 1);
+        p.sharers = 1;
+        for (int64_t split = 2; gram && split * p.tiles <= slots && 8 * split <= steps && split * p.tiles * kFewTile * kFewTile * 4 <= room; split *= 2) {
+            const double split_time = 2 * kNsLaunch + time(split * p.tiles, (double)steps / (double)split) + kNsSplitJoin + kNsSplitPart * (double)split;
+            if (split_time < p.time) p.sharers = split, p.time = split_time;
+        }
+    }
     // A last round that does not fill the chip is dealt out in shares of its steps instead, where the steps saved are
     // worth the sums' way through memory (at about 4 TB/s, one after the other for a tile) and one more kernel (step of
     // two matrices of 2048 x 5500 in 22 bits, 352 tiles for 256 CUs: 340 us in two rounds, 251 + 19 with shares).
@@ -876,6 +995,20 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
     return p;
 }
 
+// poly and step in one kernel, 32 columns of the result to a workgroup: its own
+// chain of loads and products, and a share of a full chip's time (measured
+// alone on 1 to 3072 workgroups; operands of 22 bits take about 2 and 3 times as long).
+constexpr int64_t kNarrow = 256;        // most rows
+static NsProduct ns_narrow(int64_t mp, int64_t np, int64_t count, int passes)
+{
+    NsProduct p{};
+    const double groups = (double)mp / 64.0;
+    p.tiles = np / kPanel * count, p.whole = p.groups = p.tiles;
+    p.time = kNsLaunch + 0.5 + 0.75 * groups * (passes > 1 ? 2.0 : 1.0) +
+             (double)p.tiles * (0.001 * groups + 0.00033 * groups * groups) * (passes > 1 ? 3.2 : 1.0);
+    return p;
+}
+
 // The tile of each product that its estimate is shortest on.  Padding: whole
 // tiles of the largest size used.
 static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
@@ -887,18 +1020,20 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
     for (const NsTileRate& most : kNsRates) {
         NsPlan p{};
         p.mp = up(m, most.tile), p.np = up(n, most.tile);
-        auto pick = [&](int64_t rows, int64_t cols, bool sym, int64_t k) {
+        auto pick = [&](int64_t rows, int64_t cols, int kind, int64_t k) {
             NsProduct b{};
             for (const NsTileRate& r : kNsRates) {
                 if (r.tile > most.tile) continue;       // (the sizes divide one another)
-                const NsProduct q = ns_product(r, rows, cols, sym, k, count, passes);
+                const NsProduct q = ns_product(r, rows, cols, kind, k, count, passes);
                 if (b.tile == 0 || q.time < b.time) b = q;
             }
             return b;
         };
-        p.gram = pick(p.mp, p.mp, true, p.np);
-        p.poly = pick(p.mp, p.mp, true, p.mp);
-        p.step = pick(p.mp, p.np, false, p.mp);
+        p.gram = pick(p.mp, p.mp, kGram, p.np);
+        p.poly = pick(p.mp, p.mp, kPoly, p.mp);
+        p.step = pick(p.mp, p.np, kStep, p.mp);
+        const NsProduct both = ns_narrow(p.mp, p.np, count, passes);
+        if (p.mp <= kNarrow && both.time < p.poly.time + p.step.time) p.narrow = true, p.poly = NsProduct{}, p.step = both;
         const double time = p.gram.time + p.poly.time + p.step.time;
         if (best.mp == 0 || time < best_time) best = p, best_time = time;
     }
@@ -906,7 +1041,7 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
     p.x_bytes = p.size(p.np) * 2 * count * (precise ? 2 : 1);
     p.a_bytes = p.size(p.mp) * 2 * count * (precise ? 2 : 1);
     p.parts_bytes = (kNsParts * 8 * count + 255) / 256 * 256;
-    for (const NsProduct& q : {p.gram, p.poly, p.step}) p.share_bytes = std::max(p.share_bytes, q.sharers * 2 * q.tile * q.tile * 4);
+    for (const NsProduct& q : {p.gram, p.poly, p.step}) if (q.tile != kFewTile) p.share_bytes = std::max(p.share_bytes, q.sharers * 2 * q.tile * q.tile * 4);
     p.total = 2 * p.x_bytes + 2 * p.a_bytes + p.parts_bytes + p.share_bytes;
     return p;
 }
@@ -940,7 +1075,19 @@ static void ns_launch(NsGemm g, const NsPlan& plan, const NsProduct& p, const Ns
     else if (p.tile == 128)
         ns_launch_cfg<NsMiddle, KIND>(g, p, mats, st);
     else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_few_kernel<KIND>), dim3((uint32_t)p.tiles), dim3(256), 0, st, g, ns_given<KIND>(mats));
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_few_kernel<KIND>), dim3((uint32_t)(p.tiles * p.sharers)), dim3(256), 0, st, g, ns_given<KIND>(mats));
+    if (KIND == kGram && p.tile == kFewTile && p.sharers > 1)
+        hipLaunchKernelGGL(ns_few_join_kernel, dim3((uint32_t)p.tiles), dim3(256), 0, st, g);
+}
+
+template <int KIND, bool LOW>
+static void ns_launch_narrow(NsGemm g, const NsPlan& plan, const NsMatrices& mats, hipStream_t st)
+{
+    g.tiles_n = (int)(plan.np / kPanel);
+    const int groups = (int)(plan.mp / 64);
+    auto* kernel = groups == 1 ? ns_narrow_kernel<KIND, 1, LOW> : groups == 2 ? ns_narrow_kernel<KIND, 2, LOW>
+                   : groups == 3 ? ns_narrow_kernel<KIND, 3, LOW> : ns_narrow_kernel<KIND, 4, LOW>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)plan.step.tiles), dim3(128 * groups), 0, st, g, ns_given<KIND>(mats));
 }
 
 struct NsWork {
@@ -956,19 +1103,23 @@ static void ns_products(const NsPlan& p, const NsWork& w, NsGemm g, const NsMatr
         gram.p = gram.q = x, gram.p_size = gram.q_size = x_size, gram.p_low = gram.q_low = x_size * count;
         gram.pitch = (int)p.pitch(), gram.k_steps = (int)(p.np / kPanel);
         gram.out = w.a, gram.out_size = a_size, gram.out_low = a_size * count;
+        if (p.gram.tile == kFewTile) gram.part = reinterpret_cast<float*>(y);
         ns_launch<kGram>(gram, p, p.gram, mats, st);
         NsGemm poly = gram;
+        poly.part = g.part;
         poly.p = poly.q = w.a, poly.p_size = poly.q_size = a_size, poly.p_low = poly.q_low = a_size * count;
         poly.k_steps = (int)(p.mp / kPanel);
         poly.out = w.b;
-        ns_launch<kPoly>(poly, p, p.poly, mats, st);
+        if (!p.narrow) ns_launch<kPoly>(poly, p, p.poly, mats, st);
         NsGemm step = poly;
-        step.p = w.b, step.q = x, step.q_size = x_size, step.q_low = x_size * count;
+        step.p = p.narrow ? w.a : w.b, step.q = x, step.q_size = x_size, step.q_low = x_size * count;
         step.out = y, step.out_size = x_size, step.out_low = x_size * count;
-        if (k + 1 < steps)
-            ns_launch<kStep>(step, p, p.step, mats, st);
+        if (p.narrow && g.passes == 1)
+            k + 1 < steps ? ns_launch_narrow<kStep, false>(step, p, mats, st) : ns_launch_narrow<kLast, false>(step, p, mats, st);
+        else if (p.narrow)
+            k + 1 < steps ? ns_launch_narrow<kStep, true>(step, p, mats, st) : ns_launch_narrow<kLast, true>(step, p, mats, st);
         else
-            ns_launch<kLast>(step, p, p.step, mats, st);
+            k + 1 < steps ? ns_launch<kStep>(step, p, p.step, mats, st) : ns_launch<kLast>(step, p, p.step, mats, st);
     }
 }
 
@@ -982,9 +1133,9 @@ static int64_t ns_together(int64_t m, int64_t n, int64_t count, bool precise)
     return most;
 }
 
-// Whether all X but the last, and all A and B, stay where fp16 holds them.  Their elements are no larger than their
-// largest singular values: from s <= 1 on, q(s^2) of B and s q(s^2) of the next X with q(t) = a + b t + c t^2, whose
-// extremes lie at the ends or where a derivative is 0.
+// Whether all X but the last, A, B and Z stay where fp16 holds them.  Their elements are no larger than their
+// largest singular values: from s <= 1 on, q(s^2) of B, s q(s^2) of the next X and s (b + c s^2) of the narrow kernel's Z,
+// with q(t) = a + b t + c t^2; extremes lie at the ends or where a derivative is 0.
 static bool ns_in_range(double a, double b, double c, int steps)
 {
     constexpr double kMost = 15.0;      // (65504 / kHeld = 15.99, less the products' own errors)
@@ -992,14 +1143,15 @@ static bool ns_in_range(double a, double b, double c, int steps)
     double s = 1.0;
     for (int k = 0; k < steps; k++) {
         const double end = s * s, root = std::sqrt(std::max(0.0, 9.0 * b * b - 20.0 * a * c));
-        double most_b = 0.0, most_x = 0.0;
-        for (double t : {0.0, end, -b / (2.0 * c), (-3.0 * b + root) / (10.0 * c), (-3.0 * b - root) / (10.0 * c), -a / (3.0 * b)}) {
+        double most_b = 0.0, most_x = 0.0, most_z = 0.0;
+        for (double t : {0.0, end, -b / (2.0 * c), (-3.0 * b + root) / (10.0 * c), (-3.0 * b - root) / (10.0 * c), -a / (3.0 * b), -b / (3.0 * c)}) {
             if (!(t >= 0.0 && t <= end)) continue;      // (nor where a divisor is 0)
             const double q = std::fabs(a + b * t + c * t * t);
             most_b = std::max(most_b, q);
             most_x = std::max(most_x, std::sqrt(t) * q);
+            most_z = std::max(most_z, std::sqrt(t) * std::fabs(b + c * t));
         }
-        if (end > kMost || most_b > kMost || (k + 1 < steps && most_x > kMost)) return false;
+        if (end > kMost || most_b > kMost || most_z > kMost || (k + 1 < steps && most_x > kMost)) return false;
         s = most_x;
     }
     return true;
@@ -1057,7 +1209,7 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         // (a last group with fewer matrices: its plan may want more workspace than the full one's, so its tiles have workgroups of their own)
         NsPlan p = full;
         if (here < together) {
-            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = 0, q.groups = std::min(q.tiles, q.groups); };       // (a few-tiles product: as many groups as tiles)
+            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = q.tile == kFewTile ? q.sharers : 0, q.groups = std::min(q.tiles, q.groups); };       // (a few-tiles product: as many groups as tiles)
             fewer(p.gram);
             fewer(p.poly);
             fewer(p.step);

@@ -199,7 +199,11 @@ def test_update_in_place_of_views():
     M.muon_update_([W], [G], [mom], lr=0.1)
     assert torch.equal(W, plain)
     changed = buf != before
-    assert changed[10:60, 7:140].all()
+    # (an update of less than half a unit of its weight's last place leaves the weight as it is)
+    step = torch.zeros_like(plain)
+    M.muon_update_([step], [G.contiguous()], [torch.zeros(50, 133, device="cuda")], lr=0.1)
+    lost = step.abs() <= before[10:60, 7:140].abs() * 2.0 ** -24
+    assert (changed[10:60, 7:140] | lost).all() and lost.sum() < 10
     changed[10:60, 7:140] = False
     assert not changed.any()
 
@@ -350,3 +354,17 @@ def test_shared_tiles(B, R, C, precise):
         assert _err(got, _exact(G)) < 2.0e-3
     else:
         _check(G, got)
+
+
+@pytest.mark.parametrize("B,R,C", [(1, 64, 8200), (3, 200, 9000), (2, 130, 600), (70, 48, 100), (5, 256, 256), (1, 16000, 190)])
+@pytest.mark.parametrize("precise", [False, True])
+def test_few_rows(B, R, C, precise):
+    """Up to 256 rows, whose polynomial is not formed; long K, which is split over workgroups; the bars of the other
+    shapes."""
+    G = _grads(B, R, C, 15).to(BF)
+    got = _mod().orthogonalize(G, precise=precise)
+    if precise:
+        assert _err(got, _exact(G)) < 2.0e-3
+    else:
+        _check(G, got)
+    assert torch.equal(got, _mod().orthogonalize(G, precise=precise))
