@@ -483,11 +483,8 @@ __device__ __forceinline__ f16x8 ns_col_frag(const char* t, int c0, int lane)
 // Such a product is bound by latency: a wave has five steps of loads in flight
 // (with all of a CU's LDS, as much as its share of L2 delivers), and the
 // products take a quarter of the steps one after the other that they take in
-// workgroups that split the tile instead (gram of 256 x 1024, 10 tiles: 7.5 us
-// against 9.9; of 1001 x 2731, 136 tiles: 12.8 against 18.2 with its shares).
-// A gram of few tiles and long K has g.sharers workgroups a tile, whose sums
-// ns_few_join_kernel adds (256 x 16384: 8.8 + 5.4 us; 128 x 128 tiles with
-// shares 41 + 5).
+// workgroups that split the tile instead (gram of 1001 x 2731, 136 tiles: 12.8
+// us against 18.2 with its shares; of 256 x 1024, 10 tiles: 7.5 against 9.9).
 constexpr int kFewTile = 64, kFewStages = 5, kFewStage = 2 * kFewTile * kPanel * 2;
 template <int KIND>
 __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mats)
@@ -501,10 +498,9 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
         const int group = id / kNsCus * kNsCus, here = min(kNsCus, (int)gridDim.x - group);
         if (here == kNsCus) id = group + (id - group) % kNsXcds * (kNsCus / kNsXcds) + (id - group) / kNsXcds;
     }
-    const int split = KIND == kGram ? g.sharers : 1, quarter = 4 * (id % split) + wave;
-    NsTile t = ns_tile<kSym>(g, id / split);
+    NsTile t = ns_tile<kSym>(g, id);
     t = {(int)uniform_u32((uint32_t)t.batch), (int)uniform_u32((uint32_t)t.ti), (int)uniform_u32((uint32_t)t.tj)};
-    const int k_total = g.k_steps * g.passes, from = (int)((int64_t)k_total * quarter / (4 * split)), to = (int)((int64_t)k_total * (quarter + 1) / (4 * split));
+    const int k_total = g.k_steps * g.passes, from = k_total * wave / 4, to = k_total * (wave + 1) / 4;
     const _Float16* p = g.p + t.batch * g.p_size + (int64_t)t.ti * kFewTile * kPanel;
     const _Float16* q = g.q + t.batch * g.q_size + (kSym ? (int64_t)t.tj * kFewTile * kPanel : (int64_t)t.tj * kFewTile * g.pitch);
     const bool low = g.passes > 1;
@@ -588,32 +584,114 @@ __global__ __launch_bounds__(256) void ns_few_kernel(NsGemm g, NsGiven<KIND> mat
 #pragma unroll
         for (int w = 0; w < 4; w++) sum.q[q] += w == wave ? mine : meet[((wave * 3 + (w < wave ? w : w - 1)) * 4 + q) * 64 + lane];
     }
-    if (split > 1) {
-        float* const part = g.part + ((int64_t)id * 4 + wave) * 1024 + lane * 4;
-#pragma unroll
-        for (int q = 0; q < 4; q++) *reinterpret_cast<f32x4*>(part + q * 256) = sum.q[q];
-        return;
-    }
     ns_finish<KIND>(g, mats, t.batch, r0, c0, kSym && t.ti != t.tj, sum, s_mem + 12 * 4096 + wave * kScratch, old);
 }
 
-// The tiles of a gram whose K is split over workgroups too: their sums added
-// in order, a wave a block of 32 x 32.
-__global__ __launch_bounds__(256) void ns_few_join_kernel(NsGemm g)
+// Symmetric products of few tiles: 32 x 32 a workgroup, an eighth of K to each
+// of its waves, whose operands go from memory into registers in the matrix
+// instructions' own order, without LDS, four steps of loads at once.  With
+// g.sharers workgroups a tile (long K) their sums meet in ns_fine_join_kernel.
+// Gram of 256 x 1024: 5.2 us (64 x 64 tiles: 7.5), of 256 x 16384: 10.8 + 3.9
+// (128 x 128 tiles with shares: 41 + 5); bound by latency.
+constexpr int kFineTile = 32;
+template <int KIND, bool LOW>
+__global__ __launch_bounds__(512) void ns_fine_kernel(NsGemm g)
 {
-    __shared__ __attribute__((aligned(16))) char s_mem[4 * kScratch];
+    constexpr int kParts = LOW ? 2 : 1, kAhead = 4 / kParts;
+    __shared__ __attribute__((aligned(16))) f32x4 s_sum[8][4][64];
+    __shared__ __attribute__((aligned(16))) char s_out[kScratch];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int id = (int)blockIdx.x, eighth = 8 * (id % g.sharers) + wave;
+    NsTile t = ns_tile<true>(g, id / g.sharers);
+    t = {(int)uniform_u32((uint32_t)t.batch), (int)uniform_u32((uint32_t)t.ti), (int)uniform_u32((uint32_t)t.tj)};
+    const int from = (int)((int64_t)g.k_steps * eighth / (8 * g.sharers)), to = (int)((int64_t)g.k_steps * (eighth + 1) / (8 * g.sharers));
+    const int r0 = t.ti * kFineTile, c0 = t.tj * kFineTile;
+    const _Float16* const p = g.p + t.batch * g.p_size + (lane & 15) * kPanel + (lane >> 4) * 8;
+    NsOld old;
+    if constexpr (KIND == kPoly)
+        if (wave == 0) old = ns_old(g, t.batch, r0, c0);
+    f32x4 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // steps k on, all their loads before the first product; of the last ones those past the end with nothing for Q
+    auto steps = [&](int k, auto n, auto last) {
+        constexpr int kN = decltype(n)::value;
+        f16x8 fp[kN][kParts][2], fq[kN][kParts][2];
+#pragma unroll
+        for (int s = 0; s < kN; s++) {
+            const _Float16* const at = p + (int64_t)(decltype(last)::value ? min(k + s, to - 1) : k + s) * g.pitch * kPanel;
+#pragma unroll
+            for (int part = 0; part < kParts; part++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    fp[s][part][i] = *reinterpret_cast<const f16x8*>(at + (part ? g.p_low : 0) + (r0 + 16 * i) * kPanel);
+                    fq[s][part][i] = *reinterpret_cast<const f16x8*>(at + (part ? g.p_low : 0) + (c0 + 16 * i) * kPanel);
+                }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < kN; s++) {
+            if (decltype(last)::value && k + s >= to)
+#pragma unroll
+                for (int part = 0; part < kParts; part++) fq[s][part][0] = fq[s][part][1] = f16x8{};
+#pragma unroll
+            for (int pass = 0; pass < 2 * kParts - 1; pass++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fq[s][pass == 1][j], fp[s][pass / 2][i], acc[i][j], 0, 0, 0);
+        }
+    };
+    typedef std::integral_constant<int, kAhead> All;
+    typedef std::integral_constant<int, kAhead / 2> Half;
+    int k = from;
+    for (; k + kAhead <= to; k += kAhead) steps(k, All{}, std::false_type{});
+    if (k + kAhead / 2 < to)
+        steps(k, All{}, std::true_type{});
+    else if (k < to)
+        steps(k, Half{}, std::true_type{});
+#pragma unroll
+    for (int q = 0; q < 4; q++) s_sum[wave][q][lane] = acc[q >> 1][q & 1];
+    __syncthreads();
+    if (wave < 4) {         // a quarter of the block each, the waves' sums in order
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 8; w++) sum += s_sum[w][wave][lane];
+        if (g.sharers > 1)
+            *reinterpret_cast<f32x4*>(g.part + (int64_t)id * 1024 + wave * 256 + lane * 4) = sum;
+        else
+            s_sum[0][wave][lane] = sum;
+    }
+    if (g.sharers > 1) return;
+    __syncthreads();
+    if (wave) return;
+    NsBlock sum;
+#pragma unroll
+    for (int q = 0; q < 4; q++) sum.q[q] = s_sum[0][q][lane];
+    ns_finish<KIND>(g, {}, t.batch, r0, c0, t.ti != t.tj, sum, s_out, old);
+}
+
+// The tiles of more than one workgroup: their sums added in order.
+template <int KIND>
+__global__ __launch_bounds__(64) void ns_fine_join_kernel(NsGemm g)
+{
+    __shared__ __attribute__((aligned(16))) char s_out[kScratch];
+    const int lane = threadIdx.x & 63;
     const NsTile t = ns_tile<true>(g, (int)blockIdx.x);
-    const float* part = g.part + ((int64_t)blockIdx.x * g.sharers * 4 + wave) * 1024 + lane * 4;
+    const float* part = g.part + (int64_t)blockIdx.x * g.sharers * 1024 + lane * 4;
+    NsOld old;
+    if constexpr (KIND == kPoly) old = ns_old(g, t.batch, t.ti * kFineTile, t.tj * kFineTile);
     NsBlock sum;
 #pragma unroll
     for (int q = 0; q < 4; q++) sum.q[q] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < g.sharers; i++)
 #pragma unroll
-        for (int q = 0; q < 4; q++) sum.q[q] += *reinterpret_cast<const f32x4*>(part + (int64_t)i * 4096 + q * 256);
-    ns_finish<kGram>(g, {}, t.batch, t.ti * kFewTile + 32 * (wave >> 1), t.tj * kFewTile + 32 * (wave & 1), t.ti != t.tj, sum,
-                     s_mem + wave * kScratch, NsOld{});
+        for (int q = 0; q < 4; q++) sum.q[q] += *reinterpret_cast<const f32x4*>(part + (int64_t)i * 1024 + q * 256);
+    ns_finish<KIND>(g, {}, t.batch, t.ti * kFineTile, t.tj * kFineTile, t.ti != t.tj, sum, s_out, old);
 }
 
 // Matrices of up to 256 rows: X' = a X + A (b X + c A X), so poly and step are
@@ -951,11 +1029,10 @@ struct NsTileRate {
     double alone, full, round;
 };
 constexpr NsTileRate kNsRates[] = {{256, 1, 0.6, 0.85, 5.0}, {128, 2, 0.25, 0.70, 3.0}, {kFewTile, 1, 0.08, 0.145, 1.7}};
-constexpr double kNsLaunch = 4.0, kNsSplitJoin = 0.5, kNsSplitPart = 0.05;
+constexpr double kNsLaunch = 4.0;
 
-static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, int kind, int64_t k, int64_t count, int passes)
+static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, bool sym, int64_t k, int64_t count, int passes)
 {
-    const bool gram = kind == kGram, sym = gram || kind == kPoly;
     NsProduct p{};
     const int64_t tm = rows / r.tile, tn = cols / r.tile, steps = k / kPanel * passes, slots = (int64_t)kNsCus * r.per_cu;
     p.tile = r.tile;
@@ -967,15 +1044,6 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, int
         return (r.alone + (r.full - r.alone) * std::min(1.0, (double)tiles / (double)slots)) * k_steps + r.round;
     };
     p.time = kNsLaunch + (double)(rounds - 1) * time(slots, (double)steps) + time(rounds > 1 ? slots : p.tiles, (double)steps);
-    if (r.tile == kFewTile) {
-        // a gram's K split over workgroups: their sums lie where the next X will
-        const int64_t room = (rows + kPanel) * k * 2 * count * (passes > 1 ? 2 : 1);
-        p.sharers = 1;
-        for (int64_t split = 2; gram && split * p.tiles <= slots && 8 * split <= steps && split * p.tiles * kFewTile * kFewTile * 4 <= room; split *= 2) {
-            const double split_time = 2 * kNsLaunch + time(split * p.tiles, (double)steps / (double)split) + kNsSplitJoin + kNsSplitPart * (double)split;
-            if (split_time < p.time) p.sharers = split, p.time = split_time;
-        }
-    }
     // A last round that does not fill the chip is dealt out in shares of its steps instead, where the steps saved are
     // worth the sums' way through memory (at about 4 TB/s, one after the other for a tile) and one more kernel (step of
     // two matrices of 2048 x 5500 in 22 bits, 352 tiles for 256 CUs: 340 us in two rounds, 251 + 19 with shares).
@@ -993,6 +1061,28 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, int
         }
     }
     return p;
+}
+
+// A symmetric product in 32 x 32 tiles, with as many workgroups a tile as its K
+// is worth; their sums lie where the next X will (`room` bytes).  Up to 512 rows:
+// every row is read rows / 32 times (orthogonalize of 512 x 2048 105 us against
+// 130 without these tiles, 22 bits 141 against 181; of 768 x 3072 177 against
+// 178, 22 bits 323 against 314).
+constexpr int64_t kFineRows = 512;
+constexpr double kFineStep = 0.035, kFineFull = 0.05, kFineRound = 1.2, kFineJoin = 0.8, kFinePart = 0.05;
+static NsProduct ns_fine(int64_t rows, int64_t k, int64_t count, int passes, int64_t room)
+{
+    NsProduct best{};
+    const int64_t n = rows / kFineTile, steps = k / kPanel;
+    const double step_bytes = passes > 1 ? 2.0 : 1.0;
+    for (int64_t split = 1; split == 1 || (split * best.tiles <= kNsCus && 16 * split <= steps && split * best.tiles * kFineTile * kFineTile * 4 <= room); split *= 2) {
+        NsProduct p{};
+        p.tile = kFineTile, p.tiles = n * (n + 1) / 2 * count, p.whole = p.groups = p.tiles, p.sharers = split;
+        const double fill = (double)(p.tiles * split) / (double)kNsCus, each = (double)steps / (double)split * step_bytes;
+        p.time = kNsLaunch + kFineRound + each * std::max(kFineStep, kFineFull * std::ceil(fill)) + (split > 1 ? kNsLaunch + kFineJoin + kFinePart * (double)split : 0.0);
+        if (split == 1 || p.time < best.time) best = p;
+    }
+    return best;
 }
 
 // poly and step in one kernel, 32 columns of the result to a workgroup: its own
@@ -1015,23 +1105,27 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
 {
     NsPlan best{};
     auto up = [](int64_t v, int64_t t) { return (v + t - 1) / t * t; };
-    const int passes = precise ? 3 : 1;
+    const int passes = precise ? 3 : 1, passes_held = precise ? 2 : 1;
     double best_time = 0;
     for (const NsTileRate& most : kNsRates) {
         NsPlan p{};
         p.mp = up(m, most.tile), p.np = up(n, most.tile);
-        auto pick = [&](int64_t rows, int64_t cols, int kind, int64_t k) {
+        auto pick = [&](int64_t rows, int64_t cols, bool sym, int64_t k) {
             NsProduct b{};
             for (const NsTileRate& r : kNsRates) {
                 if (r.tile > most.tile) continue;       // (the sizes divide one another)
-                const NsProduct q = ns_product(r, rows, cols, kind, k, count, passes);
+                const NsProduct q = ns_product(r, rows, cols, sym, k, count, passes);
                 if (b.tile == 0 || q.time < b.time) b = q;
+            }
+            if (sym && rows <= kFineRows) {
+                const NsProduct q = ns_fine(rows, k, count, passes, p.size(p.np) * 2 * count * passes_held);
+                if (q.time < b.time) b = q;
             }
             return b;
         };
-        p.gram = pick(p.mp, p.mp, kGram, p.np);
-        p.poly = pick(p.mp, p.mp, kPoly, p.mp);
-        p.step = pick(p.mp, p.np, kStep, p.mp);
+        p.gram = pick(p.mp, p.mp, true, p.np);
+        p.poly = pick(p.mp, p.mp, true, p.mp);
+        p.step = pick(p.mp, p.np, false, p.mp);
         const NsProduct both = ns_narrow(p.mp, p.np, count, passes);
         if (p.mp <= kNarrow && both.time < p.poly.time + p.step.time) p.narrow = true, p.poly = NsProduct{}, p.step = both;
         const double time = p.gram.time + p.poly.time + p.step.time;
@@ -1041,7 +1135,7 @@ static NsPlan ns_plan(int64_t m, int64_t n, int64_t count, bool precise)
     p.x_bytes = p.size(p.np) * 2 * count * (precise ? 2 : 1);
     p.a_bytes = p.size(p.mp) * 2 * count * (precise ? 2 : 1);
     p.parts_bytes = (kNsParts * 8 * count + 255) / 256 * 256;
-    for (const NsProduct& q : {p.gram, p.poly, p.step}) if (q.tile != kFewTile) p.share_bytes = std::max(p.share_bytes, q.sharers * 2 * q.tile * q.tile * 4);
+    for (const NsProduct& q : {p.gram, p.poly, p.step}) if (q.tile > kFewTile) p.share_bytes = std::max(p.share_bytes, q.sharers * 2 * q.tile * q.tile * 4);
     p.total = 2 * p.x_bytes + 2 * p.a_bytes + p.parts_bytes + p.share_bytes;
     return p;
 }
@@ -1070,14 +1164,19 @@ static void ns_launch(NsGemm g, const NsPlan& plan, const NsProduct& p, const Ns
     g.tiles = (int)p.tiles, g.whole = (int)p.whole, g.sharers = (int)p.sharers, g.lanes = (int)p.lanes;
     g.tiles_m = (int)(plan.mp / p.tile);
     g.tiles_n = (int)((KIND == kGram || KIND == kPoly ? plan.mp : plan.np) / p.tile);
+    if constexpr (KIND == kGram || KIND == kPoly)
+        if (p.tile == kFineTile) {
+            auto* kernel = g.passes > 1 ? ns_fine_kernel<KIND, true> : ns_fine_kernel<KIND, false>;
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)(p.tiles * p.sharers)), dim3(512), 0, st, g);
+            if (p.sharers > 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_fine_join_kernel<KIND>), dim3((uint32_t)p.tiles), dim3(64), 0, st, g);
+            return;
+        }
     if (p.tile == 256)
         ns_launch_cfg<NsLarge, KIND>(g, p, mats, st);
     else if (p.tile == 128)
         ns_launch_cfg<NsMiddle, KIND>(g, p, mats, st);
     else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_few_kernel<KIND>), dim3((uint32_t)(p.tiles * p.sharers)), dim3(256), 0, st, g, ns_given<KIND>(mats));
-    if (KIND == kGram && p.tile == kFewTile && p.sharers > 1)
-        hipLaunchKernelGGL(ns_few_join_kernel, dim3((uint32_t)p.tiles), dim3(256), 0, st, g);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_few_kernel<KIND>), dim3((uint32_t)p.tiles), dim3(256), 0, st, g, ns_given<KIND>(mats));
 }
 
 template <int KIND, bool LOW>
@@ -1103,15 +1202,16 @@ static void ns_products(const NsPlan& p, const NsWork& w, NsGemm g, const NsMatr
         gram.p = gram.q = x, gram.p_size = gram.q_size = x_size, gram.p_low = gram.q_low = x_size * count;
         gram.pitch = (int)p.pitch(), gram.k_steps = (int)(p.np / kPanel);
         gram.out = w.a, gram.out_size = a_size, gram.out_low = a_size * count;
-        if (p.gram.tile == kFewTile) gram.part = reinterpret_cast<float*>(y);
+        if (p.gram.tile == kFineTile) gram.part = reinterpret_cast<float*>(y);
         ns_launch<kGram>(gram, p, p.gram, mats, st);
         NsGemm poly = gram;
-        poly.part = g.part;
+        poly.part = p.poly.tile == kFineTile ? reinterpret_cast<float*>(y) : g.part;
         poly.p = poly.q = w.a, poly.p_size = poly.q_size = a_size, poly.p_low = poly.q_low = a_size * count;
         poly.k_steps = (int)(p.mp / kPanel);
         poly.out = w.b;
         if (!p.narrow) ns_launch<kPoly>(poly, p, p.poly, mats, st);
         NsGemm step = poly;
+        step.part = g.part;
         step.p = p.narrow ? w.a : w.b, step.q = x, step.q_size = x_size, step.q_low = x_size * count;
         step.out = y, step.out_size = x_size, step.out_low = x_size * count;
         if (p.narrow && g.passes == 1)
@@ -1209,7 +1309,7 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         // (a last group with fewer matrices: its plan may want more workspace than the full one's, so its tiles have workgroups of their own)
         NsPlan p = full;
         if (here < together) {
-            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = q.tile == kFewTile ? q.sharers : 0, q.groups = std::min(q.tiles, q.groups); };       // (a few-tiles product: as many groups as tiles)
+            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = q.tile == kFineTile ? q.sharers : 0, q.groups = std::min(q.tiles, q.groups); };       // (a few-tiles product: as many groups as tiles)
             fewer(p.gram);
             fewer(p.poly);
             fewer(p.step);
