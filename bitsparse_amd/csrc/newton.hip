@@ -674,16 +674,13 @@ __global__ __launch_bounds__(512) void ns_fine_kernel(NsGemm g)
     ns_finish<KIND>(g, {}, t.batch, r0, c0, t.ti != t.tj, sum, s_out, old);
 }
 
-// The tiles of more than one workgroup: their sums added in order.
-template <int KIND>
+// A gram's tiles of more than one workgroup: their sums added in order.
 __global__ __launch_bounds__(64) void ns_fine_join_kernel(NsGemm g)
 {
     __shared__ __attribute__((aligned(16))) char s_out[kScratch];
     const int lane = threadIdx.x & 63;
     const NsTile t = ns_tile<true>(g, (int)blockIdx.x);
     const float* part = g.part + (int64_t)blockIdx.x * g.sharers * 1024 + lane * 4;
-    NsOld old;
-    if constexpr (KIND == kPoly) old = ns_old(g, t.batch, t.ti * kFineTile, t.tj * kFineTile);
     NsBlock sum;
 #pragma unroll
     for (int q = 0; q < 4; q++) sum.q[q] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -691,7 +688,7 @@ __global__ __launch_bounds__(64) void ns_fine_join_kernel(NsGemm g)
     for (int i = 0; i < g.sharers; i++)
 #pragma unroll
         for (int q = 0; q < 4; q++) sum.q[q] += *reinterpret_cast<const f32x4*>(part + (int64_t)i * 1024 + q * 256);
-    ns_finish<KIND>(g, {}, t.batch, t.ti * kFineTile, t.tj * kFineTile, t.ti != t.tj, sum, s_out, old);
+    ns_finish<kGram>(g, {}, t.batch, t.ti * kFineTile, t.tj * kFineTile, t.ti != t.tj, sum, s_out, NsOld{});
 }
 
 // Matrices of up to 256 rows: X' = a X + A (b X + c A X), so poly and step are
@@ -1063,11 +1060,12 @@ static NsProduct ns_product(const NsTileRate& r, int64_t rows, int64_t cols, boo
     return p;
 }
 
-// A symmetric product in 32 x 32 tiles, with as many workgroups a tile as its K
-// is worth; their sums lie where the next X will (`room` bytes).  Up to 512 rows:
-// every row is read rows / 32 times (orthogonalize of 512 x 2048 105 us against
-// 130 without these tiles, 22 bits 141 against 181; of 768 x 3072 177 against
-// 178, 22 bits 323 against 314).
+// A symmetric product in 32 x 32 tiles; a gram's with as many workgroups a tile
+// as its K is worth, whose sums lie where the next X will (`room` bytes; poly's
+// K is too short for more than one).  Up to 512 rows, as every row is read
+// rows / 32 times: orthogonalize of 512 x 2048 takes 105 us against 130 without
+// these tiles (22 bits 141 against 181), of 768 x 3072 177 against 178 (323
+// against 314).  Rates as above: microseconds a step of K, a tile, a join.
 constexpr int64_t kFineRows = 512;
 constexpr double kFineStep = 0.035, kFineFull = 0.05, kFineRound = 1.2, kFineJoin = 0.8, kFinePart = 0.05;
 static NsProduct ns_fine(int64_t rows, int64_t k, int64_t count, int passes, int64_t room)
@@ -1168,7 +1166,7 @@ static void ns_launch(NsGemm g, const NsPlan& plan, const NsProduct& p, const Ns
         if (p.tile == kFineTile) {
             auto* kernel = g.passes > 1 ? ns_fine_kernel<KIND, true> : ns_fine_kernel<KIND, false>;
             hipLaunchKernelGGL(kernel, dim3((uint32_t)(p.tiles * p.sharers)), dim3(512), 0, st, g);
-            if (p.sharers > 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(ns_fine_join_kernel<KIND>), dim3((uint32_t)p.tiles), dim3(64), 0, st, g);
+            if (KIND == kGram && p.sharers > 1) hipLaunchKernelGGL(ns_fine_join_kernel, dim3((uint32_t)p.tiles), dim3(64), 0, st, g);
             return;
         }
     if (p.tile == 256)
@@ -1205,13 +1203,12 @@ static void ns_products(const NsPlan& p, const NsWork& w, NsGemm g, const NsMatr
         if (p.gram.tile == kFineTile) gram.part = reinterpret_cast<float*>(y);
         ns_launch<kGram>(gram, p, p.gram, mats, st);
         NsGemm poly = gram;
-        poly.part = p.poly.tile == kFineTile ? reinterpret_cast<float*>(y) : g.part;
+        poly.part = g.part;
         poly.p = poly.q = w.a, poly.p_size = poly.q_size = a_size, poly.p_low = poly.q_low = a_size * count;
         poly.k_steps = (int)(p.mp / kPanel);
         poly.out = w.b;
         if (!p.narrow) ns_launch<kPoly>(poly, p, p.poly, mats, st);
         NsGemm step = poly;
-        step.part = g.part;
         step.p = p.narrow ? w.a : w.b, step.q = x, step.q_size = x_size, step.q_low = x_size * count;
         step.out = y, step.out_size = x_size, step.out_low = x_size * count;
         if (p.narrow && g.passes == 1)
