@@ -1085,7 +1085,7 @@ static NsProduct ns_fine(int64_t rows, int64_t k, int64_t count, int passes, int
 
 // poly and step in one kernel, 32 columns of the result to a workgroup: its own
 // chain of loads and products, and a share of a full chip's time (measured
-// alone on 1 to 3072 workgroups; operands of 22 bits take about 2 and 3 times as long).
+// on 1 workgroup to 12 a CU; operands of 22 bits take about 2 and 3 times as long).
 constexpr int64_t kNarrow = 256;        // most rows
 static NsProduct ns_narrow(int64_t mp, int64_t np, int64_t count, int passes)
 {

@@ -37,7 +37,7 @@ def orthogonalize(G: Tensor, *, steps: int = 5, coefficients: tuple[float, float
     65536 rows and columns and fewer than 2^29 elements each), in bfloat16, contiguous.
 
     ``precise``: products of 22-bit operands (see above).  Coefficients that
-    could take X, A or B past 15 raise ValueError.  No gradient flows
+    could take X, A, b A + c A^2 + a or b X + c A X past 15 raise ValueError.  No gradient flows
     through it (an optimiser's operator)."""
     a, b, c = coefficients
     with torch.no_grad():

@@ -119,6 +119,7 @@ def test_newton_schulz_refusals(kw, word):
     (4.5, 0.0, 0.0, 1, True), (4.5, 0.0, 0.0, 2, False),            # the last X is no operand; A of 1 and 20.25
     (14.9, 0.0, 0.0, 1, True), (15.1, 0.0, 0.0, 1, False), (-15.1, 0.0, 0.0, 1, False), (0.0, 0.0, 16.0, 1, False),
     (0.0, 70.0, -70.0, 1, False),                                   # B is largest inside the range, 17.5 at t = 0.5
+    (-10.0, 20.0, 0.0, 1, False), (-7.0, 14.0, 0.0, 1, True),       # b X + c A X
     (float("nan"), 0.0, 0.0, 1, False), (0.0, float("inf"), 0.0, 1, False)])
 def test_newton_schulz_range(a, b, c, steps, ok):
     """Coefficients whose operands fp16 does not hold; what is held gets as far as the workspace."""
