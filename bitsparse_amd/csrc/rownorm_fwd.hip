@@ -5,8 +5,8 @@
 //
 // Bound by memory: x and y are read and x' and h written once, all four in
 // the row's own registers between the two statistics (rownorm.h).  The
-// vectors are held in registers over the rows that a workgroup goes through,
-// gate * weight_post and gate * bias_post multiplied beforehand, and the next
+// vectors are held in registers over the rows that a workgroup goes through
+// (without a bias gate * weight_post multiplied beforehand), and the next
 // row's loads are in flight while this row's sums meet.  16384 x 4096 in bf16:
 // 105 us, 5.1 TB/s (a copy reaches 5.15); 32 x 4096: 5.5 us, latency.
 #include <algorithm>
@@ -58,18 +58,18 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
     };
     load(row);
 
-    float sc[C][8], gw[C][8], gb[C][8], w2[C][8], b2[C][8];
+    const bool bias = a.b_post.p != nullptr;
+    float sc[C][8], gw[C][8], gv[C][8], gb[C][8], w2[C][8], b2[C][8];
     auto vectors = [&](int k) {
         if constexpr (JOIN) {
             param_chunk(a.scale, at.col[k], at.in_row[k], a.scale_value, sc[k]);
-            float g[8];
-            param_chunk(a.gate, at.col[k], at.in_row[k], 1.f, g);
+            param_chunk(a.gate, at.col[k], at.in_row[k], 1.f, gv[k]);
             param_chunk(a.w_post, at.col[k], at.in_row[k], 1.f, gw[k]);
-            param_chunk(a.b_post, at.col[k], at.in_row[k], 0.f, gb[k]);
+            if (bias) {
+                param_chunk(a.b_post, at.col[k], at.in_row[k], 0.f, gb[k]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                gw[k][e] *= g[e];
-                gb[k][e] *= g[e];
+                for (int e = 0; e < 8; e++) gw[k][e] *= gv[k][e];
             }
         }
         if (a.pre) {
@@ -115,11 +115,14 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                     param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, g);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    // (rstd last: with RMS norms of 16-bit x, y and vectors every product before is exact, and the
-                    // sum the only rounding in 32 bits)
-                    const float gate = per_element ? g[e] : rg;
-                    const float t = (y[k][e] - mean) * gw[k][e] * gate;
-                    v[k][e] = fmaf(t, rstd, fmaf(sc[k][e], v[k][e], gb[k][e] * gate));
+                    // Without a bias rstd comes last: with RMS norms of 16-bit x, y and vectors every product before is exact,
+                    // and the sum the only rounding in 32 bits.  With one p is whole before its gate: an infinite gate times
+                    // two terms of different signs would be NaN (and times an absent bias's 0).
+                    const float gate = per_element ? g[e] : rg, c = (y[k][e] - mean) * gw[k][e];
+                    if (bias)
+                        v[k][e] = fmaf(gv[k][e] * gate, fmaf(c, rstd, gb[k][e]), sc[k][e] * v[k][e]);
+                    else
+                        v[k][e] = fmaf(c * gate, rstd, sc[k][e] * v[k][e]);
                 }
                 const Raw<XT> o = to_raw<XT>(v[k]);
                 store_raw<WHOLE>(static_cast<XT*>(a.x1) + row * a.cols + at.col[k], o, nv[k]);
