@@ -201,14 +201,15 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
             if (a.post || (per_row && d_row_gate)) row_sums(s, at, s_sums, turn);
             if (per_row && d_row_gate && mine && at.lane_in_row == 0) param_store(d_row_gate, a.row_gate_f32, row, s[2]);
             if (a.dy) {
-                const float m0 = layer_post ? s[0] * at.inv_cols : 0.f, m1 = a.post ? s[1] * at.inv_cols : 0.f;
+                const float m0 = layer_post ? s[0] * at.inv_cols : 0.f, m1 = s[1] * at.inv_cols;
 #pragma unroll
                 for (int k = 0; k < C; k++) {
                     float o[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
+                        // (without a norm dp alone: y may hold what 0 times makes a NaN)
                         const float n = (raw_get(now.y[k], e) - st.x) * st.y;
-                        o[e] = st.y * (G[k][e] - m0 - n * m1);
+                        o[e] = a.post ? st.y * (G[k][e] - m0 - n * m1) : G[k][e];
                     }
                     store_raw<WHOLE>(static_cast<YT*>(a.dy) + row * a.cols + at.col[k], to_raw<YT>(o), nv[k]);
                 }
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
             for (int e = 0; e < 8; e++) {
                 if (e >= at.in_row[k]) continue;
                 t[0] += acc[kSumScale][k][e];
-                t[1] += w1[e] * acc[kSumA][k][e] + b1[e] * acc[kSumB][k][e];
+                t[1] += w1[e] * acc[kSumA][k][e] + (a.b_post.p ? b1[e] * acc[kSumB][k][e] : 0.f);    // (B may be infinite)
             }
         }
         const int wave = (int)threadIdx.x >> 6, waves = (int)blockDim.x >> 6;

@@ -35,6 +35,21 @@ def _randn(*s, seed=0):
 SHAPES = {"one": lambda T, D: (1,), "channel": lambda T, D: (D,), "row": lambda T, D: (T, 1), "element": lambda T, D: (T, D)}
 
 
+@pytest.mark.parametrize("T,D", [(5, 64), (7, 2001), (3, 5000)])
+@pytest.mark.parametrize("gate", [None, "one", "channel", "row", "element"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gradient_of_a_block_output_that_overflowed(T, D, gate, dtype):
+    """Without a norm after the block dy = gate dx', whatever y is."""
+    x, y, g = (_randn(T, D, seed=i).to(dtype) for i in range(3))
+    y[0, 3], y[1, 5], y[2, 7] = math.inf, -math.inf, math.nan
+    gv = None if gate is None else (0.5 + 0.3 * _randn(*SHAPES[gate](T, D), seed=3))
+    y.requires_grad_()
+    x1 = _mod().block_join(x, y, gate=gv)
+    dy, = torch.autograd.grad(x1, y, g)
+    want = g.double() * (1.0 if gv is None else gv.double())
+    _same(dy, want, want.abs(), "dy " + ("bf16" if dtype == BF else "fp32"))
+
+
 @pytest.mark.parametrize("T,D", [(5, 64), (7, 2001), (3, 9000)])
 @pytest.mark.parametrize("gate", ["one", "channel", "row", "element"])
 @pytest.mark.parametrize("post,bias", [(None, False), ("rms", False), ("layer", False), ("rms", True), ("layer", True)])
@@ -57,3 +72,16 @@ def test_gates_past_the_range(T, D, gate, post, bias, big):
         p = c * r * w.double() + b
     want = 0.75 * x.double() + gv.double() * p
     _same(x1, want, 0.75 * x.double().abs() + (gv.double() * mag).abs().nan_to_num(posinf=0.0), "x1 fp32")
+
+
+@pytest.mark.parametrize("post", ["rms", "layer"])
+def test_gradient_of_one_gate_with_an_infinite_gradient(post):
+    """dgate = sum G p is infinite where one G is; the bias that is not there adds nothing to it."""
+    R = _mod()
+    x, y, g = (_randn(9, 300, seed=i) for i in range(3))
+    g[4, 100] = math.inf
+    gv = torch.full((1,), 0.5, device="cuda").requires_grad_()
+    x1 = R.block_join(x, y, post=R.RowNorm(None, None, post, EPS), gate=gv)
+    d, = torch.autograd.grad(x1, gv, g)
+    c = y - y.mean(-1, keepdim=True) if post == "layer" else y
+    assert d.item() == math.copysign(math.inf, c[4, 100].item())
