@@ -9,6 +9,7 @@
 
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
@@ -625,9 +626,12 @@ block_backward(const Tensor& g, const Tensor& x, const Tensor& W1, const Tensor&
 // the step between two blocks (residual.py)
 // ---------------------------------------------------------------------------
 // A tensor the kernels can read at its address: on the GPU, with storage of its
-// own, not inside a tracer's or a transform's wrapper.
+// own, not inside a tracer's or a transform's wrapper, and without a tangent:
+// results of these operators have none, which forward mode reads as 0.
 void plain_on_gpu(const Tensor& t, const char* what)
 {
+    TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), what,
+                                ": bitsparse_amd has no forward-mode derivatives");
     TORCH_CHECK(t.is_cuda(), what, ": bitsparse_amd runs on a ROCm GPU; got a tensor on ", t.device());
     TORCH_CHECK_NOT_IMPLEMENTED(
         t.has_storage() && t.layout() == at::kStrided &&

@@ -38,7 +38,7 @@ def orthogonalize(G: Tensor, *, steps: int = 5, coefficients: tuple[float, float
 
     ``precise``: products of 22-bit operands (see above).  Coefficients that
     could take X, A, b A + c A^2 + a or b X + c A X past 15 raise ValueError.  No gradient flows
-    through it (an optimiser's operator)."""
+    through it (an optimiser's operator), and a tangent is refused."""
     a, b, c = coefficients
     with torch.no_grad():
         return native().orthogonalize(G, steps, a, b, c, eps, precise)

@@ -61,7 +61,8 @@ def block_norm(x: Tensor, norm: RowNorm, *, dtype: torch.dtype | None = None) ->
     of a float32 x for a block that takes it).
 
     x: [..., D], bfloat16 or float32, 0 < D <= 32768, rows of any stride.
-    Differentiable once in x and the norm's vectors."""
+    Differentiable once in x and the norm's vectors, in reverse mode; a tangent
+    (forward mode) is refused."""
     weight, bias, kind, eps = _parts(norm, "norm")
     if kind == 0:
         raise TypeError("block_norm needs a RowNorm")
@@ -83,7 +84,7 @@ def block_join(x: Tensor, y: Tensor, *, post: RowNorm | None = None, gate: Tenso
     scale: None (1), a Python number, or a tensor of one value or one a
     channel [D].
     Returns x' (x's dtype), with ``pre`` the pair (x', h) (h in y's dtype).
-    Differentiable once in every tensor; the gradients are sums in 32 bits in
+    Differentiable once in every tensor, in reverse mode (a tangent is refused); the gradients are sums in 32 bits in
     a fixed order, each rounded once to its tensor's dtype."""
     w_post, b_post, kind_post, eps_post = _parts(post, "post")
     w_pre, b_pre, kind_pre, eps_pre = _parts(pre, "pre")
