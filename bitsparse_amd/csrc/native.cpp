@@ -979,7 +979,7 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         rule.momentum = 1, rule.nesterov = nesterov, rule.update = 1;
         rule.precise = precise.value_or(key.w == BS_DT_F32);
         rule.steps = (int)steps;
-        rule.a = (float)a, rule.b = (float)b, rule.c = (float)c, rule.eps = (float)eps, rule.mu = (float)mu;
+        rule.a = (float)a, rule.b = (float)b, rule.c = (float)c, rule.eps = (float)eps, rule.mu = (float)mu, rule.fresh = (float)(1.0 - mu);
         rule.keep = (float)(1.0 - lr * decay), rule.rate = (float)(lr * key.s);
         newton_group(mats, key.m, key.n, rule, like);
     }

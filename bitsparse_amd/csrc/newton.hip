@@ -76,7 +76,7 @@ using NsGiven = std::conditional_t<KIND == kLast, NsMatrices, NsNone>;
 struct NsPrep {
     int64_t m, n, pitch, np;
     int g_f32, m_f32, momentum, nesterov, parts, precise;
-    float mu, eps;
+    float mu, fresh, eps;               // fresh: 1 - mu
     double* parts_at;                   // [count][kNsParts]
     _Float16* x;                        // [count] matrices, precise: and the low parts behind all of them
     int64_t low;                        // elements from a value to its low part
@@ -104,7 +104,7 @@ __device__ __forceinline__ void ns_u(const NsPrep& a, const NsMatrix& t, int64_t
     ns_chunk(t.m, a.m_f32, r * t.m_stride + c, nv, m);
     if (update) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) m[e] = a.mu * m[e] + (1.f - a.mu) * u[e];
+        for (int e = 0; e < 8; e++) m[e] = a.mu * m[e] + a.fresh * u[e];
         if (a.m_f32) {
             store_raw(static_cast<float*>(t.m) + r * t.m_stride + c, to_raw<float>(m), nv);
         } else {
@@ -115,7 +115,7 @@ __device__ __forceinline__ void ns_u(const NsPrep& a, const NsMatrix& t, int64_t
         }
     }
 #pragma unroll
-    for (int e = 0; e < 8; e++) u[e] = a.nesterov ? (1.f - a.mu) * u[e] + a.mu * m[e] : m[e];
+    for (int e = 0; e < 8; e++) u[e] = a.nesterov ? a.fresh * u[e] + a.mu * m[e] : m[e];
 }
 
 // The momentum's update and partial sums of squares of U (in 64 bits: any
@@ -1321,7 +1321,7 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         NsPrep a{};
         a.m = m, a.n = n, a.np = p.np;
         a.g_f32 = r.grad_type == BS_DT_F32, a.m_f32 = r.momentum_type == BS_DT_F32, a.momentum = r.momentum, a.nesterov = r.nesterov;
-        a.mu = r.mu, a.eps = r.eps, a.precise = precise, a.low = p.size(p.np) * here, a.pitch = p.pitch();
+        a.mu = r.mu, a.fresh = r.fresh, a.eps = r.eps, a.precise = precise, a.low = p.size(p.np) * here, a.pitch = p.pitch();
         // about 4096 elements or more to a workgroup, and no more of them than 8 a CU over all matrices
         a.parts = (int)std::max<int64_t>(1, std::min({(int64_t)kNsParts, (m * n + 8191) / 8192, (8 * kNsCus + here - 1) / here}));
         a.parts_at = reinterpret_cast<double*>(ws);

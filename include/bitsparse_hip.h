@@ -49,7 +49,7 @@ extern "C" {
 const char* bs_last_error(void);
 
 /* ABI version (bumped when an entry point changes): of this header, and of a built library. */
-#define BS_ABI_VERSION 18
+#define BS_ABI_VERSION 19
 int bs_abi_version(void);
 
 /*
@@ -714,7 +714,7 @@ int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* work
  * Orthogonalised updates of weight matrices (no counterpart in the reference,
  * which leaves its weight gradients to torch's optimisers).  For each of
  * `count` matrices, [rows, cols] or (transposed) [cols, rows]:
- *   with a momentum: M <- mu M + (1 - mu) G and U = (1 - mu) G + mu M
+ *   with a momentum: M <- mu M + fresh G and U = fresh G + mu M
  *   (nesterov) or M, of M as stored; without: U = G
  *   X = U / (||U||_F + eps); `steps` times X <- (a I + b A + c A^2) X with
  *   A = X X^T (of the transpose, where U has more rows than columns)
@@ -740,6 +740,7 @@ typedef struct bs_newton_schulz_rule {
     int precise;                     /* flag: operands of 22 bits */
     int steps;
     float a, b, c, eps, mu, keep, rate;
+    float fresh;                     /* 1 - mu, rounded by itself: 1 - (float)mu is off by 2^-25 / (1 - mu) of it */
 } bs_newton_schulz_rule;
 int64_t bs_newton_schulz_workspace_bytes(int64_t rows, int64_t cols, int64_t count, int precise);
 int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_t rows, int64_t cols,

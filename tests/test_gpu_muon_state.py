@@ -1,0 +1,22 @@
+"""What an optimiser step leaves in the momentum."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _randn(*s, seed=0):
+    return torch.randn(s, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+@pytest.mark.parametrize("mu", [0.0, 0.5, 0.9, 0.95, 0.999, 0.9999])
+@pytest.mark.parametrize("shape", [(40, 70), (129, 33)])
+def test_momentum_in_32_bits(mu, shape):
+    """M' = mu M + (1 - mu) G of the mu that was given.  Bar: mu and 1 - mu rounded, two products and a sum, each to
+    2^-24: four roundings of each term at most."""
+    from bitsparse_amd.muon import muon_update_
+    G, W = _randn(*shape, seed=1), _randn(*shape, seed=2)
+    for M in (torch.zeros(shape, device="cuda"), _randn(*shape, seed=3)):
+        old, fresh = mu * M.double(), (1 - mu) * G.double()
+        muon_update_([W], [G], [M], lr=0.1, momentum=mu)
+        assert ((M.double() - (old + fresh)).abs() <= 4 * 2.0 ** -24 * (old.abs() + fresh.abs())).all()
