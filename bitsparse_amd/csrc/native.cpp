@@ -667,26 +667,16 @@ struct JoinKind {
     at::ScalarType h_type;
 };
 
+// address of an operand that is there and that this call does not read
+alignas(16) char kUnread[16];
+
 struct JoinCall {
     bs_join a{};
     Tensor x, y, gate;          // as the kernels read them
-    int64_t rows, cols;
+    int64_t rows = 0, cols = 0;
     std::vector<Tensor> held;   // copies the pointers above point into
 
-    bs_vector vector(const Maybe& v, const char* what, bool whole)
-    {
-        if (!v) return {nullptr, BS_DT_BF16};
-        plain_on_gpu(*v, what);
-        TORCH_CHECK(v->device() == x.device(), what, " is on ", v->device(), ", x on ", x.device());
-        const int type = row_type(*v, what);
-        if (whole) TORCH_CHECK_VALUE(v->dim() == 1 && v->size(0) == cols, what, ": expected shape [", cols, "], got ", v->sizes());
-        if (!v->is_contiguous()) {
-            held.push_back(v->contiguous());
-            return {held.back().data_ptr(), type};
-        }
-        return {v->data_ptr(), type};
-    }
-
+    JoinCall() = default;
     JoinCall(const Tensor& x_in, const Maybe& y_in, const Maybe& w_post, const Maybe& b_post, const Maybe& gate_in,
              const Maybe& scale, const Maybe& w_pre, const Maybe& b_pre, const JoinKind& k)
     {
@@ -694,9 +684,9 @@ struct JoinCall {
         TORCH_CHECK_VALUE(x_in.dim() >= 1 && x_in.size(-1) > 0, "x: expected rows [..., D] with D > 0, got ", x_in.sizes());
         cols = x_in.size(-1);
         a.x_type = row_type(x_in, "x");
-        x = as_rows(x_in, cols);
+        put_x(x_in);
         rows = x.size(0);
-        a.rows = rows, a.cols = cols, a.x = x.data_ptr(), a.x_stride = row_stride(x);
+        a.rows = rows, a.cols = cols;
         a.norm_post = (int)k.post, a.norm_pre = (int)k.pre, a.eps_post = (float)k.eps_post, a.eps_pre = (float)k.eps_pre;
         a.y_type = k.h_type == at::kFloat ? BS_DT_F32 : BS_DT_BF16;
         if (y_in) {
@@ -704,9 +694,7 @@ struct JoinCall {
             a.y_type = row_type(*y_in, "y");
             TORCH_CHECK(y_in->device() == x_in.device(), "y is on ", y_in->device(), ", x on ", x_in.device());
             TORCH_CHECK_VALUE(y_in->sizes() == x_in.sizes(), "y: expected x's shape ", x_in.sizes(), ", got ", y_in->sizes());
-            y = as_rows(*y_in, cols);
-            // (no rows: torch gives a null address, the ABI's sign of an absent y)
-            a.y = rows ? y.data_ptr() : &a, a.y_stride = row_stride(y);
+            put_y(*y_in);
         }
         TORCH_CHECK_TYPE(a.x_type == BS_DT_F32 || a.y_type == BS_DT_BF16, y_in ? "y" : "dtype",
                          " float32 needs a float32 x: the residual stream has at least the block's precision");
@@ -722,6 +710,44 @@ struct JoinCall {
             a.scale_per = scale->numel() == 1 ? BS_PER_TENSOR : BS_PER_CHANNEL;
         }
         if (gate_in) set_gate(*gate_in, x_in.sizes());
+    }
+
+    void put_x(const Tensor& t)
+    {
+        x = as_rows(t, cols);
+        a.x = x.data_ptr(), a.x_stride = row_stride(x);
+    }
+    void put_y(const Tensor& t)
+    {
+        y = as_rows(t, cols);
+        // (no rows: torch gives a null address, the ABI's sign of an absent y)
+        a.y = rows ? y.data_ptr() : kUnread, a.y_stride = row_stride(y);
+    }
+    bs_vector put_vector(const Tensor& v, int type)
+    {
+        if (v.is_contiguous()) return {v.data_ptr(), type};
+        held.push_back(v.contiguous());
+        return {held.back().data_ptr(), type};
+    }
+    void put_gate(const Tensor& g)
+    {
+        if (a.gate_per <= BS_PER_CHANNEL) {
+            a.gate = put_vector(g, a.gate.type);
+            return;
+        }
+        gate = as_rows(g, a.gate_per == BS_PER_ELEMENT ? cols : 1);
+        a.gate.data = rows ? gate.data_ptr() : kUnread;
+        a.gate_stride = row_stride(gate);
+    }
+
+    bs_vector vector(const Maybe& v, const char* what, bool whole)
+    {
+        if (!v) return {nullptr, BS_DT_BF16};
+        plain_on_gpu(*v, what);
+        TORCH_CHECK(v->device() == x.device(), what, " is on ", v->device(), ", x on ", x.device());
+        const int type = row_type(*v, what);
+        if (whole) TORCH_CHECK_VALUE(v->dim() == 1 && v->size(0) == cols, what, ": expected shape [", cols, "], got ", v->sizes());
+        return put_vector(*v, type);
     }
 
     void set_gate(const Tensor& g, at::IntArrayRef shape)
@@ -741,10 +767,9 @@ struct JoinCall {
                           at::IntArrayRef(per_row), " or ", shape, ", got ", g.sizes());
         plain_on_gpu(g, "gate");
         TORCH_CHECK(g.device() == x.device(), "gate is on ", g.device(), ", x on ", x.device());
-        gate = as_rows(g, element ? cols : 1);
-        a.gate = {rows ? gate.data_ptr() : &a, row_type(g, "gate")};
+        a.gate.type = row_type(g, "gate");
         a.gate_per = element ? BS_PER_ELEMENT : BS_PER_ROW;
-        a.gate_stride = row_stride(gate);
+        put_gate(g);
     }
 };
 
@@ -763,6 +788,19 @@ std::array<Tensor, 3> join_forward(JoinCall& c, at::IntArrayRef shape, bool stat
     return {x1, h, st};
 }
 
+// What a step's backward has of its operands besides those it reads: the
+// call as it was made (its addresses are taken anew) and the operands' shapes.
+struct JoinNode : torch::CustomClassHolder {
+    bs_join a;
+    int64_t rows, cols;
+    at::TensorOptions options;      // of x
+    struct Operand {
+        bool there = false;
+        at::ScalarType type;
+        c10::SmallVector<int64_t, 4> shape;
+    } operands[8];                  // x, y, w_post, b_post, gate, scale, w_pre, b_pre
+};
+
 struct Join : torch::autograd::Function<Join> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Maybe& y,
                                                   const Maybe& w_post, const Maybe& b_post, const Maybe& gate,
@@ -772,15 +810,25 @@ struct Join : torch::autograd::Function<Join> {
         const c10::DeviceGuard guard(x.device());
         JoinCall c(x, y, w_post, b_post, gate, scale, w_pre, b_pre, k);
         const auto [x1, h, st] = join_forward(c, x.sizes(), true);
-        auto or_none = [](const Maybe& m) { return m ? *m : Tensor(); };
-        ctx->save_for_backward({x, or_none(y), or_none(w_post), or_none(b_post), or_none(gate), or_none(scale),
-                                or_none(w_pre), or_none(b_pre), x1, st});
-        ctx->saved_data["post"] = k.post;
-        ctx->saved_data["pre"] = k.pre;
-        ctx->saved_data["eps_post"] = k.eps_post;
-        ctx->saved_data["eps_pre"] = k.eps_pre;
-        ctx->saved_data["scale"] = k.scale_value;
-        ctx->saved_data["h"] = (int64_t)k.h_type;
+        auto node = c10::make_intrusive<JoinNode>();
+        node->a = c.a, node->rows = c.rows, node->cols = c.cols, node->options = x.options();
+        const Maybe first(x);
+        const Maybe* all[8] = {&first, &y, &w_post, &b_post, &gate, &scale, &w_pre, &b_pre};
+        for (int i = 0; i < 8; i++) {
+            if (!*all[i]) continue;
+            const Tensor& t = **all[i];
+            node->operands[i].there = true, node->operands[i].type = t.scalar_type();
+            node->operands[i].shape.assign(t.sizes().begin(), t.sizes().end());
+        }
+        // Only what some gradient is formed of: x for the scale's (or where it is what is normalised), y for the gate's and
+        // through its norm, x' through the norm that follows, post's bias for the gate's.  The rest may be freed or changed.
+        auto learns = [](const Maybe& m) { return m && m->requires_grad(); };
+        auto if_read = [](bool read, const Maybe& m) { return read && m ? *m : Tensor(); };
+        ctx->save_for_backward({if_read(!y || learns(scale), x),
+                                if_read(learns(gate) || (k.post != BS_NORM_NONE && (learns(y) || learns(w_post))), y),
+                                if_read(true, w_post), if_read(learns(gate), b_post), if_read(true, gate), if_read(true, scale),
+                                if_read(true, w_pre), y && k.pre != BS_NORM_NONE ? x1 : Tensor(), st});
+        ctx->saved_data["node"] = c10::IValue::make_capsule(node);
         ctx->set_materialize_grads(false);
         if (!c.a.y) return {h};
         if (!c.a.norm_pre) return {x1};
@@ -793,37 +841,53 @@ struct Join : torch::autograd::Function<Join> {
         TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(),
                                     "bitsparse_amd: the step between two blocks has no second derivative (create_graph)");
         const auto saved = ctx->get_saved_variables();
-        const Tensor& x = saved[0];
-        const c10::DeviceGuard guard(x.device());
-        auto maybe = [&](int i) { return saved[i].defined() ? Maybe(saved[i]) : std::nullopt; };
-        const JoinKind k{ctx->saved_data["post"].toInt(), ctx->saved_data["pre"].toInt(),
-                         ctx->saved_data["eps_post"].toDouble(), ctx->saved_data["eps_pre"].toDouble(),
-                         ctx->saved_data["scale"].toDouble(), (at::ScalarType)ctx->saved_data["h"].toInt()};
-        JoinCall c(x, maybe(1), maybe(2), maybe(3), maybe(4), maybe(5), maybe(6), maybe(7), k);
+        const auto capsule = ctx->saved_data["node"].toCapsule();
+        const JoinNode& node = static_cast<const JoinNode&>(*capsule);
+        const c10::DeviceGuard guard(node.options.device());
+        JoinCall c;
+        c.a = node.a, c.rows = node.rows, c.cols = node.cols;
         // the tensors among the operands, in order, are the node's edges
         bool wanted[8];
-        for (int i = 0, edge = 0; i < 8; i++) wanted[i] = saved[i].defined() && ctx->needs_input_grad(edge++);
+        for (int i = 0, edge = 0; i < 8; i++) wanted[i] = node.operands[i].there && ctx->needs_input_grad(edge++);
         torch::autograd::variable_list out(9);
         const Tensor gx = c.a.y ? grads[0] : Tensor(), gh = c.a.norm_pre ? grads.back() : Tensor();
         if (!gx.defined() && !gh.defined()) return out;
-        for (int i = 0; i < 8; i++)
-            if (wanted[i]) out[i] = c.rows ? at::empty(saved[i].sizes(), saved[i].options()) : at::zeros_like(saved[i]);
+        for (int i = 0; i < 8; i++) {
+            if (!wanted[i]) continue;
+            const auto options = node.options.dtype(node.operands[i].type);
+            out[i] = c.rows ? at::empty(node.operands[i].shape, options) : at::zeros(node.operands[i].shape, options);
+        }
         if (c.rows == 0) return out;
 
+        c.a.x = kUnread;
+        if (saved[0].defined()) c.put_x(saved[0]);
+        if (c.a.y) c.a.y = kUnread;
+        if (saved[1].defined()) c.put_y(saved[1]);
+        auto put = [&](bs_vector& v, const Tensor& t) {
+            if (v.data) v.data = kUnread;
+            if (t.defined()) v = c.put_vector(t, v.type);
+        };
+        put(c.a.weight_post, saved[2]);
+        put(c.a.bias_post, saved[3]);
+        if (saved[4].defined()) c.put_gate(saved[4]);
+        put(c.a.scale, saved[5]);
+        put(c.a.weight_pre, saved[6]);
+        put(c.a.bias_pre, Tensor());
         bs_join_grads g{};
-        const Tensor st = saved[9];
+        const Tensor st = saved[8];
         if (st.defined()) {
             c.a.stats_post = st.data_ptr<float>();
             c.a.stats_pre = c.a.stats_post + 2 * c.rows;
         }
         Tensor x1, gxr, ghr;
-        if (saved[8].defined()) {
-            x1 = saved[8].contiguous();
+        if (saved[7].defined()) {
+            x1 = saved[7].contiguous();
             g.x1 = x1.data_ptr();
         }
         auto grad_rows = [&](const Tensor& t, int type, const char* what) {
             plain_on_gpu(t, what);
-            TORCH_CHECK_VALUE(t.sizes() == x.sizes(), what, ": expected ", x.sizes(), ", got ", t.sizes());
+            TORCH_CHECK_VALUE(t.sizes() == at::IntArrayRef(node.operands[0].shape), what, ": expected ",
+                              at::IntArrayRef(node.operands[0].shape), ", got ", t.sizes());
             TORCH_CHECK_TYPE(row_type(t, what) == type, what, ": unexpected dtype ", t.scalar_type());
             return as_rows(t, c.cols);
         };
@@ -838,8 +902,10 @@ struct Join : torch::autograd::Function<Join> {
         g.d_x = raw(out[0]), g.d_y = raw(out[1]), g.d_weight_post = raw(out[2]), g.d_bias_post = raw(out[3]);
         g.d_gate = raw(out[4]), g.d_scale = raw(out[5]), g.d_weight_pre = raw(out[6]), g.d_bias_pre = raw(out[7]);
         const int64_t need = L.bs_join_backward_workspace_bytes(c.rows, c.cols);
-        const Tensor ws = empty({need}, c.x, at::kByte);
-        check(L.bs_join_backward(&c.a, &g, ws.data_ptr(), need, stream_of(c.x)), "bs_join_backward");
+        const Tensor ws = at::empty({need}, node.options.dtype(at::kByte));
+        check(L.bs_join_backward(&c.a, &g, ws.data_ptr(), need,
+                                 c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(node.options.device().index()).stream()),
+              "bs_join_backward");
         return out;
     }
 };

@@ -13,7 +13,7 @@
 // B = sum G, dw_post = gate A, db_post = gate B and dgate = w_post A +
 // b_post B, so five sums a column serve all six vectors.
 //
-// Bound by memory: dx', dh, x', y (and x for dscale) read once, dx and dy
+// Bound by memory: dx', dh, x', y (and x for dscale; y not where no gradient is formed of it) read once, dx and dy
 // written once, a row in registers throughout.  Each workgroup keeps its
 // column sums in registers over all its rows and writes one row of partial
 // sums; the second kernel adds those in order.  No atomics: the same bits at
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
             o.gh[k] = load_raw<WHOLE>(static_cast<const YT*>(a.gh) + row * a.gh_stride + at.col[k], nv_gh);
             o.x1[k] = load_raw<WHOLE>(static_cast<const XT*>(a.x1) + row * a.x1_stride + at.col[k], nv_gh);
             if constexpr (JOIN) {
-                o.y[k] = load_raw<WHOLE>(static_cast<const YT*>(a.y) + row * a.y_stride + at.col[k], nv);
+                o.y[k] = load_raw<WHOLE>(static_cast<const YT*>(a.y) + row * a.y_stride + at.col[k], a.y ? nv : 0);
                 o.x[k] = load_raw<WHOLE>(static_cast<const XT*>(a.x) + row * a.x_stride + at.col[k], a.x ? nv : 0);
             }
         }
@@ -437,9 +437,9 @@ extern "C" int bs_join_backward(const bs_join* args, const bs_join_grads* grads,
     a.rows = j.rows, a.cols = j.cols;
     a.x = g.d_scale ? j.x : nullptr, a.x_stride = j.x_stride;
     a.x1 = join ? g.x1 : j.x, a.x1_stride = join ? j.cols : j.x_stride;
-    a.y = j.y, a.y_stride = j.y_stride;
+    a.y = g.d_gate || (j.norm_post && (g.d_y || g.d_weight_post)) ? j.y : nullptr, a.y_stride = j.y_stride;
     a.gx = g.grad_x1, a.gx_stride = g.grad_x1_stride, a.gh = g.grad_h, a.gh_stride = g.grad_h_stride;
-    a.w_post = row_param(j.weight_post, 0), a.b_post = row_param(j.bias_post, 0), a.w_pre = row_param(j.weight_pre, 0);
+    a.w_post = row_param(j.weight_post, 0), a.b_post = g.d_gate ? row_param(j.bias_post, 0) : RowParam{nullptr, 0, 0}, a.w_pre = row_param(j.weight_pre, 0);
     a.gate = fixed_gate ? row_param(j.gate, j.gate_per) : RowParam{nullptr, 0, 0};
     a.scale = row_param(j.scale, j.scale_per), a.scale_value = j.scale_value;
     a.row_gate = fixed_gate ? nullptr : j.gate.data, a.row_gate_f32 = j.gate.type == BS_DT_F32;

@@ -695,7 +695,9 @@ int bs_join_forward(const bs_join* args, void* x1, void* h, void* stream);
  * y; row stride cols).  Every result may be NULL; those there are written
  * whole, in the type of what they are the gradient of: d_x, d_y [rows, cols];
  * d_gate in the gate's own shape, d_scale, and those of the four vectors.
- * bs_join.x is read for d_scale (and, without y, for everything).  Sums over
+ * bs_join.x is read for d_scale (and, without y, for everything), y for d_gate
+ * and, behind norm_post, d_y and d_weight_post, bias_post for d_gate, bias_pre
+ * not at all; of what is not read only that it is there counts.  Sums over
  * the rows go through `workspace` in a fixed order: the same call gives the
  * same bits.
  */
