@@ -1220,15 +1220,32 @@ static void ns_products(const NsPlan& p, const NsWork& w, NsGemm g, const NsMatr
     }
 }
 
-// Matrices that go through the products together: as many as keep every
-// offset inside a buffer under 2^32 bytes.
+// Matrices that go through the products together: no more than 64, and no more
+// than 1 GiB holds two X, A and B of (or one), which also keeps every offset
+// inside a buffer under 2^32 bytes.  Few large matrices fill the chip: of 8
+// of 4096 x 16384 each takes 3.74 ms together (2.7 GiB) and 3.86 in threes, of
+// 64 of 2048 x 8192 0.51 together (5.2 GiB) and 0.54 in tens (1.1).
+constexpr int64_t kNsScratch = int64_t(1) << 30;
 static int64_t ns_together(int64_t m, int64_t n, int64_t count, bool precise)
 {
-    int64_t most = std::min<int64_t>(count, kNsBatch);
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-    while (most > 1 && precise && (most + 1) * (up(m) + kPanel) * up(n) * 2 >= (int64_t(1) << 32)) most--;
-    return most;
+    const int64_t one = 4 * (up(m) + kPanel) * (up(n) + up(m)) * (precise ? 2 : 1);
+    return std::min({count, (int64_t)kNsBatch, std::max<int64_t>(1, kNsScratch / one)});
 }
+
+// More than go together go in as many groups as they need, even to one matrix,
+// each with the plan of its own size: 72 of 768 x 3072 take 2.89 ms as 36 and
+// 36 (3.30 as 64 and 8).
+struct NsGroups {
+    int64_t most, groups, small, larger;        // `larger` groups of small + 1, the others of small
+    NsGroups(int64_t m, int64_t n, int64_t count, bool precise)
+    {
+        most = ns_together(m, n, count, precise);
+        groups = (count + most - 1) / most;
+        small = count / groups;
+        larger = count % groups;
+    }
+};
 
 // Whether all X but the last, A, B and Z stay where fp16 holds them.  Their elements are no larger than their
 // largest singular values: from s <= 1 on, q(s^2) of B, s q(s^2) of the next X and s (b + c s^2) of the narrow kernel's Z,
@@ -1262,7 +1279,11 @@ extern "C" int64_t bs_newton_schulz_workspace_bytes(int64_t rows, int64_t cols, 
 {
     if (rows <= 0 || cols <= 0 || count <= 0 || rows > 65536 || cols > 65536) return 0;
     const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
-    return ns_plan(m, n, ns_together(m, n, count, precise != 0), precise != 0).total;
+    const NsGroups g(m, n, count, precise != 0);
+    int64_t total = ns_plan(m, n, g.most, precise != 0).total;      // (what any number of matrices needs)
+    if (g.groups > 1) total = std::max(total, ns_plan(m, n, g.small, precise != 0).total);
+    if (g.groups > 1 && g.larger) total = std::max(total, ns_plan(m, n, g.small + 1, precise != 0).total);
+    return total;
 }
 
 extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_t rows, int64_t cols,
@@ -1299,18 +1320,13 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
     if (workspace == nullptr || ((uintptr_t)workspace & 255u) || workspace_bytes < bs_newton_schulz_workspace_bytes(rows, cols, count, precise))
         return set_error(BS_ERR_INVALID, "%s: workspace too small or misaligned", what);
     const hipStream_t st = (hipStream_t)stream;
-    const int64_t together = ns_together(m, n, count, precise);
-    const NsPlan full = ns_plan(m, n, together, precise);
-    for (int64_t first = 0; first < count; first += together) {
-        const int64_t here = std::min<int64_t>(count - first, together);
-        // (a last group with fewer matrices: its plan may want more workspace than the full one's, so its tiles have workgroups of their own)
-        NsPlan p = full;
-        if (here < together) {
-            auto fewer = [&](NsProduct& q) { q.tiles = q.tiles / together * here, q.whole = q.tiles, q.sharers = q.tile == kFineTile ? q.sharers : 0, q.groups = std::min(q.tiles, q.groups); };       // (a few-tiles product: as many groups as tiles)
-            fewer(p.gram);
-            fewer(p.poly);
-            fewer(p.step);
-        }
+    const NsGroups groups(m, n, count, precise);
+    NsPlan p{};
+    int64_t first = 0, here = 0;
+    for (int64_t group = 0; group < groups.groups; group++, first += here) {
+        const int64_t size = groups.small + (group < groups.larger);
+        if (size != here) p = ns_plan(m, n, size, precise);
+        here = size;
         NsMatrices mats{};
         for (int64_t i = 0; i < here; i++) {
             const bs_matrix& t = matrices[first + i];
