@@ -954,6 +954,14 @@ void newton_group(const std::vector<bs_matrix>& mats, int64_t m, int64_t n, cons
     check(L.bs_newton_schulz(mats.data(), count, m, n, &rule, ws.data_ptr(), need, stream_of(on)), "bs_newton_schulz");
 }
 
+// (before anything of that size is allocated)
+template <class... What>
+void check_size(int64_t R, int64_t C, const What&... what)
+{
+    TORCH_CHECK_VALUE(std::max(R, C) <= 65536 && R * C < (int64_t(1) << 29), what..., ": ", R, " x ", C,
+                      " is past 65536 rows or columns or 2^29 elements");
+}
+
 void check_matrix(const Tensor& t, const char* what)
 {
     plain_on_gpu(t, what);
@@ -964,6 +972,7 @@ Tensor orthogonalize(const Tensor& G, int64_t steps, double a, double b, double 
 {
     plain_on_gpu(G, "G");
     TORCH_CHECK_VALUE(G.dim() >= 2, "G: expected matrices [..., R, C], got ", G.sizes());
+    if (G.numel() > 0) check_size(G.size(-2), G.size(-1), "G");
     const c10::DeviceGuard guard(G.device());
     bs_newton_schulz_rule rule{};
     rule.grad_type = row_type(G, "G");
@@ -1021,8 +1030,7 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         TORCH_CHECK_VALUE(written.insert(W[i].data_ptr()).second && written.insert(M[i].data_ptr()).second,
                           "parameter ", i, " or its momentum is in the lists twice");
         const int64_t R = W[i].size(0), C = W[i].size(1);
-        TORCH_CHECK_VALUE(std::max(R, C) <= 65536 && R * C < (int64_t(1) << 29), "parameter ", i, ": ", W[i].sizes(),
-                          " is past 65536 rows or columns or 2^29 elements");
+        check_size(R, C, "parameter ", i);
         Tensor g = G[i];
         if (C > 1 && g.stride(1) != 1) held.push_back(g = g.contiguous());
         bs_matrix t{};

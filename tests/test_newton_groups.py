@@ -34,3 +34,18 @@ def test_groups(B, R, C, precise):
         alone = orthogonalize(G[i], precise=precise).float()
         assert (got[i].float() - alone).norm() < 4e-3 * alone.norm(), i
     assert torch.equal(got, orthogonalize(G, precise=precise))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(32768, 32768), (16384, 65536), (8, 65537)])
+def test_refused_before_memory_is_taken(R, C):
+    """(a view that takes no memory itself)"""
+    from bitsparse_amd.muon import muon_update_, orthogonalize
+    G = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(R, C)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    with pytest.raises(ValueError, match="65536"):
+        orthogonalize(G)
+    with pytest.raises(ValueError):
+        muon_update_([G], [G], [G], lr=0.1)
+    assert torch.cuda.max_memory_allocated() == before
