@@ -1009,11 +1009,7 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
     struct Key {
         int64_t m, n;
         int g, mt, w, dev;
-        double s;
-        bool operator<(const Key& o) const
-        {
-            return std::tie(m, n, g, mt, w, dev, s) < std::tie(o.m, o.n, o.g, o.mt, o.w, o.dev, o.s);
-        }
+        bool operator<(const Key& o) const { return std::tie(m, n, g, mt, w, dev) < std::tie(o.m, o.n, o.g, o.mt, o.w, o.dev); }
     };
     std::map<Key, std::vector<bs_matrix>> groups;
     std::map<int, Tensor> on;
@@ -1040,8 +1036,9 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         t.transposed = R > C;
         // 0.2 sqrt(max): updates of the size of Adam's; sqrt(rows / columns) for tall ones
         const double s = by_rms ? 0.2 * std::sqrt((double)std::max(R, C)) : scale < 0 ? std::sqrt(std::max(1.0, (double)R / (double)C)) : scale;
+        t.rate = (float)(lr * s);
         const Key key{std::min(R, C), std::max(R, C), row_type(g, "a gradient"), row_type(M[i], "a momentum"),
-                      row_type(W[i], "a parameter"), W[i].get_device(), s};
+                      row_type(W[i], "a parameter"), W[i].get_device()};
         groups[key].push_back(t);
         on.emplace(key.dev, W[i]);
     }
@@ -1054,7 +1051,7 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         rule.precise = precise.value_or(key.w == BS_DT_F32);
         rule.steps = (int)steps;
         rule.a = (float)a, rule.b = (float)b, rule.c = (float)c, rule.eps = (float)eps, rule.mu = (float)mu, rule.fresh = (float)(1.0 - mu);
-        rule.keep = (float)(1.0 - lr * decay), rule.rate = (float)(lr * key.s);
+        rule.keep = (float)(1.0 - lr * decay);
         newton_group(mats, key.m, key.n, rule, like);
     }
     // (autograd's saved copies of the parameters are stale now)

@@ -60,6 +60,7 @@ struct NsMatrix {
     void* w;                            // weights, or the result
     int64_t g_stride, m_stride, w_stride;
     int tall;                           // given as [n, m]
+    float rate;                         // of its update
 };
 struct NsMatrices {
     NsMatrix at[kNsBatch];
@@ -236,7 +237,7 @@ struct NsGemm {
     // last
     int64_t m, n;
     int w_f32, update;
-    float keep, rate;
+    float keep;
 };
 
 constexpr int kScratch = 16 * 36 * 4;  // bytes of LDS for a wave's results on their way out
@@ -386,7 +387,7 @@ __device__ __forceinline__ void ns_finish(const NsGemm& g, const NsGiven<KIND>& 
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 o[e] = s[(lane >> 2) * 36 + 8 * (lane & 3) + e] * (1.f / (kHeld * kHeld));
-                if (g.update) o[e] = g.keep * w[e] - g.rate * o[e];
+                if (g.update) o[e] = g.keep * w[e] - mat.rate * o[e];
             }
             if (g.w_f32)
                 store_raw(static_cast<float*>(mat.w) + at, to_raw<float>(o), nv);
@@ -1331,7 +1332,7 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         for (int64_t i = 0; i < here; i++) {
             const bs_matrix& t = matrices[first + i];
             const bool tall = (t.transposed ? cols : rows) > (t.transposed ? rows : cols);
-            mats.at[i] = {t.grad, t.momentum, t.out, t.grad_stride, t.momentum_stride, t.out_stride, tall};
+            mats.at[i] = {t.grad, t.momentum, t.out, t.grad_stride, t.momentum_stride, t.out_stride, tall, t.rate};
         }
         char* ws = static_cast<char*>(workspace);
         NsPrep a{};
@@ -1353,7 +1354,7 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
         NsGemm g{};
         g.passes = precise ? 3 : 1, g.a = r.a, g.b = r.b, g.c = r.c;
         g.part = reinterpret_cast<float*>(at + 2 * p.x_bytes + 2 * p.a_bytes);
-        g.m = m, g.n = n, g.w_f32 = r.out_type == BS_DT_F32, g.update = r.update, g.keep = r.keep, g.rate = r.rate;
+        g.m = m, g.n = n, g.w_f32 = r.out_type == BS_DT_F32, g.update = r.update, g.keep = r.keep;
         ns_products(p, w, g, mats, here, r.steps, st);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));

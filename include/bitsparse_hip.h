@@ -49,7 +49,7 @@ extern "C" {
 const char* bs_last_error(void);
 
 /* ABI version (bumped when an entry point changes): of this header, and of a built library. */
-#define BS_ABI_VERSION 19
+#define BS_ABI_VERSION 20
 int bs_abi_version(void);
 
 /*
@@ -735,13 +735,14 @@ typedef struct bs_matrix {
     void* out;
     int64_t grad_stride, momentum_stride, out_stride;
     int transposed;
+    float rate;                      /* of its update */
 } bs_matrix;
 typedef struct bs_newton_schulz_rule {
     int grad_type, momentum_type, out_type;     /* BS_DT_BF16 or BS_DT_F32 */
     int momentum, nesterov, update;             /* flags */
     int precise;                     /* flag: operands of 22 bits */
     int steps;
-    float a, b, c, eps, mu, keep, rate;
+    float a, b, c, eps, mu, keep;
     float fresh;                     /* 1 - mu, rounded by itself: 1 - (float)mu is off by 2^-25 / (1 - mu) of it */
 } bs_newton_schulz_rule;
 int64_t bs_newton_schulz_workspace_bytes(int64_t rows, int64_t cols, int64_t count, int precise);

@@ -49,3 +49,29 @@ def test_refused_before_memory_is_taken(R, C):
     with pytest.raises(ValueError):
         muon_update_([G], [G], [G], lr=0.1)
     assert torch.cuda.max_memory_allocated() == before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("adjust", ["shape", "rms", 0.3])
+def test_transposes_go_together(adjust):
+    """W1 [H, D] and W2 [D, H] of two blocks in one call of the products, whatever the scale of each one's step: the call's
+    scratch is that of four matrices.  Each is stepped as orthogonalize says, both in half a unit of bf16 (2^-8 at most, and
+    1.7e-3 of the 2-norm) and 1e-3 of the exact one."""
+    import math
+
+    from bitsparse_amd.muon import muon_update_, orthogonalize
+    D, H = 256, 1024
+    g = torch.Generator(device="cuda").manual_seed(3)
+    shapes = [(H, D), (D, H), (H, D), (D, H)]
+    G = [torch.randn(s, generator=g, device="cuda").to(torch.bfloat16) for s in shapes]
+    W = [torch.zeros(s, device="cuda", dtype=torch.bfloat16) for s in shapes]
+    M = [torch.zeros(s, device="cuda") for s in shapes]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    muon_update_(W, G, M, lr=0.5, momentum=0.0, adjust=adjust)
+    assert torch.cuda.max_memory_allocated() - before >= _lib.load().bs_newton_schulz_workspace_bytes(D, H, 4, 0)
+    for w, x, (r, c) in zip(W, G, shapes):
+        s = {"shape": math.sqrt(max(1, r / c)), "rms": 0.2 * math.sqrt(max(r, c))}.get(adjust, adjust)
+        want = -0.5 * s * orthogonalize(x).float()
+        assert (w.float() - want).norm() < 5.4e-3 * want.norm()
