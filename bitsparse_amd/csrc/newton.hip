@@ -1299,6 +1299,8 @@ extern "C" int bs_newton_schulz(const bs_matrix* matrices, int64_t count, int64_
     if (m * n >= (int64_t(1) << 29)) return set_error(BS_ERR_INVALID, "%s: rows*cols must be < 2^29", what);
     const bs_newton_schulz_rule& r = *rule;
     if (r.steps < 1 || r.steps > 100) return set_error(BS_ERR_INVALID, "%s: steps must be in 1..100, got %d", what, r.steps);
+    // (the bounds on X start from ||X_0|| <= 1)
+    if (!(r.eps >= 0.f)) return set_error(BS_ERR_INVALID, "%s: eps must not be negative, got %g", what, r.eps);
     if (!ns_in_range(r.a, r.b, r.c, r.steps))
         return set_error(BS_ERR_INVALID, "%s: the coefficients %g, %g, %g take values past 15, out of the operands' range", what, r.a, r.b, r.c);
     auto known = [](int t) { return t == BS_DT_BF16 || t == BS_DT_F32; };

@@ -718,7 +718,7 @@ int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* work
  * `count` matrices, [rows, cols] or (transposed) [cols, rows]:
  *   with a momentum: M <- mu M + fresh G and U = fresh G + mu M
  *   (nesterov) or M, of M as stored; without: U = G
- *   X = U / (||U||_F + eps); `steps` times X <- (a I + b A + c A^2) X with
+ *   X = U / (||U||_F + eps), eps >= 0; `steps` times X <- (a I + b A + c A^2) X with
  *   A = X X^T (of the transpose, where U has more rows than columns)
  *   out <- X, or (update) out <- keep * out - rate * X
  * G, M and out are bf16 or fp32, each type the same for all matrices, with

@@ -20,3 +20,17 @@ def test_momentum_in_32_bits(mu, shape):
         old, fresh = mu * M.double(), (1 - mu) * G.double()
         muon_update_([W], [G], [M], lr=0.1, momentum=mu)
         assert ((M.double() - (old + fresh)).abs() <= 4 * 2.0 ** -24 * (old.abs() + fresh.abs())).all()
+
+
+@pytest.mark.parametrize("eps", [-1e-3, -1e30, float("nan")])
+def test_eps(eps):
+    """An X_0 past a norm of 1 would leave the operands' range unseen: refused, with nothing touched."""
+    from bitsparse_amd.muon import muon_update_, orthogonalize
+    G = _randn(20, 30)
+    with pytest.raises(ValueError, match="eps"):
+        orthogonalize(G, eps=eps)
+    W, M = G.clone(), G.clone()
+    with pytest.raises(ValueError, match="eps"):
+        muon_update_([W], [G], [M], lr=0.1, eps=eps)
+    assert torch.equal(W, G) and torch.equal(M, G)
+    assert orthogonalize(G, eps=0.0).isfinite().all()
