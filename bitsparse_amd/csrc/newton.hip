@@ -198,7 +198,9 @@ __global__ __launch_bounds__(256) void ns_scale_kernel(NsPrep a, NsMatrices mats
         if ((int)threadIdx.x < w) s_q[threadIdx.x] += s_q[threadIdx.x + w];
         __syncthreads();
     }
-    const float norm = (float)sqrt(s_q[0]) + a.eps;
+    // (a norm past fp32's range, of elements inside it: of U 2^-40 instead)
+    const double norm64 = sqrt(s_q[0]);
+    const float down = norm64 > 1e38 ? 0x1p-40f : 1.f, norm = (float)(norm64 * (double)down) + a.eps * down;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const int r = k * 32 + (int)threadIdx.x / 8, c = (int)threadIdx.x % 8 * 8;
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(256) void ns_scale_kernel(NsPrep a, NsMatrices mats
         f16x8 h;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            v[e] = (t.tall ? s_t[r][c + e] : u[k][e]) / norm * kHeld;
+            v[e] = (t.tall ? s_t[r][c + e] : u[k][e]) * down / norm * kHeld;
             h[e] = (_Float16)v[e];
         }
         _Float16* out = a.x + (int64_t)blockIdx.z * a.pitch * a.np + panel_at(a.pitch, i0 + r, j0 + c);

@@ -34,3 +34,12 @@ def test_eps(eps):
         muon_update_([W], [G], [M], lr=0.1, eps=eps)
     assert torch.equal(W, G) and torch.equal(M, G)
     assert orthogonalize(G, eps=0.0).isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,C", [(200, 300), (300, 200), (1, 5000)])
+def test_norm_past_fp32(dtype, R, C):
+    """Elements near fp32's largest, whose norm is past it: a power of two off, the same bits (eps counts in neither)."""
+    from bitsparse_amd.muon import orthogonalize
+    G = (_randn(R, C).clamp(-3, 3) * 2.0 ** 126 / 3).to(dtype)
+    assert torch.equal(orthogonalize(G), orthogonalize(G * 2.0 ** -60)) and orthogonalize(G).any()
