@@ -14,9 +14,9 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <map>
 #include <memory>
-#include <set>
 
 #include "bitsparse_hip.h"
 
@@ -996,6 +996,42 @@ Tensor orthogonalize(const Tensor& G, int64_t steps, double a, double b, double 
     return out;
 }
 
+// The memory of one matrix of an update: `rows` runs of `run` bytes, `stride` apart.
+struct MatrixSpan {
+    const char *from, *to;
+    int64_t stride, run, rows;
+    char list;                      // W, M or G
+    size_t at;                      // place in it
+    MatrixSpan(const void* p, int64_t stride_, int64_t cols, int64_t rows_, int64_t size, char list_, size_t at_)
+        : from(static_cast<const char*>(p)), stride(stride_ * size), run(cols * size), rows(rows_), list(list_), at(at_)
+    {
+        to = from + (rows - 1) * stride + run;
+    }
+    bool meets(const MatrixSpan& o) const       // (columns of one buffer may lie between each other's)
+    {
+        for (int64_t i = 0, j = 0; i < rows && j < o.rows;) {
+            const char *a = from + i * stride, *b = o.from + j * o.stride;
+            if (a < b + o.run && b < a + run) return true;
+            (a + run < b + o.run ? i : j)++;
+        }
+        return false;
+    }
+};
+
+// M is written between two reads of every G, and a W after the Gs of its group
+// are read: what is written lies apart, and a G from every M and other W.
+void check_apart(std::vector<MatrixSpan>& spans)
+{
+    std::sort(spans.begin(), spans.end(), [](const MatrixSpan& a, const MatrixSpan& b) { return a.from < b.from; });
+    for (size_t i = 0; i < spans.size(); i++)
+        for (size_t j = i + 1; j < spans.size() && spans[j].from < spans[i].to; j++) {
+            const MatrixSpan &a = spans[i], &b = spans[j];
+            if ((a.list == 'G' && b.list == 'G') || (a.at == b.at && a.list + b.list == 'G' + 'W')) continue;
+            auto name = [](char list) { return list == 'W' ? "parameter " : list == 'M' ? "the momentum of parameter " : "the gradient of parameter "; };
+            TORCH_CHECK_VALUE(!a.meets(b), name(a.list), a.at, " and ", name(b.list), b.at, " share memory");
+        }
+}
+
 // The update of lists of weights: matrices of one shape (up to transposition)
 // and set of types go together.  All are checked before the first is touched.
 void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, const std::vector<Tensor>& M, double lr, double mu,
@@ -1014,7 +1050,8 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
     std::map<Key, std::vector<bs_matrix>> groups;
     std::map<int, Tensor> on;
     std::vector<Tensor> held;
-    std::set<const void*> written;
+    std::vector<MatrixSpan> spans;
+    spans.reserve(3 * W.size());
     for (size_t i = 0; i < W.size(); i++) {
         check_matrix(W[i], "a parameter");
         check_matrix(G[i], "a gradient");
@@ -1023,8 +1060,6 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
                           ", its gradient ", G[i].sizes(), " and momentum ", M[i].sizes(), " differ in shape");
         TORCH_CHECK(G[i].device() == W[i].device() && M[i].device() == W[i].device(), "parameter ", i,
                     ", its gradient and momentum are on different devices");
-        TORCH_CHECK_VALUE(written.insert(W[i].data_ptr()).second && written.insert(M[i].data_ptr()).second,
-                          "parameter ", i, " or its momentum is in the lists twice");
         const int64_t R = W[i].size(0), C = W[i].size(1);
         check_size(R, C, "parameter ", i);
         Tensor g = G[i];
@@ -1034,6 +1069,9 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         t.momentum = M[i].data_ptr(), t.momentum_stride = matrix_stride(M[i], "a momentum");
         t.out = W[i].data_ptr(), t.out_stride = matrix_stride(W[i], "a parameter");
         t.transposed = R > C;
+        spans.emplace_back(t.grad, t.grad_stride, C, R, g.element_size(), 'G', i);
+        spans.emplace_back(t.momentum, t.momentum_stride, C, R, M[i].element_size(), 'M', i);
+        spans.emplace_back(t.out, t.out_stride, C, R, W[i].element_size(), 'W', i);
         // 0.2 sqrt(max): updates of the size of Adam's; sqrt(rows / columns) for tall ones
         const double s = by_rms ? 0.2 * std::sqrt((double)std::max(R, C)) : scale < 0 ? std::sqrt(std::max(1.0, (double)R / (double)C)) : scale;
         t.rate = (float)(lr * s);
@@ -1042,6 +1080,7 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         groups[key].push_back(t);
         on.emplace(key.dev, W[i]);
     }
+    check_apart(spans);
     for (const auto& [key, mats] : groups) {
         const Tensor& like = on.at(key.dev);
         const c10::DeviceGuard guard(like.device());

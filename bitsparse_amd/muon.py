@@ -59,7 +59,8 @@ def muon_update_(params: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seq
     (``"rms"``: updates of the size that Adam's have) or the number given.
     precise: products of 22-bit operands, by default for float32 weights.
     Each of the three lists is bfloat16 or float32; W and M have contiguous
-    rows, their own memory, and are updated on the current stream."""
+    rows, their own memory (shared with no other matrix of the lists; a G with its own W
+    at most), and are updated on the current stream."""
     if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0:
         raise ValueError(f"lr and weight_decay must not be negative and momentum be in [0, 1), got lr={lr}, "
                          f"weight_decay={weight_decay}, momentum={momentum}")
