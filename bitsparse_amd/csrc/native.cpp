@@ -11,6 +11,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 
@@ -1056,6 +1057,9 @@ void muon_update(const std::vector<Tensor>& W, const std::vector<Tensor>& G, con
         check_matrix(W[i], "a parameter");
         check_matrix(G[i], "a gradient");
         check_matrix(M[i], "a momentum");
+        for (const Tensor* t : {&W[i], &M[i]})
+            TORCH_CHECK(!t->is_inference() || c10::InferenceMode::is_enabled(), "parameter ", i,
+                        " or its momentum is an inference tensor: no update in place outside InferenceMode");
         TORCH_CHECK_VALUE(G[i].sizes() == W[i].sizes() && M[i].sizes() == W[i].sizes(), "parameter ", i, " ", W[i].sizes(),
                           ", its gradient ", G[i].sizes(), " and momentum ", M[i].sizes(), " differ in shape");
         TORCH_CHECK(G[i].device() == W[i].device() && M[i].device() == W[i].device(), "parameter ", i,

@@ -42,3 +42,21 @@ def test_apart():
         _update(*apart)
         _update(W, G, M)
         assert all(torch.equal(t, u) for ts, us in zip((W, M), (apart[0], apart[2])) for t, u in zip(ts, us))
+
+
+def test_inference_tensors():
+    """Not updated outside inference mode, like any tensor made there: refused before the first matrix is touched."""
+    with torch.inference_mode():
+        made = torch.randn(20, 30, device="cuda")
+    for k in range(2):
+        W, G, M = (_randn(20, 30, seed=i) for i in range(3))
+        V = W.clone()
+        lists = ([W, made], [G, G], [M, V]) if k == 0 else ([W, V], [G, G], [M, made])
+        before = [t.clone() for t in (W, M, V, made)]
+        with pytest.raises(RuntimeError, match="inference"):
+            _update(*lists)
+        assert all(torch.equal(t, u) for t, u in zip((W, M, V, made), before))
+    with torch.inference_mode():
+        W, N = made.clone(), made.clone()
+        _update([W], [G], [N])
+        assert not torch.equal(W, made)
