@@ -14,8 +14,10 @@
 // A and B are held as fp16 times 2^12: ||X_0|| <= 1 keeps every singular
 // value of the iteration below 1.21 and so every element of X, A and B below
 // 3.5 (other coefficients: refused where they leave fp16's range), and elements down to 2^-26 keep all 11 bits.
-// On gradients the result is 1.0-2.4e-3 from the exact one so (bf16 operands,
-// three bits shorter: 1.0-2.0e-2), where rounding it to bf16 costs 1.7e-3.
+// On gradients of full rank the result is 1.0-2.4e-3 from the exact one so (bf16
+// operands, three bits shorter: 1.0-2.0e-2), where rounding it to bf16 costs
+// 1.7e-3.  With t tokens, fewer than rows, the rounding noise in the directions
+// without a gradient is raised by a = 3.44 a step, to about 0.16 / sqrt(t).
 //
 // Where the result goes into fp32 weights that is not enough: there each of X,
 // A and B is held as two fp16 numbers, the value and what is left of it (22

@@ -724,8 +724,9 @@ int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* work
  * G, M and out are bf16 or fp32, each type the same for all matrices, with
  * contiguous rows `*_stride` elements apart.  Products have fp16 operands and
  * fp32 sums: X comes to 1-3e-3 of the exact result for a gradient of full
- * rank.  With `precise` every operand is two fp16 numbers and a product three:
- * 2e-6, at a third of the speed.  Coefficients that take X (but the last), A,
+ * rank, to about 0.16 / sqrt(t) for one of t tokens, fewer than rows.  With
+ * `precise` every operand is two fp16 numbers and a product three:
+ * 2e-6 (one token: 1e-4), at a third of the speed.  Coefficients that take X (but the last), A,
  * a I + b A + c A^2 or b X + c A X past 15 for some U are refused: fp16
  * operands do not hold them.
  */
