@@ -5,8 +5,8 @@
 // A row of D elements is D / 8 chunks.  ceil(D / 512) waves hold a row, a
 // chunk a lane, and a workgroup holds as many rows as its eight waves make
 // (longer rows: 16 waves, and two or four chunks a lane).  The whole row then
-// stays in registers between the passes that its statistics take, and it is
-// read once.
+// stays with its lanes between the passes that its statistics take, and it is
+// read once; with one chunk a lane all of it is in registers.
 #pragma once
 
 #include "bs_device.h"

@@ -14,11 +14,15 @@
 // b_post B, so five sums a column serve all six vectors.
 //
 // Bound by memory: dx', dh, x', y (and x for dscale; y not where no gradient is formed of it) read once, dx and dy
-// written once, a row in registers throughout.  Each workgroup keeps its
-// column sums in registers over all its rows and writes one row of partial
-// sums; the second kernel adds those in order.  No atomics: the same bits at
-// every call.  16384 x 4096 in bf16: 182 us, 5.2 TB/s (a copy reaches 5.15);
-// 8192 x 768, which stays in the last level cache: 23 us, 3.8 TB/s.
+// written once, a row with its lanes throughout.  Each workgroup keeps its
+// column sums over all its rows and writes one row of partial sums; the second
+// kernel adds those in order.  No atomics: the same bits at every call.
+// 16384 x 4096 in bf16: 182 us, 5.2 TB/s (a copy reaches 5.15); 8192 x 768,
+// which stays in the last level cache: 23 us, 3.8 TB/s.  Up to 4096 elements
+// row, sums and vectors are in registers.  Past that they do not all fit (the
+// join's spill 40 to 90 registers a lane up to 8192 elements, 630 to 960 up to
+// 16384, 1200 to 1600 beyond): 8192 x 8192 297 us, 3.2 TB/s; 4096 x 16384 1.49
+// ms, 0.63 TB/s; 2048 x 32768 1.94 ms.
 #include <algorithm>
 
 #include "bs_host.h"
