@@ -860,6 +860,20 @@ struct Join : torch::autograd::Function<Join> {
         }
         if (c.rows == 0) return out;
 
+        // (hooks on saved tensors may hand back others than were saved)
+        const at::IntArrayRef shape(node.operands[0].shape);
+        auto as_saved = [&](const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const char* what) {
+            if (!t.defined()) return;
+            plain_on_gpu(t, what);
+            TORCH_CHECK(t.device() == node.options.device() && t.scalar_type() == type && t.sizes() == sizes, what,
+                        ": expected what was saved, ", type, " ", sizes, " on ", node.options.device(), ", got ", t.scalar_type(),
+                        " ", t.sizes(), " on ", t.device());
+        };
+        static constexpr const char* names[8] = {"x", "y", "post.weight", "post.bias", "gate", "scale", "pre.weight", "x'"};
+        for (int i = 0; i < 7; i++) as_saved(saved[i], node.operands[i].shape, node.operands[i].type, names[i]);
+        as_saved(saved[7], shape, node.operands[0].type, names[7]);
+        as_saved(saved[8], {2, c.rows, 2}, at::kFloat, "the rows' statistics");
+
         c.a.x = kUnread;
         if (saved[0].defined()) c.put_x(saved[0]);
         if (c.a.y) c.a.y = kUnread;
@@ -875,7 +889,7 @@ struct Join : torch::autograd::Function<Join> {
         put(c.a.weight_pre, saved[6]);
         put(c.a.bias_pre, Tensor());
         bs_join_grads g{};
-        const Tensor st = saved[8];
+        const Tensor st = saved[8].defined() ? saved[8].contiguous() : Tensor();
         if (st.defined()) {
             c.a.stats_post = st.data_ptr<float>();
             c.a.stats_pre = c.a.stats_post + 2 * c.rows;
@@ -887,8 +901,7 @@ struct Join : torch::autograd::Function<Join> {
         }
         auto grad_rows = [&](const Tensor& t, int type, const char* what) {
             plain_on_gpu(t, what);
-            TORCH_CHECK_VALUE(t.sizes() == at::IntArrayRef(node.operands[0].shape), what, ": expected ",
-                              at::IntArrayRef(node.operands[0].shape), ", got ", t.sizes());
+            TORCH_CHECK_VALUE(t.sizes() == shape, what, ": expected ", shape, ", got ", t.sizes());
             TORCH_CHECK_TYPE(row_type(t, what) == type, what, ": unexpected dtype ", t.scalar_type());
             return as_rows(t, c.cols);
         };

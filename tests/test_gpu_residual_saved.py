@@ -108,3 +108,29 @@ def test_changed_in_place():
                           (lambda c, out: c["y"].zero_(), ("gate",))):
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             grads(change, "rms", "rms", (g_x, g_h), names)
+
+
+@pytest.mark.parametrize("change", [lambda t: t.cpu(), lambda t: t.to(torch.float64), lambda t: t[..., :1].contiguous(),
+                                    lambda t: t.flatten()[:1], lambda t: t[None]])
+def test_hooks_that_hand_back_something_else(change):
+    """Refused on the host, whichever of the saved tensors it is; the same values at another address are taken."""
+    t, g_x, g_h = _operands("element", F32)
+    n = len(_saved(_learn(t, NAMES), "rms", "layer")[0])
+    assert n == 9                       # x, y, three of the vectors and post's bias, gate, x', statistics
+    for which in range(n):
+        c, seen = _learn(t, NAMES), []
+
+        def pack(v):
+            seen.append(v)
+            return len(seen) - 1, v
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda p: change(p[1]) if p[0] == which else p[1].clone()):
+            out = _call(c, "rms", "layer")
+            with pytest.raises((RuntimeError, ValueError, TypeError)):
+                torch.autograd.grad(out, [c[k] for k in NAMES], (g_x, g_h))
+                pytest.fail(str(which))
+    want = _learn(t, NAMES)
+    want = torch.autograd.grad(_call(want, "rms", "layer"), [want[k] for k in NAMES], (g_x, g_h))
+    c = _learn(t, NAMES)
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: v.T.contiguous().T if v.dim() == 2 else v.clone()):
+        got = torch.autograd.grad(_call(c, "rms", "layer"), [c[k] for k in NAMES], (g_x, g_h))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
