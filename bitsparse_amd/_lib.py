@@ -17,7 +17,7 @@ LIB_NAME = "libbitsparse_hip.so"
 # BITSPARSE_HIP_LIB points at another build of the same sources (tuning sweeps)
 LIB_PATH = os.environ.get("BITSPARSE_HIP_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 BS_OK = 0
 BS_ERR_INVALID = 1
@@ -95,6 +95,19 @@ _SIGNATURES = {
     "bs_join_forward": [_vp, _vp, _vp, _vp],
     "bs_join_backward_workspace_bytes": [_i64, _i64],
     "bs_join_backward": [_vp, _vp, _vp, _i64, _vp],
+    "bs_dropout": [_vp, _vp, _int, _i64, _i64, _i64, _vp, _vp],
+    "bs_join_drop_forward": [_vp, _vp, _vp, _vp, _vp],
+    "bs_join_drop_backward": [_vp, _vp, _vp, _vp, _i64, _vp],
+    "bs_route_forward": [_vp, _vp, _vp, _vp],
+    "bs_route_backward": [_vp, _vp, _vp, _vp, _vp],
+    "bs_expert_plan": [_vp, _i64, _int, _vp, _vp, _vp, _vp],
+    "bs_expert_linear": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _int, _f32, _vp, _vp],
+    "bs_expert_linear_dx": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
+    "bs_expert_linear_dw": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
+    "bs_pad_rows": [_vp, _i64, _i64, _i64, _vp, _i64, _vp],
+    "bs_expert_combine": [_vp, _i64, _vp, _vp, _i64, _int, _i64, _i64, _vp, _vp],
+    "bs_expert_combine_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _int, _i64, _i64, _vp, _vp, _vp],
+    "bs_experts_act_grad": [_vp, _vp, _i64, _i64, _int, _f32, _vp, _vp, _vp, _i64, _vp, _vp],
     "bs_newton_schulz_workspace_bytes": [_i64, _i64, _i64, _int],
     "bs_newton_schulz": [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp],
     "bs_launch_timing": [_int],

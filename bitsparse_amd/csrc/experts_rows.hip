@@ -1,0 +1,219 @@
+// The experts' rows back into tokens: the weighted sum over a token's choices,
+// its gradients, and the step between the two products of an expert's backward.
+//
+//   out[t] = sum over j of w[t, j] y[place[t, j]]        (32-bit sums in the order of j)
+//   dy[place[t, j]] = w[t, j] dout[t];  dw[t, j] = <dout[t], y[place[t, j]]>
+//
+// Bound by memory: y, dout and the results once.  A workgroup a token.
+#include <algorithm>
+
+#include "bs_host.h"
+#include "rownorm.h"
+
+namespace bs {
+
+constexpr int kMaxChoices = 64;
+constexpr int kTailBlocks = 64;     // workgroups that clear the rows behind the last expert's
+
+struct CombineArgs {
+    int64_t tokens, rows, cols;
+    int top_k;
+    const bf16* y;
+    int64_t y_stride;
+    const float* weights;       // null: 1
+    const int32_t *place, *used;        // used: rows that belong to an expert
+    bf16* out;
+    // backward
+    const bf16* g;
+    int64_t g_stride;
+    bf16* dy;
+    float* dw;
+};
+
+template <bool WHOLE>
+__global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
+{
+    const int64_t t = blockIdx.x;
+    const int32_t* place = a.place + t * a.top_k;
+    for (int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8; c < a.cols; c += (int64_t)gridDim.y * 2048) {
+        const int nv = (int)min((int64_t)8, a.cols - c);
+        float acc[8] = {};
+        for (int j = 0; j < a.top_k; j++) {
+            const int p = place[j];
+            if (p < 0 || p >= a.rows) continue;
+            const float w = a.weights ? a.weights[t * a.top_k + j] : 1.f;
+            const Raw<bf16> y = load_raw<WHOLE>(a.y + p * a.y_stride + c, nv);
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[e] = fmaf(w, raw_get(y, e), acc[e]);
+        }
+        store_raw<WHOLE>(a.out + t * a.cols + c, to_raw<bf16>(acc), nv);
+    }
+}
+
+// dy and dw; either may be absent
+template <bool WHOLE>
+__global__ __launch_bounds__(256) void combine_backward_kernel(CombineArgs a)
+{
+    __shared__ float s_dot[4][kMaxChoices];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if ((int64_t)blockIdx.x >= a.tokens) {
+        if (a.dy == nullptr) return;
+        for (int64_t r = max(0, *a.used) + (blockIdx.x - a.tokens); r < a.rows; r += kTailBlocks)
+            for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048)
+                store_raw<WHOLE>(a.dy + r * a.cols + c, Raw<bf16>{}, (int)min((int64_t)8, a.cols - c));
+        return;
+    }
+    const int64_t t = blockIdx.x;
+    for (int j = 0; j < a.top_k; j++) {
+        const int p = a.place[t * a.top_k + j];
+        const bool there = p >= 0 && p < a.rows;
+        const float w = a.weights ? a.weights[t * a.top_k + j] : 1.f;
+        float dot = 0.f;
+        if (there)
+            for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+                const int nv = (int)min((int64_t)8, a.cols - c);
+                const Raw<bf16> g = load_raw<WHOLE>(a.g + t * a.g_stride + c, nv);
+                if (a.dy) {
+                    float o[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) o[e] = w * raw_get(g, e);
+                    store_raw<WHOLE>(a.dy + p * a.cols + c, to_raw<bf16>(o), nv);
+                }
+                if (a.dw) {
+                    const Raw<bf16> y = load_raw<WHOLE>(a.y + p * a.y_stride + c, nv);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) dot = fmaf(raw_get(g, e), raw_get(y, e), dot);
+                }
+            }
+        if (a.dw) {
+            dot = wave_sum_f32(dot);
+            if (lane == 0) s_dot[wave][j] = dot;
+        }
+    }
+    if (a.dw == nullptr) return;
+    __syncthreads();
+    if ((int)threadIdx.x < a.top_k)
+        a.dw[t * a.top_k + threadIdx.x] = (s_dot[0][threadIdx.x] + s_dot[1][threadIdx.x]) + (s_dot[2][threadIdx.x] + s_dot[3][threadIdx.x]);
+}
+
+// The backward of y = sum w act(z) W2^T between its products, a workgroup a
+// row.  g = dout W2 (of the row's token), r = the saved activation relu(z);
+// h = r or bf16(bf16(r r) k):
+//   dw = <g, h>;  dz = w g [r > 0] or w g 2 k r;  and w h, W2's right operand
+struct ActGradArgs {
+    int64_t rows, cols, pairs;
+    int square;
+    float k;
+    const float* weights;
+    const int32_t *order, *used;
+    bf16 *g, *r;                // in: g, r; out: dz, w h
+    float* dw;
+};
+
+template <bool WHOLE>
+__global__ __launch_bounds__(256) void experts_act_grad_kernel(ActGradArgs a)
+{
+    __shared__ float s_dot[4];
+    const int64_t row = blockIdx.x;
+    const int pair = row < *a.used ? a.order[row] : -1;
+    const bool there = pair >= 0 && pair < a.pairs;
+    const float w = there ? a.weights[pair] : 0.f;
+    float dot = 0.f;
+    for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+        const int nv = (int)min((int64_t)8, a.cols - c);
+        const Raw<bf16> g = load_raw<WHOLE>(a.g + row * a.cols + c, nv), r = load_raw<WHOLE>(a.r + row * a.cols + c, nv);
+        float dz[8], wh[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float x = raw_get(r, e), ge = raw_get(g, e);
+            const float h = a.square ? bf16_to_f32(relu2_sq_bits(__float_as_uint(x) >> 16, a.k)) : x;
+            // (select, not a product: a gradient of infinity where nothing came through is 0)
+            dz[e] = !there || x == 0.f ? 0.f : a.square ? w * ge * (2.f * a.k * x) : w * ge;
+            wh[e] = there ? w * h : 0.f;
+            dot += h == 0.f ? 0.f : ge * h;
+        }
+        store_raw<WHOLE>(a.g + row * a.cols + c, to_raw<bf16>(dz), nv);
+        store_raw<WHOLE>(a.r + row * a.cols + c, to_raw<bf16>(wh), nv);
+    }
+    if (a.dw == nullptr) return;
+    dot = wave_sum_f32(dot);
+    if ((threadIdx.x & 63) == 0) s_dot[threadIdx.x >> 6] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0 && there) a.dw[pair] = (s_dot[0] + s_dot[1]) + (s_dot[2] + s_dot[3]);
+}
+
+static int combine_check(const char* what, int64_t tokens, int top_k, int64_t rows, int64_t cols)
+{
+    if (tokens < 0 || rows < 0 || cols < 0 || top_k < 1 || top_k > kMaxChoices || tokens >= (1ll << 31) - kTailBlocks || rows >= (1ll << 31) ||
+        (cols && std::max(tokens, rows) >= (1ll << 40) / cols))
+        return set_error(BS_ERR_INVALID, "%s: top_k must be in 1..%d, tokens and rows below 2^31, rows*cols below 2^40, got %lld, %d, %lld x %lld",
+                         what, kMaxChoices, (long long)tokens, top_k, (long long)rows, (long long)cols);
+    return BS_OK;
+}
+
+}  // namespace bs
+
+using namespace bs;
+
+extern "C" int bs_expert_combine(const void* y, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
+                                 int64_t rows, int64_t cols, void* out, void* stream)
+{
+    clear_error();
+    const char* what = "bs_expert_combine";
+    if (const int rc = combine_check(what, tokens, top_k, rows, cols); rc != BS_OK) return rc;
+    if (tokens == 0 || cols == 0) return BS_OK;
+    if ((rows && y == nullptr) || place == nullptr || out == nullptr) return set_error(BS_ERR_INVALID, "%s: null pointer", what);
+    if (y_stride < 0) return set_error(BS_ERR_INVALID, "%s: negative row stride", what);
+    if ((((uintptr_t)y | (uintptr_t)out) & 1u) || (((uintptr_t)weights | (uintptr_t)place) & 3u))
+        return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
+    CombineArgs a{};
+    a.tokens = tokens, a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = static_cast<const bf16*>(y), a.y_stride = y_stride;
+    a.weights = weights, a.place = place, a.out = static_cast<bf16*>(out);
+    const dim3 grid((uint32_t)tokens, (uint32_t)std::min<int64_t>((cols + 2047) / 2048, 65535));
+    auto* kernel = cols % 8 == 0 ? combine_kernel<true> : combine_kernel<false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+}
+
+extern "C" int bs_expert_combine_backward(const void* g, int64_t g_stride, const void* y, int64_t y_stride, const float* weights,
+                                          const int32_t* place, const int32_t* used, int64_t tokens, int top_k, int64_t rows, int64_t cols,
+                                          void* dy, float* dw, void* stream)
+{
+    clear_error();
+    const char* what = "bs_expert_combine_backward";
+    if (const int rc = combine_check(what, tokens, top_k, rows, cols); rc != BS_OK) return rc;
+    if ((dy == nullptr && dw == nullptr) || (tokens == 0 && rows == 0)) return BS_OK;
+    if ((tokens && cols && g == nullptr) || (tokens && place == nullptr) || (dy && used == nullptr) || (dw && rows && cols && y == nullptr))
+        return set_error(BS_ERR_INVALID, "%s: null pointer", what);
+    if (g_stride < 0 || y_stride < 0) return set_error(BS_ERR_INVALID, "%s: negative row stride", what);
+    if ((((uintptr_t)g | (uintptr_t)y | (uintptr_t)dy) & 1u) || (((uintptr_t)weights | (uintptr_t)place | (uintptr_t)used | (uintptr_t)dw) & 3u))
+        return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
+    CombineArgs a{};
+    a.tokens = tokens, a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = static_cast<const bf16*>(y), a.y_stride = y_stride;
+    a.weights = weights, a.place = place, a.used = used, a.g = static_cast<const bf16*>(g), a.g_stride = g_stride;
+    a.dy = static_cast<bf16*>(dy), a.dw = dw;
+    auto* kernel = cols % 8 == 0 ? combine_backward_kernel<true> : combine_backward_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tokens + (dy ? kTailBlocks : 0))), dim3(256), 0, (hipStream_t)stream, a);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+}
+
+extern "C" int bs_experts_act_grad(void* g, void* r, int64_t rows, int64_t cols, int square, float k, const float* weights,
+                                   const int32_t* order, const int32_t* used, int64_t pairs, float* dw, void* stream)
+{
+    clear_error();
+    const char* what = "bs_experts_act_grad";
+    if (rows < 0 || cols < 0 || rows >= (1ll << 31) || (cols && rows >= (1ll << 40) / cols) || pairs < 0)
+        return set_error(BS_ERR_INVALID, "%s: rows must be below 2^31 and rows*cols below 2^40, got %lld x %lld", what, (long long)rows, (long long)cols);
+    if (rows == 0) return BS_OK;
+    if ((cols && (g == nullptr || r == nullptr)) || weights == nullptr || order == nullptr || used == nullptr)
+        return set_error(BS_ERR_INVALID, "%s: null pointer", what);
+    if ((((uintptr_t)g | (uintptr_t)r) & 1u) || (((uintptr_t)weights | (uintptr_t)order | (uintptr_t)used | (uintptr_t)dw) & 3u))
+        return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
+    ActGradArgs a{rows, cols, pairs, square, k, weights, order, used, static_cast<bf16*>(g), static_cast<bf16*>(r), dw};
+    auto* kernel = cols % 8 == 0 ? experts_act_grad_kernel<true> : experts_act_grad_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+}

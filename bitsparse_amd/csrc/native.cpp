@@ -37,7 +37,10 @@ using at::Tensor;
     F(bs_gemm_compressed_b_packed_workspace_bytes) F(bs_gemm_compressed_b_packed)                                \
     F(bs_gemm_compressed_b_fp8_workspace_bytes) F(bs_gemm_compressed_b_fp8) F(bs_gemm_compressed_b_fp8_packed)   \
     F(bs_workspace_amax_slot) F(bs_join_forward) F(bs_join_backward_workspace_bytes) F(bs_join_backward) \
-    F(bs_newton_schulz_workspace_bytes) F(bs_newton_schulz)
+    F(bs_newton_schulz_workspace_bytes) F(bs_newton_schulz) F(bs_dropout) F(bs_join_drop_forward)                \
+    F(bs_join_drop_backward) F(bs_route_forward) F(bs_route_backward) F(bs_expert_plan) F(bs_expert_linear)      \
+    F(bs_expert_linear_dx) F(bs_expert_linear_dw) F(bs_pad_rows) F(bs_expert_combine)                            \
+    F(bs_expert_combine_backward) F(bs_experts_act_grad)
 struct Lib {
 #define F(name) decltype(&::name) name = nullptr;
     BS_FUNCS(F)
@@ -661,11 +664,14 @@ int64_t row_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0
 
 using Maybe = std::optional<Tensor>;
 
+#include "native_experts.h"
+
 // what a step is besides its tensors
 struct JoinKind {
     int64_t post, pre;          // BS_NORM_*
     double eps_post, eps_pre, scale_value;
     at::ScalarType h_type;
+    std::optional<DropKind> drop;
 };
 
 // address of an operand that is there and that this call does not read
@@ -775,8 +781,10 @@ struct JoinCall {
 };
 
 // (x', h, statistics), the undefined ones absent
-std::array<Tensor, 3> join_forward(JoinCall& c, at::IntArrayRef shape, bool stats)
+std::array<Tensor, 3> join_forward(JoinCall& c, at::IntArrayRef shape, bool stats, const std::optional<DropKind>& drop)
 {
+    bs_drop d{};
+    if (drop) d = drop_args(*drop, c.x);
     Tensor x1, h, st;
     if (c.a.y) x1 = at::empty(shape, c.x.options());
     if (c.a.norm_pre) h = at::empty(shape, c.x.options().dtype(c.a.y_type == BS_DT_F32 ? at::kFloat : at::kBFloat16));
@@ -785,7 +793,10 @@ std::array<Tensor, 3> join_forward(JoinCall& c, at::IntArrayRef shape, bool stat
         c.a.stats_post = st.data_ptr<float>();
         c.a.stats_pre = c.a.stats_post + 2 * c.rows;
     }
-    if (c.rows) check(L.bs_join_forward(&c.a, raw(x1), raw(h), stream_of(c.x)), "bs_join_forward");
+    if (c.rows && drop)
+        check(L.bs_join_drop_forward(&c.a, &d, raw(x1), raw(h), stream_of(c.x)), "bs_join_drop_forward");
+    else if (c.rows)
+        check(L.bs_join_forward(&c.a, raw(x1), raw(h), stream_of(c.x)), "bs_join_forward");
     return {x1, h, st};
 }
 
@@ -794,6 +805,7 @@ std::array<Tensor, 3> join_forward(JoinCall& c, at::IntArrayRef shape, bool stat
 struct JoinNode : torch::CustomClassHolder {
     bs_join a;
     int64_t rows, cols;
+    std::optional<DropKind> drop;   // its state is among the saved tensors
     at::TensorOptions options;      // of x
     struct Operand {
         bool there = false;
@@ -810,9 +822,11 @@ struct Join : torch::autograd::Function<Join> {
     {
         const c10::DeviceGuard guard(x.device());
         JoinCall c(x, y, w_post, b_post, gate, scale, w_pre, b_pre, k);
-        const auto [x1, h, st] = join_forward(c, x.sizes(), true);
+        const auto [x1, h, st] = join_forward(c, x.sizes(), true, k.drop);
         auto node = c10::make_intrusive<JoinNode>();
         node->a = c.a, node->rows = c.rows, node->cols = c.cols, node->options = x.options();
+        node->drop = k.drop;
+        if (k.drop) node->drop->state.reset();
         const Maybe first(x);
         const Maybe* all[8] = {&first, &y, &w_post, &b_post, &gate, &scale, &w_pre, &b_pre};
         for (int i = 0; i < 8; i++) {
@@ -828,7 +842,7 @@ struct Join : torch::autograd::Function<Join> {
         ctx->save_for_backward({if_read(!y || learns(scale), x),
                                 if_read(learns(gate) || (k.post != BS_NORM_NONE && (learns(y) || learns(w_post))), y),
                                 if_read(true, w_post), if_read(learns(gate), b_post), if_read(true, gate), if_read(true, scale),
-                                if_read(true, w_pre), y && k.pre != BS_NORM_NONE ? x1 : Tensor(), st});
+                                if_read(true, w_pre), y && k.pre != BS_NORM_NONE ? x1 : Tensor(), st, k.drop && k.drop->state ? *k.drop->state : Tensor()});
         ctx->saved_data["node"] = c10::IValue::make_capsule(node);
         ctx->set_materialize_grads(false);
         if (!c.a.y) return {h};
@@ -917,9 +931,15 @@ struct Join : torch::autograd::Function<Join> {
         g.d_gate = raw(out[4]), g.d_scale = raw(out[5]), g.d_weight_pre = raw(out[6]), g.d_bias_pre = raw(out[7]);
         const int64_t need = L.bs_join_backward_workspace_bytes(c.rows, c.cols);
         const Tensor ws = at::empty({need}, node.options.dtype(at::kByte));
-        check(L.bs_join_backward(&c.a, &g, ws.data_ptr(), need,
-                                 c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(node.options.device().index()).stream()),
-              "bs_join_backward");
+        void* const stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(node.options.device().index()).stream();
+        if (node.drop) {
+            DropKind k = *node.drop;
+            if (saved[9].defined()) k.state = saved[9];
+            const bs_drop d = drop_args(k, ws);
+            check(L.bs_join_drop_backward(&c.a, &g, &d, ws.data_ptr(), need, stream), "bs_join_drop_backward");
+        } else {
+            check(L.bs_join_backward(&c.a, &g, ws.data_ptr(), need, stream), "bs_join_backward");
+        }
         return out;
     }
 };
@@ -927,9 +947,10 @@ struct Join : torch::autograd::Function<Join> {
 // x' and h, each where there is one
 std::vector<Tensor> join(const Tensor& x, const Maybe& y, const Maybe& w_post, const Maybe& b_post, const Maybe& gate,
                          const Maybe& scale, const Maybe& w_pre, const Maybe& b_pre, int64_t post, int64_t pre,
-                         double eps_post, double eps_pre, double scale_value, at::ScalarType h_type)
+                         double eps_post, double eps_pre, double scale_value, at::ScalarType h_type,
+                         const std::optional<DropKind>& drop)
 {
-    const JoinKind k{post, pre, eps_post, eps_pre, scale_value, h_type};
+    const JoinKind k{post, pre, eps_post, eps_pre, scale_value, h_type, drop};
     if (at::GradMode::is_enabled()) {
         bool any = x.requires_grad();
         for (const Maybe* m : {&y, &w_post, &b_post, &gate, &scale, &w_pre, &b_pre}) any = any || (*m && (*m)->requires_grad());
@@ -937,7 +958,7 @@ std::vector<Tensor> join(const Tensor& x, const Maybe& y, const Maybe& w_post, c
     }
     const c10::DeviceGuard guard(x.device());
     JoinCall c(x, y, w_post, b_post, gate, scale, w_pre, b_pre, k);
-    const auto [x1, h, st] = join_forward(c, x.sizes(), false);
+    const auto [x1, h, st] = join_forward(c, x.sizes(), false, k.drop);
     if (!c.a.y) return {h};
     if (!c.a.norm_pre) return {x1};
     return {x1, h};
@@ -1159,7 +1180,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
                                optional(a.cols.scale));
     });
     m.def("col_sum", &col_sum);
-    m.def("join", &join);
+    m.def("join", [](const Tensor& x, const Maybe& y, const Maybe& w_post, const Maybe& b_post, const Maybe& gate, const Maybe& scale,
+                     const Maybe& w_pre, const Maybe& b_pre, int64_t post, int64_t pre, double eps_post, double eps_pre, double scale_value,
+                     at::ScalarType h_type) {
+        return join(x, y, w_post, b_post, gate, scale, w_pre, b_pre, post, pre, eps_post, eps_pre, scale_value, h_type, std::nullopt);
+    });
+    m.def("join_drop", [](const Tensor& x, const Maybe& y, const Maybe& w_post, const Maybe& b_post, const Maybe& gate, const Maybe& scale,
+                          const Maybe& w_pre, const Maybe& b_pre, int64_t post, int64_t pre, double eps_post, double eps_pre,
+                          double scale_value, at::ScalarType h_type, int64_t below, uint64_t seed, uint64_t offset, const Maybe& state) {
+        return join(x, y, w_post, b_post, gate, scale, w_pre, b_pre, post, pre, eps_post, eps_pre, scale_value, h_type,
+                    DropKind{below, seed, offset, state});
+    });
+    m.def("dropout", &dropout);
+    m.def("route", &route);
+    m.def("plan_experts", &plan_experts);
+    m.def("expert_linear", &expert_linear);
+    m.def("expert_combine", &expert_combine);
     m.def("orthogonalize", &orthogonalize);
     m.def("muon_update", &muon_update, py::call_guard<py::gil_scoped_release>());
     m.def("quantize_t", [](const Tensor& x, bool rows) {

@@ -50,13 +50,14 @@ struct JoinBwd {
     float* part;            // [blocks, sums wanted, cols]
     float* part_one;        // [blocks, 2]
     int waves, rows_here;       // of a row, of a workgroup at a time
+    DropRule drop;
 };
 
-// JOIN: there is a y.  C chunks a lane; HOLD: the vectors fit the registers; AHEAD: and the next row's loads.
+// JOIN: there is a y.  DROP: p was dropped out of, by the same factors here.  C chunks a lane; HOLD: the vectors fit the registers; AHEAD: and the next row's loads.
 // WHOLE: rows of a multiple of 8 elements.
 // PLAIN: RMS norms (or none), no gate that differs from row to row, no sums for biases: a third fewer instructions, which
 // two waves a SIMD do not hide behind the loads (16384 x 4096: 182 against 232 us).
-template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD, bool AHEAD, bool PLAIN, bool WHOLE>
+template <typename XT, typename YT, bool JOIN, bool DROP, int C, int MAXT, bool HOLD, bool AHEAD, bool PLAIN, bool WHOLE>
 __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
 {
     __shared__ RowSums s_sums;
@@ -66,6 +67,8 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
     const bool per_row = !PLAIN && a.gate_per == BS_PER_ROW, per_element = !PLAIN && a.gate_per == BS_PER_ELEMENT;
     const bool layer_post = !PLAIN && a.post == BS_NORM_LAYER, layer_pre = !PLAIN && a.pre == BS_NORM_LAYER;
     void* const d_row_gate = PLAIN ? nullptr : a.d_row_gate;
+    DropKey key;
+    if constexpr (DROP) key = drop_key(a.drop);
 
     // the next row's loads are in flight while this row's sums meet
     struct Row {
@@ -175,14 +178,23 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                 if (per_element)
                     param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, ge);
                 if (d_row_gate) param_chunk(a.b_post, at.col[k], nv[k], 0.f, b1);
+                float drop[8];
+                if constexpr (DROP) drop_factors(a.drop, key, (uint32_t)(at.col[k] >> 3), (uint32_t)row, drop);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     // (past the row's end x' and the gradients are 0, and so is G but for a layer norm's mean)
                     const float g0 = PLAIN || e < nv[k] ? G[k][e] : 0.f;
                     o[e] = sc[k][e] * g0;
                     acc[kSumScale][k][e] += g0 * raw_get(now.x[k], e);
-                    const float n = (raw_get(now.y[k], e) - st.x) * st.y;
-                    const float gg = PLAIN ? g0 : per_element ? g0 * ge[e] : rg * g0;    // G of the gate's part that is not a vector
+                    float n = (raw_get(now.y[k], e) - st.x) * st.y;
+                    float gg = PLAIN ? g0 : per_element ? g0 * ge[e] : rg * g0;    // G of the gate's part that is not a vector
+                    float gp = g0;                                                 // G as the gate's gradient has it
+                    if constexpr (DROP) {       // (a dropped element passes nothing, whatever it and its gradient are)
+                        const bool kept = drop[e] != 0.f;
+                        gg = kept ? gg * drop[e] : 0.f;
+                        gp = kept ? g0 * drop[e] : 0.f;
+                        n = kept || a.post ? n : 0.f;
+                    }
                     acc[kSumA][k][e] += gg * n;
                     if (!PLAIN) acc[kSumB][k][e] += gg;
                     const float dm = gg * gw[k][e];
@@ -190,7 +202,7 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                     s[1] += dm * n;
                     G[k][e] = dm;
                     if (d_row_gate) {
-                        ge[e] = g0 * (n * gw[k][e] + b1[e]);      // (such a gate is no vector: gw is weight_post)
+                        ge[e] = gp * (n * gw[k][e] + b1[e]);      // (such a gate is no vector: gw is weight_post)
                         s[2] += ge[e];
                     }
                 }
@@ -372,7 +384,7 @@ static int64_t backward_blocks(int64_t rows, const RowLaunch& l)
 // Sixteen waves would leave 128 registers a lane, fewer than the sums take: rows past 4096 have two chunks a lane.
 static RowLaunch backward_launch(int64_t cols) { return row_launch(cols, cols <= 16384 ? 4096 : 8192); }
 
-template <typename XT, typename YT, bool JOIN>
+template <typename XT, typename YT, bool JOIN, bool DROP>
 static void launch_backward(const JoinBwd& a, const RowLaunch& l, int64_t blocks, hipStream_t st)
 {
     const dim3 grid((uint32_t)blocks), block(l.threads);
@@ -380,13 +392,13 @@ static void launch_backward(const JoinBwd& a, const RowLaunch& l, int64_t blocks
     const bool plain = a.post != BS_NORM_LAYER && a.pre != BS_NORM_LAYER && a.gate_per <= BS_PER_CHANNEL &&
                        !(a.want & (1 << kSumB | 1 << kSumB2)) && !(a.one_gate && a.b_post.p);
     const bool whole = a.cols % 8 == 0;
-    auto* kernel = l.chunks == 1 ? (plain ? whole ? join_backward_kernel<XT, YT, JOIN, 1, 512, true, true, true, true>
-                                                  : join_backward_kernel<XT, YT, JOIN, 1, 512, true, true, true, false>
-                                          : whole ? join_backward_kernel<XT, YT, JOIN, 1, 512, true, true, false, true>
-                                                  : join_backward_kernel<XT, YT, JOIN, 1, 512, true, true, false, false>)
-                   : l.chunks == 2    ? join_backward_kernel<XT, YT, JOIN, 2, 512, false, false, false, false>
-                   : l.threads <= 512 ? join_backward_kernel<XT, YT, JOIN, 4, 512, false, false, false, false>
-                                      : join_backward_kernel<XT, YT, JOIN, 4, 1024, false, false, false, false>;
+    auto* kernel = l.chunks == 1 ? (plain ? whole ? join_backward_kernel<XT, YT, JOIN, DROP, 1, 512, true, true, true, true>
+                                                  : join_backward_kernel<XT, YT, JOIN, DROP, 1, 512, true, true, true, false>
+                                          : whole ? join_backward_kernel<XT, YT, JOIN, DROP, 1, 512, true, true, false, true>
+                                                  : join_backward_kernel<XT, YT, JOIN, DROP, 1, 512, true, true, false, false>)
+                   : l.chunks == 2    ? join_backward_kernel<XT, YT, JOIN, DROP, 2, 512, false, false, false, false>
+                   : l.threads <= 512 ? join_backward_kernel<XT, YT, JOIN, DROP, 4, 512, false, false, false, false>
+                                      : join_backward_kernel<XT, YT, JOIN, DROP, 4, 1024, false, false, false, false>;
     hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
 }
 
@@ -400,15 +412,19 @@ extern "C" int64_t bs_join_backward_workspace_bytes(int64_t rows, int64_t cols)
     return backward_blocks(rows, backward_launch(cols)) * (kColSums * cols + 2) * 4;
 }
 
-extern "C" int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* workspace,
-                                int64_t workspace_bytes, void* stream)
+namespace bs {
+
+static int join_backward(const char* what, const bs_join* args, const bs_join_grads* grads, const bs_drop* drop, void* workspace,
+                         int64_t workspace_bytes, void* stream)
 {
     clear_error();
-    const char* what = "bs_join_backward";
     if (const int rc = join_check(args, what); rc != BS_OK) return rc;
     if (grads == nullptr) return set_error(BS_ERR_INVALID, "%s: null arguments", what);
     const bs_join& j = *args;
     const bs_join_grads& g = *grads;
+    DropRule rule{};
+    if (drop)
+        if (const int rc = join_drop_check(j, drop, what, &rule); rc != BS_OK) return rc;
     if (j.rows == 0) return set_error(BS_ERR_INVALID, "%s: no rows", what);
     const bool join = j.y != nullptr;
     const bool fixed_gate = j.gate_per <= BS_PER_CHANNEL;
@@ -463,10 +479,13 @@ extern "C" int bs_join_backward(const bs_join* args, const bs_join_grads* grads,
     a.waves = l.waves, a.rows_here = l.rows;
     const hipStream_t st = (hipStream_t)stream;
     const bool xb = j.x_type == BS_DT_BF16, yb = j.y_type == BS_DT_BF16;
-    if (join)
-        (xb ? launch_backward<bf16, bf16, true> : yb ? launch_backward<float, bf16, true> : launch_backward<float, float, true>)(a, l, blocks, st);
+    a.drop = rule;
+    if (drop)
+        (xb ? launch_backward<bf16, bf16, true, true> : yb ? launch_backward<float, bf16, true, true> : launch_backward<float, float, true, true>)(a, l, blocks, st);
+    else if (join)
+        (xb ? launch_backward<bf16, bf16, true, false> : yb ? launch_backward<float, bf16, true, false> : launch_backward<float, float, true, false>)(a, l, blocks, st);
     else
-        (xb ? launch_backward<bf16, bf16, false> : yb ? launch_backward<float, bf16, false> : launch_backward<float, float, false>)(a, l, blocks, st);
+        (xb ? launch_backward<bf16, bf16, false, false> : yb ? launch_backward<float, bf16, false, false> : launch_backward<float, float, false, false>)(a, l, blocks, st);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 
@@ -486,4 +505,19 @@ extern "C" int bs_join_backward(const bs_join* args, const bs_join_grads* grads,
     hipLaunchKernelGGL(join_finish_kernel, dim3((uint32_t)f.col_blocks + ones), dim3(kFinishThreads), 0, st, f);
     e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s finish launch: %s", what, hipGetErrorString(e));
+}
+
+}  // namespace bs
+
+extern "C" int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* workspace, int64_t workspace_bytes,
+                                void* stream)
+{
+    return join_backward("bs_join_backward", args, grads, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int bs_join_drop_backward(const bs_join* args, const bs_join_grads* grads, const bs_drop* drop, void* workspace,
+                                     int64_t workspace_bytes, void* stream)
+{
+    if (drop == nullptr) return set_error(BS_ERR_INVALID, "bs_join_drop_backward: null drop");
+    return join_backward("bs_join_drop_backward", args, grads, drop, workspace, workspace_bytes, stream);
 }

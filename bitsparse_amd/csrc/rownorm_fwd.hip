@@ -1,7 +1,7 @@
 // The step between two MLP blocks, forward: norm of the block's output, gate,
 // scaled residual and the next block's norm in one pass over the rows.
 //
-//   p = norm_post(y) or y;  x' = scale x + gate p;  h = norm_pre(x')
+//   p = norm_post(y) or y, dropped out of or not;  x' = scale x + gate p;  h = norm_pre(x')
 //
 // Bound by memory: x and y are read and x' and h written once, all four with
 // the row's own lanes between the two statistics (rownorm.h).  The next row's
@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "bs_host.h"
+#include "philox.h"
 #include "rownorm.h"
 #include "rownorm_host.h"
 
@@ -33,17 +34,20 @@ struct JoinFwd {
     float *stats_post, *stats_pre;
     void *x1, *h;
     int waves, rows_here;       // of a row, of a workgroup at a time
+    DropRule drop;
 };
 
-// JOIN: there is a y.  C chunks a lane; HOLD: the vectors fit the registers;
-// WHOLE: rows of a multiple of 8 elements.
-template <typename XT, typename YT, bool JOIN, int C, int MAXT, bool HOLD, bool WHOLE>
+// JOIN: there is a y.  DROP: p is dropped out of (philox.h) before its gate.  C chunks a lane; HOLD: the vectors fit the
+// registers; WHOLE: rows of a multiple of 8 elements.
+template <typename XT, typename YT, bool JOIN, bool DROP, int C, int MAXT, bool HOLD, bool WHOLE>
 __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
 {
     __shared__ RowSums s_sums;
     const RowPlace<C> at(a.cols, a.waves);
     int turn = 0;
     const bool per_row = a.gate_per == BS_PER_ROW, per_element = a.gate_per == BS_PER_ELEMENT;
+    DropKey key;
+    if constexpr (DROP) key = drop_key(a.drop);
 
     const int64_t step = (int64_t)gridDim.x * a.rows_here;
     int64_t row = (int64_t)blockIdx.x * a.rows_here + at.sub;
@@ -112,13 +116,16 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                 float g[8];
                 if (per_element)
                     param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, g);
+                float drop[8];
+                if constexpr (DROP) drop_factors(a.drop, key, (uint32_t)(at.col[k] >> 3), (uint32_t)row, drop);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     // (p whole before its gate: an infinite gate times two terms of different signs would be NaN, and times
                     // an absent bias's 0; rstd last: with RMS norms of 16-bit x, y and vectors p and the sum are the only
                     // roundings in 32 bits)
                     const float gate = gv[k][e] * (per_element ? g[e] : rg);
-                    const float p = fmaf((y[k][e] - mean) * w1[k][e], rstd, b1[k][e]);
+                    float p = fmaf((y[k][e] - mean) * w1[k][e], rstd, b1[k][e]);
+                    if constexpr (DROP) p = drop[e] == 0.f ? 0.f : p * drop[e];     // (a dropped infinity is 0)
                     v[k][e] = fmaf(gate, p, sc[k][e] * v[k][e]);
                 }
                 const Raw<XT> o = to_raw<XT>(v[k]);
@@ -145,7 +152,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
     }
 }
 
-template <typename XT, typename YT, bool JOIN>
+template <typename XT, typename YT, bool JOIN, bool DROP>
 static int launch_forward(const JoinFwd& a, const RowLaunch& l, hipStream_t st)
 {
     // as many workgroups as are resident at once (16 waves a CU: 106 us at 16384 x 4096; 32 take 112, 8 take 140), each
@@ -154,11 +161,11 @@ static int launch_forward(const JoinFwd& a, const RowLaunch& l, hipStream_t st)
     const int64_t most = 256ll * std::max(1, 1024 / l.threads);
     const dim3 grid((uint32_t)std::min(need, most)), block(l.threads);
     const bool whole = a.cols % 8 == 0;
-    auto* kernel = l.chunks == 1 ? (l.threads <= 512 ? whole ? join_forward_kernel<XT, YT, JOIN, 1, 512, true, true>
-                                                             : join_forward_kernel<XT, YT, JOIN, 1, 512, true, false>
-                                                     : join_forward_kernel<XT, YT, JOIN, 1, 1024, true, false>)
-                   : l.chunks == 2 ? join_forward_kernel<XT, YT, JOIN, 2, 1024, false, false>
-                                   : join_forward_kernel<XT, YT, JOIN, 4, 1024, false, false>;
+    auto* kernel = l.chunks == 1 ? (l.threads <= 512 ? whole ? join_forward_kernel<XT, YT, JOIN, DROP, 1, 512, true, true>
+                                                             : join_forward_kernel<XT, YT, JOIN, DROP, 1, 512, true, false>
+                                                     : join_forward_kernel<XT, YT, JOIN, DROP, 1, 1024, true, false>)
+                   : l.chunks == 2 ? join_forward_kernel<XT, YT, JOIN, DROP, 2, 1024, false, false>
+                                   : join_forward_kernel<XT, YT, JOIN, DROP, 4, 1024, false, false>;
     hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "bs_join_forward launch: %s", hipGetErrorString(e));
@@ -214,16 +221,27 @@ RowParam row_param(const bs_vector& v, int per) { return {v.data, v.type == BS_D
 
 using namespace bs;
 
-extern "C" int bs_join_forward(const bs_join* args, void* x1, void* h, void* stream)
+namespace bs {
+
+int join_drop_check(const bs_join& j, const bs_drop* drop, const char* what, DropRule* r)
+{
+    if (j.y == nullptr) return set_error(BS_ERR_INVALID, "%s: drop needs y", what);
+    if (j.rows >= (1ll << 32)) return set_error(BS_ERR_INVALID, "%s: drop takes fewer than 2^32 rows", what);
+    return drop_rule(drop, what, r);
+}
+
+static int join_forward(const char* what, const bs_join* args, const bs_drop* drop, void* x1, void* h, void* stream)
 {
     clear_error();
-    if (const int rc = join_check(args, "bs_join_forward"); rc != BS_OK) return rc;
+    if (const int rc = join_check(args, what); rc != BS_OK) return rc;
     const bs_join& j = *args;
+    DropRule rule{};
+    if (drop)
+        if (const int rc = join_drop_check(j, drop, what, &rule); rc != BS_OK) return rc;
     if (j.rows == 0) return BS_OK;
-    if ((j.y && x1 == nullptr) || (j.norm_pre && h == nullptr))
-        return set_error(BS_ERR_INVALID, "bs_join_forward: null result");
+    if ((j.y && x1 == nullptr) || (j.norm_pre && h == nullptr)) return set_error(BS_ERR_INVALID, "%s: null result", what);
     if (!aligned_to_type(x1, j.x_type) || !aligned_to_type(h, j.y_type))
-        return set_error(BS_ERR_INVALID, "bs_join_forward: result misaligned for its type");
+        return set_error(BS_ERR_INVALID, "%s: result misaligned for its type", what);
     const RowLaunch l = row_launch(j.cols, 8192);
     const bool whole = j.gate_per == BS_PER_TENSOR || j.gate_per == BS_PER_CHANNEL;
     JoinFwd a{};
@@ -236,13 +254,25 @@ extern "C" int bs_join_forward(const bs_join* args, void* x1, void* h, void* str
     a.gate_per = j.gate_per, a.gate_stride = j.gate_stride, a.scale_value = j.scale_value;
     a.post = j.norm_post, a.pre = j.norm_pre, a.eps_post = j.eps_post, a.eps_pre = j.eps_pre;
     a.stats_post = j.stats_post, a.stats_pre = j.stats_pre, a.x1 = x1, a.h = h, a.waves = l.waves, a.rows_here = l.rows;
+    a.drop = rule;
     const hipStream_t st = (hipStream_t)stream;
-    if (j.y == nullptr) {
-        if (j.x_type == BS_DT_BF16) return launch_forward<bf16, bf16, false>(a, l, st);
-        if (j.y_type == BS_DT_BF16) return launch_forward<float, bf16, false>(a, l, st);
-        return launch_forward<float, float, false>(a, l, st);
-    }
-    if (j.x_type == BS_DT_BF16) return launch_forward<bf16, bf16, true>(a, l, st);
-    if (j.y_type == BS_DT_BF16) return launch_forward<float, bf16, true>(a, l, st);
-    return launch_forward<float, float, true>(a, l, st);
+    const bool xb = j.x_type == BS_DT_BF16, yb = j.y_type == BS_DT_BF16;
+    if (j.y == nullptr)
+        return (xb ? launch_forward<bf16, bf16, false, false> : yb ? launch_forward<float, bf16, false, false> : launch_forward<float, float, false, false>)(a, l, st);
+    if (drop)
+        return (xb ? launch_forward<bf16, bf16, true, true> : yb ? launch_forward<float, bf16, true, true> : launch_forward<float, float, true, true>)(a, l, st);
+    return (xb ? launch_forward<bf16, bf16, true, false> : yb ? launch_forward<float, bf16, true, false> : launch_forward<float, float, true, false>)(a, l, st);
+}
+
+}  // namespace bs
+
+extern "C" int bs_join_forward(const bs_join* args, void* x1, void* h, void* stream)
+{
+    return join_forward("bs_join_forward", args, nullptr, x1, h, stream);
+}
+
+extern "C" int bs_join_drop_forward(const bs_join* args, const bs_drop* drop, void* x1, void* h, void* stream)
+{
+    if (drop == nullptr) return set_error(BS_ERR_INVALID, "bs_join_drop_forward: null drop");
+    return join_forward("bs_join_drop_forward", args, drop, x1, h, stream);
 }

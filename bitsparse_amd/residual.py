@@ -6,7 +6,7 @@ block, the norm after it with its gate, and the scaled residual.
 pass over the rows (csrc/rownorm_fwd.hip; the gradients in one more,
 csrc/rownorm_bwd.hip):
 
-    p  = post(y)                   (y itself without ``post``)
+    p  = post(y)                   (y itself without ``post``), dropped out of with ``drop``
     x' = scale * x + gate * p      rounded to x's dtype
     h  = pre(x')                   of x' as stored, in y's dtype
 
@@ -29,6 +29,7 @@ import torch
 from torch import Tensor
 
 from ._lib import native
+from .dropout import Dropout, drop_parts
 
 _KINDS = {"rms": 1, "layer": 2}
 
@@ -74,7 +75,7 @@ def block_norm(x: Tensor, norm: RowNorm, *, dtype: torch.dtype | None = None) ->
 
 def block_join(x: Tensor, y: Tensor, *, post: RowNorm | None = None, gate: Tensor | None = None,
                scale: Tensor | float | None = None,
-               pre: RowNorm | None = None) -> Tensor | tuple[Tensor, Tensor]:
+               pre: RowNorm | None = None, drop: Dropout | None = None) -> Tensor | tuple[Tensor, Tensor]:
     """x' = scale * x + gate * post(y), and with ``pre`` also h = pre(x').
 
     x: the residual stream [..., D]; y: the block's output, of the same shape.
@@ -83,6 +84,7 @@ def block_join(x: Tensor, y: Tensor, *, post: RowNorm | None = None, gate: Tenso
     token [..., 1] or an element [..., D].
     scale: None (1), a Python number, or a tensor of one value or one a
     channel [D].
+    drop: dropout of post(y), in front of the gate, with the mask that ``dropout`` has for [..., D] (fewer than 2^32 rows); none is stored.
     Returns x' (x's dtype), with ``pre`` the pair (x', h) (h in y's dtype).
     Differentiable once in every tensor, in reverse mode (a tangent is refused); the gradients are sums in 32 bits in
     a fixed order, each rounded once to its tensor's dtype."""
@@ -93,6 +95,6 @@ def block_join(x: Tensor, y: Tensor, *, post: RowNorm | None = None, gate: Tenso
     value = 1.0
     if scale is not None and not isinstance(scale, Tensor):
         value, scale = float(scale), None
-    out = native().join(x, y, w_post, b_post, gate, scale, w_pre, b_pre, kind_post, kind_pre, eps_post, eps_pre, value,
-                        y.dtype)
+    args = (x, y, w_post, b_post, gate, scale, w_pre, b_pre, kind_post, kind_pre, eps_post, eps_pre, value, y.dtype)
+    out = native().join(*args) if drop is None else native().join_drop(*args, *drop_parts(drop))
     return out[0] if pre is None else (out[0], out[1])

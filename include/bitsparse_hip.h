@@ -49,7 +49,7 @@ extern "C" {
 const char* bs_last_error(void);
 
 /* ABI version (bumped when an entry point changes): of this header, and of a built library. */
-#define BS_ABI_VERSION 20
+#define BS_ABI_VERSION 21
 int bs_abi_version(void);
 
 /*
@@ -711,6 +711,120 @@ typedef struct bs_join_grads {
 int64_t bs_join_backward_workspace_bytes(int64_t rows, int64_t cols);
 int bs_join_backward(const bs_join* args, const bs_join_grads* grads, void* workspace, int64_t workspace_bytes,
                      void* stream);
+
+/*
+ * Dropout (no counterpart in the reference): element (row, column) of
+ * [rows, cols] is dropped where its 16 random bits are less than `below`, and
+ * times 65536 / (65536 - below) elsewhere (below = 65536: all dropped).  The
+ * bits are half column % 2 of word column / 2 % 4 of Philox 4x32 (10 rounds)
+ * with the key seed and the counter (column / 8, row, offset), low words
+ * first: of seed, offset, row and column alone, so the same call on a gradient
+ * is the backward pass.  state (NULL, or the address of [seed, offset] on the
+ * device) takes the place of seed and offset.  A dropped element is 0 whatever
+ * it was.
+ */
+typedef struct bs_drop {
+    uint64_t seed, offset;
+    const int64_t* state;
+    int below;                       /* 0..65536 */
+} bs_drop;
+int bs_dropout(const bs_drop* drop, const void* x, int type, int64_t rows, int64_t cols, int64_t stride, void* out, void* stream);
+/* The step between two blocks with p dropped out of before its gate: x' = scale * x + gate * drop(p). */
+int bs_join_drop_forward(const bs_join* args, const bs_drop* drop, void* x1, void* h, void* stream);
+int bs_join_drop_backward(const bs_join* args, const bs_join_grads* grads, const bs_drop* drop, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/*
+ * MLP blocks as experts (no counterpart in the reference, whose blocks are
+ * dense): the routing of tokens, the products of each expert's rows with its
+ * weights, the weighted sum back to tokens.
+ *
+ * bs_route_forward: s = softmax or sigmoid of a token's logits [tokens,
+ * experts]; c = s + bias; of `groups` groups of consecutive experts the
+ * top_groups with the largest sum of their group_best largest c are kept, and
+ * of their experts the top_k largest c are chosen, the largest first.  The
+ * choice is between 64-bit values; of equal ones the lowest index goes first
+ * and a NaN before all.  weights = scale * s / sum(s of the chosen)
+ * (renormalize; 0 where that sum is 0) or scale * s.  An expert whose logit or
+ * c is -infinity is not chosen; a choice that is left without an expert is -1
+ * with weight 0.  weights and chosen: [tokens, top_k], contiguous.
+ * bs_route_backward: the gradient of the logits (their type, contiguous) from
+ * that of the weights; the choice and the bias have none.
+ */
+#define BS_SCORE_SOFTMAX 0
+#define BS_SCORE_SIGMOID 1
+typedef struct bs_route {
+    int64_t tokens;
+    int experts, top_k;              /* up to 1024; up to 64 */
+    const void* logits;
+    int logits_type;                 /* BS_DT_BF16 or BS_DT_F32 */
+    int64_t logits_stride;
+    const float* bias;               /* [experts] or NULL */
+    int score, groups, top_groups, group_best, renormalize;
+    float scale;
+} bs_route;
+int bs_route_forward(const bs_route* route, float* weights, int32_t* chosen, void* stream);
+int bs_route_backward(const bs_route* route, const int32_t* chosen, const float* d_weights, void* d_logits, void* stream);
+
+/*
+ * The order of `pairs` ids by expert: rows offsets[e] up to offsets[e + 1] are
+ * expert e's, order[row] is the row's pair and place[pair] the pair's row;
+ * equal ids stay in order.  Ids outside 0..experts-1 have place -1 and no
+ * row; order is -1 in the rows that are left at the end.
+ */
+int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts, int32_t* offsets, int32_t* order, int32_t* place, void* stream);
+
+/*
+ * Products of the experts' rows with their bf16 weights [experts, out, in]
+ * (w_stride elements from row to row), fp32 sums rounded once:
+ *   y[r] = act(x[src r] W[e]^T), dx[r] = dy[r] W[e], dW[e] = sum dy[r]^T x[src r]
+ * src r = order[r] / top_k, a row of the `tokens` of x, or (order NULL) r.
+ * Rows that belong to no expert, or whose order is out of range, come out as
+ * 0 (as act(0)); an expert without rows gets dW = 0.  Offsets out of range are
+ * taken as the nearest in it.  Results are contiguous.  Operands have rows at
+ * 16-byte addresses, a multiple of 8 elements apart, and zeros from their
+ * last column to the next multiple of 8 (bs_pad_rows makes such rows).
+ * BS_ACT_RELU2: bf16(bf16(r r) act_k) of r = bf16(relu(.)), as the ReLU^2
+ * layers form it; BS_ACT_RELU: r.
+ */
+#define BS_ACT_NONE 0
+#define BS_ACT_RELU 1
+#define BS_ACT_RELU2 2
+typedef struct bs_experts {
+    int64_t rows, tokens;
+    int experts, top_k;
+    const int32_t* offsets;          /* [experts + 1] */
+    const int32_t* order;            /* [rows], or NULL: operands are rows themselves */
+} bs_experts;
+int bs_expert_linear(const bs_experts* experts, const void* x, int64_t x_stride, const void* W, int64_t w_stride, int64_t in,
+                     int64_t out, int act, float act_k, void* y, void* stream);
+int bs_expert_linear_dx(const bs_experts* experts, const void* dy, int64_t dy_stride, const void* W, int64_t w_stride, int64_t in,
+                        int64_t out, void* dx, void* stream);
+int bs_expert_linear_dw(const bs_experts* experts, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int64_t in,
+                        int64_t out, void* dW, void* stream);
+/* bf16 rows of `cols` copied into rows of `width`, a multiple of 8, with zeros behind. */
+int bs_pad_rows(const void* x, int64_t rows, int64_t cols, int64_t stride, void* out, int64_t width, void* stream);
+
+/*
+ * out[t] = sum over j of weights[t, j] y[place[t, j]] in the order of j (bf16,
+ * fp32 sums; weights NULL: 1); a place outside 0..rows-1 adds nothing.
+ * Backward: dy[place[t, j]] = weights[t, j] g[t], 0 in the rows from *used
+ * (a device address: offsets[experts]) on; dweights[t, j] = <g[t],
+ * y[place[t, j]]>.  dy or dweights may be NULL.
+ */
+int bs_expert_combine(const void* y, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
+                      int64_t rows, int64_t cols, void* out, void* stream);
+int bs_expert_combine_backward(const void* g, int64_t g_stride, const void* y, int64_t y_stride, const float* weights,
+                               const int32_t* place, const int32_t* used, int64_t tokens, int top_k, int64_t rows, int64_t cols,
+                               void* dy, float* dweights, void* stream);
+/*
+ * Between the two products of a backward through y = sum of w act(z) W2^T: g
+ * [rows, cols] holds the gradient of act(z) before its weight, r the saved
+ * relu(z) (or, not `square`, any activation with relu's gradient).  In place g becomes w g act'(z) and r becomes w act(z);
+ * dweights[pair] = <g, act(z)> for every pair that has a row.  w = weights[order[row]], 0 from row *used on.
+ */
+int bs_experts_act_grad(void* g, void* r, int64_t rows, int64_t cols, int square, float k, const float* weights,
+                        const int32_t* order, const int32_t* used, int64_t pairs, float* dweights, void* stream);
 
 /*
  * Orthogonalised updates of weight matrices (no counterpart in the reference,
