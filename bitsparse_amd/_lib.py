@@ -100,7 +100,8 @@ _SIGNATURES = {
     "bs_join_drop_backward": [_vp, _vp, _vp, _vp, _i64, _vp],
     "bs_route_forward": [_vp, _vp, _vp, _vp],
     "bs_route_backward": [_vp, _vp, _vp, _vp, _vp],
-    "bs_expert_plan": [_vp, _i64, _int, _vp, _vp, _vp, _vp],
+    "bs_expert_plan_workspace_bytes": [_i64, _int],
+    "bs_expert_plan": [_vp, _i64, _int, _vp, _vp, _vp, _vp, _i64, _vp],
     "bs_expert_linear": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _int, _f32, _vp, _vp],
     "bs_expert_linear_dx": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
     "bs_expert_linear_dw": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
@@ -127,6 +128,7 @@ _RESTYPES = {
     "bs_col_sum_workspace_bytes": _i64,
     "bs_join_backward_workspace_bytes": _i64,
     "bs_newton_schulz_workspace_bytes": _i64,
+    "bs_expert_plan_workspace_bytes": _i64,
     "bs_nontemporal_min_bytes": _i64,
     "bs_workspace_amax_slot": _vp,
     "bs_workspace_fallback_counter": _vp,

@@ -195,8 +195,11 @@ std::vector<Tensor> plan_experts(const Tensor& chosen, int64_t experts)
     const Tensor ids = chosen.contiguous();
     const Tensor offsets = at::empty({experts + 1}, ids.options()), order = at::empty({ids.numel()}, ids.options()),
                  place = at::empty(chosen.sizes(), ids.options());
+    const int64_t need = L.bs_expert_plan_workspace_bytes(ids.numel(), (int)experts);
+    Tensor ws;
+    if (need) ws = at::empty({need}, ids.options().dtype(at::kByte));
     check(L.bs_expert_plan(ptr<int32_t>(ids), ids.numel(), (int)experts, offsets.data_ptr<int32_t>(), ptr<int32_t>(order), ptr<int32_t>(place),
-                           stream_of(ids)),
+                           raw(ws), need, stream_of(ids)),
           "bs_expert_plan");
     return {offsets, order, place};
 }

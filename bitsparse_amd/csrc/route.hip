@@ -6,12 +6,13 @@
 //   the top_k largest c of those groups; w = scale s / sum(s) or scale s
 //
 // The choice is made between 64-bit values, as what lies next to each other in
-// 32 bits would be ordered by its roundings; equal values go by index.  A wave
-// a token, an expert a lane and a round.
+// 32 bits would be ordered by its roundings; equal values go by index.  Where
+// c has the order of the logits it is between those.
 //
 //   dw -> ds = (scale / S) (dw - <dw, s> / S) or scale dw, 0 elsewhere
 //   softmax: dl = s (ds - <ds, s>);  sigmoid: dl = s (1 - s) ds
 #include <algorithm>
+#include <type_traits>
 
 #include "bs_host.h"
 #include "rownorm.h"
@@ -28,6 +29,7 @@ struct RouteArgs {
     int f32;
     const float* bias;
     int sigmoid, groups, top_groups, group_best, renorm;
+    int by_logit;               // the order of c is that of the logits
     float scale;
     float* weights;
     int32_t* chosen;
@@ -36,291 +38,447 @@ struct RouteArgs {
     void* d_logits;
 };
 
-__device__ __forceinline__ float route_logit(const RouteArgs& a, int64_t row, int e)
-{
-    const int64_t i = row * a.stride + e;
-    return a.f32 ? static_cast<const float*>(a.logits)[i] : (float)static_cast<const bf16*>(a.logits)[i];
-}
-
-// 64-bit values as integers in the same order; NaN above all, 0: none
-__device__ __forceinline__ uint64_t order_key(double v)
-{
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    if (v != v) return ~0ull;
-    return b >> 63 ? ~b : b | 1ull << 63;
-}
-__device__ __forceinline__ double key_value(uint64_t k)
-{
-    return __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k);
-}
-
-struct Best {
-    uint64_t key;
-    int at;
-};
-__device__ __forceinline__ Best better(const Best& a, const Best& b)
-{
-    return b.key > a.key || (b.key == a.key && b.at < a.at) ? b : a;
-}
-// the best over the wave, in every lane
-__device__ __forceinline__ Best wave_best(Best v)
-{
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        Best o;
-        o.key = (uint64_t)(uint32_t)__shfl_xor((int)(v.key >> 32), d) << 32 | (uint32_t)__shfl_xor((int)v.key, d);
-        o.at = __shfl_xor(v.at, d);
-        v = better(v, o);
+// L lanes have a token, 64 / L tokens a wave; lane l of them has the V experts
+// from V l on.
+template <int L>
+struct Lanes {
+    // x of the lane 1, 2, 4 (mirrored in 8), 8 (mirrored in 16), 16, 32 away: enough for what is the same on both sides so far
+    template <int D>
+    static __device__ __forceinline__ uint32_t other(uint32_t x)
+    {
+        if constexpr (D == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true);
+        if constexpr (D == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true);
+        if constexpr (D == 4) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xf, 0xf, true);
+        if constexpr (D == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xf, 0xf, true);
+        if constexpr (D >= 16) return (uint32_t)__shfl_xor((int)x, D);
     }
-    return v;
-}
-__device__ __forceinline__ double wave_max_f64(double v)
+    template <int D>
+    static __device__ __forceinline__ float other(float x) { return __uint_as_float(other<D>(__float_as_uint(x))); }
+    template <int D>
+    static __device__ __forceinline__ double other(double x)
+    {
+        const uint64_t b = __builtin_bit_cast(uint64_t, x);
+        return __builtin_bit_cast(double, (uint64_t)other<D>((uint32_t)(b >> 32)) << 32 | other<D>((uint32_t)b));
+    }
+    // v joined over the token's lanes, the same in all of them
+    template <int D = 1, typename T, typename F>
+    static __device__ __forceinline__ T all(T v, F&& join)
+    {
+        if constexpr (D < L) {
+            v = join(v, other<D>(v));
+            return all<2 * D>(v, join);
+        }
+        return v;
+    }
+};
+
+// V logits of a row from its element e0 on, -infinity behind its end
+template <int V, typename T>
+__device__ __forceinline__ void load_logits(const T* row, int e0, int experts, float (&v)[V])
 {
+    if constexpr (V % 8 == 0) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = fmax(v, __shfl_xor(v, d));
-    return v;
+        for (int c = 0; c < V; c += 8) {
+            const int nv = max(0, min(8, experts - e0 - c));
+            const Raw<T> r = load_raw(row + e0 + c, nv);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[c + i] = i < nv ? raw_get(r, i) : -INFINITY;
+        }
+    } else if (V == 4 && e0 + 4 <= experts) {
+        uint32_t w[sizeof(T)];
+        __builtin_memcpy(w, row + e0, sizeof(w));
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            v[i] = sizeof(T) == 4 ? __uint_as_float(w[i % (int)sizeof(T)]) : __uint_as_float(i & 1 ? w[i / 2 % (int)sizeof(T)] & 0xffff0000u : w[i / 2 % (int)sizeof(T)] << 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = e0 + i < experts ? (float)row[e0 + i] : -INFINITY;
+    }
 }
-__device__ __forceinline__ double wave_sum_f64(double v)
+template <int V>
+__device__ __forceinline__ void load_logits(const RouteArgs& a, int64_t row, int e0, float (&v)[V])
 {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
+    if (a.f32)
+        load_logits(static_cast<const float*>(a.logits) + row * a.stride, e0, a.experts, v);
+    else
+        load_logits(static_cast<const bf16*>(a.logits) + row * a.stride, e0, a.experts, v);
 }
 
-// V: experts of a lane
-template <int V>
+// LDS written by some lanes of a wave and read by others of it
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// What is chosen by, c, is -infinity where there is no expert (any more) and
+// infinity for a NaN.
+template <int L, int V>
 __global__ __launch_bounds__(256) void route_forward_kernel(RouteArgs a)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.tokens) return;
-    double s[V];
-    uint64_t key[V];
-    double top = -INFINITY;
+    constexpr int TOKENS = 64 / L, SLOTS = (kMaxTopK + L - 1) / L;
+    __shared__ double s_score[4][TOKENS][64];
+    typedef Lanes<L> Ln;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % L, sub = lane / L;
+    const int64_t token = ((int64_t)blockIdx.x * 4 + wave) * TOKENS + sub, row = min(token, a.tokens - 1);
+    const auto larger = [](auto x, auto y) { return x > y ? x : y; };
+    const auto sum_of = [](auto x, auto y) { return x + y; };
+    const int e0 = l * V;
+    float lg[V];
+    load_logits(a, row, e0, lg);
+
+    // softmax: the largest logit and the sum of exponentials over it (a NaN makes the sum NaN)
+    float top = -INFINITY, sum = 0.f;
+    if (!a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int e = lane + 64 * i;
-        s[i] = e < a.experts ? (double)route_logit(a, row, e) : -INFINITY;
-        top = s[i] != s[i] ? s[i] : top != top ? top : fmax(top, s[i]);
+        for (int i = 0; i < V; i++) top = fmaxf(top, lg[i]);
+        top = Ln::all(top, [](float x, float y) { return fmaxf(x, y); });
     }
-    bool there[V];
+    double c[V];
+    if (a.by_logit) {
+        if (!a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < V; i++) there[i] = lane + 64 * i < a.experts && s[i] != -INFINITY;
-    if (a.sigmoid) {
+            for (int i = 0; i < V; i++) sum += lg[i] == -INFINITY ? 0.f : expf(lg[i] - top);
+            sum = Ln::all(sum, sum_of);
+        }
 #pragma unroll
-        for (int i = 0; i < V; i++) s[i] = 1.0 / (1.0 + exp(-s[i]));
+        for (int i = 0; i < V; i++) c[i] = lg[i];
+    } else if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < V; i++) c[i] = lg[i] == -INFINITY ? -INFINITY : 1.0 / (1.0 + exp(-(double)lg[i]));
     } else {
-        const bool nan = __any(top != top);
-        top = wave_max_f64(nan ? 0.0 : top);
-        double sum = 0.0;
+        double total = 0.0;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            s[i] = there[i] ? exp(s[i] - top) : 0.0;
-            sum += s[i];
+            c[i] = lg[i] == -INFINITY ? -INFINITY : exp((double)lg[i] - (double)top);
+            total += lg[i] == -INFINITY ? 0.0 : c[i];
         }
-        sum = wave_sum_f64(sum);
+        total = Ln::all(total, sum_of);
+        sum = (float)total;
+        const double part = 1.0 / total;
 #pragma unroll
-        for (int i = 0; i < V; i++) s[i] /= sum;
+        for (int i = 0; i < V; i++) c[i] = lg[i] == -INFINITY ? -INFINITY : c[i] * part;
+    }
+    if (a.bias) {
+        float b[V];
+        load_logits(a.bias, e0, a.experts, b);
+#pragma unroll
+        for (int i = 0; i < V; i++) c[i] += (double)b[i];
     }
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int e = lane + 64 * i;
-        double c = s[i];
-        if (a.bias && e < a.experts) c += (double)a.bias[e];
-        key[i] = there[i] && c != -INFINITY ? order_key(c) : 0;
-    }
+    for (int i = 0; i < V; i++) c[i] = c[i] != c[i] ? (double)INFINITY : c[i];
+
     if (a.top_groups < a.groups) {
-        // group g's score to lane g
         const int size = a.experts / a.groups;
-        Best mine = {0, lane};
-        for (int g = 0; g < a.groups; g++) {
-            Best first = {0, 1 << 30}, second = {0, 1 << 30};
+        // the best and the second best of two pairs of such
+        struct Pair {
+            double x, y;
+        };
+        auto add = [](Pair p, double v) {
+            const bool more = v > p.x;
+            return Pair{more ? v : p.x, more ? p.x : v > p.y ? v : p.y};
+        };
+        auto score = [&](Pair p) { return a.group_best == 1 || p.y == -INFINITY ? p.x : p.x + p.y; };
+        const int span = size / V;          // lanes of a group, where it has whole lanes
+        if (span * V == size && (span & (span - 1)) == 0 && span <= 16) {
+            Pair p = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < V; i++) p = add(p, c[i]);
+            auto meet = [&](auto d) {
+                constexpr int D = decltype(d)::value;
+                if (span > D) p = add(add(p, Ln::template other<D>(p.x)), Ln::template other<D>(p.y));
+            };
+            meet(std::integral_constant<int, 1>{});
+            meet(std::integral_constant<int, 2>{});
+            meet(std::integral_constant<int, 4>{});
+            meet(std::integral_constant<int, 8>{});
+            if (l % span == 0 && l / span < a.groups) s_score[wave][sub][l / span] = score(p);
+        } else {
+            for (int g = 0; g < a.groups; g++) {
+                Pair p = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < V; i++) p = add(p, e0 + i >= g * size && e0 + i < (g + 1) * size ? c[i] : -INFINITY);
+                const double best = Ln::all(p.x, larger);
+                // (one lane gives its best up, the first of those that have it)
+                const uint64_t have = __ballot(p.x == best) >> (sub * L) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1);
+                const bool first = l == __builtin_ctzll(have);
+                const double second = Ln::all(first ? p.y : p.x, larger);
+                if (l == 0) s_score[wave][sub][g] = score(Pair{best, second});
+            }
+        }
+        wave_fence();
+        // group g stays if fewer than top_groups come before it
+        uint32_t low = 0, high = 0;
+        for (int g = l; g < a.groups; g += L) {
+            const double mine = s_score[wave][sub][g];
+            int before = 0;
+            for (int h = 0; h < a.groups; h++) {
+                const double v = s_score[wave][sub][h];
+                before += v > mine || (v == mine && h < g);
+            }
+            if (before < a.top_groups && mine != -INFINITY) (g < 32 ? low : high) |= 1u << (g & 31);
+        }
+        const auto either = [](uint32_t x, uint32_t y) { return x | y; };
+        const uint64_t kept = (uint64_t)Ln::all(high, either) << 32 | Ln::all(low, either);
+        const uint32_t part = ((1u << 22) + size - 1) / size;       // e / size = e part >> 22 for e, size <= 1024
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (!(kept >> ((uint32_t)(e0 + i) * part >> 22 & 63) & 1)) c[i] = -INFINITY;
+    }
+
+    int id[SLOTS];
+    float of[SLOTS];        // its logit
+#pragma unroll
+    for (int s = 0; s < SLOTS; s++) {
+        id[s] = -1;
+        of[s] = 0.f;
+        for (int j = 0; j < L && s * L + j < a.top_k; j++) {
+            double best = c[0];
+#pragma unroll
+            for (int i = 1; i < V; i++) best = fmax(best, c[i]);
+            uint32_t at = ~0u;
+#pragma unroll
+            for (int i = V - 1; i >= 0; i--) at = c[i] == best ? e0 + i : at;
+            const double most = Ln::all(best, larger);
+            at = Ln::all(best == most ? at : ~0u, [](uint32_t x, uint32_t y) { return min(x, y); });
+            float logit = 0.f;
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const int e = lane + 64 * i;
-                if (e / size == g && key[i]) first = better(first, Best{key[i], e});
+                const bool here = at == (uint32_t)(e0 + i);
+                logit = here ? lg[i] : logit;
+                c[i] = here ? -INFINITY : c[i];
             }
-            first = wave_best(first);
-            double score = first.key == ~0ull ? NAN : key_value(first.key);
-            if (a.group_best == 2) {
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const int e = lane + 64 * i;
-                    if (e / size == g && key[i] && e != first.at) second = better(second, Best{key[i], e});
-                }
-                second = wave_best(second);
-                if (second.key) score += second.key == ~0ull ? NAN : key_value(second.key);
+            logit = __shfl(logit, (int)(sub * L + at / V) & 63);
+            if (l == j) {
+                id[s] = most == -INFINITY ? -1 : (int)at;
+                of[s] = logit;
             }
-            if (lane == g) mine.key = first.key ? order_key(score) : 0;
-        }
-        uint64_t kept = 0;
-        for (int j = 0; j < a.top_groups; j++) {
-            const Best b = wave_best(mine);
-            if (b.key) kept |= 1ull << b.at;
-            if (lane == b.at) mine.key = 0;
-        }
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            if (!(kept >> min(63, (lane + 64 * i) / size) & 1)) key[i] = 0;
-    }
-    double total = 0.0, own = 0.0;
-    int chosen = -1;
-    for (int j = 0; j < a.top_k; j++) {
-        Best b = {0, 1 << 30};
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            if (key[i]) b = better(b, Best{key[i], lane + 64 * i});
-        b = wave_best(b);
-        double v = 0.0;
-        if (b.key) {
-#pragma unroll
-            for (int i = 0; i < V; i++)
-                if (lane + 64 * i == b.at) {
-                    key[i] = 0;
-                    v = s[i];
-                }
-            v = __shfl(v, b.at & 63);
-        }
-        total += v;
-        if (lane == j) {
-            own = v;
-            chosen = b.key ? b.at : -1;
         }
     }
-    if (lane < a.top_k) {
-        double w = own;
-        if (a.renorm) w = total == 0.0 ? 0.0 : w / total;
-        a.weights[row * a.top_k + lane] = (float)(w * (double)a.scale);
-        a.chosen[row * a.top_k + lane] = chosen;
+    float w[SLOTS], total = 0.f;
+#pragma unroll
+    for (int s = 0; s < SLOTS; s++) {
+        w[s] = id[s] < 0 ? 0.f : a.sigmoid ? 1.f / (1.f + expf(-of[s])) : expf(of[s] - top) / sum;
+        total += w[s];
+    }
+    if (a.renorm) total = Ln::all(total, sum_of);
+#pragma unroll
+    for (int s = 0; s < SLOTS; s++) {
+        const int j = s * L + l;
+        if (j >= a.top_k || token >= a.tokens) continue;
+        a.weights[token * a.top_k + j] = a.scale * (!a.renorm ? w[s] : total == 0.f ? 0.f : w[s] / total);
+        a.chosen[token * a.top_k + j] = id[s];
     }
 }
 
-template <int V>
+template <int L, int V>
 __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.tokens) return;
-    float s[V], top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int e = lane + 64 * i;
-        s[i] = e < a.experts ? route_logit(a, row, e) : -INFINITY;
-        top = fmaxf(top, s[i]);
-    }
+    constexpr int TOKENS = 64 / L, SLOTS = (kMaxTopK + L - 1) / L;
+    typedef Lanes<L> Ln;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % L, sub = lane / L;
+    const int64_t token = ((int64_t)blockIdx.x * 4 + wave) * TOKENS + sub, row = min(token, a.tokens - 1);
+    const auto sum_of = [](float x, float y) { return x + y; };
+    const int e0 = l * V;
+    float s[V];
+    load_logits(a, row, e0, s);
     if (a.sigmoid) {
 #pragma unroll
         for (int i = 0; i < V; i++) s[i] = 1.f / (1.f + expf(-s[i]));
     } else {
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        float sum = 0.f;
+        for (int i = 0; i < V; i++) top = fmaxf(top, s[i]);
+        top = Ln::all(top, [](float x, float y) { return fmaxf(x, y); });
 #pragma unroll
         for (int i = 0; i < V; i++) {
             s[i] = s[i] == -INFINITY ? 0.f : expf(s[i] - top);
             sum += s[i];
         }
-        sum = wave_sum_f32(sum);
+        sum = Ln::all(sum, sum_of);
+        const float part = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int i = 0; i < V; i++) s[i] = sum == 0.f ? 0.f : s[i] / sum;
+        for (int i = 0; i < V; i++) s[i] *= part;
     }
-    // lane j: the j-th choice, its score and gradient
-    int e = -1;
-    float g = 0.f, sc = 0.f;
-    if (lane < a.top_k) {
-        e = a.chosen[row * a.top_k + lane];
-        if (e >= a.experts) e = -1;
-        g = e >= 0 ? a.d_weights[row * a.top_k + lane] * a.scale : 0.f;
-    }
+    // lane l has the choices l, l + L, ...: experts, scores, gradients
+    int e[SLOTS];
+    float g[SLOTS], sc[SLOTS], total = 0.f, dot = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const float v = __shfl(s[i], e & 63);
-        if (e >> 6 == i) sc = v;
+    for (int t = 0; t < SLOTS; t++) {
+        const int j = t * L + l;
+        e[t] = j < a.top_k ? a.chosen[row * a.top_k + j] : -1;
+        if (e[t] >= a.experts) e[t] = -1;
+        g[t] = e[t] >= 0 ? a.d_weights[row * a.top_k + j] * a.scale : 0.f;
+        sc[t] = 0.f;
+        if (t * L < a.top_k) {
+            const int from = (sub * L + max(0, e[t]) / V) & 63;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float v = __shfl(s[i], from);
+                if (e[t] >= 0 && e[t] % V == i) sc[t] = v;
+            }
+        }
+        total += sc[t];
+        dot += e[t] >= 0 ? g[t] * sc[t] : 0.f;
     }
+    dot = Ln::all(dot, sum_of);
     if (a.renorm) {
-        const float total = wave_sum_f32(sc), dot = wave_sum_f32(g * sc);
-        g = total == 0.f || e < 0 ? 0.f : (g - dot / total) / total;
+        total = Ln::all(total, sum_of);
+        const float part = total == 0.f ? 0.f : 1.f / total, mean = dot * part;
+#pragma unroll
+        for (int t = 0; t < SLOTS; t++) g[t] = e[t] < 0 ? 0.f : (g[t] - mean) * part;
+        dot = 0.f;              // of the renormalised weights' gradient with s
     }
-    const float dot = a.sigmoid ? 0.f : wave_sum_f32(g * sc);
     float ds[V];
 #pragma unroll
     for (int i = 0; i < V; i++) ds[i] = 0.f;
-    for (int j = 0; j < a.top_k; j++) {
-        const int at = __shfl(e, j);
-        const float v = __shfl(g, j);
+#pragma unroll
+    for (int t = 0; t < SLOTS; t++)
+        for (int j = 0; j < L && t * L + j < a.top_k; j++) {
+            const int at = __shfl(e[t], sub * L + j);
+            const float v = __shfl(g[t], sub * L + j);
+#pragma unroll
+            for (int i = 0; i < V; i++) ds[i] += at == e0 + i ? v : 0.f;
+        }
+    if (token >= a.tokens) return;
+    float d[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) d[i] = a.sigmoid ? s[i] * (1.f - s[i]) * ds[i] : s[i] * (ds[i] - dot);
+    const int64_t at = token * a.experts + e0;
+    if constexpr (V % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 8) {
+            float o[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) o[k] = d[i + k];
+            const int nv = max(0, min(8, a.experts - e0 - i));
+            if (a.f32)
+                store_raw(static_cast<float*>(a.d_logits) + at + i, to_raw<float>(o), nv);
+            else
+                store_raw(static_cast<bf16*>(a.d_logits) + at + i, to_raw<bf16>(o), nv);
+        }
+    } else {
 #pragma unroll
         for (int i = 0; i < V; i++)
-            if (at == lane + 64 * i) ds[i] += v;
-    }
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int x = lane + 64 * i;
-        if (x >= a.experts) continue;
-        const float d = a.sigmoid ? s[i] * (1.f - s[i]) * ds[i] : s[i] * (ds[i] - dot);
-        param_store(a.d_logits, a.f32, row * a.experts + x, d);
+            if (e0 + i < a.experts) param_store(a.d_logits, a.f32, at + i, d[i]);
     }
 }
 
 // ---------------------------------------------------------------------------
 // The pairs by expert: a counting sort that keeps equal ones in order, without
-// atomics.  A workgroup an expert, each reads all ids: once to count its own
-// and those of lower experts, once to place its own; a wave has a run of them,
-// so their order needs no more than the waves' counts.
+// atomics.  A block of pairs is a run of each of 16 waves; a wave counts 64 of
+// them at a time, the lanes with the same expert told by a ballot for each bit of it.
+// One block does it all by itself; of more, each writes its counts and a
+// second kernel adds those of the blocks before it.
 // ---------------------------------------------------------------------------
+constexpr int kPlanBlock = 8192;        // pairs of a block where there are several
+constexpr int kPlanBlocks = 256;        // most blocks
+
 struct PlanArgs {
     const int32_t* chosen;
-    int32_t pairs;
-    int experts;
+    int64_t pairs, run;         // run: pairs of a wave, a multiple of 64
+    int experts, bits, blocks;
     int32_t *offsets, *order, *place;
+    int32_t* counts;            // [blocks, experts], of several blocks
 };
 
+// the lanes whose expert is this lane's
+__device__ __forceinline__ uint64_t same_expert(uint32_t e, int bits)
+{
+    uint64_t same = ~0ull;
+    for (int b = 0; b < bits; b++) {
+        const bool one = e >> b & 1;
+        const uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
+}
+
+// COUNT: the first of two kernels
+template <bool COUNT>
 __global__ __launch_bounds__(1024) void expert_plan_kernel(PlanArgs a)
 {
-    __shared__ int s_own[16], s_lower[16];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int mine = (int)blockIdx.x;
-    const int64_t run = (((int64_t)a.pairs + 15) / 16 + 63) / 64 * 64;
-    const int64_t from = wave * run, to = min((int64_t)a.pairs, from + run);
-    int own = 0, lower = 0;
-    for (int64_t i = from + lane; i < to; i += 64) {
-        const int e = a.chosen[i];
-        own += e == mine;
-        lower += e >= 0 && e < mine;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        own += __shfl_xor(own, d);
-        lower += __shfl_xor(lower, d);
-    }
-    if (lane == 0) {
-        s_own[wave] = own;
-        s_lower[wave] = lower;
+    extern __shared__ int s_mem[];
+    int* const s_count = s_mem;                         // [16][experts]
+    int* const s_total = s_mem + 16 * a.experts;        // [experts]
+    __shared__ int s_wave[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), E = a.experts;
+    for (int i = tid; i < 16 * E; i += 1024) s_count[i] = 0;
+    __syncthreads();
+    const int64_t from = ((int64_t)blockIdx.x * 16 + wave) * a.run, to = min(a.pairs, from + a.run);
+    int* const mine = s_count + wave * E;
+    for (int64_t i = from; i < to; i += 64) {
+        const uint32_t id = i + lane < to ? (uint32_t)a.chosen[i + lane] : ~0u;
+        const uint32_t e = min(id, (uint32_t)E);        // (all that are none of the experts' at one)
+        const uint64_t same = same_expert(e, a.bits);
+        if (e < (uint32_t)E && popc_below(same) == 0) mine[e] += __popcll(same);
     }
     __syncthreads();
-    int first = 0, before = 0, all = 0;
-    for (int w = 0; w < 16; w++) {
-        first += s_lower[w];
-        before += w < wave ? s_own[w] : 0;
-        all += s_own[w];
-    }
-    if (threadIdx.x == 0) a.offsets[mine] = first;
-    if (mine == a.experts - 1) {
-        if (threadIdx.x == 0) a.offsets[a.experts] = first + all;
-        for (int64_t r = first + all + (int)threadIdx.x; r < a.pairs; r += 1024) a.order[r] = -1;
-    }
-    int row = first + before;
-    for (int64_t i0 = from; i0 < to; i0 += 64) {
-        const int64_t i = i0 + lane;
-        const int e = i < to ? a.chosen[i] : -1;
-        const uint64_t hit = __ballot(i < to && e == mine);
-        if (i < to && e == mine) {
-            const int r = row + (int)popc_below(hit);
-            a.order[r] = (int)i;
-            a.place[i] = r;
-        } else if (i < to && mine == 0 && (e < 0 || e >= a.experts)) {
-            a.place[i] = -1;
+    // each wave's counts become the rows of the waves before it
+    for (int e = tid; e < E; e += 1024) {
+        int sum = 0;
+        for (int w = 0; w < 16; w++) {
+            const int n = s_count[w * E + e];
+            s_count[w * E + e] = sum;
+            sum += n;
         }
-        row += __popcll(hit);
+        if (COUNT)
+            a.counts[(int64_t)blockIdx.x * E + e] = sum;
+        else
+            s_total[e] = sum;
+    }
+    if (COUNT) return;
+    __syncthreads();
+    // the experts' first rows
+    int all = 0, before = 0;            // of expert `tid`, in all blocks and in those before this one
+    if (tid < E) {
+        if (a.blocks > 1) {
+#pragma unroll 8
+            for (int b = 0; b < a.blocks; b++) {
+                const int n = a.counts[(int64_t)b * E + tid];
+                all += n;
+                before += b < (int)blockIdx.x ? n : 0;
+            }
+        } else {
+            all = s_total[tid];
+        }
+    }
+    int sum = all;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(sum, d);
+        sum += lane >= d ? o : 0;
+    }
+    if (lane == 63) s_wave[wave] = sum;
+    __syncthreads();
+    int used = 0;
+    for (int w = 0; w < 16; w++) {
+        const int n = s_wave[w];
+        sum += w < wave ? n : 0;
+        used += n;
+    }
+    if (tid < E) {
+        s_total[tid] = sum - all + before;
+        if (blockIdx.x == 0) a.offsets[tid] = sum - all;
+    }
+    if (blockIdx.x == 0 && tid == 0) a.offsets[E] = used;
+    for (int64_t r = used + (int64_t)blockIdx.x * 1024 + tid; r < a.pairs; r += (int64_t)a.blocks * 1024) a.order[r] = -1;
+    __syncthreads();
+    for (int64_t i = from; i < to; i += 64) {
+        const bool there = i + lane < to;
+        const uint32_t id = there ? (uint32_t)a.chosen[i + lane] : ~0u;
+        const uint32_t e = min(id, (uint32_t)E);
+        const uint64_t same = same_expert(e, a.bits);
+        int r = -1;
+        if (e < (uint32_t)E) {
+            const int rank = (int)popc_below(same);
+            r = s_total[e] + mine[e] + rank;
+            wave_fence();
+            if (rank == 0) mine[e] += __popcll(same);
+            a.order[r] = (int)(i + lane);
+        }
+        wave_fence();
+        if (there) a.place[i + lane] = r;
     }
 }
 
@@ -350,6 +508,7 @@ static RouteArgs route_args(const bs_route& r)
     a.tokens = r.tokens, a.experts = r.experts, a.top_k = r.top_k, a.logits = r.logits, a.stride = r.logits_stride;
     a.f32 = r.logits_type == BS_DT_F32, a.bias = r.bias, a.sigmoid = r.score == BS_SCORE_SIGMOID, a.groups = r.groups;
     a.top_groups = r.top_groups, a.group_best = r.group_best, a.renorm = r.renormalize, a.scale = r.scale;
+    a.by_logit = r.bias == nullptr && (r.top_groups == r.groups || r.group_best == 1);
     return a;
 }
 
@@ -367,10 +526,10 @@ extern "C" int bs_route_forward(const bs_route* route, float* weights, int32_t* 
         return set_error(BS_ERR_INVALID, "%s: null or misaligned result", what);
     RouteArgs a = route_args(*route);
     a.weights = weights, a.chosen = chosen;
-    const int v = (a.experts + 63) / 64;
-    auto* kernel = v <= 1 ? route_forward_kernel<1> : v <= 2 ? route_forward_kernel<2> : v <= 4 ? route_forward_kernel<4>
-                   : v <= 8 ? route_forward_kernel<8> : route_forward_kernel<16>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.tokens + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+    const int E = a.experts, tokens = E <= 256 ? 16 : 4;        // of a workgroup
+    auto* kernel = E <= 16 ? route_forward_kernel<16, 1> : E <= 64 ? route_forward_kernel<16, 4> : E <= 128 ? route_forward_kernel<16, 8>
+                   : E <= 256 ? route_forward_kernel<16, 16> : E <= 512 ? route_forward_kernel<64, 8> : route_forward_kernel<64, 16>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.tokens + tokens - 1) / tokens)), dim3(256), 0, (hipStream_t)stream, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }
@@ -386,16 +545,28 @@ extern "C" int bs_route_backward(const bs_route* route, const int32_t* chosen, c
         return set_error(BS_ERR_INVALID, "%s: null or misaligned operand", what);
     RouteArgs a = route_args(*route);
     a.chosen = const_cast<int32_t*>(chosen), a.d_weights = d_weights, a.d_logits = d_logits;
-    const int v = (a.experts + 63) / 64;
-    auto* kernel = v <= 1 ? route_backward_kernel<1> : v <= 2 ? route_backward_kernel<2> : v <= 4 ? route_backward_kernel<4>
-                   : v <= 8 ? route_backward_kernel<8> : route_backward_kernel<16>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.tokens + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+    const int E = a.experts, tokens = E <= 256 ? 16 : 4;        // of a workgroup
+    auto* kernel = E <= 16 ? route_backward_kernel<16, 1> : E <= 64 ? route_backward_kernel<16, 4> : E <= 128 ? route_backward_kernel<16, 8>
+                   : E <= 256 ? route_backward_kernel<16, 16> : E <= 512 ? route_backward_kernel<64, 8> : route_backward_kernel<64, 16>;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.tokens + tokens - 1) / tokens)), dim3(256), 0, (hipStream_t)stream, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }
 
+static int64_t plan_blocks(int64_t pairs)
+{
+    return pairs <= 2 * kPlanBlock ? 1 : std::min<int64_t>((pairs + kPlanBlock - 1) / kPlanBlock, kPlanBlocks);
+}
+
+extern "C" int64_t bs_expert_plan_workspace_bytes(int64_t pairs, int experts)
+{
+    if (pairs <= 0 || pairs >= (1ll << 31) || experts < 1 || experts > kMaxExperts) return 0;
+    const int64_t blocks = plan_blocks(pairs);
+    return blocks > 1 ? blocks * experts * 4 : 0;
+}
+
 extern "C" int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts, int32_t* offsets, int32_t* order, int32_t* place,
-                              void* stream)
+                              void* workspace, int64_t workspace_bytes, void* stream)
 {
     clear_error();
     const char* what = "bs_expert_plan";
@@ -404,8 +575,17 @@ extern "C" int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts,
     if (offsets == nullptr || (pairs && (chosen == nullptr || order == nullptr || place == nullptr)))
         return set_error(BS_ERR_INVALID, "%s: null pointer", what);
     if (((uintptr_t)chosen | (uintptr_t)offsets | (uintptr_t)order | (uintptr_t)place) & 3u) return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
-    const PlanArgs a{chosen, (int32_t)pairs, experts, offsets, order, place};
-    hipLaunchKernelGGL(expert_plan_kernel, dim3((uint32_t)experts), dim3(1024), 0, (hipStream_t)stream, a);
+    const int64_t blocks = plan_blocks(pairs), run = ((pairs + blocks * 16 - 1) / (blocks * 16) + 63) / 64 * 64;
+    const int64_t need = bs_expert_plan_workspace_bytes(pairs, experts);
+    if (need && (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 3u)))
+        return set_error(BS_ERR_INVALID, "%s: workspace too small or misaligned", what);
+    int bits = 0;
+    while (experts >> bits) bits++;         // (ids up to and with `experts`)
+    const PlanArgs a{chosen, pairs, run, experts, bits, (int)blocks, offsets, order, place, static_cast<int32_t*>(workspace)};
+    const uint32_t lds = 17u * experts * 4;
+    const hipStream_t st = (hipStream_t)stream;
+    if (blocks > 1) hipLaunchKernelGGL(expert_plan_kernel<true>, dim3((uint32_t)blocks), dim3(1024), lds, st, a);
+    hipLaunchKernelGGL(expert_plan_kernel<false>, dim3((uint32_t)blocks), dim3(1024), lds, st, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }

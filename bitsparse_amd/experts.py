@@ -42,10 +42,11 @@ def route(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Tensor | 
     balance; it has no part in the weights and no gradient), with ``groups``
     among the experts of the ``top_groups`` groups (all by default) whose
     ``group_best`` (1 or 2) best ones have the largest sum; of equal ones the
-    lower index, as 64-bit values.  weights = scale * s, divided by the sum over the
+    lower index.  The choice is as between 64-bit values (between the logits
+    themselves where the order is theirs).  weights = scale * s, divided by the sum over the
     token's choices with ``renormalize``.
     An expert whose logit (or whose biased score) is -inf is not chosen; a choice left without
-    one is -1 with weight 0, which is how a padded token (all -inf) goes nowhere.  A NaN score goes before all others.
+    one is -1 with weight 0, which is how a padded token (all -inf) goes nowhere.  A NaN counts as +inf.
     Differentiable once in logits."""
     if score not in _SCORES:
         raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")

@@ -772,7 +772,9 @@ int bs_route_backward(const bs_route* route, const int32_t* chosen, const float*
  * equal ids stay in order.  Ids outside 0..experts-1 have place -1 and no
  * row; order is -1 in the rows that are left at the end.
  */
-int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts, int32_t* offsets, int32_t* order, int32_t* place, void* stream);
+int64_t bs_expert_plan_workspace_bytes(int64_t pairs, int experts);
+int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts, int32_t* offsets, int32_t* order, int32_t* place,
+                   void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Products of the experts' rows with their bf16 weights [experts, out, in]
