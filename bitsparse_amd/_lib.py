@@ -103,10 +103,10 @@ _SIGNATURES = {
     "bs_expert_plan_workspace_bytes": [_i64, _int],
     "bs_expert_plan": [_vp, _i64, _int, _vp, _vp, _vp, _vp, _i64, _vp],
     "bs_expert_linear": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _int, _f32, _vp, _vp],
-    "bs_expert_linear_dx": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
+    "bs_expert_linear_dx": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _int, _vp],
     "bs_expert_linear_dw": [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
     "bs_pad_rows": [_vp, _i64, _i64, _i64, _vp, _i64, _vp],
-    "bs_expert_combine": [_vp, _i64, _vp, _vp, _i64, _int, _i64, _i64, _vp, _vp],
+    "bs_expert_combine": [_vp, _int, _i64, _vp, _vp, _i64, _int, _i64, _i64, _vp, _vp],
     "bs_expert_combine_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _int, _i64, _i64, _vp, _vp, _vp],
     "bs_experts_act_grad": [_vp, _vp, _i64, _i64, _int, _f32, _vp, _vp, _vp, _i64, _vp, _vp],
     "bs_newton_schulz_workspace_bytes": [_i64, _i64, _i64, _int],

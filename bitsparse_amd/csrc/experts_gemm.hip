@@ -10,6 +10,7 @@
 // tiles of ragged groups are found on the device, so the host knows nothing
 // of the routing and waits for nothing.
 #include <algorithm>
+#include <cmath>
 
 #include "bs_host.h"
 #include "gemm_common.h"
@@ -32,10 +33,11 @@ struct ExpertGemm {
     int64_t rows, tokens;                       // tokens: rows of a gathered operand
     const bf16 *a, *b;
     int64_t a_stride, b_stride, b_expert;       // elements
-    bf16* c;
+    void* c;
+    int c_f32;                                  // results in 32 bits
     int64_t c_expert;
     int m, n, k;                                // of one expert's product; m or k of the rows is -1
-    int tiles_m, tiles_n;
+    int tiles_m, tiles_n, panel;
     int act;
     float act_k;
 };
@@ -44,10 +46,15 @@ struct ExpertGemm {
 // LDS tiles of a K-step of 64.  K contiguous: rows of 128 bytes, the 16-byte
 // chunk c of row r at c ^ r % 8, so the 16 lanes that a fragment read serves at a
 // time meet all 64 banks.  K down the rows: T columns a row, the chunk u of
-// row k at u ^ 2 (k % 4 + 4 (k / 8 % 2)): 32 lanes of a transposing read take
-// half of eight rows.
+// row k at u ^ col_turn(k): 32 lanes of a transposing read take two chunks of
+// eight rows, k % 4 + 8 (k / 8 % 2), which lie 16 chunks or (T = 64) 8 apart.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ int col_turn(int k) { return 2 * ((k & 3) + 4 * (k >> 3 & 1)); }
+template <int T>
+__device__ __forceinline__ int col_turn(int k)
+{
+    static_assert(T % 64 == 0 && (T & (T - 1)) == 0, "whole loads of rows, chunks that a turn stays among");
+    return T == 64 ? 2 * ((k >> 1 & 1) + 2 * (k >> 3 & 1)) : 2 * ((k & 3) + 4 * (k >> 3 & 1));
+}
 
 template <int T, bool ALONG_K>
 __device__ __forceinline__ bf16x8 read_fragment(const char* tile, int r0, int k0, int lane)
@@ -58,7 +65,7 @@ __device__ __forceinline__ bf16x8 read_fragment(const char* tile, int r0, int k0
     } else {
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
         const int j = lane & 15, k = k0 + 8 * (lane >> 4) + (j >> 2), u = r0 / 8 + ((j & 3) >> 1);
-        const char* at = tile + k * (T * 2) + ((u ^ col_turn(k)) * 16) + (j & 1) * 8;
+        const char* at = tile + k * (T * 2) + ((u ^ col_turn<T>(k)) * 16) + (j & 1) * 8;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * (T * 2)));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -94,6 +101,17 @@ __device__ __forceinline__ int group_bound(const ExpertGemm& g, int e)
 {
     return (int)max((int64_t)0, min((int64_t)g.offsets[e], g.rows));
 }
+// the sum over this lane and those below it: four steps inside rows of 16 lanes, two across them
+__device__ __forceinline__ int wave_scan(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);     // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);     // last lane of rows 0, 2 into rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);     // last lane of row 1 into rows 2, 3
+    return v;
+}
 __device__ __forceinline__ Group find_group(const ExpertGemm& g, int tile, int size)
 {
     const int lane = threadIdx.x & 63;
@@ -101,21 +119,16 @@ __device__ __forceinline__ Group find_group(const ExpertGemm& g, int tile, int s
     for (int e0 = 0; e0 < g.experts; e0 += 64) {
         const int e = e0 + lane;
         const int from = group_bound(g, min(e, g.experts)), to = max(from, group_bound(g, min(e + 1, g.experts)));
-        const int tiles = (to - from + size - 1) / size;
-        int sum = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(sum, d);
-            sum += lane >= d ? o : 0;
-        }
+        const int tiles = (int)((uint32_t)(to - from + size - 1) / (uint32_t)size);
+        const int sum = wave_scan(tiles);
         const uint64_t past = __ballot(before + sum > tile);
         if (past) {
             const int at = __builtin_ctzll(past);
             const int mine = before + sum - tiles;
-            return {e0 + at, (int64_t)(int)uniform_u32((uint32_t)__shfl(from, at)), (int64_t)(int)uniform_u32((uint32_t)__shfl(to, at)),
-                    (int64_t)(tile - (int)uniform_u32((uint32_t)__shfl(mine, at)))};
+            return {e0 + at, (int64_t)__builtin_amdgcn_readlane(from, at), (int64_t)__builtin_amdgcn_readlane(to, at),
+                    (int64_t)(tile - __builtin_amdgcn_readlane(mine, at))};
         }
-        before += (int)uniform_u32((uint32_t)__shfl(sum, 63));
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
     return {-1, (int64_t)group_bound(g, g.experts), g.rows, (int64_t)(tile - before)};
 }
@@ -137,22 +150,63 @@ __device__ __forceinline__ float activated(float z, int act, float k)
     return bf16_to_f32(act == BS_ACT_RELU ? r : relu2_sq_bits(r, k));
 }
 
-// WGM x WGN waves, each 16 IM x 16 JN results
-template <int KIND, bool GATHER, int WGM, int WGN, int IM, int JN>
+// four results of a row from column `col` on; `row`: the row's first element
+template <int KIND>
+__device__ __forceinline__ void store_four(const ExpertGemm& g, int64_t row, int64_t col, const f32x4& v)
+{
+    if (col >= g.n) return;
+    const int nv = (int)min((int64_t)4, g.n - col);
+    if (KIND == kDx && g.c_f32) {
+        float* to = static_cast<float*>(g.c) + row + col;
+        if (g.n % 4 == 0) {
+            *reinterpret_cast<f32x4*>(to) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (e < nv) to[e] = v[e];
+        }
+        return;
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = f32_to_bf16(KIND == kForward ? activated(v[e], g.act, g.act_k) : v[e]);
+    uint16_t* to = static_cast<uint16_t*>(g.c) + row + col;
+    if (g.n % 4 == 0) {
+        *reinterpret_cast<uint2*>(to) = uint2{o[0] | o[1] << 16, o[2] | o[3] << 16};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < nv) to[e] = (uint16_t)o[e];
+    }
+}
+
+// WGM x WGN waves, each 16 IM x 16 JN results.  AHEAD: fragments are read ahead of the barrier, for a workgroup that has a
+// CU to itself.
+template <int KIND, bool GATHER, int WGM, int WGN, int IM, int JN, int STAGES, bool AHEAD>
 __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm g)
 {
     constexpr int WAVES = WGM * WGN, TM = 16 * IM * WGM, TN = 16 * JN * WGN;
     constexpr bool A_ALONG = KIND != kDw, B_ALONG = KIND == kForward;
-    constexpr bool GA = GATHER && KIND == kForward, GB = GATHER && KIND == kDw;
+    static_assert(!GATHER || KIND == kForward, "x is gathered by the forward product alone");
     constexpr int A_BYTES = TM * kRowBytes, B_BYTES = TN * kRowBytes, STAGE = A_BYTES + B_BYTES;
     constexpr int LA = TM / 8 / WAVES, LB = TN / 8 / WAVES;     // loads of a wave, 1 KiB each
     static_assert(LA * 8 * WAVES == TM && LB * 8 * WAVES == TN, "a stage is whole loads of every wave");
-    static_assert(2 * STAGE <= 160 * 1024, "LDS budget");
-    __shared__ __attribute__((aligned(16))) char s_mem[2 * STAGE];
+    static_assert(STAGES * STAGE <= 160 * 1024 && (!AHEAD || STAGES == 2), "LDS budget");
+    constexpr int AT_ONCE = kCus * (160 * 1024 / (STAGES * STAGE));
+    __shared__ __attribute__((aligned(16))) char s_mem[STAGES * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
 
-    const int tn = (int)blockIdx.x % g.tiles_n, tm = (int)blockIdx.x / g.tiles_n;
+    // Workgroups go round the XCDs in turn: of as many as are resident at once each XCD takes a run, in panels of g.panel rows
+    // of tiles, whose neighbours share rows of A and of B.
+    int id = (int)blockIdx.x;
+    if (g.panel > 1) {
+        const int group = id / AT_ONCE * AT_ONCE;
+        if (group + AT_ONCE <= (int)gridDim.x) id = group + (id - group) % kXcds * (AT_ONCE / kXcds) + (id - group) / kXcds;
+    }
+    const int panel = id / (g.panel * g.tiles_n), in_panel = id - panel * g.panel * g.tiles_n;
+    const int high = min(g.panel, (int)gridDim.x / g.tiles_n - panel * g.panel);
+    const int tm = panel * g.panel + in_panel % high, tn = in_panel / high;
     Group grp;
     int64_t c_row, c_rows, k_total;
     if constexpr (KIND == kDw) {
@@ -173,18 +227,19 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
     const bf16* b_base = g.b + (KIND == kDw ? 0 : max(0, grp.expert) * g.b_expert);
     const int64_t a_row_bytes = g.a_stride * 2, b_row_bytes = g.b_stride * 2;
     // K down the rows: this lane's row of a load and its chunk of columns
-    auto along_m = [&](int i, int loads, int t, int& k, int& unit) {
-        k = (wave * loads + i) * (512 / t) + lane / (t / 8);
-        unit = (lane % (t / 8)) ^ col_turn(k);
+    auto along_m = [&](int i, int loads, auto t, int& k, int& unit) {
+        constexpr int T = decltype(t)::value;
+        k = (wave * loads + i) * (512 / T) + lane / (T / 8);
+        unit = (lane % (T / 8)) ^ col_turn<T>(k);
     };
     i32x4 ra, rb;
     if constexpr (A_ALONG) {
-        const bf16* base = GA ? g.a : g.a + c_row * g.a_stride;
-        ra = rsrc_words(base, GA ? ((g.tokens - 1) * g.a_stride + g.k + 7) / 8 * 16 : (int64_t)kNoRow);
+        const bf16* base = GATHER ? g.a : g.a + c_row * g.a_stride;
+        ra = rsrc_words(base, GATHER ? ((g.tokens - 1) * g.a_stride + g.k + 7) / 8 * 16 : (int64_t)kNoRow);
 #pragma unroll
         for (int i = 0; i < LA; i++) {
             const int64_t r = (wave * LA + i) * 8 + (lane >> 3);
-            const int64_t at = c_row + r < c_rows && k_total ? (GA ? source_row<GA>(g, c_row + r) : r) : -1;
+            const int64_t at = c_row + r < c_rows && k_total ? (GATHER ? source_row<GATHER>(g, c_row + r) : r) : -1;
             a_off[i] = at < 0 ? kNoRow : (uint32_t)(at * a_row_bytes) + chunk * 16;
         }
     }
@@ -198,13 +253,12 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
     }
     const int steps = (int)((k_total + kBK - 1) / kBK);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem;
-    auto load = [&](int step, int stage) {
-        const uint32_t lds = lds0 + stage * STAGE;
-        const bool in_k = chunk * 8 + step * kBK < g.k;        // of an operand with K along its rows
+    auto load_a = [&](int step, int stage) {
+        const uint32_t lds = lds0 + stage * STAGE + wave * LA * 1024;
         if constexpr (A_ALONG) {
+            const bool in_k = chunk * 8 + step * kBK < g.k;
 #pragma unroll
-            for (int i = 0; i < LA; i++)
-                load_lds16(ra, lds + (wave * LA + i) * 1024, in_k ? a_off[i] : kNoRow, (uint32_t)step * kRowBytes);
+            for (int i = 0; i < LA; i++) load_lds16(ra, lds + i * 1024, in_k ? a_off[i] : kNoRow, (uint32_t)step * kRowBytes);
         } else {
             // (the rows that are left bound the operand: those behind them are zeros)
             const int64_t at = grp.first + (int64_t)step * kBK, left = grp.end - at;
@@ -212,100 +266,267 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
 #pragma unroll
             for (int i = 0; i < LA; i++) {
                 int k, unit;
-                along_m(i, LA, TM, k, unit);
-                load_lds16(r, lds + (wave * LA + i) * 1024, (uint32_t)(k * a_row_bytes) + (uint32_t)(c_row * 2) + unit * 16, 0);
+                along_m(i, LA, IC<TM>{}, k, unit);
+                load_lds16(r, lds + i * 1024, (uint32_t)(k * a_row_bytes) + (uint32_t)(c_row * 2) + unit * 16, 0);
             }
         }
+    };
+    auto load_b = [&](int step, int stage) {
+        const uint32_t lds = lds0 + stage * STAGE + A_BYTES + wave * LB * 1024;
         if constexpr (B_ALONG) {
+            const bool in_k = chunk * 8 + step * kBK < g.k;
 #pragma unroll
-            for (int i = 0; i < LB; i++)
-                load_lds16(rb, lds + A_BYTES + (wave * LB + i) * 1024, in_k ? b_off[i] : kNoRow, (uint32_t)step * kRowBytes);
+            for (int i = 0; i < LB; i++) load_lds16(rb, lds + i * 1024, in_k ? b_off[i] : kNoRow, (uint32_t)step * kRowBytes);
         } else {
             const int64_t at = (KIND == kDw ? grp.first : 0) + (int64_t)step * kBK, end = KIND == kDw ? grp.end : g.k;
-            const bf16* base = GB ? g.b : b_base + at * g.b_stride;
-            const i32x4 r = rsrc_words(base, ((GB ? g.tokens : end - at) - 1) * b_row_bytes + (g.n + 7) / 8 * 16);
+            const i32x4 r = rsrc_words(b_base + at * g.b_stride, (end - at - 1) * b_row_bytes + (g.n + 7) / 8 * 16);
 #pragma unroll
             for (int i = 0; i < LB; i++) {
                 int k, unit;
-                along_m(i, LB, TN, k, unit);
-                int64_t src = k;
-                if constexpr (GB) src = at + k < end ? source_row<GB>(g, at + k) : -1;
-                load_lds16(r, lds + A_BYTES + (wave * LB + i) * 1024,
-                           src < 0 ? kNoRow : (uint32_t)(src * b_row_bytes) + (uint32_t)(c_col * 2) + unit * 16, 0);
+                along_m(i, LB, IC<TN>{}, k, unit);
+                load_lds16(r, lds + i * 1024, (uint32_t)(k * b_row_bytes) + (uint32_t)(c_col * 2) + unit * 16, 0);
             }
         }
     };
 
+    // A step is two halves of 32 of K.  A fragment of A is read again, for the next half, as soon as its last product is
+    // under way, those of B into a second set.  The one barrier of a step stands a quarter into its second half: by then
+    // all of the step's stage is in registers, so that it is loaded again, and the next step's stage has come, a whole
+    // step after its loads.
+    constexpr int MEET = IM / 4;
+    bf16x8 fa[IM], fb[2][JN];
+    auto read_a = [&](int stage, int i, int k0) { fa[i] = read_fragment<TM, A_ALONG>(s_mem + stage * STAGE, wm * 16 * IM + 16 * i, k0, lane); };
+    auto read_b = [&](int stage, int j, int k0) {
+        fb[k0 / 32][j] = read_fragment<TN, B_ALONG>(s_mem + stage * STAGE + A_BYTES, wn * 16 * JN + 16 * j, k0, lane);
+    };
     f32x4 acc[IM][JN];
 #pragma unroll
     for (int i = 0; i < IM; i++)
 #pragma unroll
         for (int j = 0; j < JN; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (steps) load(0, 0);
-    for (int step = 0; step < steps; step++) {
-        // this step's parts are there and the other stage has been read, in every wave
-        wait_for_loads();
+    if constexpr (!AHEAD) {
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++)
+            if (i < steps) {
+                load_a(i, i);
+                load_b(i, i);
+            }
+        for (int step = 0, stage = 0; step < steps; step++) {
+            // this step's stage has come and the last one's has been read, in every wave
+            if (step + STAGES - 2 < steps)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * (LA + LB)) : "memory");
+            else
+                wait_for_loads();
+            barrier_only();
+            if (step + STAGES - 1 < steps) {
+                const int last = stage == 0 ? STAGES - 1 : stage - 1;
+                load_a(step + STAGES - 1, last);
+                load_b(step + STAGES - 1, last);
+            }
+#pragma unroll
+            for (int k0 = 0; k0 < kBK; k0 += 32) {
+#pragma unroll
+                for (int i = 0; i < IM; i++) read_a(stage, i, k0);
+#pragma unroll
+                for (int j = 0; j < JN; j++) read_b(stage, j, k0);
+#pragma unroll
+                for (int i = 0; i < IM; i++)
+#pragma unroll
+                    for (int j = 0; j < JN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[k0 / 32][j], fa[i], acc[i][j], 0, 0, 0);
+            }
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+        }
+    }
+    if (AHEAD && steps) {
+        load_a(0, 0);
+        load_b(0, 0);
+        if (steps > 1) {
+            load_a(1, 1);
+            load_b(1, 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LA + LB) : "memory");
+        } else {
+            wait_for_loads();
+        }
         barrier_only();
-        if (step + 1 < steps) load(step + 1, (step + 1) & 1);
-        const char* ta = s_mem + (step & 1) * STAGE;
 #pragma unroll
-        for (int k0 = 0; k0 < kBK; k0 += 32) {
-            bf16x8 fa[IM], fb[JN];
+        for (int i = 0; i < IM; i++) read_a(0, i, 0);
 #pragma unroll
-            for (int i = 0; i < IM; i++) fa[i] = read_fragment<TM, A_ALONG>(ta, wm * 16 * IM + 16 * i, k0, lane);
+        for (int j = 0; j < JN; j++) read_b(0, j, 0);
+    }
+    for (int step = 0; AHEAD && step < steps; step++) {
+        const int stage = step & 1;
 #pragma unroll
-            for (int j = 0; j < JN; j++) fb[j] = read_fragment<TN, B_ALONG>(ta + A_BYTES, wn * 16 * JN + 16 * j, k0, lane);
+        for (int i = 0; i < IM; i++) {
 #pragma unroll
-            for (int i = 0; i < IM; i++)
+            for (int j = i; j < JN; j += IM) read_b(stage, j, 32);
 #pragma unroll
-                for (int j = 0; j < JN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < JN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[0][j], fa[i], acc[i][j], 0, 0, 0);
+            read_a(stage, i, 32);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // (behind the last step the next stage holds what it held: read, not used)
+#pragma unroll
+        for (int i = 0; i < IM; i++) {
+            if (i == MEET) {
+                wait_for_loads();
+                barrier_only();
+            }
+#pragma unroll
+            for (int j = i - MEET; j < JN && j >= 0; j += IM - MEET) read_b(stage ^ 1, j, 0);
+#pragma unroll
+            for (int j = 0; j < JN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[1][j], fa[i], acc[i][j], 0, 0, 0);
+            if (i >= MEET) read_a(stage ^ 1, i, 0);
+            if (i == MEET)
+#pragma unroll
+                for (int o = 0; o < MEET; o++) read_a(stage ^ 1, o, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (step + 2 < steps) {
+                if (i == MEET) load_a(step + 2, stage);
+                if (i == MEET + 1) load_b(step + 2, stage);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
     // a lane has row lane % 16 and columns 4 (lane / 16) on of each block
-    bf16* c = g.c + (KIND == kDw ? grp.expert * g.c_expert : 0);
-    const bool wide = g.n % 4 == 0;
+    const int64_t c0 = KIND == kDw ? grp.expert * g.c_expert : 0;
 #pragma unroll
     for (int i = 0; i < IM; i++) {
         const int64_t r = c_row + (wm * IM + i) * 16 + (lane & 15);
         if (r >= c_rows) continue;
 #pragma unroll
-        for (int j = 0; j < JN; j++) {
-            const int64_t col = c_col + (wn * JN + j) * 16 + 4 * (lane >> 4);
-            if (col >= g.n) continue;
-            uint32_t o[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = f32_to_bf16(KIND == kForward ? activated(acc[i][j][e], g.act, g.act_k) : acc[i][j][e]);
-            uint16_t* to = reinterpret_cast<uint16_t*>(c) + r * g.n + col;
-            if (wide) {
-                *reinterpret_cast<uint2*>(to) = uint2{o[0] | o[1] << 16, o[2] | o[3] << 16};
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (col + e < g.n) to[e] = (uint16_t)o[e];
-            }
-        }
+        for (int j = 0; j < JN; j++) store_four<KIND>(g, c0 + r * g.n, c_col + (wn * JN + j) * 16 + 4 * (lane >> 4), acc[i][j]);
     }
 }
 
-template <int KIND, bool GATHER, int WGM, int WGN, int IM, int JN>
+// ---------------------------------------------------------------------------
+// Forward for few rows an expert: bound by reading the experts' weights.  A
+// workgroup has 16 columns and up to 32 rows, each of its eight waves an eighth
+// of K, whose operands go from memory straight into registers, eight steps of
+// 32 of K at once; the waves' sums meet in LDS, in order.
+// ---------------------------------------------------------------------------
+constexpr int kFewRows = 32, kFewCols = 16, kFewAhead = 8;
+
+template <bool GATHER, int MR>
+__device__ __forceinline__ void few_products(const ExpertGemm& g, const Group& grp, int64_t c_row, int64_t c_rows, int64_t c_col, f32x4 (*s_sum)[2][64])
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int steps = grp.expert < 0 ? 0 : (g.k + 31) / 32, from = steps * wave / 8, to = steps * (wave + 1) / 8;
+    const int k_lane = (lane >> 4) * 8;
+    const bf16* w = nullptr;
+    if (c_col + (lane & 15) < g.n) w = g.b + max(0, grp.expert) * g.b_expert + (c_col + (lane & 15)) * g.b_stride + k_lane;
+    const bf16* x[MR];
+#pragma unroll
+    for (int m = 0; m < MR; m++) {
+        const int64_t r = c_row + 16 * m + (lane & 15), at = r < c_rows && steps ? source_row<GATHER>(g, r) : -1;
+        x[m] = at < 0 ? nullptr : g.a + at * g.a_stride + k_lane;
+    }
+    f32x4 acc[MR];
+#pragma unroll
+    for (int m = 0; m < MR; m++) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = from; s0 < to; s0 += kFewAhead) {
+        bf16x8 fw[kFewAhead], fx[MR][kFewAhead];
+#pragma unroll
+        for (int u = 0; u < kFewAhead; u++) {
+            const int k = (s0 + u) * 32;
+            const bool in = s0 + u < to && k + k_lane < g.k;
+            fw[u] = w && in ? *reinterpret_cast<const bf16x8*>(w + k) : bf16x8{};
+#pragma unroll
+            for (int m = 0; m < MR; m++) fx[m][u] = x[m] && in ? *reinterpret_cast<const bf16x8*>(x[m] + k) : bf16x8{};
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < kFewAhead; u++)
+#pragma unroll
+            for (int m = 0; m < MR; m++) acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[u], fx[m][u], acc[m], 0, 0, 0);
+    }
+#pragma unroll
+    for (int m = 0; m < MR; m++) s_sum[wave][m][lane] = acc[m];
+    __syncthreads();
+    if (wave >= MR) return;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum += s_sum[i][wave][lane];
+    const int64_t r = c_row + 16 * wave + (lane & 15);
+    if (r < c_rows) store_four<kForward>(g, r * g.n, c_col + 4 * (lane >> 4), sum);
+}
+
+template <bool GATHER>
+__global__ __launch_bounds__(512) void expert_few_kernel(ExpertGemm g)
+{
+    __shared__ __attribute__((aligned(16))) f32x4 s_sum[8][2][64];
+    const int tn = (int)blockIdx.x % g.tiles_n, tm = (int)blockIdx.x / g.tiles_n;
+    const Group grp = find_group(g, tm, kFewRows);
+    const int64_t c_row = grp.first + grp.tile * kFewRows, c_rows = min(grp.end, c_row + kFewRows);
+    if (c_row >= c_rows) return;
+    if (c_rows - c_row <= 16)
+        few_products<GATHER, 1>(g, grp, c_row, c_rows, (int64_t)tn * kFewCols, s_sum);
+    else
+        few_products<GATHER, 2>(g, grp, c_row, c_rows, (int64_t)tn * kFewCols, s_sum);
+}
+
+template <int KIND, bool GATHER, int WGM, int WGN, int IM, int JN, int STAGES, bool AHEAD>
 static int launch_gemm(ExpertGemm g, const char* what, hipStream_t st)
 {
     constexpr int TM = 16 * IM * WGM, TN = 16 * JN * WGN;
     g.tiles_n = (g.n + TN - 1) / TN;
     g.tiles_m = KIND == kDw ? (g.m + TM - 1) / TM : 0;
-    // every expert's last tile may be a part of one, and so may that of the rows behind them
-    const int64_t tiles_m = KIND == kDw ? (int64_t)g.experts * g.tiles_m : g.rows / TM + g.experts + 2;
+    // (parts of tiles: one at most for each expert that has rows, and one of the rows behind them)
+    const int64_t tiles_m = KIND == kDw ? (int64_t)g.experts * g.tiles_m : g.rows / TM + std::min<int64_t>(g.experts + 1, g.rows);
+    g.panel = 8;
     if (tiles_m * g.tiles_n >= (1ll << 31)) return set_error(BS_ERR_INVALID, "%s: too many tiles", what);
-    hipLaunchKernelGGL((expert_gemm_kernel<KIND, GATHER, WGM, WGN, IM, JN>), dim3((uint32_t)(tiles_m * g.tiles_n)), dim3(64 * WGM * WGN), 0, st, g);
+    hipLaunchKernelGGL((expert_gemm_kernel<KIND, GATHER, WGM, WGN, IM, JN, STAGES, AHEAD>), dim3((uint32_t)(tiles_m * g.tiles_n)), dim3(64 * WGM * WGN), 0, st, g);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }
 
+template <bool GATHER>
+static int launch_few(ExpertGemm g, const char* what, hipStream_t st)
+{
+    g.tiles_n = (g.n + kFewCols - 1) / kFewCols;
+    const int64_t tiles_m = g.rows / kFewRows + std::min<int64_t>(g.experts + 1, g.rows);
+    hipLaunchKernelGGL(expert_few_kernel<GATHER>, dim3((uint32_t)(tiles_m * g.tiles_n)), dim3(512), 0, st, g);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+}
+
+// What a product takes on tiles of one size, in us: rounds of as many as are
+// resident at once, each its steps and a start and an end.  The host knows how
+// many rows there are, not how they lie: half a tile is left over for each
+// expert, and the longest of dW's sums has 1.4 times the mean's steps.
+static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_once, double step)
+{
+    const double columns = (g.n + tn - 1) / tn;
+    if (kind == kDw) {
+        const double tiles = (double)g.experts * ((g.m + tm - 1) / tm) * columns, time = (double)g.rows / g.experts / kBK * step;
+        return std::max(1.0, tiles / at_once) * (time + 5.0) + 0.4 * time;
+    }
+    const double tiles = ((double)g.rows / tm + 0.5 * (double)std::min<int64_t>(g.experts, g.rows)) * columns;
+    return std::ceil(std::max(1.0, tiles) / at_once) * ((double)g.k / kBK * step + 5.0);
+}
+
+// Forward for up to two rows an expert: expert_few_kernel (8 rows of 64 experts of 4096 -> 1024 13.2 us, on tiles of 64 x 64
+// 20.9; 64 rows 50 and 65; 32 rows of 8 experts of 4096 -> 2048 24.3 and 22.0).  Else the tile whose time is least by
+// tile_time (measured in us, forward / dx / dW, x gathered in forward):
+//   rows, experts, in -> out           64 x 64       128 x 128     192 x 128   256 x 256
+//   16384,  8,  768 -> 2048         122 / 98 / 100   82 / 67 / 72   76 / 76 / -   87 / 62 / 80
+//   16384,  8, 2048 ->  768          94 / 109 / 95   67 / 73 / 70   74 / 67 / -   55 / 83 / 79
+//   32768, 16, 2048 -> 4096               -         619 / 571 / 591 571 / 533 / - 530 / 520 / 540
+//   16384,  4,  512 -> 1024          50 / 39 / 41    37 / 33 / 62   32 / 28 / -   44 / 34 / 133
+//     512,  8, 2048 -> 2048          21 / 22 / 46    27 / 25 / 28   32 / 29 / -   45 / 47 / 29
 template <int KIND, bool GATHER>
 static int launch_kind(const ExpertGemm& g, const char* what, hipStream_t st)
 {
-    return launch_gemm<KIND, GATHER, 2, 2, 4, 4>(g, what, st);
+    if constexpr (KIND == kForward)
+        if (g.rows <= 2 * std::min<int64_t>(g.experts, g.rows)) return launch_few<GATHER>(g, what, st);
+    const double small = tile_time(g, KIND, 64, 64, kCus * 2, 0.45), middle = tile_time(g, KIND, 128, 128, kCus * 2, 0.98),
+                 wide = tile_time(g, KIND, 192, 128, kCus * 2, 1.33), large = tile_time(g, KIND, 256, 256, kCus, 1.7);
+    const double best = std::min(std::min(small, middle), KIND == kDw ? large : std::min(wide, large));
+    if (best == large) return launch_gemm<KIND, GATHER, 2, 4, 8, 4, 2, true>(g, what, st);
+    if constexpr (KIND != kDw)
+        if (best == wide) return launch_gemm<KIND, GATHER, 2, 2, 6, 4, 2, false>(g, what, st);
+    if (best == middle) return launch_gemm<KIND, GATHER, 2, 2, 4, 4, 2, false>(g, what, st);
+    return launch_gemm<KIND, GATHER, 2, 2, 2, 2, 4, false>(g, what, st);
 }
 
 static int experts_check(const bs_experts* x, int64_t in, int64_t out, const char* what)
@@ -374,25 +595,25 @@ extern "C" int bs_expert_linear(const bs_experts* experts, const void* x, int64_
     if (y == nullptr || ((uintptr_t)y & 7u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned y", what);
     ExpertGemm g = gemm_args(*experts, gather);
     g.a = static_cast<const bf16*>(x), g.a_stride = x_stride, g.b = static_cast<const bf16*>(W), g.b_stride = w_stride, g.b_expert = out * w_stride;
-    g.c = static_cast<bf16*>(y), g.m = -1, g.n = (int)out, g.k = (int)in, g.act = act, g.act_k = act_k;
+    g.c = y, g.m = -1, g.n = (int)out, g.k = (int)in, g.act = act, g.act_k = act_k;
     return gather ? launch_kind<kForward, true>(g, what, (hipStream_t)stream) : launch_kind<kForward, false>(g, what, (hipStream_t)stream);
 }
 
 extern "C" int bs_expert_linear_dx(const bs_experts* experts, const void* dy, int64_t dy_stride, const void* W, int64_t w_stride, int64_t in,
-                                   int64_t out, void* dx, void* stream)
+                                   int64_t out, void* dx, int dx_type, void* stream)
 {
     clear_error();
     const char* what = "bs_expert_linear_dx";
     if (const int rc = experts_check(experts, in, out, what); rc != BS_OK) return rc;
     if (experts->rows == 0) return BS_OK;
-    const bool gather = experts->order != nullptr;
-    (void)gather;
+    if (experts->order) return set_error(BS_ERR_INVALID, "%s: dx is rows in the experts' order, so order must be null", what);
+    if (dx_type != BS_DT_BF16 && dx_type != BS_DT_F32) return set_error(BS_ERR_INVALID, "%s: dx dtype %d must be bf16 or fp32", what, dx_type);
     if (const int rc = operand_check(what, "dy", dy, experts->rows, dy_stride, out, false); rc != BS_OK) return rc;
     if (const int rc = operand_check(what, "W", W, out, w_stride, in, false); rc != BS_OK) return rc;
-    if (dx == nullptr || ((uintptr_t)dx & 7u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned dx", what);
+    if (dx == nullptr || ((uintptr_t)dx & 15u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned dx", what);
     ExpertGemm g = gemm_args(*experts, false);
     g.a = static_cast<const bf16*>(dy), g.a_stride = dy_stride, g.b = static_cast<const bf16*>(W), g.b_stride = w_stride, g.b_expert = out * w_stride;
-    g.c = static_cast<bf16*>(dx), g.m = -1, g.n = (int)in, g.k = (int)out;
+    g.c = dx, g.c_f32 = dx_type == BS_DT_F32, g.m = -1, g.n = (int)in, g.k = (int)out;
     return launch_kind<kDx, false>(g, what, (hipStream_t)stream);
 }
 
@@ -402,14 +623,14 @@ extern "C" int bs_expert_linear_dw(const bs_experts* experts, const void* dy, in
     clear_error();
     const char* what = "bs_expert_linear_dw";
     if (const int rc = experts_check(experts, in, out, what); rc != BS_OK) return rc;
-    const bool gather = experts->order != nullptr;
+    if (experts->order) return set_error(BS_ERR_INVALID, "%s: x is rows in the experts' order, so order must be null", what);
     if (const int rc = operand_check(what, "dy", dy, experts->rows, dy_stride, out, false); rc != BS_OK) return rc;
-    if (const int rc = operand_check(what, "x", x, experts->rows == 0 ? 0 : gather ? experts->tokens : experts->rows, x_stride, in, gather); rc != BS_OK) return rc;
+    if (const int rc = operand_check(what, "x", x, experts->rows, x_stride, in, false); rc != BS_OK) return rc;
     if (dW == nullptr || ((uintptr_t)dW & 7u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned dW", what);
-    ExpertGemm g = gemm_args(*experts, gather);
+    ExpertGemm g = gemm_args(*experts, false);
     g.a = static_cast<const bf16*>(dy), g.a_stride = dy_stride, g.b = static_cast<const bf16*>(x), g.b_stride = x_stride;
-    g.c = static_cast<bf16*>(dW), g.c_expert = in * out, g.m = (int)out, g.n = (int)in, g.k = -1;
-    return gather ? launch_kind<kDw, true>(g, what, (hipStream_t)stream) : launch_kind<kDw, false>(g, what, (hipStream_t)stream);
+    g.c = dW, g.c_expert = in * out, g.m = (int)out, g.n = (int)in, g.k = -1;
+    return launch_kind<kDw, false>(g, what, (hipStream_t)stream);
 }
 
 extern "C" int bs_pad_rows(const void* x, int64_t rows, int64_t cols, int64_t stride, void* out, int64_t width, void* stream)

@@ -18,7 +18,7 @@ constexpr int kTailBlocks = 64;     // workgroups that clear the rows behind the
 struct CombineArgs {
     int64_t tokens, rows, cols;
     int top_k;
-    const bf16* y;
+    const void* y;
     int64_t y_stride;
     const float* weights;       // null: 1
     const int32_t *place, *used;        // used: rows that belong to an expert
@@ -30,7 +30,7 @@ struct CombineArgs {
     float* dw;
 };
 
-template <bool WHOLE>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
 {
     const int64_t t = blockIdx.x;
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
             const int p = place[j];
             if (p < 0 || p >= a.rows) continue;
             const float w = a.weights ? a.weights[t * a.top_k + j] : 1.f;
-            const Raw<bf16> y = load_raw<WHOLE>(a.y + p * a.y_stride + c, nv);
+            const Raw<T> y = load_raw<WHOLE>(static_cast<const T*>(a.y) + p * a.y_stride + c, nv);
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[e] = fmaf(w, raw_get(y, e), acc[e]);
         }
@@ -50,7 +50,38 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
     }
 }
 
-// dy and dw; either may be absent
+// dy alone
+template <bool WHOLE>
+__global__ __launch_bounds__(256) void spread_kernel(CombineArgs a)
+{
+    const int64_t chunks = (a.cols + 7) / 8;
+    if ((int64_t)blockIdx.x >= a.tokens) {
+        for (int64_t r = max(0, *a.used) + (blockIdx.x - a.tokens); r < a.rows; r += kTailBlocks)
+            for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048)
+                store_raw<WHOLE>(a.dy + r * a.cols + c, Raw<bf16>{}, (int)min((int64_t)8, a.cols - c));
+        return;
+    }
+    const int64_t t = blockIdx.x;
+    // (choices one after the other in a thread's chunks: a short row's threads are all at work)
+    for (int64_t i = threadIdx.x; i < chunks * a.top_k; i += 256) {
+        const int64_t j = i / chunks, c = (i - j * chunks) * 8;
+        const int p = a.place[t * a.top_k + j];
+        if (p < 0 || p >= a.rows) continue;
+        const int nv = (int)min((int64_t)8, a.cols - c);
+        const Raw<bf16> g = load_raw<WHOLE>(a.g + t * a.g_stride + c, nv);
+        if (a.weights == nullptr) {
+            store_raw<WHOLE>(a.dy + p * a.cols + c, g, nv);
+            continue;
+        }
+        const float w = a.weights[t * a.top_k + j];
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = w * raw_get(g, e);
+        store_raw<WHOLE>(a.dy + p * a.cols + c, to_raw<bf16>(o), nv);
+    }
+}
+
+// dw, and dy where it is asked for
 template <bool WHOLE>
 __global__ __launch_bounds__(256) void combine_backward_kernel(CombineArgs a)
 {
@@ -79,18 +110,13 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(CombineArgs a)
                     for (int e = 0; e < 8; e++) o[e] = w * raw_get(g, e);
                     store_raw<WHOLE>(a.dy + p * a.cols + c, to_raw<bf16>(o), nv);
                 }
-                if (a.dw) {
-                    const Raw<bf16> y = load_raw<WHOLE>(a.y + p * a.y_stride + c, nv);
+                const Raw<bf16> y = load_raw<WHOLE>(static_cast<const bf16*>(a.y) + p * a.y_stride + c, nv);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) dot = fmaf(raw_get(g, e), raw_get(y, e), dot);
-                }
+                for (int e = 0; e < 8; e++) dot = fmaf(raw_get(g, e), raw_get(y, e), dot);
             }
-        if (a.dw) {
-            dot = wave_sum_f32(dot);
-            if (lane == 0) s_dot[wave][j] = dot;
-        }
+        dot = wave_sum_f32(dot);
+        if (lane == 0) s_dot[wave][j] = dot;
     }
-    if (a.dw == nullptr) return;
     __syncthreads();
     if ((int)threadIdx.x < a.top_k)
         a.dw[t * a.top_k + threadIdx.x] = (s_dot[0][threadIdx.x] + s_dot[1][threadIdx.x]) + (s_dot[2][threadIdx.x] + s_dot[3][threadIdx.x]);
@@ -155,7 +181,7 @@ static int combine_check(const char* what, int64_t tokens, int top_k, int64_t ro
 
 using namespace bs;
 
-extern "C" int bs_expert_combine(const void* y, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
+extern "C" int bs_expert_combine(const void* y, int y_type, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
                                  int64_t rows, int64_t cols, void* out, void* stream)
 {
     clear_error();
@@ -163,14 +189,17 @@ extern "C" int bs_expert_combine(const void* y, int64_t y_stride, const float* w
     if (const int rc = combine_check(what, tokens, top_k, rows, cols); rc != BS_OK) return rc;
     if (tokens == 0 || cols == 0) return BS_OK;
     if ((rows && y == nullptr) || place == nullptr || out == nullptr) return set_error(BS_ERR_INVALID, "%s: null pointer", what);
+    if (y_type != BS_DT_BF16 && y_type != BS_DT_F32) return set_error(BS_ERR_INVALID, "%s: y dtype %d must be bf16 or fp32", what, y_type);
     if (y_stride < 0) return set_error(BS_ERR_INVALID, "%s: negative row stride", what);
-    if ((((uintptr_t)y | (uintptr_t)out) & 1u) || (((uintptr_t)weights | (uintptr_t)place) & 3u))
+    if (((uintptr_t)y & (y_type == BS_DT_F32 ? 3u : 1u)) || ((uintptr_t)out & 1u) || (((uintptr_t)weights | (uintptr_t)place) & 3u))
         return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
     CombineArgs a{};
-    a.tokens = tokens, a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = static_cast<const bf16*>(y), a.y_stride = y_stride;
+    a.tokens = tokens, a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride;
     a.weights = weights, a.place = place, a.out = static_cast<bf16*>(out);
     const dim3 grid((uint32_t)tokens, (uint32_t)std::min<int64_t>((cols + 2047) / 2048, 65535));
-    auto* kernel = cols % 8 == 0 ? combine_kernel<true> : combine_kernel<false>;
+    const bool whole = cols % 8 == 0;
+    auto* kernel = y_type == BS_DT_F32 ? (whole ? combine_kernel<float, true> : combine_kernel<float, false>)
+                                       : (whole ? combine_kernel<bf16, true> : combine_kernel<bf16, false>);
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
@@ -190,10 +219,11 @@ extern "C" int bs_expert_combine_backward(const void* g, int64_t g_stride, const
     if ((((uintptr_t)g | (uintptr_t)y | (uintptr_t)dy) & 1u) || (((uintptr_t)weights | (uintptr_t)place | (uintptr_t)used | (uintptr_t)dw) & 3u))
         return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
     CombineArgs a{};
-    a.tokens = tokens, a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = static_cast<const bf16*>(y), a.y_stride = y_stride;
+    a.tokens = tokens, a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride;
     a.weights = weights, a.place = place, a.used = used, a.g = static_cast<const bf16*>(g), a.g_stride = g_stride;
     a.dy = static_cast<bf16*>(dy), a.dw = dw;
-    auto* kernel = cols % 8 == 0 ? combine_backward_kernel<true> : combine_backward_kernel<false>;
+    auto* kernel = dw ? (cols % 8 == 0 ? combine_backward_kernel<true> : combine_backward_kernel<false>)
+                      : (cols % 8 == 0 ? spread_kernel<true> : spread_kernel<false>);
     hipLaunchKernelGGL(kernel, dim3((uint32_t)(tokens + (dy ? kTailBlocks : 0))), dim3(256), 0, (hipStream_t)stream, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));

@@ -288,12 +288,13 @@ void check_weights(const Tensor& W, const Plan& plan, const char* what)
                       " experts, out, in], got ", W.sizes());
 }
 
-// A gathered operand.  One of 4 GiB or more is past the loads' offsets: its rows are written out first.
+// A gathered operand.  `written`, and one of 4 GiB or more, which is past the
+// loads' offsets: its rows are written out in the plan's order.
 struct Gathered {
     Rows16 rows;
     bool gather;
-    Gathered(const Tensor& x, const Plan& plan, bool gather_)
-        : rows(gather_ && too_far(x) ? written_out(x, plan) : x), gather(gather_ && !too_far(x))
+    Gathered(const Tensor& x, const Plan& plan, bool gather_, bool written)
+        : rows(gather_ && (written || too_far(x)) ? written_out(x, plan) : x), gather(gather_ && !written && !too_far(x))
     {
     }
     static bool too_far(const Tensor& x)
@@ -319,7 +320,7 @@ Tensor expert_product(const Tensor& x, const Tensor& W, const Plan& plan, bool g
     TORCH_CHECK_VALUE(W.size(2) == rows.size(1), "W: expected ", rows.size(1), " columns, as x has, got ", W.sizes());
     Tensor y = at::empty({plan.rows, W.size(1)}, x.options());
     if (plan.rows == 0) return y;
-    const Gathered a(rows, plan, gather);
+    const Gathered a(rows, plan, gather, false);
     const Rows16 w = expert_weights(W);
     const bs_experts e = plan.args(a.gather);
     check(L.bs_expert_linear(&e, raw(a.rows.t), a.rows.stride, raw(w.t), w.stride, W.size(2), W.size(1), (int)act, (float)act_k, raw(y), stream_of(y)),
@@ -327,34 +328,35 @@ Tensor expert_product(const Tensor& x, const Tensor& W, const Plan& plan, bool g
     return y;
 }
 // in the plan's order
-Tensor expert_product_dx(const Tensor& dy, const Tensor& W, const Plan& plan)
+Tensor expert_product_dx(const Tensor& dy, const Tensor& W, const Plan& plan, at::ScalarType type)
 {
     const c10::DeviceGuard guard(plan.offsets.device());
-    Tensor dx = at::empty({plan.rows, W.size(2)}, dy.options());
+    Tensor dx = at::empty({plan.rows, W.size(2)}, dy.options().dtype(type));
     if (plan.rows == 0) return dx;
     const Rows16 g(dy), w = expert_weights(W);
     const bs_experts e = plan.args(false);
-    check(L.bs_expert_linear_dx(&e, raw(g.t), g.stride, raw(w.t), w.stride, W.size(2), W.size(1), raw(dx), stream_of(dx)), "bs_expert_linear_dx");
+    check(L.bs_expert_linear_dx(&e, raw(g.t), g.stride, raw(w.t), w.stride, W.size(2), W.size(1), raw(dx), type == at::kFloat ? BS_DT_F32 : BS_DT_BF16,
+                                stream_of(dx)),
+          "bs_expert_linear_dx");
     return dx;
 }
-Tensor expert_product_dw(const Tensor& dy, const Tensor& x, const Plan& plan, bool dy_gathered, bool x_gathered)
+Tensor expert_product_dw(const Tensor& dy, const Tensor& x, const Plan& plan, bool x_gathered)
 {
     const c10::DeviceGuard guard(plan.offsets.device());
     Tensor dW = at::empty({plan.experts, dy.size(1), x.size(1)}, x.options());
     const Rows16 g(dy);
-    (void)dy_gathered;
-    const Gathered b(x, plan, x_gathered && plan.rows);
-    const bs_experts e = plan.args(b.gather);
+    const Gathered b(x, plan, x_gathered && plan.rows, true);
+    const bs_experts e = plan.args(false);
     check(L.bs_expert_linear_dw(&e, raw(g.t), g.stride, raw(b.rows.t), b.rows.stride, x.size(1), dy.size(1), raw(dW), stream_of(dW)), "bs_expert_linear_dw");
     return dW;
 }
-// sums over the choices of each token
+// sums over the choices of each token, in bf16
 Tensor combined(const Tensor& y, const Tensor& weights, const Plan& plan)
 {
     const c10::DeviceGuard guard(plan.offsets.device());
-    Tensor out = at::empty(plan.token_shape(y.size(1)), y.options());
+    Tensor out = at::empty(plan.token_shape(y.size(1)), y.options().dtype(at::kBFloat16));
     if (out.numel() == 0) return out;
-    check(L.bs_expert_combine(raw(y), row_stride(y), ptr<float>(weights), ptr<int32_t>(plan.place), plan.tokens, plan.top_k, plan.rows, y.size(1),
+    check(L.bs_expert_combine(raw(y), y.scalar_type() == at::kFloat ? BS_DT_F32 : BS_DT_BF16, row_stride(y), ptr<float>(weights), ptr<int32_t>(plan.place), plan.tokens, plan.top_k, plan.rows, y.size(1),
                               raw(out), stream_of(out)),
           "bs_expert_combine");
     return out;
@@ -413,12 +415,13 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
         const Tensor g = as_rows(grads[0], node.shape[1][1]);
         if (ctx->needs_input_grad(0) && node.need[0]) {
             as_saved(saved[1], node.shape[1], at::kBFloat16, device, "W");
-            const Tensor dx = expert_product_dx(g, saved[1], plan);
+            // (a gathered token's rows are rounded once, in their sum)
+            const Tensor dx = expert_product_dx(g, saved[1], plan, node.gather && plan.top_k > 1 ? at::kFloat : at::kBFloat16);
             out[0] = (node.gather ? combined(dx, Tensor(), plan) : dx).view(node.shape[0]);
         }
         if (ctx->needs_input_grad(1) && node.need[1]) {
             as_saved(saved[0], node.shape[0], at::kBFloat16, device, "x");
-            out[1] = expert_product_dw(g, as_rows(saved[0], node.shape[0].back()), plan, false, node.gather);
+            out[1] = expert_product_dw(g, as_rows(saved[0], node.shape[0].back()), plan, node.gather);
         }
         return out;
     }

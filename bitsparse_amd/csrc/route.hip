@@ -371,8 +371,9 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a)
 // One block does it all by itself; of more, each writes its counts and a
 // second kernel adds those of the blocks before it.
 // ---------------------------------------------------------------------------
-constexpr int kPlanBlock = 8192;        // pairs of a block where there are several
-constexpr int kPlanBlocks = 256;        // most blocks
+constexpr int kPlanBlock = 1024;        // pairs of a block, at least, where there are several
+constexpr int kPlanBlocks = 64;         // most blocks
+constexpr int kPlanAhead = 4;           // loads of a wave at a time
 
 struct PlanArgs {
     const int32_t* chosen;
@@ -407,12 +408,25 @@ __global__ __launch_bounds__(1024) void expert_plan_kernel(PlanArgs a)
     __syncthreads();
     const int64_t from = ((int64_t)blockIdx.x * 16 + wave) * a.run, to = min(a.pairs, from + a.run);
     int* const mine = s_count + wave * E;
-    for (int64_t i = from; i < to; i += 64) {
-        const uint32_t id = i + lane < to ? (uint32_t)a.chosen[i + lane] : ~0u;
-        const uint32_t e = min(id, (uint32_t)E);        // (all that are none of the experts' at one)
+    // f(pair, its expert, or E for all that are none of the experts')
+    auto each = [&](auto f) {
+        for (int64_t i0 = from; i0 < to; i0 += 64 * kPlanAhead) {
+            uint32_t e[kPlanAhead];
+#pragma unroll
+            for (int u = 0; u < kPlanAhead; u++) {
+                const int64_t i = i0 + 64 * u + lane;
+                e[u] = i < to ? (uint32_t)a.chosen[i] : ~0u;
+            }
+#pragma unroll
+            for (int u = 0; u < kPlanAhead; u++)
+                if (i0 + 64 * u < to) f(i0 + 64 * u + lane, min(e[u], (uint32_t)E));
+        }
+    };
+    each([&](int64_t, uint32_t e) {
         const uint64_t same = same_expert(e, a.bits);
         if (e < (uint32_t)E && popc_below(same) == 0) mine[e] += __popcll(same);
-    }
+        wave_fence();
+    });
     __syncthreads();
     // each wave's counts become the rows of the waves before it
     for (int e = tid; e < E; e += 1024) {
@@ -431,17 +445,28 @@ __global__ __launch_bounds__(1024) void expert_plan_kernel(PlanArgs a)
     __syncthreads();
     // the experts' first rows
     int all = 0, before = 0;            // of expert `tid`, in all blocks and in those before this one
-    if (tid < E) {
-        if (a.blocks > 1) {
+    if (a.blocks > 1) {
+        // (as many threads to an expert as there are; sums of whole numbers, in any order)
+        int* const s_all = s_mem + 17 * E;
+        for (int i = tid; i < E; i += 1024) s_total[i] = s_all[i] = 0;
+        __syncthreads();
+        const int parts = min(1024 / E, a.blocks), part = tid / E, e = tid - part * E;
+        if (part < parts) {
+            int n_all = 0, n_before = 0;
 #pragma unroll 8
-            for (int b = 0; b < a.blocks; b++) {
-                const int n = a.counts[(int64_t)b * E + tid];
-                all += n;
-                before += b < (int)blockIdx.x ? n : 0;
+            for (int b = part; b < a.blocks; b += parts) {
+                const int n = a.counts[(int64_t)b * E + e];
+                n_all += n;
+                n_before += b < (int)blockIdx.x ? n : 0;
             }
-        } else {
-            all = s_total[tid];
+            atomicAdd(&s_all[e], n_all);
+            atomicAdd(&s_total[e], n_before);
         }
+        __syncthreads();
+        if (tid < E) all = s_all[tid], before = s_total[tid];
+        __syncthreads();
+    } else if (tid < E) {
+        all = s_total[tid];
     }
     int sum = all;
 #pragma unroll
@@ -464,10 +489,7 @@ __global__ __launch_bounds__(1024) void expert_plan_kernel(PlanArgs a)
     if (blockIdx.x == 0 && tid == 0) a.offsets[E] = used;
     for (int64_t r = used + (int64_t)blockIdx.x * 1024 + tid; r < a.pairs; r += (int64_t)a.blocks * 1024) a.order[r] = -1;
     __syncthreads();
-    for (int64_t i = from; i < to; i += 64) {
-        const bool there = i + lane < to;
-        const uint32_t id = there ? (uint32_t)a.chosen[i + lane] : ~0u;
-        const uint32_t e = min(id, (uint32_t)E);
+    each([&](int64_t i, uint32_t e) {
         const uint64_t same = same_expert(e, a.bits);
         int r = -1;
         if (e < (uint32_t)E) {
@@ -475,11 +497,11 @@ __global__ __launch_bounds__(1024) void expert_plan_kernel(PlanArgs a)
             r = s_total[e] + mine[e] + rank;
             wave_fence();
             if (rank == 0) mine[e] += __popcll(same);
-            a.order[r] = (int)(i + lane);
+            a.order[r] = (int)i;
         }
         wave_fence();
-        if (there) a.place[i + lane] = r;
-    }
+        if (i < to) a.place[i] = r;
+    });
 }
 
 static int route_check(const bs_route* r, const char* what)
@@ -555,7 +577,7 @@ extern "C" int bs_route_backward(const bs_route* route, const int32_t* chosen, c
 
 static int64_t plan_blocks(int64_t pairs)
 {
-    return pairs <= 2 * kPlanBlock ? 1 : std::min<int64_t>((pairs + kPlanBlock - 1) / kPlanBlock, kPlanBlocks);
+    return pairs <= 4 * kPlanBlock ? 1 : std::min<int64_t>((pairs + kPlanBlock - 1) / kPlanBlock, kPlanBlocks);
 }
 
 extern "C" int64_t bs_expert_plan_workspace_bytes(int64_t pairs, int experts)
@@ -582,7 +604,7 @@ extern "C" int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts,
     int bits = 0;
     while (experts >> bits) bits++;         // (ids up to and with `experts`)
     const PlanArgs a{chosen, pairs, run, experts, bits, (int)blocks, offsets, order, place, static_cast<int32_t*>(workspace)};
-    const uint32_t lds = 17u * experts * 4;
+    const uint32_t lds = 18u * experts * 4;
     const hipStream_t st = (hipStream_t)stream;
     if (blocks > 1) hipLaunchKernelGGL(expert_plan_kernel<true>, dim3((uint32_t)blocks), dim3(1024), lds, st, a);
     hipLaunchKernelGGL(expert_plan_kernel<false>, dim3((uint32_t)blocks), dim3(1024), lds, st, a);

@@ -68,8 +68,7 @@ def expert_linear(x: Tensor, W: Tensor, plan: ExpertPlan, *, gather: bool = Fals
     x: [rows, d_in], or with ``gather`` the tokens [..., d_in], each read where
     its rows need it; W: [E, d_out, d_in]; both bfloat16.  Rows behind the last
     expert's are 0, and the gradients of x (as x is given) and W take nothing
-    from them.  Sums in 32 bits, each result rounded once (the gradient of
-    gathered tokens: each row's, and their sum).  Differentiable once in x and W."""
+    from them.  Sums in 32 bits, each result rounded once.  Differentiable once in x and W."""
     return native().expert_linear(x, W, *plan, gather)
 
 

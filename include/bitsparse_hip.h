@@ -780,10 +780,12 @@ int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts, int32_t* o
  * Products of the experts' rows with their bf16 weights [experts, out, in]
  * (w_stride elements from row to row), fp32 sums rounded once:
  *   y[r] = act(x[src r] W[e]^T), dx[r] = dy[r] W[e], dW[e] = sum dy[r]^T x[src r]
- * src r = order[r] / top_k, a row of the `tokens` of x, or (order NULL) r.
+ * src r = order[r] / top_k, a row of the `tokens` of x, or (order NULL) r; dx
+ * and dW are of rows in the experts' order and take no order.
  * Rows that belong to no expert, or whose order is out of range, come out as
  * 0 (as act(0)); an expert without rows gets dW = 0.  Offsets out of range are
- * taken as the nearest in it.  Results are contiguous.  Operands have rows at
+ * taken as the nearest in it.  Results are contiguous; dx is bf16 or, for the
+ * sum over a token's rows that follows where they were gathered, fp32 (dx_type).  Operands have rows at
  * 16-byte addresses, a multiple of 8 elements apart, and zeros from their
  * last column to the next multiple of 8 (bs_pad_rows makes such rows).
  * BS_ACT_RELU2: bf16(bf16(r r) act_k) of r = bf16(relu(.)), as the ReLU^2
@@ -796,25 +798,25 @@ typedef struct bs_experts {
     int64_t rows, tokens;
     int experts, top_k;
     const int32_t* offsets;          /* [experts + 1] */
-    const int32_t* order;            /* [rows], or NULL: operands are rows themselves */
+    const int32_t* order;            /* [rows], or NULL: x is rows itself */
 } bs_experts;
 int bs_expert_linear(const bs_experts* experts, const void* x, int64_t x_stride, const void* W, int64_t w_stride, int64_t in,
                      int64_t out, int act, float act_k, void* y, void* stream);
 int bs_expert_linear_dx(const bs_experts* experts, const void* dy, int64_t dy_stride, const void* W, int64_t w_stride, int64_t in,
-                        int64_t out, void* dx, void* stream);
+                        int64_t out, void* dx, int dx_type, void* stream);
 int bs_expert_linear_dw(const bs_experts* experts, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int64_t in,
                         int64_t out, void* dW, void* stream);
 /* bf16 rows of `cols` copied into rows of `width`, a multiple of 8, with zeros behind. */
 int bs_pad_rows(const void* x, int64_t rows, int64_t cols, int64_t stride, void* out, int64_t width, void* stream);
 
 /*
- * out[t] = sum over j of weights[t, j] y[place[t, j]] in the order of j (bf16,
- * fp32 sums; weights NULL: 1); a place outside 0..rows-1 adds nothing.
+ * out[t] = sum over j of weights[t, j] y[place[t, j]] in the order of j (bf16;
+ * y bf16 or fp32; fp32 sums; weights NULL: 1); a place outside 0..rows-1 adds nothing.
  * Backward: dy[place[t, j]] = weights[t, j] g[t], 0 in the rows from *used
  * (a device address: offsets[experts]) on; dweights[t, j] = <g[t],
  * y[place[t, j]]>.  dy or dweights may be NULL.
  */
-int bs_expert_combine(const void* y, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
+int bs_expert_combine(const void* y, int y_type, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
                       int64_t rows, int64_t cols, void* out, void* stream);
 int bs_expert_combine_backward(const void* g, int64_t g_stride, const void* y, int64_t y_stride, const float* weights,
                                const int32_t* place, const int32_t* used, int64_t tokens, int top_k, int64_t rows, int64_t cols,
