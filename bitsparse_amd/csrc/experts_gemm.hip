@@ -40,6 +40,7 @@ struct ExpertGemm {
     int tiles_m, tiles_n, panel;
     int act;
     float act_k;
+    int stream;                                 // results past the caches' size, stored around them
 };
 
 // ---------------------------------------------------------------------------
@@ -89,6 +90,13 @@ __device__ __forceinline__ void barrier_only()
 {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+}
+
+// LDS written by some lanes of a wave and read by others of it, or the other way round
+__device__ __forceinline__ void wave_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // A tile's expert: the tile'th tile of `size` rows in the order of the experts, or behind the last expert's
@@ -232,7 +240,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
         k = (wave * loads + i) * (512 / T) + lane / (T / 8);
         unit = (lane % (T / 8)) ^ col_turn<T>(k);
     };
-    i32x4 ra, rb;
+    i32x4 ra = {}, rb = {};
     if constexpr (A_ALONG) {
         const bf16* base = GATHER ? g.a : g.a + c_row * g.a_stride;
         ra = rsrc_words(base, GATHER ? ((g.tokens - 1) * g.a_stride + g.k + 7) / 8 * 16 : (int64_t)kNoRow);
@@ -251,42 +259,54 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
             b_off[i] = r < g.n ? (uint32_t)(r * b_row_bytes) + chunk * 16 : kNoRow;
         }
     }
+    if constexpr (!A_ALONG) {
+#pragma unroll
+        for (int i = 0; i < LA; i++) {
+            int k, unit;
+            along_m(i, LA, IC<TM>{}, k, unit);
+            a_off[i] = (uint32_t)(k * a_row_bytes) + (uint32_t)(c_row * 2) + unit * 16;
+        }
+    }
+    if constexpr (!B_ALONG) {
+#pragma unroll
+        for (int i = 0; i < LB; i++) {
+            int k, unit;
+            along_m(i, LB, IC<TN>{}, k, unit);
+            b_off[i] = (uint32_t)(k * b_row_bytes) + (uint32_t)(c_col * 2) + unit * 16;
+        }
+    }
     const int steps = (int)((k_total + kBK - 1) / kBK);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem;
-    auto load_a = [&](int step, int stage) {
-        const uint32_t lds = lds0 + stage * STAGE + wave * LA * 1024;
-        if constexpr (A_ALONG) {
-            const bool in_k = chunk * 8 + step * kBK < g.k;
-#pragma unroll
-            for (int i = 0; i < LA; i++) load_lds16(ra, lds + i * 1024, in_k ? a_off[i] : kNoRow, (uint32_t)step * kRowBytes);
+    // the q-th of this wave's loads of a step: first those of A
+    constexpr int LOADS = LA + LB;
+    i32x4 step_a = ra, step_b = rb;
+    auto load_one = [&](int q, int step, int stage) {
+        const uint32_t lds = lds0 + stage * STAGE;
+        if (q < LA) {
+            const uint32_t to = lds + (wave * LA + q) * 1024;
+            if constexpr (A_ALONG) {
+                load_lds16(ra, to, chunk * 8 + step * kBK < g.k ? a_off[q] : kNoRow, (uint32_t)step * kRowBytes);
+            } else {
+                // (the rows that are left bound the operand: those behind them are zeros)
+                const int64_t at = grp.first + (int64_t)step * kBK, left = grp.end - at;
+                if (q == 0) step_a = rsrc_words(g.a + at * g.a_stride, (left - 1) * a_row_bytes + (g.m + 7) / 8 * 16);
+                load_lds16(step_a, to, a_off[q], 0);
+            }
         } else {
-            // (the rows that are left bound the operand: those behind them are zeros)
-            const int64_t at = grp.first + (int64_t)step * kBK, left = grp.end - at;
-            const i32x4 r = rsrc_words(g.a + at * g.a_stride, (left - 1) * a_row_bytes + (g.m + 7) / 8 * 16);
-#pragma unroll
-            for (int i = 0; i < LA; i++) {
-                int k, unit;
-                along_m(i, LA, IC<TM>{}, k, unit);
-                load_lds16(r, lds + i * 1024, (uint32_t)(k * a_row_bytes) + (uint32_t)(c_row * 2) + unit * 16, 0);
+            const int i = q - LA;
+            const uint32_t to = lds + A_BYTES + (wave * LB + i) * 1024;
+            if constexpr (B_ALONG) {
+                load_lds16(rb, to, chunk * 8 + step * kBK < g.k ? b_off[i] : kNoRow, (uint32_t)step * kRowBytes);
+            } else {
+                const int64_t at = (KIND == kDw ? grp.first : 0) + (int64_t)step * kBK, end = KIND == kDw ? grp.end : g.k;
+                if (i == 0) step_b = rsrc_words(b_base + at * g.b_stride, (end - at - 1) * b_row_bytes + (g.n + 7) / 8 * 16);
+                load_lds16(step_b, to, b_off[i], 0);
             }
         }
     };
-    auto load_b = [&](int step, int stage) {
-        const uint32_t lds = lds0 + stage * STAGE + A_BYTES + wave * LB * 1024;
-        if constexpr (B_ALONG) {
-            const bool in_k = chunk * 8 + step * kBK < g.k;
+    auto load_all = [&](int step, int stage) {
 #pragma unroll
-            for (int i = 0; i < LB; i++) load_lds16(rb, lds + i * 1024, in_k ? b_off[i] : kNoRow, (uint32_t)step * kRowBytes);
-        } else {
-            const int64_t at = (KIND == kDw ? grp.first : 0) + (int64_t)step * kBK, end = KIND == kDw ? grp.end : g.k;
-            const i32x4 r = rsrc_words(b_base + at * g.b_stride, (end - at - 1) * b_row_bytes + (g.n + 7) / 8 * 16);
-#pragma unroll
-            for (int i = 0; i < LB; i++) {
-                int k, unit;
-                along_m(i, LB, IC<TN>{}, k, unit);
-                load_lds16(r, lds + i * 1024, (uint32_t)(k * b_row_bytes) + (uint32_t)(c_col * 2) + unit * 16, 0);
-            }
-        }
+        for (int q = 0; q < LOADS; q++) load_one(q, step, stage);
     };
 
     // A step is two halves of 32 of K.  A fragment of A is read again, for the next half, as soon as its last product is
@@ -307,10 +327,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
     if constexpr (!AHEAD) {
 #pragma unroll
         for (int i = 0; i < STAGES - 1; i++)
-            if (i < steps) {
-                load_a(i, i);
-                load_b(i, i);
-            }
+            if (i < steps) load_all(i, i);
         for (int step = 0, stage = 0; step < steps; step++) {
             // this step's stage has come and the last one's has been read, in every wave
             if (step + STAGES - 2 < steps)
@@ -320,8 +337,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
             barrier_only();
             if (step + STAGES - 1 < steps) {
                 const int last = stage == 0 ? STAGES - 1 : stage - 1;
-                load_a(step + STAGES - 1, last);
-                load_b(step + STAGES - 1, last);
+                load_all(step + STAGES - 1, last);
             }
 #pragma unroll
             for (int k0 = 0; k0 < kBK; k0 += 32) {
@@ -338,11 +354,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
         }
     }
     if (AHEAD && steps) {
-        load_a(0, 0);
-        load_b(0, 0);
+        load_all(0, 0);
         if (steps > 1) {
-            load_a(1, 1);
-            load_b(1, 1);
+            load_all(1, 1);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LA + LB) : "memory");
         } else {
             wait_for_loads();
@@ -363,6 +377,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
             for (int j = 0; j < JN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[0][j], fa[i], acc[i][j], 0, 0, 0);
             read_a(stage, i, 32);
             __builtin_amdgcn_sched_barrier(0);
+            // (the last of the loads that began in the step before)
+            if (step > 0 && step + 1 < steps && IM - MEET + i < LOADS) load_one(IM - MEET + i, step + 1, stage ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
         }
         // (behind the last step the next stage holds what it held: read, not used)
 #pragma unroll
@@ -380,16 +397,58 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
 #pragma unroll
                 for (int o = 0; o < MEET; o++) read_a(stage ^ 1, o, 0);
             __builtin_amdgcn_sched_barrier(0);
-            if (step + 2 < steps) {
-                if (i == MEET) load_a(step + 2, stage);
-                if (i == MEET + 1) load_b(step + 2, stage);
-            }
+            // (a load at a time: more at once hold up the products behind them)
+            if (step + 2 < steps && i >= MEET && i - MEET < LOADS) load_one(i - MEET, step + 2, stage);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
 
     // a lane has row lane % 16 and columns 4 (lane / 16) on of each block
-    const int64_t c0 = KIND == kDw ? grp.expert * g.c_expert : 0;
+    const int64_t c0 = KIND == kDw ? (int64_t)grp.expert * g.c_expert : 0;
+    // Out as whole rows of the wave's columns through LDS, 16 rows at a time: stored from the lanes that hold them, 8 bytes
+    // of 16 rows each, the results take a seventh of 16384 x 768 -> 2048's time (82 us instead of 72).
+    auto store_rows = [&](auto wide) {
+        constexpr int SIZE = decltype(wide)::value;                                     // bytes of a result
+        constexpr int ROW = 16 * JN * SIZE, CHUNKS = ROW / 16, ROWS = 64 / CHUNKS;      // of a row; rows of a store
+        static_assert(WAVES * 16 * ROW <= STAGES * STAGE, "LDS budget");
+        char* const out = s_mem + wave * (16 * ROW);
+        if (steps) {
+            wait_for_loads();
+            barrier_only();     // (the stages have been read)
+        }
+#pragma unroll
+        for (int i = 0; i < IM; i++) {
+            const int r = lane & 15;
+            auto at_chunk = [&](int row, int c) { return out + row * ROW + ((c ^ (row & (CHUNKS - 1))) * 16); };
+#pragma unroll
+            for (int j = 0; j < JN; j++) {
+                if constexpr (SIZE == 4) {
+                    *reinterpret_cast<f32x4*>(at_chunk(r, 4 * j + (lane >> 4))) = acc[i][j];
+                } else {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[e] = f32_to_bf16(KIND == kForward ? activated(acc[i][j][e], g.act, g.act_k) : acc[i][j][e]);
+                    *reinterpret_cast<uint2*>(at_chunk(r, 2 * j + (lane >> 5)) + (lane >> 4 & 1) * 8) = uint2{o[0] | o[1] << 16, o[2] | o[3] << 16};
+                }
+            }
+            wave_order();
+#pragma unroll
+            for (int u = 0; u < 16 / ROWS; u++) {
+                const int row = u * ROWS + lane / CHUNKS, c = lane % CHUNKS;
+                const uint4 v = *reinterpret_cast<const uint4*>(at_chunk(row, c));
+                const int64_t at = c_row + (wm * IM + i) * 16 + row, col = c_col + wn * 16 * JN + c * (16 / SIZE);
+                if (at >= c_rows || col >= g.n) continue;
+                char* const to = static_cast<char*>(g.c) + (c0 + at * g.n + col) * SIZE;
+                if (g.stream)
+                    st16<true>(to, v);
+                else
+                    st16<false>(to, v);
+            }
+            wave_order();
+        }
+    };
+    if (KIND == kDx && g.c_f32 && g.n % 4 == 0) return store_rows(IC<4>{});
+    if (!(KIND == kDx && g.c_f32) && g.n % 8 == 0) return store_rows(IC<2>{});
 #pragma unroll
     for (int i = 0; i < IM; i++) {
         const int64_t r = c_row + (wm * IM + i) * 16 + (lane & 15);
@@ -474,6 +533,8 @@ static int launch_gemm(ExpertGemm g, const char* what, hipStream_t st)
     // (parts of tiles: one at most for each expert that has rows, and one of the rows behind them)
     const int64_t tiles_m = KIND == kDw ? (int64_t)g.experts * g.tiles_m : g.rows / TM + std::min<int64_t>(g.experts + 1, g.rows);
     g.panel = 8;
+    // (32768 rows of 16 experts 2048 -> 4096 510 us without, 489 with; dW of 64 experts 1024 -> 2048 147 and 110)
+    g.stream = use_nontemporal((KIND == kDw ? (int64_t)g.experts * g.m : g.rows) * g.n * (KIND == kDx && g.c_f32 ? 4 : 2));
     if (tiles_m * g.tiles_n >= (1ll << 31)) return set_error(BS_ERR_INVALID, "%s: too many tiles", what);
     hipLaunchKernelGGL((expert_gemm_kernel<KIND, GATHER, WGM, WGN, IM, JN, STAGES, AHEAD>), dim3((uint32_t)(tiles_m * g.tiles_n)), dim3(64 * WGM * WGN), 0, st, g);
     const hipError_t e = hipGetLastError();
@@ -509,18 +570,18 @@ static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_on
 // 20.9; 64 rows 50 and 65; 32 rows of 8 experts of 4096 -> 2048 24.3 and 22.0).  Else the tile whose time is least by
 // tile_time (measured in us, forward / dx / dW, x gathered in forward):
 //   rows, experts, in -> out           64 x 64       128 x 128     192 x 128   256 x 256
-//   16384,  8,  768 -> 2048         122 / 98 / 100   82 / 67 / 72   76 / 76 / -   87 / 62 / 80
-//   16384,  8, 2048 ->  768          94 / 109 / 95   67 / 73 / 70   74 / 67 / -   55 / 83 / 79
-//   32768, 16, 2048 -> 4096               -         619 / 571 / 591 571 / 533 / - 530 / 520 / 540
-//   16384,  4,  512 -> 1024          50 / 39 / 41    37 / 33 / 62   32 / 28 / -   44 / 34 / 133
-//     512,  8, 2048 -> 2048          21 / 22 / 46    27 / 25 / 28   32 / 29 / -   45 / 47 / 29
+//   16384,  8,  768 -> 2048         119 / 91 / 95    78 / 65 / 72   73 / 72 / -   72 / 55 / 74
+//   16384,  8, 2048 ->  768          92 / 102 / 93   68 / 66 / 68   73 / 59 / -   56 / 68 / 73
+//   32768, 16, 2048 -> 4096         976 / 929 / 996 621 / 570 / 572 559 / 532 / - 489 / 497 / 501
+//   16384,  4,  512 -> 1024          49 / 38 / 40    34 / 31 / 63   30 / 26 / -   36 / 27 / 116
+//     512,  8, 2048 -> 2048          22 / 22 / 41    27 / 24 / 21   31 / 30 / -   42 / 42 / 23
 template <int KIND, bool GATHER>
 static int launch_kind(const ExpertGemm& g, const char* what, hipStream_t st)
 {
     if constexpr (KIND == kForward)
         if (g.rows <= 2 * std::min<int64_t>(g.experts, g.rows)) return launch_few<GATHER>(g, what, st);
-    const double small = tile_time(g, KIND, 64, 64, kCus * 2, 0.45), middle = tile_time(g, KIND, 128, 128, kCus * 2, 0.98),
-                 wide = tile_time(g, KIND, 192, 128, kCus * 2, 1.33), large = tile_time(g, KIND, 256, 256, kCus, 1.7);
+    const double small = tile_time(g, KIND, 64, 64, kCus * 2, 0.45), middle = tile_time(g, KIND, 128, 128, kCus * 2, 0.95),
+                 wide = tile_time(g, KIND, 192, 128, kCus * 2, 1.3), large = tile_time(g, KIND, 256, 256, kCus, 1.55);
     const double best = std::min(std::min(small, middle), KIND == kDw ? large : std::min(wide, large));
     if (best == large) return launch_gemm<KIND, GATHER, 2, 4, 8, 4, 2, true>(g, what, st);
     if constexpr (KIND != kDw)
@@ -592,7 +653,7 @@ extern "C" int bs_expert_linear(const bs_experts* experts, const void* x, int64_
     const bool gather = experts->order != nullptr;
     if (const int rc = operand_check(what, "x", x, gather ? experts->tokens : experts->rows, x_stride, in, gather); rc != BS_OK) return rc;
     if (const int rc = operand_check(what, "W", W, out, w_stride, in, false); rc != BS_OK) return rc;
-    if (y == nullptr || ((uintptr_t)y & 7u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned y", what);
+    if (y == nullptr || ((uintptr_t)y & 15u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned y", what);
     ExpertGemm g = gemm_args(*experts, gather);
     g.a = static_cast<const bf16*>(x), g.a_stride = x_stride, g.b = static_cast<const bf16*>(W), g.b_stride = w_stride, g.b_expert = out * w_stride;
     g.c = y, g.m = -1, g.n = (int)out, g.k = (int)in, g.act = act, g.act_k = act_k;
@@ -626,7 +687,7 @@ extern "C" int bs_expert_linear_dw(const bs_experts* experts, const void* dy, in
     if (experts->order) return set_error(BS_ERR_INVALID, "%s: x is rows in the experts' order, so order must be null", what);
     if (const int rc = operand_check(what, "dy", dy, experts->rows, dy_stride, out, false); rc != BS_OK) return rc;
     if (const int rc = operand_check(what, "x", x, experts->rows, x_stride, in, false); rc != BS_OK) return rc;
-    if (dW == nullptr || ((uintptr_t)dW & 7u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned dW", what);
+    if (dW == nullptr || ((uintptr_t)dW & 15u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned dW", what);
     ExpertGemm g = gemm_args(*experts, false);
     g.a = static_cast<const bf16*>(dy), g.a_stride = dy_stride, g.b = static_cast<const bf16*>(x), g.b_stride = x_stride;
     g.c = dW, g.c_expert = in * out, g.m = (int)out, g.n = (int)in, g.k = -1;
