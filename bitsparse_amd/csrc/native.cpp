@@ -1197,6 +1197,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("plan_experts", &plan_experts);
     m.def("expert_linear", &expert_linear);
     m.def("expert_combine", &expert_combine);
+    m.def("expert_product", &expert_product_act);
+    m.def("experts_backward", &experts_backward);
     m.def("orthogonalize", &orthogonalize);
     m.def("muon_update", &muon_update, py::call_guard<py::gil_scoped_release>());
     m.def("quantize_t", [](const Tensor& x, bool rows) {

@@ -503,3 +503,52 @@ Tensor expert_combine(const Tensor& y, const Tensor& weights, const Tensor& offs
     const CombineCall c(y, weights, plan);
     return combined(c.y, c.w, plan);
 }
+
+// ---------------------------------------------------------------------------
+// a block of experts (experts.py's ExpertsRelu and ExpertsRelu2)
+// ---------------------------------------------------------------------------
+Tensor expert_product_act(const Tensor& x, const Tensor& W, const Tensor& offsets, const Tensor& order, const Tensor& place, bool gather,
+                          int64_t act, double act_k)
+{
+    return expert_product(x, W, Plan(offsets, order, place), gather, act, act_k);
+}
+
+// The gradients of out = sum of w act(x W1^T) W2^T over a token's choices, of
+// (x, W1, W2, weights) those that are wanted.  r: the saved relu(x W1^T)
+// [rows, H], overwritten.  The result y of the second product is not needed:
+// the weights' gradient is <dout W2, act>.
+std::vector<std::optional<Tensor>> experts_backward(const Tensor& grad, const Tensor& x, const Tensor& W1, const Tensor& W2, const Tensor& weights,
+                                                    const Tensor& offsets, const Tensor& order, const Tensor& place, const Tensor& r, bool square,
+                                                    double k, std::vector<bool> need)
+{
+    const Plan plan(offsets, order, place);
+    const c10::DeviceGuard guard(plan.offsets.device());
+    // (those that this walk through the graph asks for; the node's edges are its tensors in order)
+    if (const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node(); node && node->name() == "_ExpertsBlockBackward")
+        for (size_t i = 0; i < need.size(); i++) need[i] = need[i] && node->task_should_compute_output(i);
+    TORCH_CHECK_VALUE(need.size() == 4, "four gradients, each wanted or not");
+    const Tensor tokens = expert_operand(x, plan, true, "x");
+    check_weights(W1, plan, "W1");
+    check_weights(W2, plan, "W2");
+    const int64_t H = W1.size(1), O = W2.size(1);
+    const CombineCall w(r, weights, plan);
+    TORCH_CHECK_VALUE(W1.size(2) == tokens.size(1) && W2.size(2) == H && r.dim() == 2 && r.size(1) == H && r.is_contiguous(),
+                      "the operands are not those of the forward pass");
+    as_saved(grad, plan.token_shape(O), at::kBFloat16, plan.offsets.device(), "the gradient");
+    std::vector<std::optional<Tensor>> out(4);
+    const Tensor g_tokens = as_rows(grad, O);
+    Tensor dy = plan.rows ? Gathered::written_out(g_tokens, plan) : at::empty({0, O}, grad.options());      // before its weights
+    const Tensor dz = expert_product_dx(dy, W2, plan, at::kBFloat16);
+    Tensor dw;
+    if (need[3]) dw = at::zeros(weights.sizes(), weights.options());
+    if (plan.rows)
+        check(L.bs_experts_act_grad(raw(dz), raw(r), plan.rows, H, square, (float)k, ptr<float>(w.w), ptr<int32_t>(plan.order), plan.used(), plan.rows,
+                                    ptr<float>(dw), stream_of(dz)),
+              "bs_experts_act_grad");
+    if (need[3]) out[3] = dw;
+    if (need[2]) out[2] = expert_product_dw(dy, r, plan, false);
+    dy = Tensor();
+    if (need[0]) out[0] = combined(expert_product_dx(dz, W1, plan, plan.top_k > 1 ? at::kFloat : at::kBFloat16), Tensor(), plan).view(x.sizes());
+    if (need[1]) out[1] = expert_product_dw(dz, tokens, plan, true);
+    return out;
+}

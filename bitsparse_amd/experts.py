@@ -3,6 +3,10 @@ rows with its weights, and the weighted sum back to tokens.
 
     w, experts = route(x @ Wr.T, top_k)               # [T, k] each
     plan = plan_experts(experts, n_experts)           # rows by expert
+    out = ExpertsRelu2.apply(x, W1, W2, w, plan, sparse_data=buf)
+
+or, step by step,
+
     z = expert_linear(x, W1, plan, gather=True)       # [T k, d_ff], by expert
     y = expert_linear(act(z), W2, plan)               # [T k, d_out]
     out = expert_combine(y, w, plan)                  # [T, d_out]
@@ -16,8 +20,14 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd import Function
 
 from ._lib import native
+from .bitsparse import BitsparseTensor, TensorBuffer
+from .config import RELU2_SCALE
+from .src.functions import relu2_and_compress, relu2_fused_ok, relu_and_compress
+from .src.hip_operators import relu2_square_amax_
+from .src.sparse_matmul import decoded
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 
@@ -79,3 +89,73 @@ def expert_combine(y: Tensor, weights: Tensor, plan: ExpertPlan) -> Tensor:
     y: bfloat16 [rows, d_out]; weights: float32 [..., top_k].  Sums in 32 bits
     in the order of the choices.  Differentiable once in y and weights."""
     return native().expert_combine(y, weights, *plan)
+
+
+# ------------------------------------------------------------
+# blocks of experts whose activation is saved compressed
+# ------------------------------------------------------------
+class ExpertsRelu:
+    """FFNRelu as experts: the weighted sum over a token's experts of
+    relu(x @ W1[e].T) @ W2[e].T."""
+
+    @staticmethod
+    def apply(x: Tensor, W1: Tensor, W2: Tensor, weights: Tensor, plan: ExpertPlan, *,
+              sparse_data: TensorBuffer | None = None, pack_sbit: bool = False) -> Tensor:
+        """x [..., d_in], W1 [E, d_ff, d_in], W2 [E, d_out, d_ff], all bfloat16; weights float32 [..., top_k] and the plan as
+        ``route`` and ``plan_experts`` give them -> [..., d_out].
+
+        The activation of all rows [tokens * top_k, d_ff] is saved compressed, as the dense blocks save theirs (``sparse_data``,
+        ``pack_sbit``); the second product's result is not saved at all.  Without a gradient to come nothing is, and the
+        activation is part of the first product.  Differentiable once in x, W1, W2 and weights."""
+        return _experts(x, W1, W2, weights, plan, sparse_data, pack_sbit, False)
+
+
+class ExpertsRelu2:
+    """FFNRelu2 as experts: the weighted sum over a token's experts of
+    k * relu(x @ W1[e].T)^2 @ W2[e].T.  Arguments as ``ExpertsRelu``'s."""
+
+    @staticmethod
+    def apply(x: Tensor, W1: Tensor, W2: Tensor, weights: Tensor, plan: ExpertPlan, *,
+              sparse_data: TensorBuffer | None = None, pack_sbit: bool = False) -> Tensor:
+        return _experts(x, W1, W2, weights, plan, sparse_data, pack_sbit, True)
+
+
+def _experts(x, W1, W2, weights, plan, sparse_data, pack_sbit, square) -> Tensor:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, W1, W2, weights)):
+        return _ExpertsBlock.apply(x, W1, W2, weights, *plan, sparse_data, pack_sbit, square)
+    h = native().expert_product(x, W1, *plan, True, 2 if square else 1, float(RELU2_SCALE))
+    return native().expert_combine(native().expert_product(h, W2, *plan, False, 0, 0.0), weights, *plan)
+
+
+class _ExpertsBlock(Function):
+    @staticmethod
+    def forward(ctx, x, W1, W2, weights, offsets, order, place, sparse_data, pack_sbit, square):
+        plan = (offsets, order, place)
+        h, ctx.h_sparse = _activate(native().expert_product(x, W1, *plan, True, 0, 0.0), sparse_data, pack_sbit, square)
+        ctx.square = square
+        ctx.save_for_backward(x, W1, W2, weights, *plan)
+        return native().expert_combine(native().expert_product(h, W2, *plan, False, 0, 0.0), weights, *plan)
+
+    @staticmethod
+    @torch.compiler.disable
+    def backward(ctx, grad_output: Tensor):
+        if torch.is_grad_enabled():
+            raise NotImplementedError("bitsparse_amd: a block of experts has no second derivative (create_graph)")
+        if ctx.h_sparse is None:
+            raise RuntimeError("a block of experts goes backward once: its compressed activation is freed with it")
+        h = ctx.h_sparse
+        r = decoded(h, False) if h.shape[0] else grad_output.new_empty(h.shape)
+        del h
+        ctx.h_sparse = None
+        grads = native().experts_backward(grad_output, *ctx.saved_tensors, r, ctx.square, float(RELU2_SCALE), ctx.needs_input_grad[:4])
+        return *grads, None, None, None, None, None, None
+
+
+def _activate(z: Tensor, sparse_data: TensorBuffer | None, pack_sbit: bool, square: bool) -> tuple[Tensor, BitsparseTensor]:
+    """(the activation of z, which it overwrites; relu(z) compressed)"""
+    if square and relu2_fused_ok(z, sparse_data, pack_sbit, RELU2_SCALE):
+        return z, relu2_and_compress(z, sparse_data, RELU2_SCALE)
+    h, h_sparse = relu_and_compress(z, sparse_data, pack_sbit)
+    if square:
+        relu2_square_amax_(h, RELU2_SCALE)
+    return h, h_sparse
