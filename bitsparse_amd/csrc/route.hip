@@ -111,77 +111,61 @@ __device__ __forceinline__ void wave_fence()
     __builtin_amdgcn_wave_barrier();
 }
 
-// What is chosen by, c, is -infinity where there is no expert (any more) and
-// infinity for a NaN.
-template <int L, int V>
-__global__ __launch_bounds__(256) void route_forward_kernel(RouteArgs a)
+// The groups that stay, a bit each, from their scores in LDS: fewer than
+// top_groups come before each.  worst: the least score that stays, next: the
+// largest that does not (over the lane's groups).
+template <int L, typename T>
+__device__ __forceinline__ uint64_t route_groups(const RouteArgs& a, const T* s_score, int l, T& worst, T& next)
 {
-    constexpr int TOKENS = 64 / L, SLOTS = (kMaxTopK + L - 1) / L;
-    __shared__ double s_score[4][TOKENS][64];
+    uint32_t low = 0, high = 0;
+    worst = INFINITY, next = -INFINITY;
+    for (int g = l; g < a.groups; g += L) {
+        const T mine = s_score[g];
+        int before = 0;
+        for (int h = 0; h < a.groups; h++) {
+            const T v = s_score[h];
+            before += v > mine || (v == mine && h < g);
+        }
+        if (before < a.top_groups && mine != (T)-INFINITY) {
+            (g < 32 ? low : high) |= 1u << (g & 31);
+            worst = mine < worst ? mine : worst;
+        } else {
+            next = mine > next ? mine : next;
+        }
+    }
+    const auto either = [](uint32_t x, uint32_t y) { return x | y; };
+    return (uint64_t)Lanes<L>::all(high, either) << 32 | Lanes<L>::all(low, either);
+}
+// whether expert e's group stays
+__device__ __forceinline__ bool group_kept(uint64_t kept, int e, uint32_t part)
+{
+    return kept >> ((uint32_t)e * part >> 22 & 63) & 1;     // part: 2^22 / size rounded up, e / size = e part >> 22 for e, size <= 1024
+}
+
+// The choice between 64-bit values c, -infinity where there is no expert (any
+// more): choice j in lane j % L's place j / L.
+template <int L, int V, int SLOTS>
+__device__ __forceinline__ void route_exact(const RouteArgs& a, double (&c)[V], int lane, double* s_score, int (&id)[SLOTS])
+{
+    typedef double T;
     typedef Lanes<L> Ln;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % L, sub = lane / L;
-    const int64_t token = ((int64_t)blockIdx.x * 4 + wave) * TOKENS + sub, row = min(token, a.tokens - 1);
-    const auto larger = [](auto x, auto y) { return x > y ? x : y; };
-    const auto sum_of = [](auto x, auto y) { return x + y; };
-    const int e0 = l * V;
-    float lg[V];
-    load_logits(a, row, e0, lg);
-
-    // softmax: the largest logit and the sum of exponentials over it (a NaN makes the sum NaN)
-    float top = -INFINITY, sum = 0.f;
-    if (!a.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < V; i++) top = fmaxf(top, lg[i]);
-        top = Ln::all(top, [](float x, float y) { return fmaxf(x, y); });
-    }
-    double c[V];
-    if (a.by_logit) {
-        if (!a.sigmoid) {
-#pragma unroll
-            for (int i = 0; i < V; i++) sum += lg[i] == -INFINITY ? 0.f : expf(lg[i] - top);
-            sum = Ln::all(sum, sum_of);
-        }
-#pragma unroll
-        for (int i = 0; i < V; i++) c[i] = lg[i];
-    } else if (a.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < V; i++) c[i] = lg[i] == -INFINITY ? -INFINITY : 1.0 / (1.0 + exp(-(double)lg[i]));
-    } else {
-        double total = 0.0;
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            c[i] = lg[i] == -INFINITY ? -INFINITY : exp((double)lg[i] - (double)top);
-            total += lg[i] == -INFINITY ? 0.0 : c[i];
-        }
-        total = Ln::all(total, sum_of);
-        sum = (float)total;
-        const double part = 1.0 / total;
-#pragma unroll
-        for (int i = 0; i < V; i++) c[i] = lg[i] == -INFINITY ? -INFINITY : c[i] * part;
-    }
-    if (a.bias) {
-        float b[V];
-        load_logits(a.bias, e0, a.experts, b);
-#pragma unroll
-        for (int i = 0; i < V; i++) c[i] += (double)b[i];
-    }
-#pragma unroll
-    for (int i = 0; i < V; i++) c[i] = c[i] != c[i] ? (double)INFINITY : c[i];
-
+    constexpr T kNone = -INFINITY;
+    const int l = lane % L, sub = lane / L, e0 = l * V;
+    const auto larger = [](T x, T y) { return x > y ? x : y; };
     if (a.top_groups < a.groups) {
         const int size = a.experts / a.groups;
-        // the best and the second best of two pairs of such
+        // the best and the second best
         struct Pair {
-            double x, y;
+            T x, y;
         };
-        auto add = [](Pair p, double v) {
+        auto add = [](Pair p, T v) {
             const bool more = v > p.x;
             return Pair{more ? v : p.x, more ? p.x : v > p.y ? v : p.y};
         };
-        auto score = [&](Pair p) { return a.group_best == 1 || p.y == -INFINITY ? p.x : p.x + p.y; };
+        auto score = [&](Pair p) { return a.group_best == 1 || p.y == kNone ? p.x : p.x + p.y; };
         const int span = size / V;          // lanes of a group, where it has whole lanes
         if (span * V == size && (span & (span - 1)) == 0 && span <= 16) {
-            Pair p = {-INFINITY, -INFINITY};
+            Pair p = {kNone, kNone};
 #pragma unroll
             for (int i = 0; i < V; i++) p = add(p, c[i]);
             auto meet = [&](auto d) {
@@ -192,73 +176,237 @@ __global__ __launch_bounds__(256) void route_forward_kernel(RouteArgs a)
             meet(std::integral_constant<int, 2>{});
             meet(std::integral_constant<int, 4>{});
             meet(std::integral_constant<int, 8>{});
-            if (l % span == 0 && l / span < a.groups) s_score[wave][sub][l / span] = score(p);
+            if (l % span == 0 && l / span < a.groups) s_score[l / span] = score(p);
         } else {
             for (int g = 0; g < a.groups; g++) {
-                Pair p = {-INFINITY, -INFINITY};
+                Pair p = {kNone, kNone};
 #pragma unroll
-                for (int i = 0; i < V; i++) p = add(p, e0 + i >= g * size && e0 + i < (g + 1) * size ? c[i] : -INFINITY);
-                const double best = Ln::all(p.x, larger);
+                for (int i = 0; i < V; i++) p = add(p, e0 + i >= g * size && e0 + i < (g + 1) * size ? c[i] : kNone);
+                const T best = Ln::all(p.x, larger);
                 // (one lane gives its best up, the first of those that have it)
                 const uint64_t have = __ballot(p.x == best) >> (sub * L) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1);
                 const bool first = l == __builtin_ctzll(have);
-                const double second = Ln::all(first ? p.y : p.x, larger);
-                if (l == 0) s_score[wave][sub][g] = score(Pair{best, second});
+                const T second = Ln::all(first ? p.y : p.x, larger);
+                if (l == 0) s_score[g] = score(Pair{best, second});
             }
         }
         wave_fence();
-        // group g stays if fewer than top_groups come before it
-        uint32_t low = 0, high = 0;
-        for (int g = l; g < a.groups; g += L) {
-            const double mine = s_score[wave][sub][g];
-            int before = 0;
-            for (int h = 0; h < a.groups; h++) {
-                const double v = s_score[wave][sub][h];
-                before += v > mine || (v == mine && h < g);
-            }
-            if (before < a.top_groups && mine != -INFINITY) (g < 32 ? low : high) |= 1u << (g & 31);
-        }
-        const auto either = [](uint32_t x, uint32_t y) { return x | y; };
-        const uint64_t kept = (uint64_t)Ln::all(high, either) << 32 | Ln::all(low, either);
-        const uint32_t part = ((1u << 22) + size - 1) / size;       // e / size = e part >> 22 for e, size <= 1024
+        T worst, next;
+        const uint64_t kept = route_groups<L>(a, s_score, l, worst, next);
+        wave_fence();
+        const uint32_t part = ((1u << 22) + size - 1) / size;
 #pragma unroll
         for (int i = 0; i < V; i++)
-            if (!(kept >> ((uint32_t)(e0 + i) * part >> 22 & 63) & 1)) c[i] = -INFINITY;
+            if (!group_kept(kept, e0 + i, part)) c[i] = kNone;
     }
-
-    int id[SLOTS];
-    float of[SLOTS];        // its logit
 #pragma unroll
     for (int s = 0; s < SLOTS; s++) {
         id[s] = -1;
-        of[s] = 0.f;
         for (int j = 0; j < L && s * L + j < a.top_k; j++) {
-            double best = c[0];
+            T best = c[0];
 #pragma unroll
-            for (int i = 1; i < V; i++) best = fmax(best, c[i]);
+            for (int i = 1; i < V; i++) best = larger(best, c[i]);
             uint32_t at = ~0u;
 #pragma unroll
             for (int i = V - 1; i >= 0; i--) at = c[i] == best ? e0 + i : at;
-            const double most = Ln::all(best, larger);
+            const T most = Ln::all(best, larger);
             at = Ln::all(best == most ? at : ~0u, [](uint32_t x, uint32_t y) { return min(x, y); });
-            float logit = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; i++) c[i] = at == (uint32_t)(e0 + i) ? kNone : c[i];
+            if (l == j) id[s] = most == kNone ? -1 : (int)at;
+        }
+    }
+}
+
+// The same between 32-bit values cut to 28 bits, the place in the lane in the
+// other four: their order as integers (0: none) is that of the values, and among equal ones
+// that of the places.  A lane's are sorted once, so that a choice is the largest of the lanes' first
+// ones.  True where what decides lies closer together than `near` and the cut:
+// the choice is then not sure.
+__device__ __forceinline__ uint32_t place_key(float v, int place)
+{
+    const uint32_t b = __float_as_uint(v);
+    return v == -INFINITY ? 0u : ((b >> 31 ? ~b : b | 1u << 31) & ~15u) | (uint32_t)(15 - place);
+}
+__device__ __forceinline__ float key_value(uint32_t k)
+{
+    k &= ~15u;
+    return k == 0 ? -INFINITY : __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
+}
+
+template <int L, int V, int SLOTS>
+__device__ __forceinline__ bool route_fast(const RouteArgs& a, const float (&c)[V], int lane, float* s_score, float near, int (&id)[SLOTS])
+{
+    static_assert(V <= 16, "four bits of place");
+    typedef Lanes<L> Ln;
+    const int l = lane % L, e0 = l * V;
+    const auto larger = [](uint32_t x, uint32_t y) { return max(x, y); };
+    const auto apart = [&](float x, float y, float times) { return near < 0.f || x - y > times * (near + 0x1p-18f * fabsf(x)); };
+    uint32_t k[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) k[i] = place_key(c[i], i);
+    bool unsure = false;
+    if (a.top_groups < a.groups) {
+        const int size = a.experts / a.groups, span = size / V;
+        if (span * V != size || (span & (span - 1)) != 0 || span > 16) return true;      // (no whole lanes, or no power of two of them)
+        uint32_t x = 0, y = 0;          // the best and the second best
+        auto add = [&](uint32_t v) {
+            y = max(y, min(x, v));
+            x = max(x, v);
+        };
+#pragma unroll
+        for (int i = 0; i < V; i++) add(k[i]);
+        auto meet = [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            if (span > D) {
+                const uint32_t ox = Ln::template other<D>(x), oy = Ln::template other<D>(y);
+                add(ox);
+                add(oy);
+            }
+        };
+        meet(std::integral_constant<int, 1>{});
+        meet(std::integral_constant<int, 2>{});
+        meet(std::integral_constant<int, 4>{});
+        meet(std::integral_constant<int, 8>{});
+        const float vx = key_value(x), vy = key_value(y);
+        if (l % span == 0 && l / span < a.groups) s_score[l / span] = a.group_best == 1 || y == 0 ? vx : vx + vy;
+        wave_fence();
+        float worst, next;
+        const uint64_t kept = route_groups<L>(a, s_score, l, worst, next);
+        wave_fence();
+        worst = Ln::all(worst, [](float p, float q) { return p < q ? p : q; });
+        next = Ln::all(next, [](float p, float q) { return p > q ? p : q; });
+        unsure = next != -INFINITY && !apart(worst, next, 4.f);
+        const bool mine = kept >> (l / span & 63) & 1;
+#pragma unroll
+        for (int i = 0; i < V; i++) k[i] = mine ? k[i] : 0u;
+    }
+    // (merging networks of pairs, fours, ...: the largest first)
+#pragma unroll
+    for (int p = 1; p < V; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < V; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; i++)
+                    if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t hi = max(k[i + j], k[i + j + q]), lo = min(k[i + j], k[i + j + q]);
+                        k[i + j] = hi, k[i + j + q] = lo;
+                    }
+    float last = 0.f;
+#pragma unroll
+    for (int s = 0; s < SLOTS; s++) {
+        id[s] = -1;
+        for (int j = 0; j < L && s * L + j < a.top_k; j++) {
+            // (of the lanes with the largest value the lowest index)
+            const uint32_t most = Ln::all(k[0] & ~15u, larger);
+            const uint32_t at = Ln::all((k[0] & ~15u) == most ? (uint32_t)e0 + 15 - (k[0] & 15) : ~0u, [](uint32_t x, uint32_t y) { return min(x, y); });
+            const float value = key_value(most);
+            if (s + j > 0) unsure |= most != 0 && !apart(last, value, 1.f);
+            last = value;
+            if (l == j) id[s] = most == 0 ? -1 : (int)at;
+            const bool mine = at - (uint32_t)e0 < (uint32_t)V;
+#pragma unroll
+            for (int i = 0; i < V; i++) k[i] = mine ? (i + 1 < V ? k[i + 1 < V ? i + 1 : i] : 0u) : k[i];
+        }
+    }
+    const uint32_t left = Ln::all(k[0] & ~15u, larger);         // the first that is left out
+    return unsure || (left != 0 && !apart(last, key_value(left), 1.f));
+}
+
+// First the fast choice, then where it is not sure the exact one (32768 tokens,
+// 8 of 256 experts in 4 of 8 groups, by sigmoid and bias: 47 us if all were exact).
+template <int L, int V>
+__global__ __launch_bounds__(256) void route_forward_kernel(RouteArgs a)
+{
+    constexpr int TOKENS = 64 / L, SLOTS = (kMaxTopK + L - 1) / L;
+    __shared__ double s_score[4][TOKENS][64];
+    typedef Lanes<L> Ln;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % L, sub = lane / L;
+    const int64_t token = ((int64_t)blockIdx.x * 4 + wave) * TOKENS + sub, row = min(token, a.tokens - 1);
+    const auto sum_of = [](auto x, auto y) { return x + y; };
+    const int e0 = l * V;
+    float lg[V], bias[V];
+    load_logits(a, row, e0, lg);
+    if (a.bias)
+        load_logits(a.bias, e0, a.experts, bias);
+    else
+#pragma unroll
+        for (int i = 0; i < V; i++) bias[i] = 0.f;
+
+    // softmax: the largest logit and the sum of exponentials over it (a NaN makes the sum NaN)
+    float top = -INFINITY, sum = 0.f, c[V];
+    if (!a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < V; i++) top = fmaxf(top, lg[i]);
+        top = Ln::all(top, [](float x, float y) { return fmaxf(x, y); });
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            c[i] = lg[i] == -INFINITY ? 0.f : expf(lg[i] - top);
+            sum += c[i];
+        }
+        sum = Ln::all(sum, sum_of);
+        const float part = 1.f / sum;
+#pragma unroll
+        for (int i = 0; i < V; i++) c[i] *= part;
+    } else if (!a.by_logit) {
+        // (the instructions' own precision, 2^-23: l's product with log2(e) is off by |l| 2^-24, s by a quarter of e^-|l| of that)
+#pragma unroll
+        for (int i = 0; i < V; i++) c[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * lg[i]));
+    }
+    float most_bias = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        c[i] = a.by_logit ? lg[i] : lg[i] == -INFINITY ? -INFINITY : c[i] + bias[i];
+        c[i] = c[i] != c[i] ? INFINITY : c[i];
+        most_bias = fmaxf(most_bias, bias[i] == -INFINITY ? 0.f : fabsf(bias[i]));
+    }
+    // What two scores together may be off by: a sigmoid's, at most 1, six roundings of 2^-24, a softmax's, at most 1 / sum, as
+    // many and those of a sum over lanes and their experts, 22 more; the biased one's another of both.  A bf16 logit is its key.
+    float near = -1.f;
+    if (!a.by_logit)
+        near = (a.sigmoid ? 0x1p-20f : 0x1p-18f / sum) + 0x1p-22f * Ln::all(most_bias, [](float x, float y) { return fmaxf(x, y); });
+    else if (a.f32)
+        near = 0.f;
+    int id[SLOTS];
+    if (__any(route_fast<L, V>(a, c, lane, reinterpret_cast<float*>(s_score[wave][sub]), near, id))) {
+        double d[V];
+        if (a.by_logit) {
+#pragma unroll
+            for (int i = 0; i < V; i++) d[i] = c[i];
+        } else if (a.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < V; i++) d[i] = 1.0 / (1.0 + exp(-(double)lg[i]));
+        } else {
+            double total = 0.0;
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const bool here = at == (uint32_t)(e0 + i);
-                logit = here ? lg[i] : logit;
-                c[i] = here ? -INFINITY : c[i];
+                d[i] = lg[i] == -INFINITY ? 0.0 : exp((double)lg[i] - (double)top);
+                total += d[i];
             }
-            logit = __shfl(logit, (int)(sub * L + at / V) & 63);
-            if (l == j) {
-                id[s] = most == -INFINITY ? -1 : (int)at;
-                of[s] = logit;
-            }
+            total = Ln::all(total, sum_of);
+#pragma unroll
+            for (int i = 0; i < V; i++) d[i] /= total;
         }
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            if (!a.by_logit) d[i] = lg[i] == -INFINITY ? -INFINITY : d[i] + (double)bias[i];
+            d[i] = d[i] != d[i] ? (double)INFINITY : d[i];
+        }
+        wave_fence();
+        route_exact<L, V>(a, d, lane, s_score[wave][sub], id);
     }
     float w[SLOTS], total = 0.f;
 #pragma unroll
     for (int s = 0; s < SLOTS; s++) {
-        w[s] = id[s] < 0 ? 0.f : a.sigmoid ? 1.f / (1.f + expf(-of[s])) : expf(of[s] - top) / sum;
+        w[s] = 0.f;
+        if (s * L >= a.top_k) continue;
+        // the logit again; the difference's rounding, which the exponential turns into as much of its value, is put back
+        const int64_t at = row * a.stride + max(0, id[s]);
+        const float of = a.f32 ? static_cast<const float*>(a.logits)[at] : (float)static_cast<const bf16*>(a.logits)[at];
+        const float d = of - top, back = d - of, lost = (of - (d - back)) - (top + back), e = expf(a.sigmoid ? -of : d);
+        w[s] = id[s] < 0 ? 0.f : a.sigmoid ? 1.f / (1.f + e) : fmaf(e, lost, e) / sum;
         total += w[s];
     }
     if (a.renorm) total = Ln::all(total, sum_of);
@@ -284,7 +432,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a)
     load_logits(a, row, e0, s);
     if (a.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < V; i++) s[i] = 1.f / (1.f + expf(-s[i]));
+        for (int i = 0; i < V; i++) s[i] = __builtin_amdgcn_rcpf(1.f + expf(-s[i]));      // (within a unit of the last place)
     } else {
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
