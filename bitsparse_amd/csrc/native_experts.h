@@ -252,6 +252,7 @@ void bf16_on(const Tensor& t, const char* what, const Plan& plan)
 struct Rows16 {
     Tensor t;
     int64_t stride;
+    bool padded = false;
     explicit Rows16(const Tensor& rows)
     {
         const int64_t R = rows.size(0), C = rows.size(1), width = (C + 7) / 8 * 8;
@@ -263,6 +264,7 @@ struct Rows16 {
         t = at::empty({R, width}, rows.options());
         check(L.bs_pad_rows(raw(rows), R, C, row_stride(rows), raw(t), width, stream_of(rows)), "bs_pad_rows");
         stride = width;
+        padded = true;
     }
 };
 
@@ -312,43 +314,41 @@ struct Gathered {
     }
 };
 
-Tensor expert_product(const Tensor& x, const Tensor& W, const Plan& plan, bool gather, int64_t act, double act_k)
+Tensor expert_product(const Rows16& w, const Gathered& a, const Plan& plan, int64_t in, int64_t out, int64_t act, double act_k)
 {
-    const c10::DeviceGuard guard(plan.offsets.device());
-    const Tensor rows = expert_operand(x, plan, gather, "x");
-    check_weights(W, plan, "W");
-    TORCH_CHECK_VALUE(W.size(2) == rows.size(1), "W: expected ", rows.size(1), " columns, as x has, got ", W.sizes());
-    Tensor y = at::empty({plan.rows, W.size(1)}, x.options());
+    Tensor y = at::empty({plan.rows, out}, a.rows.t.options());
     if (plan.rows == 0) return y;
-    const Gathered a(rows, plan, gather, false);
-    const Rows16 w = expert_weights(W);
     const bs_experts e = plan.args(a.gather);
-    check(L.bs_expert_linear(&e, raw(a.rows.t), a.rows.stride, raw(w.t), w.stride, W.size(2), W.size(1), (int)act, (float)act_k, raw(y), stream_of(y)),
+    check(L.bs_expert_linear(&e, raw(a.rows.t), a.rows.stride, raw(w.t), w.stride, in, out, (int)act, (float)act_k, raw(y), stream_of(y)),
           "bs_expert_linear");
     return y;
 }
 // in the plan's order
-Tensor expert_product_dx(const Tensor& dy, const Tensor& W, const Plan& plan, at::ScalarType type)
+Tensor expert_product_dx(const Rows16& g, const Rows16& w, const Plan& plan, int64_t in, int64_t out, at::ScalarType type)
 {
-    const c10::DeviceGuard guard(plan.offsets.device());
-    Tensor dx = at::empty({plan.rows, W.size(2)}, dy.options().dtype(type));
+    Tensor dx = at::empty({plan.rows, in}, g.t.options().dtype(type));
     if (plan.rows == 0) return dx;
-    const Rows16 g(dy), w = expert_weights(W);
     const bs_experts e = plan.args(false);
-    check(L.bs_expert_linear_dx(&e, raw(g.t), g.stride, raw(w.t), w.stride, W.size(2), W.size(1), raw(dx), type == at::kFloat ? BS_DT_F32 : BS_DT_BF16,
+    check(L.bs_expert_linear_dx(&e, raw(g.t), g.stride, raw(w.t), w.stride, in, out, raw(dx), type == at::kFloat ? BS_DT_F32 : BS_DT_BF16,
                                 stream_of(dx)),
           "bs_expert_linear_dx");
     return dx;
 }
-Tensor expert_product_dw(const Tensor& dy, const Tensor& x, const Plan& plan, bool x_gathered)
+// x: rows in the plan's order
+Tensor expert_product_dw(const Rows16& g, const Rows16& x, const Plan& plan, int64_t in, int64_t out)
 {
-    const c10::DeviceGuard guard(plan.offsets.device());
-    Tensor dW = at::empty({plan.experts, dy.size(1), x.size(1)}, x.options());
-    const Rows16 g(dy);
-    const Gathered b(x, plan, x_gathered && plan.rows, true);
+    Tensor dW = at::empty({plan.experts, out, in}, g.t.options());
     const bs_experts e = plan.args(false);
-    check(L.bs_expert_linear_dw(&e, raw(g.t), g.stride, raw(b.rows.t), b.rows.stride, x.size(1), dy.size(1), raw(dW), stream_of(dW)), "bs_expert_linear_dw");
+    check(L.bs_expert_linear_dw(&e, raw(g.t), g.stride, raw(x.t), x.stride, in, out, raw(dW), stream_of(dW)), "bs_expert_linear_dw");
     return dW;
+}
+// (operands checked, and the rows of x)
+Tensor expert_operands(const Tensor& x, const Tensor& W, const Plan& plan, bool gather)
+{
+    const Tensor rows = expert_operand(x, plan, gather, "x");
+    check_weights(W, plan, "W");
+    TORCH_CHECK_VALUE(W.size(2) == rows.size(1), "W: expected ", rows.size(1), " columns, as x has, got ", W.sizes());
+    return rows;
 }
 // sums over the choices of each token, in bf16
 Tensor combined(const Tensor& y, const Tensor& weights, const Plan& plan)
@@ -364,8 +364,8 @@ Tensor combined(const Tensor& y, const Tensor& weights, const Plan& plan)
 
 // the plan's tensors and an operator's other arguments, kept for a backward
 struct ExpertsNode : torch::CustomClassHolder {
-    bool gather = false, need[2] = {};
-    std::vector<int64_t> shape[2], plan_shape[3];
+    bool gather = false, gathered = false, need[2] = {}, copied[2] = {};
+    std::vector<int64_t> shape[2], operand[2], plan_shape[3];       // of what is saved, of the operands
     at::TensorOptions options;
 };
 
@@ -390,15 +390,25 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& W, const PlanTensors& p, bool gather)
     {
         const Plan plan(p.offsets, p.order, p.place);
-        Tensor y = expert_product(x, W, plan, gather, BS_ACT_NONE, 0.0);
+        const c10::DeviceGuard guard(plan.offsets.device());
+        const Tensor rows = expert_operands(x, W, plan, gather);
+        const Gathered a(rows, plan, gather, false);
+        const Rows16 w = expert_weights(W);
+        Tensor y = expert_product(w, a, plan, W.size(2), W.size(1), BS_ACT_NONE, 0.0);
         auto node = c10::make_intrusive<ExpertsNode>();
-        node->gather = gather;
+        node->gather = a.gather;        // (rows that were written out are rows)
         node->need[0] = x.requires_grad(), node->need[1] = W.requires_grad();
-        node->shape[0] = x.sizes().vec(), node->shape[1] = W.sizes().vec();
+        node->gathered = gather;
+        node->operand[0] = x.sizes().vec(), node->operand[1] = W.sizes().vec();
+        // What a gradient that is asked for is formed of; of padded operands the copies, which the backward pass would make again.
+        const bool copied = a.rows.padded || gather != a.gather;
+        const Tensor keep_x = node->need[1] ? copied ? a.rows.t : x : Tensor(), keep_W = node->need[0] ? w.padded ? w.t : W : Tensor();
+        if (keep_x.defined()) node->shape[0] = keep_x.sizes().vec();
+        if (keep_W.defined()) node->shape[1] = keep_W.sizes().vec();
+        node->copied[0] = copied, node->copied[1] = w.padded;
         keep_plan(*node, plan);
         ctx->saved_data["node"] = c10::IValue::make_capsule(node);
-        // (what a gradient that is asked for is formed of)
-        ctx->save_for_backward({node->need[1] ? x : Tensor(), node->need[0] ? W : Tensor(), plan.offsets, plan.order, plan.place});
+        ctx->save_for_backward({keep_x, keep_W, plan.offsets, plan.order, plan.place});
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads)
@@ -411,26 +421,38 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
         const c10::DeviceGuard guard(device);
         torch::autograd::variable_list out(4);
         const Plan plan = kept_plan(node, saved, 2);
-        as_saved(grads[0], {plan.rows, node.shape[1][1]}, at::kBFloat16, device, "the gradient of y");
-        const Tensor g = as_rows(grads[0], node.shape[1][1]);
+        const int64_t D = node.operand[1][2], N = node.operand[1][1];
+        as_saved(grads[0], {plan.rows, N}, at::kBFloat16, device, "the gradient of y");
+        const Rows16 g(as_rows(grads[0], N));
         if (ctx->needs_input_grad(0) && node.need[0]) {
             as_saved(saved[1], node.shape[1], at::kBFloat16, device, "W");
+            const Rows16 w = node.copied[1] ? Rows16(saved[1].contiguous()) : expert_weights(saved[1]);
             // (a gathered token's rows are rounded once, in their sum)
-            const Tensor dx = expert_product_dx(g, saved[1], plan, node.gather && plan.top_k > 1 ? at::kFloat : at::kBFloat16);
-            out[0] = (node.gather ? combined(dx, Tensor(), plan) : dx).view(node.shape[0]);
+            const Tensor dx = expert_product_dx(g, w, plan, D, N, node.gathered && plan.top_k > 1 ? at::kFloat : at::kBFloat16);
+            out[0] = (node.gathered ? combined(dx, Tensor(), plan) : dx).view(node.operand[0]);
         }
         if (ctx->needs_input_grad(1) && node.need[1]) {
             as_saved(saved[0], node.shape[0], at::kBFloat16, device, "x");
-            out[1] = expert_product_dw(g, as_rows(saved[0], node.shape[0].back()), plan, node.gather);
+            const Tensor x = as_rows(saved[0], node.shape[0].back());
+            out[1] = expert_product_dw(g, Gathered(x, plan, node.gather && plan.rows, true).rows, plan, D, N);
         }
         return out;
     }
 };
 
+Tensor expert_product_act(const Tensor& x, const Tensor& W, const Tensor& offsets, const Tensor& order, const Tensor& place, bool gather,
+                          int64_t act, double act_k)
+{
+    const Plan plan(offsets, order, place);
+    const c10::DeviceGuard guard(plan.offsets.device());
+    const Tensor rows = expert_operands(x, W, plan, gather);
+    return expert_product(expert_weights(W), Gathered(rows, plan, gather, false), plan, W.size(2), W.size(1), act, act_k);
+}
+
 Tensor expert_linear(const Tensor& x, const Tensor& W, const Tensor& offsets, const Tensor& order, const Tensor& place, bool gather)
 {
     if (at::GradMode::is_enabled() && (x.requires_grad() || W.requires_grad())) return ExpertLinear::apply(x, W, PlanTensors{offsets, order, place}, gather);
-    return expert_product(x, W, Plan(offsets, order, place), gather, BS_ACT_NONE, 0.0);
+    return expert_product_act(x, W, offsets, order, place, gather, BS_ACT_NONE, 0.0);
 }
 
 // ---------------------------------------------------------------------------
@@ -507,12 +529,6 @@ Tensor expert_combine(const Tensor& y, const Tensor& weights, const Tensor& offs
 // ---------------------------------------------------------------------------
 // a block of experts (experts.py's ExpertsRelu and ExpertsRelu2)
 // ---------------------------------------------------------------------------
-Tensor expert_product_act(const Tensor& x, const Tensor& W, const Tensor& offsets, const Tensor& order, const Tensor& place, bool gather,
-                          int64_t act, double act_k)
-{
-    return expert_product(x, W, Plan(offsets, order, place), gather, act, act_k);
-}
-
 // The gradients of out = sum of w act(x W1^T) W2^T over a token's choices, of
 // (x, W1, W2, weights) those that are wanted.  r: the saved relu(x W1^T)
 // [rows, H], overwritten.  The result y of the second product is not needed:
@@ -537,8 +553,9 @@ std::vector<std::optional<Tensor>> experts_backward(const Tensor& grad, const Te
     as_saved(grad, plan.token_shape(O), at::kBFloat16, plan.offsets.device(), "the gradient");
     std::vector<std::optional<Tensor>> out(4);
     const Tensor g_tokens = as_rows(grad, O);
-    Tensor dy = plan.rows ? Gathered::written_out(g_tokens, plan) : at::empty({0, O}, grad.options());      // before its weights
-    const Tensor dz = expert_product_dx(dy, W2, plan, at::kBFloat16);
+    // (before its weights, in the plan's order)
+    const Rows16 dy(plan.rows ? Gathered::written_out(g_tokens, plan) : at::empty({0, O}, grad.options()));
+    const Tensor dz = expert_product_dx(dy, expert_weights(W2), plan, H, O, at::kBFloat16);
     Tensor dw;
     if (need[3]) dw = at::zeros(weights.sizes(), weights.options());
     if (plan.rows)
@@ -546,9 +563,12 @@ std::vector<std::optional<Tensor>> experts_backward(const Tensor& grad, const Te
                                     ptr<float>(dw), stream_of(dz)),
               "bs_experts_act_grad");
     if (need[3]) out[3] = dw;
-    if (need[2]) out[2] = expert_product_dw(dy, r, plan, false);
-    dy = Tensor();
-    if (need[0]) out[0] = combined(expert_product_dx(dz, W1, plan, plan.top_k > 1 ? at::kFloat : at::kBFloat16), Tensor(), plan).view(x.sizes());
-    if (need[1]) out[1] = expert_product_dw(dz, tokens, plan, true);
+    if (need[2]) out[2] = expert_product_dw(dy, Rows16(r), plan, H, O);
+    if (!need[0] && !need[1]) return out;
+    const int64_t D = tokens.size(1);
+    const Rows16 g(dz);
+    if (need[0])
+        out[0] = combined(expert_product_dx(g, expert_weights(W1), plan, D, H, plan.top_k > 1 ? at::kFloat : at::kBFloat16), Tensor(), plan).view(x.sizes());
+    if (need[1]) out[1] = expert_product_dw(g, Gathered(tokens, plan, plan.rows > 0, true).rows, plan, D, H);
     return out;
 }
