@@ -2,8 +2,10 @@
 // 65536 / (65536 - bound) elsewhere (philox.h).  Its own backward: the same
 // call on the gradient.
 //
-// Bound by memory (x read once, out written once) if the 40 multiplications of
-// eight elements' bits keep up with it.
+// Bound by memory, x read once and out written once: the bits (20 64-bit
+// products for eight elements, a third of the time by themselves) are formed
+// while other waves' loads are on their way.  16384 x 4096: bf16 52 us, 5.1 TB/s, fp32 104 us
+// (a copy reaches 4.9 TB/s); 257 x 100: 3.1 us, latency.
 #include <algorithm>
 
 #include "bs_host.h"
@@ -28,10 +30,10 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a)
         const int64_t row = i / per_row, chunk = i - row * per_row;
         const int nv = (int)min((int64_t)8, a.cols - chunk * 8);
         const Raw<T> x = load_raw(static_cast<const T*>(a.x) + row * a.stride + chunk * 8, nv);
-        float f[8], o[8];
-        drop_factors(a.rule, key, (uint32_t)chunk, (uint32_t)row, f);
+        const DropMask mask(a.rule, key, (uint32_t)chunk, (uint32_t)row);
+        float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = f[e] == 0.f ? 0.f : raw_get(x, e) * f[e];    // (a dropped infinity is 0)
+        for (int e = 0; e < 8; e++) o[e] = mask.of(a.rule, e, raw_get(x, e));
         store_raw(static_cast<T*>(a.out) + row * a.cols + chunk * 8, to_raw<T>(o), nv);
     }
 }
@@ -43,7 +45,8 @@ int drop_rule(const bs_drop* d, const char* what, DropRule* r)
     if ((uintptr_t)d->state & 7u) return set_error(BS_ERR_INVALID, "%s: drop.state misaligned", what);
     r->key0 = (uint32_t)d->seed, r->key1 = (uint32_t)(d->seed >> 32);
     r->offset0 = (uint32_t)d->offset, r->offset1 = (uint32_t)(d->offset >> 32);
-    r->at = d->state, r->below = (uint32_t)d->below;
+    r->at = d->state;
+    r->bound = d->below < 65536 ? (uint32_t)d->below << 16 : ~0u, r->mask = d->below < 65536 ? ~0u : 0u;
     r->keep_scale = d->below < 65536 ? (float)(65536.0 / (65536 - d->below)) : 1.f;
     return BS_OK;
 }

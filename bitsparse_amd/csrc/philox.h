@@ -16,7 +16,8 @@ struct DropRule {
     uint32_t key0, key1;        // the seed's words
     uint32_t offset0, offset1;  // the offset's
     const int64_t* at;          // or both of these in memory, [seed, offset]
-    uint32_t below;             // a half below it: the element is dropped (65536: all)
+    uint32_t bound;             // the number that a half below it drops its element, times 65536
+    uint32_t mask;              // of the words: all of them, or 0 where everything is dropped, which no bound says
     float keep_scale;           // of those that stay
 };
 
@@ -47,13 +48,24 @@ __device__ __forceinline__ uint4 drop_bits(const DropKey& key, uint32_t chunk, u
     return uint4{c0, c1, c2, c3};
 }
 
-// the factors of a chunk's elements: keep_scale, or 0 for a dropped one
-__device__ __forceinline__ void drop_factors(const DropRule& r, const DropKey& key, uint32_t chunk, uint32_t row, float (&f)[8])
-{
-    const uint4 u = drop_bits(key, chunk, row);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = (e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu) < r.below ? 0.f : r.keep_scale;
-}
+// A chunk's mask.  A half is compared where it lies, in the upper half of a word (the lower ones moved there).
+struct DropMask {
+    uint32_t w[4];
+    __device__ __forceinline__ DropMask(const DropRule& r, const DropKey& key, uint32_t chunk, uint32_t row)
+    {
+        const uint4 u = drop_bits(key, chunk, row);
+        w[0] = u.x & r.mask, w[1] = u.y & r.mask, w[2] = u.z & r.mask, w[3] = u.w & r.mask;
+    }
+    __device__ __forceinline__ bool kept(const DropRule& r, int e) const { return (e & 1 ? w[e >> 1] : w[e >> 1] << 16) >= r.bound; }
+    // v as the dropout leaves it: 0 where it is dropped, whatever it was
+    __device__ __forceinline__ float of(const DropRule& r, int e, float v) const { return kept(r, e) ? v * r.keep_scale : 0.f; }
+};
+
+// the same of a step without dropout
+struct DropNothing {
+    __device__ __forceinline__ DropNothing(const DropRule&, const DropKey&, uint32_t, uint32_t) {}
+    __device__ __forceinline__ bool kept(const DropRule&, int) const { return true; }
+    __device__ __forceinline__ float of(const DropRule&, int, float v) const { return v; }
+};
 
 }  // namespace bs

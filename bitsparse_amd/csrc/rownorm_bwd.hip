@@ -18,12 +18,14 @@
 // column sums over all its rows and writes one row of partial sums; the second
 // kernel adds those in order.  No atomics: the same bits at every call.
 // 16384 x 4096 in bf16: 182 us, 5.2 TB/s (a copy reaches 5.15); 8192 x 768,
-// which stays in the last level cache: 23 us, 3.8 TB/s.  Up to 4096 elements
+// which stays in the last level cache: 23 us, 3.8 TB/s.  With a dropout, whose
+// bits are formed again, 199 us where the same step without takes 144.  Up to 4096 elements
 // row, sums and vectors are in registers.  Past that they do not all fit (the
 // join's spill 40 to 90 registers a lane up to 8192 elements, 630 to 960 up to
 // 16384, 1200 to 1600 beyond): 8192 x 8192 297 us, 3.2 TB/s; 4096 x 16384 1.49
 // ms, 0.63 TB/s; 2048 x 32768 1.94 ms.
 #include <algorithm>
+#include <type_traits>
 
 #include "bs_host.h"
 #include "rownorm.h"
@@ -67,8 +69,7 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
     const bool per_row = !PLAIN && a.gate_per == BS_PER_ROW, per_element = !PLAIN && a.gate_per == BS_PER_ELEMENT;
     const bool layer_post = !PLAIN && a.post == BS_NORM_LAYER, layer_pre = !PLAIN && a.pre == BS_NORM_LAYER;
     void* const d_row_gate = PLAIN ? nullptr : a.d_row_gate;
-    DropKey key;
-    if constexpr (DROP) key = drop_key(a.drop);
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
 
     // the next row's loads are in flight while this row's sums meet
     struct Row {
@@ -178,8 +179,7 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                 if (per_element)
                     param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, ge);
                 if (d_row_gate) param_chunk(a.b_post, at.col[k], nv[k], 0.f, b1);
-                float drop[8];
-                if constexpr (DROP) drop_factors(a.drop, key, (uint32_t)(at.col[k] >> 3), (uint32_t)row, drop);
+                std::conditional_t<DROP, DropMask, DropNothing> drop(a.drop, key, (uint32_t)(at.col[k] >> 3), (uint32_t)row);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     // (past the row's end x' and the gradients are 0, and so is G but for a layer norm's mean)
@@ -188,13 +188,10 @@ __global__ __launch_bounds__(MAXT) void join_backward_kernel(JoinBwd a)
                     acc[kSumScale][k][e] += g0 * raw_get(now.x[k], e);
                     float n = (raw_get(now.y[k], e) - st.x) * st.y;
                     float gg = PLAIN ? g0 : per_element ? g0 * ge[e] : rg * g0;    // G of the gate's part that is not a vector
-                    float gp = g0;                                                 // G as the gate's gradient has it
-                    if constexpr (DROP) {       // (a dropped element passes nothing, whatever it and its gradient are)
-                        const bool kept = drop[e] != 0.f;
-                        gg = kept ? gg * drop[e] : 0.f;
-                        gp = kept ? g0 * drop[e] : 0.f;
-                        n = kept || a.post ? n : 0.f;
-                    }
+                    // (a dropped element passes nothing, whatever it and its gradient are; gp: G as the gate's gradient has it)
+                    gg = drop.of(a.drop, e, gg);
+                    const float gp = drop.of(a.drop, e, g0);
+                    if (DROP && !a.post) n = drop.kept(a.drop, e) ? n : 0.f;
                     acc[kSumA][k][e] += gg * n;
                     if (!PLAIN) acc[kSumB][k][e] += gg;
                     const float dm = gg * gw[k][e];

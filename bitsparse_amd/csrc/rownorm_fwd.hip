@@ -8,10 +8,12 @@
 // loads are in flight while this row's sums meet.  Up to 8192 elements the
 // vectors are held in registers over the rows that a workgroup goes through.
 // 16384 x 4096 in bf16: 101 us, 5.3 TB/s (a copy reaches 5.15), the norm alone
-// 46 us, 5.8 TB/s; 32 x 4096: 5.6 us, latency.  Past 8192 elements the join
+// 46 us, 5.8 TB/s; 32 x 4096: 5.6 us, latency.  With a dropout 141 us: the bits' 20
+// 64-bit products of eight elements take as long as 35 us of the loads, and 16 waves a CU do not hide them.  Past 8192 elements the join
 // spills registers (70 to 100 a lane, 220 to 380 past 16384): 4096 x 16384 202
 // us, 2.7 TB/s; 2048 x 32768 387 us.
 #include <algorithm>
+#include <type_traits>
 
 #include "bs_host.h"
 #include "philox.h"
@@ -46,8 +48,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
     const RowPlace<C> at(a.cols, a.waves);
     int turn = 0;
     const bool per_row = a.gate_per == BS_PER_ROW, per_element = a.gate_per == BS_PER_ELEMENT;
-    DropKey key;
-    if constexpr (DROP) key = drop_key(a.drop);
+    const DropKey key = DROP ? drop_key(a.drop) : DropKey{};
 
     const int64_t step = (int64_t)gridDim.x * a.rows_here;
     int64_t row = (int64_t)blockIdx.x * a.rows_here + at.sub;
@@ -116,8 +117,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                 float g[8];
                 if (per_element)
                     param_chunk(RowParam{a.row_gate, a.row_gate_f32, 0}, row * a.gate_stride + at.col[k], nv[k], 0.f, g);
-                float drop[8];
-                if constexpr (DROP) drop_factors(a.drop, key, (uint32_t)(at.col[k] >> 3), (uint32_t)row, drop);
+                std::conditional_t<DROP, DropMask, DropNothing> drop(a.drop, key, (uint32_t)(at.col[k] >> 3), (uint32_t)row);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     // (p whole before its gate: an infinite gate times two terms of different signs would be NaN, and times
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(MAXT) void join_forward_kernel(JoinFwd a)
                     // roundings in 32 bits)
                     const float gate = gv[k][e] * (per_element ? g[e] : rg);
                     float p = fmaf((y[k][e] - mean) * w1[k][e], rstd, b1[k][e]);
-                    if constexpr (DROP) p = drop[e] == 0.f ? 0.f : p * drop[e];     // (a dropped infinity is 0)
+                    p = drop.of(a.drop, e, p);
                     v[k][e] = fmaf(gate, p, sc[k][e] * v[k][e]);
                 }
                 const Raw<XT> o = to_raw<XT>(v[k]);
