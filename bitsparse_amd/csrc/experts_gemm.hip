@@ -129,7 +129,7 @@ __device__ __forceinline__ int wave_scan(int v)
 __device__ __forceinline__ Group find_group(const ExpertGemm& g, int tile, int size)
 {
     const int lane = threadIdx.x & 63;
-    int before = 0;
+    int64_t before = 0;     // (64 experts' tiles are below 2^31; those of offsets that overlap add up past it)
     for (int e0 = 0; e0 < g.experts; e0 += 64) {
         const int e = e0 + lane;
         const int from = group_bound(g, min(e, g.experts)), to = max(from, group_bound(g, min(e + 1, g.experts)));
@@ -138,13 +138,12 @@ __device__ __forceinline__ Group find_group(const ExpertGemm& g, int tile, int s
         const uint64_t past = __ballot(before + sum > tile);
         if (past) {
             const int at = __builtin_ctzll(past);
-            const int mine = before + sum - tiles;
             return {e0 + at, (int64_t)__builtin_amdgcn_readlane(from, at), (int64_t)__builtin_amdgcn_readlane(to, at),
-                    (int64_t)(tile - __builtin_amdgcn_readlane(mine, at))};
+                    tile - before - __builtin_amdgcn_readlane(sum - tiles, at)};
         }
         before += __builtin_amdgcn_readlane(sum, 63);
     }
-    return {-1, (int64_t)group_bound(g, g.experts), g.rows, (int64_t)(tile - before)};
+    return {-1, (int64_t)group_bound(g, g.experts), g.rows, tile - before};
 }
 
 // The expert with the rank'th most rows, of up to 8: dW's longest sums begin first and its shortest fill the end (16384 rows of
@@ -557,7 +556,7 @@ static int launch_gemm(ExpertGemm g, const char* what, hipStream_t st)
     g.panel = 8;
     // (32768 rows of 16 experts 2048 -> 4096 510 us without, 489 with; dW of 64 experts 1024 -> 2048 147 and 110)
     g.stream = use_nontemporal((KIND == kDw ? (int64_t)g.experts * g.m : g.rows) * g.n * (KIND == kDx && g.c_f32 ? 4 : 2));
-    if (tiles_m * g.tiles_n >= (1ll << 31)) return set_error(BS_ERR_INVALID, "%s: too many tiles", what);
+    if (tiles_m * g.tiles_n >= (1ll << 32) / (64 * WGM * WGN)) return set_error(BS_ERR_INVALID, "%s: more tiles than a launch's 2^32 threads hold", what);
     hipLaunchKernelGGL((expert_gemm_kernel<KIND, GATHER, WGM, WGN, IM, JN, STAGES, AHEAD>), dim3((uint32_t)(tiles_m * g.tiles_n)), dim3(64 * WGM * WGN), 0, st, g);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
@@ -675,6 +674,7 @@ extern "C" int bs_expert_linear(const bs_experts* experts, const void* x, int64_
     const bool gather = experts->order != nullptr;
     if (const int rc = operand_check(what, "x", x, gather ? experts->tokens : experts->rows, x_stride, in, gather); rc != BS_OK) return rc;
     if (const int rc = operand_check(what, "W", W, out, w_stride, in, false); rc != BS_OK) return rc;
+    if (out * w_stride * 2 >= (int64_t)kNoRow) return set_error(BS_ERR_INVALID, "%s: an expert's W spans 4 GiB or more", what);
     if (y == nullptr || ((uintptr_t)y & 15u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned y", what);
     ExpertGemm g = gemm_args(*experts, gather);
     g.a = static_cast<const bf16*>(x), g.a_stride = x_stride, g.b = static_cast<const bf16*>(W), g.b_stride = w_stride, g.b_expert = out * w_stride;

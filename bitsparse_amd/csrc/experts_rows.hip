@@ -17,6 +17,7 @@ namespace bs {
 
 constexpr int kMaxChoices = 64;
 constexpr int kTailBlocks = 64;     // workgroups that clear the rows behind the last expert's
+constexpr int64_t kSlice = 1 << 22; // workgroups of a launch, which has fewer than 2^32 threads
 
 struct CombineArgs {
     int64_t tokens, rows, cols;
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(CombineArgs a)
 // h = r or bf16(bf16(r r) k):
 //   dw = <g, h>;  dz = w g [r > 0] or w g 2 k r;  and w h, W2's right operand
 struct ActGradArgs {
-    int64_t rows, cols, pairs;
+    int64_t first, cols, pairs;     // first: a launch's first row
     int square;
     float k;
     const float* weights;
@@ -143,7 +144,7 @@ template <bool WHOLE>
 __global__ __launch_bounds__(256) void experts_act_grad_kernel(ActGradArgs a)
 {
     __shared__ float s_dot[4];
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.first + blockIdx.x;
     const int pair = row < *a.used ? a.order[row] : -1;
     const bool there = pair >= 0 && pair < a.pairs;
     const float w = there ? a.weights[pair] : 0.f;
@@ -197,15 +198,19 @@ extern "C" int bs_expert_combine(const void* y, int y_type, int64_t y_stride, co
     if (((uintptr_t)y & (y_type == BS_DT_F32 ? 3u : 1u)) || ((uintptr_t)out & 1u) || (((uintptr_t)weights | (uintptr_t)place) & 3u))
         return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
     CombineArgs a{};
-    a.tokens = tokens, a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride;
-    a.weights = weights, a.place = place, a.out = static_cast<bf16*>(out);
-    const dim3 grid((uint32_t)tokens, (uint32_t)std::min<int64_t>((cols + 2047) / 2048, 65535));
+    a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride;
     const bool whole = cols % 8 == 0;
     auto* kernel = y_type == BS_DT_F32 ? (whole ? combine_kernel<float, true> : combine_kernel<float, false>)
                                        : (whole ? combine_kernel<bf16, true> : combine_kernel<bf16, false>);
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    const uint32_t parts = (uint32_t)std::min<int64_t>((cols + 2047) / 2048, 65535);
+    for (int64_t t = 0; t < tokens; t += kSlice) {
+        a.tokens = std::min(kSlice, tokens - t);
+        a.weights = weights ? weights + t * top_k : nullptr, a.place = place + t * top_k, a.out = static_cast<bf16*>(out) + t * cols;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)a.tokens, parts), dim3(256), 0, (hipStream_t)stream, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    }
+    return BS_OK;
 }
 
 extern "C" int bs_expert_combine_backward(const void* g, int64_t g_stride, const void* y, int64_t y_stride, const float* weights,
@@ -222,14 +227,22 @@ extern "C" int bs_expert_combine_backward(const void* g, int64_t g_stride, const
     if ((((uintptr_t)g | (uintptr_t)y | (uintptr_t)dy) & 1u) || (((uintptr_t)weights | (uintptr_t)place | (uintptr_t)used | (uintptr_t)dw) & 3u))
         return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
     CombineArgs a{};
-    a.tokens = tokens, a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride;
-    a.weights = weights, a.place = place, a.used = used, a.g = static_cast<const bf16*>(g), a.g_stride = g_stride;
-    a.dy = static_cast<bf16*>(dy), a.dw = dw;
+    a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride;
+    a.used = used, a.g_stride = g_stride, a.dy = static_cast<bf16*>(dy);
     auto* kernel = dw ? (cols % 8 == 0 ? combine_backward_kernel<true> : combine_backward_kernel<false>)
                       : (cols % 8 == 0 ? spread_kernel<true> : spread_kernel<false>);
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tokens + (dy ? kTailBlocks : 0))), dim3(256), 0, (hipStream_t)stream, a);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    // (no tokens: the rows behind alone)
+    for (int64_t t = 0; t == 0 || t < tokens; t += kSlice) {
+        a.tokens = std::min(kSlice, tokens - t);
+        const int64_t blocks = a.tokens + (dy && t + kSlice >= tokens ? kTailBlocks : 0);
+        if (blocks == 0) break;
+        a.weights = weights ? weights + t * top_k : nullptr, a.place = place + t * top_k, a.g = static_cast<const bf16*>(g) + t * g_stride;
+        a.dw = dw ? dw + t * top_k : nullptr;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(256), 0, (hipStream_t)stream, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    }
+    return BS_OK;
 }
 
 extern "C" int bs_experts_act_grad(void* g, void* r, int64_t rows, int64_t cols, int square, float k, const float* weights,
@@ -244,9 +257,12 @@ extern "C" int bs_experts_act_grad(void* g, void* r, int64_t rows, int64_t cols,
         return set_error(BS_ERR_INVALID, "%s: null pointer", what);
     if ((((uintptr_t)g | (uintptr_t)r) & 1u) || (((uintptr_t)weights | (uintptr_t)order | (uintptr_t)used | (uintptr_t)dw) & 3u))
         return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
-    ActGradArgs a{rows, cols, pairs, square, k, weights, order, used, static_cast<bf16*>(g), static_cast<bf16*>(r), dw};
+    ActGradArgs a{0, cols, pairs, square, k, weights, order, used, static_cast<bf16*>(g), static_cast<bf16*>(r), dw};
     auto* kernel = cols % 8 == 0 ? experts_act_grad_kernel<true> : experts_act_grad_kernel<false>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    for (; a.first < rows; a.first += kSlice) {
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)std::min(kSlice, rows - a.first)), dim3(256), 0, (hipStream_t)stream, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    }
+    return BS_OK;
 }

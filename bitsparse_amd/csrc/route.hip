@@ -226,7 +226,7 @@ __device__ __forceinline__ void route_exact(const RouteArgs& a, double (&c)[V], 
 // The same between 32-bit values cut to 28 bits, the place in the lane in the
 // other four: their order as integers (0: none) is that of the values, and among equal ones
 // that of the places.  A lane's are sorted once, so that a choice is the largest of the lanes' first
-// ones.  True where what decides lies closer together than `near` and the cut:
+// ones.  True where what decides lies closer together than `near` and the cut (of values up to `size`):
 // the choice is then not sure.
 __device__ __forceinline__ uint32_t place_key(float v, int place)
 {
@@ -240,7 +240,7 @@ __device__ __forceinline__ float key_value(uint32_t k)
 }
 
 template <int L, int V, int SLOTS>
-__device__ __forceinline__ bool route_fast(const RouteArgs& a, const float (&c)[V], int lane, float* s_score, float near, int (&id)[SLOTS])
+__device__ __forceinline__ bool route_fast(const RouteArgs& a, const float (&c)[V], int lane, float* s_score, float near, float size, int (&id)[SLOTS])
 {
     static_assert(V <= 16, "four bits of place");
     typedef Lanes<L> Ln;
@@ -252,8 +252,8 @@ __device__ __forceinline__ bool route_fast(const RouteArgs& a, const float (&c)[
     for (int i = 0; i < V; i++) k[i] = place_key(c[i], i);
     bool unsure = false;
     if (a.top_groups < a.groups) {
-        const int size = a.experts / a.groups, span = size / V;
-        if (span * V != size || (span & (span - 1)) != 0 || span > 16) return true;      // (no whole lanes, or no power of two of them)
+        const int experts = a.experts / a.groups, span = experts / V;
+        if (span * V != experts || (span & (span - 1)) != 0 || span > 16) return true;      // (no whole lanes, or no power of two of them)
         uint32_t x = 0, y = 0;          // the best and the second best
         auto add = [&](uint32_t v) {
             y = max(y, min(x, v));
@@ -281,7 +281,8 @@ __device__ __forceinline__ bool route_fast(const RouteArgs& a, const float (&c)[
         wave_fence();
         worst = Ln::all(worst, [](float p, float q) { return p < q ? p : q; });
         next = Ln::all(next, [](float p, float q) { return p > q ? p : q; });
-        unsure = next != -INFINITY && !apart(worst, next, 4.f);
+        // (a sum of two that cancel is cut as they are)
+        unsure = next != -INFINITY && !(near < 0.f || worst - next > 4.f * near + 0x1p-17f * fmaxf(size, fabsf(worst)));
         const bool mine = kept >> (l / span & 63) & 1;
 #pragma unroll
         for (int i = 0; i < V; i++) k[i] = mine ? k[i] : 0u;
@@ -369,13 +370,16 @@ __global__ __launch_bounds__(256) void route_forward_kernel(RouteArgs a)
     }
     // What two scores together may be off by: a sigmoid's, at most 1, six roundings of 2^-24, a softmax's, at most 1 / sum, as
     // many and those of a sum over lanes and their experts, 22 more; the biased one's another of both.  A bf16 logit is its key.
-    float near = -1.f;
-    if (!a.by_logit)
-        near = (a.sigmoid ? 0x1p-20f : 0x1p-18f / sum) + 0x1p-22f * Ln::all(most_bias, [](float x, float y) { return fmaxf(x, y); });
-    else if (a.f32)
+    float near = -1.f, size = 0.f;
+    if (!a.by_logit) {
+        most_bias = Ln::all(most_bias, [](float x, float y) { return fmaxf(x, y); });
+        near = (a.sigmoid ? 0x1p-20f : 0x1p-18f / sum) + 0x1p-22f * most_bias;
+        size = (a.sigmoid ? 1.f : 1.f / sum) + most_bias;
+    } else if (a.f32) {
         near = 0.f;
+    }
     int id[SLOTS];
-    if (__any(route_fast<L, V>(a, c, lane, reinterpret_cast<float*>(s_score[wave][sub]), near, id))) {
+    if (__any(route_fast<L, V>(a, c, lane, reinterpret_cast<float*>(s_score[wave][sub]), near, size, id))) {
         double d[V];
         if (a.by_logit) {
 #pragma unroll
@@ -665,7 +669,7 @@ static int route_check(const bs_route* r, const char* what)
     if (r->experts < 1 || r->experts > kMaxExperts) return set_error(BS_ERR_INVALID, "%s: experts must be in 1..%d, got %d", what, kMaxExperts, r->experts);
     if (r->top_k < 1 || r->top_k > std::min(kMaxTopK, r->experts))
         return set_error(BS_ERR_INVALID, "%s: top_k must be in 1..%d (at most experts), got %d", what, kMaxTopK, r->top_k);
-    if (r->tokens < 0 || r->tokens * r->top_k >= (1ll << 31)) return set_error(BS_ERR_INVALID, "%s: tokens*top_k must be in 0..2^31-1", what);
+    if (r->tokens < 0 || r->tokens >= (1ll << 31) || r->tokens * r->top_k >= (1ll << 31)) return set_error(BS_ERR_INVALID, "%s: tokens*top_k must be in 0..2^31-1", what);
     if (r->logits_type != BS_DT_BF16 && r->logits_type != BS_DT_F32) return set_error(BS_ERR_INVALID, "%s: logits dtype %d must be bf16 or fp32", what, r->logits_type);
     if (r->score != BS_SCORE_SOFTMAX && r->score != BS_SCORE_SIGMOID) return set_error(BS_ERR_INVALID, "%s: unknown score %d", what, r->score);
     if (r->groups < 1 || r->groups > 64 || r->experts % r->groups) return set_error(BS_ERR_INVALID, "%s: groups must be in 1..64 and divide experts, got %d", what, r->groups);
@@ -689,6 +693,26 @@ static RouteArgs route_args(const bs_route& r)
     return a;
 }
 
+// (a launch has fewer than 2^32 threads)
+template <typename K>
+static int launch_route(K* kernel, const RouteArgs& all, const char* what, hipStream_t st)
+{
+    const int tokens = all.experts <= 256 ? 16 : 4;     // of a workgroup
+    const int64_t slice = (int64_t)tokens << 23, size = all.f32 ? 4 : 2;
+    for (int64_t t = 0; t < all.tokens; t += slice) {
+        RouteArgs a = all;
+        a.tokens = std::min(slice, all.tokens - t);
+        a.logits = static_cast<const char*>(all.logits) + t * all.stride * size;
+        a.chosen += t * all.top_k;
+        if (all.weights) a.weights += t * all.top_k;
+        if (all.d_weights) a.d_weights += t * all.top_k, a.d_logits = static_cast<char*>(all.d_logits) + t * all.experts * size;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.tokens + tokens - 1) / tokens)), dim3(256), 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    }
+    return BS_OK;
+}
+
 }  // namespace bs
 
 using namespace bs;
@@ -703,12 +727,10 @@ extern "C" int bs_route_forward(const bs_route* route, float* weights, int32_t* 
         return set_error(BS_ERR_INVALID, "%s: null or misaligned result", what);
     RouteArgs a = route_args(*route);
     a.weights = weights, a.chosen = chosen;
-    const int E = a.experts, tokens = E <= 256 ? 16 : 4;        // of a workgroup
+    const int E = a.experts;
     auto* kernel = E <= 16 ? route_forward_kernel<16, 1> : E <= 64 ? route_forward_kernel<16, 4> : E <= 128 ? route_forward_kernel<16, 8>
                    : E <= 256 ? route_forward_kernel<16, 16> : E <= 512 ? route_forward_kernel<64, 8> : route_forward_kernel<64, 16>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.tokens + tokens - 1) / tokens)), dim3(256), 0, (hipStream_t)stream, a);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    return launch_route(kernel, a, what, (hipStream_t)stream);
 }
 
 extern "C" int bs_route_backward(const bs_route* route, const int32_t* chosen, const float* d_weights, void* d_logits, void* stream)
@@ -722,12 +744,10 @@ extern "C" int bs_route_backward(const bs_route* route, const int32_t* chosen, c
         return set_error(BS_ERR_INVALID, "%s: null or misaligned operand", what);
     RouteArgs a = route_args(*route);
     a.chosen = const_cast<int32_t*>(chosen), a.d_weights = d_weights, a.d_logits = d_logits;
-    const int E = a.experts, tokens = E <= 256 ? 16 : 4;        // of a workgroup
+    const int E = a.experts;
     auto* kernel = E <= 16 ? route_backward_kernel<16, 1> : E <= 64 ? route_backward_kernel<16, 4> : E <= 128 ? route_backward_kernel<16, 8>
                    : E <= 256 ? route_backward_kernel<16, 16> : E <= 512 ? route_backward_kernel<64, 8> : route_backward_kernel<64, 16>;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.tokens + tokens - 1) / tokens)), dim3(256), 0, (hipStream_t)stream, a);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+    return launch_route(kernel, a, what, (hipStream_t)stream);
 }
 
 static int64_t plan_blocks(int64_t pairs)

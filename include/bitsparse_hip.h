@@ -743,8 +743,8 @@ int bs_join_drop_backward(const bs_join* args, const bs_join_grads* grads, const
  * experts]; c = s + bias; of `groups` groups of consecutive experts the
  * top_groups with the largest sum of their group_best largest c are kept, and
  * of their experts the top_k largest c are chosen, the largest first.  The
- * choice is between 64-bit values; of equal ones the lowest index goes first
- * and a NaN before all.  weights = scale * s / sum(s of the chosen)
+ * choice is between 64-bit values (between the logits where the order is
+ * theirs); of equal ones the lowest index goes first and a NaN before all.  weights = scale * s / sum(s of the chosen)
  * (renormalize; 0 where that sum is 0) or scale * s.  An expert whose logit or
  * c is -infinity is not chosen; a choice that is left without an expert is -1
  * with weight 0.  weights and chosen: [tokens, top_k], contiguous.
@@ -787,7 +787,8 @@ int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts, int32_t* o
  * taken as the nearest in it.  Results are contiguous; dx is bf16 or, for the
  * sum over a token's rows that follows where they were gathered, fp32 (dx_type).  Operands have rows at
  * 16-byte addresses, a multiple of 8 elements apart, and zeros from their
- * last column to the next multiple of 8 (bs_pad_rows makes such rows).
+ * last column to the next multiple of 8 (bs_pad_rows makes such rows); of
+ * bs_expert_linear an expert's W and gathered tokens span less than 4 GiB.
  * BS_ACT_RELU2: bf16(bf16(r r) act_k) of r = bf16(relu(.)), as the ReLU^2
  * layers form it; BS_ACT_RELU: r.
  */

@@ -70,7 +70,7 @@ def test_join_with_dropout_refusals():
 
 ROUTE = dict(tokens=4, experts=16, top_k=2, logits=FAKE, logits_type=F32, logits_stride=16, groups=1, top_groups=1, group_best=1, scale=1.0)
 ROUTE_BAD = [(dict(experts=0), "experts"), (dict(experts=1025), "experts"), (dict(top_k=0), "top_k"), (dict(top_k=17), "top_k"),
-             (dict(experts=100, top_k=65), "top_k"), (dict(tokens=-1), "tokens"), (dict(tokens=1 << 30), "2^31"), (dict(logits_type=1), "dtype"),
+             (dict(experts=100, top_k=65), "top_k"), (dict(tokens=-1), "tokens"), (dict(tokens=1 << 30), "2^31"), (dict(tokens=1 << 62, experts=4), "2^31"), (dict(logits_type=1), "dtype"),
              (dict(score=2), "score"), (dict(groups=0), "groups"), (dict(groups=3), "groups"), (dict(experts=1024, groups=128), "groups"),
              (dict(groups=4, top_groups=5), "top_groups"), (dict(groups=4, top_groups=0), "top_groups"), (dict(group_best=3), "group_best"),
              (dict(groups=8, top_groups=1, top_k=3), "more than"), (dict(logits_stride=-1), "stride"), (dict(logits=None), "null"),
@@ -136,6 +136,11 @@ def test_products_and_order():
     _refused(dw(), "order")
     forward, _, _ = _products(dict(order=FAKE, tokens=(1 << 31) - 1), {})
     _refused(forward(), "4 GiB")
+    forward, _, _ = _products({}, dict(w_stride=1 << 20, out=4096))
+    _refused(forward(), "4 GiB")
+    # 2^31 / 256 tiles of rows, of which any size of tile has two or more over the columns
+    forward, _, _ = _products(dict(rows=(1 << 31) - 1), dict(x_stride=8, w_stride=8, inn=8, out=264))
+    _refused(forward(), "tiles")
     L = _lib.load()
     e = Experts(rows=32, tokens=16, experts=4, top_k=2, offsets=FAKE)
     _refused(L.bs_expert_linear(C.byref(e), FAKE, 64, FAKE, 64, 64, 64, 3, 1.0, FAKE, None), "activation")

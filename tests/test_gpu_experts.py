@@ -191,6 +191,23 @@ def test_route_of_many_equal_and_close_values(E, k, groups, top_groups, best, sc
     assert (ids.sort(-1).values.diff(dim=-1) > 0).all()
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_of_groups_whose_best_cancel(score):
+    """Biases that take a group's two best far apart on both sides of 0: the sums that decide are small and close together, the
+    values that they are of are not."""
+    g = _gen(17)
+    T, E, groups = 4096, 64, 4
+    l = 4e-5 * _rn(g, T, E)
+    b = torch.full((E,), -torch.inf, device="cuda")
+    b[::16], b[5::16] = 10.0, -10.0
+    w, ids = _mod().route(l, 2, score=score, bias=b, groups=groups, top_groups=1, group_best=2)
+    _, want, s = _route(l, 2, score, b, groups, 1, 2, True, 1.0)
+    both = s[:, ::16] + s[:, 5::16]
+    top = both.topk(2, -1).values
+    sure = top[:, 0] - top[:, 1] > 2.0 ** -47           # (four roundings of 10 in 64 bits are 2^-49 each)
+    assert sure.float().mean() > 0.99 and torch.equal(ids[sure].long(), want[sure])
+
+
 def test_route_masked_logits():
     m = _mod()
     l = _rn(_gen(1), 6, 20)

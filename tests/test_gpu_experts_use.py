@@ -119,6 +119,85 @@ def test_gathered_tokens_past_4_gib():
         assert ((dW[e].double() - a.T @ b).abs() <= tol(a.T @ b, a.T.abs() @ b.abs(), 6)).all()
 
 
+def _long_plan(T):
+    from bitsparse_amd.experts import ExpertPlan
+    at = torch.arange(T, device="cuda", dtype=torch.int32)
+    at[T - 2:] = -1                                                         # two without an expert
+    return ExpertPlan(torch.tensor([0, T - 2], device="cuda", dtype=torch.int32), at, at[:, None].clone())
+
+
+@pytest.mark.parametrize("kept", [False, True])
+def test_sums_of_more_tokens_than_a_launch_has(kept):
+    """2^24 workgroups of 256 threads are past a launch's 2^32 threads."""
+    from bitsparse_amd.experts import expert_combine
+    T, D = 2 ** 24 + 3, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    y = torch.randn(T, D, generator=g, device="cuda").to(BF).requires_grad_()
+    w = torch.rand(T, 1, generator=g, device="cuda").requires_grad_(kept)
+    go = torch.randn(T, D, generator=g, device="cuda").to(BF)
+    out = expert_combine(y, w, _long_plan(T))
+    want = (y.detach().float() * w.detach()).to(BF)                         # (one product, rounded twice on both sides)
+    want[T - 2:] = 0
+    right = torch.equal(out, want)
+    assert right
+    got = torch.autograd.grad(out, [y, w] if kept else [y], go)
+    want = (go.float() * w.detach()).to(BF)
+    want[T - 2:] = 0
+    right = torch.equal(got[0], want)
+    assert right
+    if kept:
+        a, b = go.double(), y.detach().double()
+        a[T - 2:] = 0
+        assert ((got[1][:, 0].double() - (a * b).sum(1)).abs() <= (D + 1) * 2.0 ** -24 * (a * b).abs().sum(1)).all()
+
+
+def test_a_block_of_more_rows_than_a_launch_has():
+    """Against the same tokens by themselves: products over 8 columns and sums of a row have the same bits in both."""
+    from bitsparse_amd.experts import ExpertPlan, ExpertsRelu2
+    T, D = 2 ** 24 + 3, 8
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(T, D, generator=g, device="cuda").to(BF)
+    w = torch.rand(T, 1, generator=g, device="cuda")
+    go = torch.randn(T, D, generator=g, device="cuda").to(BF)
+    W1, W2 = (torch.randn(1, D, D, generator=g, device="cuda").to(BF) for _ in range(2))
+
+    def step(at):
+        leaves = [t[at].clone().requires_grad_() for t in (x, w)]
+        n = leaves[0].shape[0]
+        order = torch.arange(n, device="cuda", dtype=torch.int32)
+        plan = ExpertPlan(torch.tensor([0, n], device="cuda", dtype=torch.int32), order, order[:, None].clone())
+        out = ExpertsRelu2.apply(leaves[0], W1, W2, leaves[1], plan)
+        return out.detach(), *torch.autograd.grad(out, leaves, go[at])
+
+    whole = step(slice(None))
+    for at in (slice(0, 40), slice(2 ** 22 - 20, 2 ** 22 + 20), slice(2 ** 23 - 20, 2 ** 23 + 20), slice(T - 40, T)):
+        for a, b in zip(whole, step(at)):
+            assert torch.equal(a[at], b)
+
+
+def test_routing_of_more_tokens_than_a_launch_has():
+    from bitsparse_amd.experts import route
+    T = 2 ** 28 + 5
+    l = torch.randint(-8, 9, (T, 2), device="cuda", dtype=torch.int8).to(BF).requires_grad_()
+    w, ids = route(l, 1, renormalize=False)
+    right = torch.equal(ids[:, 0] == 1, l[:, 1] > l[:, 0])
+    assert right                                # (nothing that a failure would print element by element)
+    gap = (l[:, 0] - l[:, 1]).abs().detach()
+    want = 1 / (1 + torch.exp(-gap.float()))
+    # (a few roundings of 2^-24 each on both sides)
+    assert (w[:, 0].detach() - want).abs().max() < 16 * 2.0 ** -24
+    del want, ids
+    dl, = torch.autograd.grad(w, l, torch.ones_like(w))
+    del w
+    for at in (slice(0, 1000), slice(2 ** 27 - 500, 2 ** 27 + 500), slice(T - 1000, T)):
+        v = l[at].detach().double()
+        s = torch.softmax(v, -1)
+        full = s[:, 0] * s[:, 1] * torch.where(v[:, 1] > v[:, 0], -1.0, 1.0)
+        want = torch.stack([full, -full], 1)
+        # (s to 8 roundings, the difference ds - s to as many of 1)
+        assert ((dl[at].double() - want).abs() <= 2.0 ** -8 * want.abs() * 1.02 + 16 * 2.0 ** -24 * s).all()
+
+
 def test_dropout_past_32_bits():
     from bitsparse_amd.dropout import Dropout, dropout
     T, D = 3, 2 ** 30 + 9
