@@ -573,9 +573,10 @@ static int launch_few(ExpertGemm g, const char* what, hipStream_t st)
 }
 
 // What a product takes on tiles of one size, in us: rounds of as many as are
-// resident at once, each its steps and a start and an end.  The host knows how
-// many rows there are, not how they lie: half a tile is left over for each
-// expert, and the longest of dW's sums has 1.4 times the mean's steps.
+// resident at once, each its steps and a start and an end, or reading the
+// weights (of 2 to 64 rows an expert: 4.1 TB/s, on larger tiles 3.2 to 3.9).  The
+// host knows how many rows there are, not how they lie: half a tile is left over for each expert, of less than three quarters
+// of a tile one in 20 has two, and the longest of dW's sums has 1.4 times the mean's steps.
 static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_once, double step)
 {
     const double columns = (g.n + tn - 1) / tn;
@@ -583,8 +584,10 @@ static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_on
         const double tiles = (double)g.experts * ((g.m + tm - 1) / tm) * columns, time = (double)g.rows / g.experts / kBK * step;
         return std::max(1.0, tiles / at_once) * (time + 5.0) + 0.4 * time;
     }
-    const double tiles = ((double)g.rows / tm + 0.5 * (double)std::min<int64_t>(g.experts, g.rows)) * columns;
-    return std::ceil(std::max(1.0, tiles) / at_once) * ((double)g.k / kBK * step + 5.0);
+    const double experts = (double)std::min<int64_t>(g.experts, g.rows), each = (double)g.rows / experts / tm;
+    const double tiles = experts * (each <= 0.25 ? 1.0 : each < 0.75 ? 1.05 * std::max(1.0, each + 0.5) : each + 0.5) * columns;
+    const double weights = experts * g.n * g.k * 2 / (tm == 64 ? 4.1e6 : 3.6e6);
+    return std::max(weights, std::ceil(tiles / at_once) * ((double)g.k / kBK * step + 5.0));
 }
 
 // Forward for up to two rows an expert: expert_few_kernel (8 rows of 64 experts of 4096 -> 1024 13.2 us, on tiles of 64 x 64
@@ -596,6 +599,9 @@ static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_on
 //   32768, 16, 2048 -> 4096         976 / 929 / 996 621 / 570 / 572 559 / 532 / - 489 / 497 / 501
 //   16384,  4,  512 -> 1024          49 / 38 / 40    34 / 31 / 63   30 / 26 / -   36 / 27 / 116
 //     512,  8, 2048 -> 2048          22 / 22 / 41    27 / 24 / 21   31 / 30 / -   42 / 42 / 23
+//    2048, 64, 4096 -> 1024         132 / 116 / 278  171 / 122 / 124     -         138 / 127 / 126
+//    2048, 256, 2048 ->  512        122 / 137 / 280  156 / 131 / 123     -         141 / 150 / 129
+//    8192, 64, 4096 -> 1024         192 / 194 / 347  174 / 159 / 165     -         217 / 164 / 158
 template <int KIND, bool GATHER>
 static int launch_kind(const ExpertGemm& g, const char* what, hipStream_t st)
 {
@@ -604,11 +610,12 @@ static int launch_kind(const ExpertGemm& g, const char* what, hipStream_t st)
     const double small = tile_time(g, KIND, 64, 64, kCus * 2, 0.45), middle = tile_time(g, KIND, 128, 128, kCus * 2, 0.95),
                  wide = tile_time(g, KIND, 192, 128, kCus * 2, 1.3), large = tile_time(g, KIND, 256, 256, kCus, 1.55);
     const double best = std::min(std::min(small, middle), KIND == kDw ? large : std::min(wide, large));
-    if (best == large) return launch_gemm<KIND, GATHER, 2, 4, 8, 4, 2, true>(g, what, st);
+    // (of equals, bound by the weights, the smallest)
+    if (best == small) return launch_gemm<KIND, GATHER, 2, 2, 2, 2, 4, false>(g, what, st);
+    if (best == middle) return launch_gemm<KIND, GATHER, 2, 2, 4, 4, 2, false>(g, what, st);
     if constexpr (KIND != kDw)
         if (best == wide) return launch_gemm<KIND, GATHER, 2, 2, 6, 4, 2, false>(g, what, st);
-    if (best == middle) return launch_gemm<KIND, GATHER, 2, 2, 4, 4, 2, false>(g, what, st);
-    return launch_gemm<KIND, GATHER, 2, 2, 2, 2, 4, false>(g, what, st);
+    return launch_gemm<KIND, GATHER, 2, 4, 8, 4, 2, true>(g, what, st);
 }
 
 static int experts_check(const bs_experts* x, int64_t in, int64_t out, const char* what)
