@@ -576,7 +576,8 @@ static int launch_few(ExpertGemm g, const char* what, hipStream_t st)
 // resident at once, each its steps and a start and an end, or reading the
 // weights (of 2 to 64 rows an expert: 4.1 TB/s, on larger tiles 3.2 to 3.9).  The
 // host knows how many rows there are, not how they lie: half a tile is left over for each expert, of less than three quarters
-// of a tile one in 20 has two, and the longest of dW's sums has 1.4 times the mean's steps.
+// of a tile one in 20 has two (one alone has them all: 4096 rows 16384 -> 4096 425 us, 538 on the tile for half a tile more), and
+// the longest of dW's sums has 1.4 times the mean's steps.
 static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_once, double step)
 {
     const double columns = (g.n + tn - 1) / tn;
@@ -585,7 +586,7 @@ static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_on
         return std::max(1.0, tiles / at_once) * (time + 5.0) + 0.4 * time;
     }
     const double experts = (double)std::min<int64_t>(g.experts, g.rows), each = (double)g.rows / experts / tm;
-    const double tiles = experts * (each <= 0.25 ? 1.0 : each < 0.75 ? 1.05 * std::max(1.0, each + 0.5) : each + 0.5) * columns;
+    const double tiles = experts * columns * (experts == 1 ? std::ceil(each) : each <= 0.25 ? 1.0 : each < 0.75 ? 1.05 * std::max(1.0, each + 0.5) : each + 0.5);
     const double weights = experts * g.n * g.k * 2 / (tm == 64 ? 4.1e6 : 3.6e6);
     return std::max(weights, std::ceil(tiles / at_once) * ((double)g.k / kBK * step + 5.0));
 }
