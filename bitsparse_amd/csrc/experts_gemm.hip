@@ -10,11 +10,10 @@
 // tiles of ragged groups are found on the device, so the host knows nothing
 // of the routing and waits for nothing.
 //
-// Bound by the products: 32768 rows of 16 experts, 2048 -> 4096, 511 us
-// forward, 519 dx, 506 dW, 1.06 to 1.09 PFLOP/s, where the library's product of 8192^3
-// reaches 1.46 (of one expert, 4096 x 4096 x 16384: 1.11 and 1.26); an eighth of that is
-// the groups' part tiles and the last round's idle CUs.  Short sums pay for their starts and ends: 16384 rows
-// of 8 experts, 768 -> 2048, 0.63 to 0.79 PFLOP/s.
+// Bound by the products: 32768 rows of 16 experts, 2048 -> 4096, 486 us
+// forward, 489 dx, 504 dW, 1.09 to 1.13 PFLOP/s; of one expert with 4096 rows, 16384 -> 4096, 1.28 to 1.39, the
+// library's 1.29.  The difference is the groups' part tiles, the last round's idle CUs and, of
+// shorter sums, the tiles' starts and ends: 16384 rows of 8 experts, 768 -> 2048, 0.79 to 0.94 PFLOP/s.
 #include <algorithm>
 #include <cmath>
 
@@ -44,6 +43,7 @@ struct ExpertGemm {
     int64_t c_expert;
     int m, n, k;                                // of one expert's product; m or k of the rows is -1
     int tiles_m, tiles_n, panel;
+    int rows_of_tiles;                          // as many as there may be
     int act;
     float act_k;
     int stream;                                 // results past the caches' size, stored around them
@@ -126,25 +126,44 @@ __device__ __forceinline__ int wave_scan(int v)
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);     // last lane of row 1 into rows 2, 3
     return v;
 }
-__device__ __forceinline__ Group find_group(const ExpertGemm& g, int tile, int size)
-{
-    const int lane = threadIdx.x & 63;
-    int64_t before = 0;     // (64 experts' tiles are below 2^31; those of offsets that overlap add up past it)
-    for (int e0 = 0; e0 < g.experts; e0 += 64) {
-        const int e = e0 + lane;
-        const int from = group_bound(g, min(e, g.experts)), to = max(from, group_bound(g, min(e + 1, g.experts)));
-        const int tiles = (int)((uint32_t)(to - from + size - 1) / (uint32_t)size);
-        const int sum = wave_scan(tiles);
-        const uint64_t past = __ballot(before + sum > tile);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            return {e0 + at, (int64_t)__builtin_amdgcn_readlane(from, at), (int64_t)__builtin_amdgcn_readlane(to, at),
-                    tile - before - __builtin_amdgcn_readlane(sum - tiles, at)};
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
+// How `size` rows a tile lie over the experts
+struct Groups {
+    int from, to, sum;          // of lane e's expert e < 64, and the tiles of those up to it
+    int64_t all;                // tiles, with those of the rows behind
+    __device__ __forceinline__ void load(const ExpertGemm& g, int e, int size)
+    {
+        from = group_bound(g, min(e, g.experts)), to = max(from, group_bound(g, min(e + 1, g.experts)));
+        sum = wave_scan((int)((uint32_t)(to - from + size - 1) / (uint32_t)size));      // (64 experts' tiles are below 2^31)
     }
-    return {-1, (int64_t)group_bound(g, g.experts), g.rows, tile - before};
-}
+    __device__ __forceinline__ Groups(const ExpertGemm& g, int size)
+    {
+        const int lane = threadIdx.x & 63;
+        all = (g.rows - group_bound(g, g.experts) + size - 1) / size;
+        for (int e = 64; e < g.experts; e += 64) {
+            load(g, e + lane, size);
+            all += __builtin_amdgcn_readlane(sum, 63);
+        }
+        load(g, lane, size);
+        all += __builtin_amdgcn_readlane(sum, 63);
+    }
+    // (once)
+    __device__ __forceinline__ Group find(const ExpertGemm& g, int tile, int size) const
+    {
+        Groups now = *this;
+        int64_t before = 0;     // (the tiles of offsets that overlap add up past 2^31)
+        for (int e0 = 0; e0 < g.experts; e0 += 64) {
+            if (e0) now.load(g, e0 + (threadIdx.x & 63), size);
+            const uint64_t past = __ballot(before + now.sum > tile);
+            if (past) {
+                const int at = __builtin_ctzll(past), from_ = __builtin_amdgcn_readlane(now.from, at), to_ = __builtin_amdgcn_readlane(now.to, at);
+                const int tiles = (int)((uint32_t)(to_ - from_ + size - 1) / (uint32_t)size);
+                return {e0 + at, from_, to_, tile - before - (__builtin_amdgcn_readlane(now.sum, at) - tiles)};
+            }
+            before += __builtin_amdgcn_readlane(now.sum, 63);
+        }
+        return {-1, (int64_t)group_bound(g, g.experts), g.rows, tile - before};
+    }
+};
 
 // The expert with the rank'th most rows, of up to 8: dW's longest sums begin first and its shortest fill the end (16384 rows of
 // 8 experts 768 -> 2048 70.5 -> 62.2 us).  More experts' shorter sums even out by themselves (of 16 no change or 33 -> 36 us,
@@ -209,10 +228,10 @@ __device__ __forceinline__ void store_four(const ExpertGemm& g, int64_t row, int
     }
 }
 
-// WGM x WGN waves, each 16 IM x 16 JN results.  AHEAD: fragments are read ahead of the barrier, for a workgroup that has a
-// CU to itself.
+// The results from (c_row, c_col) on of `grp`, rows up to c_rows: WGM x WGN waves, each 16 IM x 16 JN of them.  AHEAD:
+// fragments are read ahead of the barrier, for a workgroup that has a CU to itself.
 template <int KIND, bool GATHER, int WGM, int WGN, int IM, int JN, int STAGES, bool AHEAD>
-__global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm g)
+__device__ __forceinline__ void gemm_tile(const ExpertGemm& g, const Group& grp, int64_t c_row, int64_t c_rows, int64_t c_col, int64_t k_total, char* s_mem)
 {
     constexpr int WAVES = WGM * WGN, TM = 16 * IM * WGM, TN = 16 * JN * WGN;
     constexpr bool A_ALONG = KIND != kDw, B_ALONG = KIND == kForward;
@@ -220,35 +239,10 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
     constexpr int A_BYTES = TM * kRowBytes, B_BYTES = TN * kRowBytes, STAGE = A_BYTES + B_BYTES;
     constexpr int LA = TM / 8 / WAVES, LB = TN / 8 / WAVES;     // loads of a wave, 1 KiB each
     static_assert(LA * 8 * WAVES == TM && LB * 8 * WAVES == TN, "a stage is whole loads of every wave");
-    static_assert(STAGES * STAGE <= 160 * 1024 && (!AHEAD || STAGES == 2), "LDS budget");
-    constexpr int AT_ONCE = kCus * (160 * 1024 / (STAGES * STAGE));
-    __shared__ __attribute__((aligned(16))) char s_mem[STAGES * STAGE];
+    static_assert(!AHEAD || STAGES == 2, "two stages in turn");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
-
-    // Workgroups go round the XCDs in turn: of as many as are resident at once each XCD takes a run, in panels of g.panel rows
-    // of tiles, whose neighbours share rows of A and of B.
-    int id = (int)blockIdx.x;
-    if (g.panel > 1) {
-        const int group = id / AT_ONCE * AT_ONCE;
-        if (group + AT_ONCE <= (int)gridDim.x) id = group + (id - group) % kXcds * (AT_ONCE / kXcds) + (id - group) / kXcds;
-    }
-    const int panel = id / (g.panel * g.tiles_n), in_panel = id - panel * g.panel * g.tiles_n;
-    const int high = min(g.panel, (int)gridDim.x / g.tiles_n - panel * g.panel);
-    const int tm = panel * g.panel + in_panel % high, tn = in_panel / high;
-    Group grp;
-    int64_t c_row, c_rows, k_total;
-    if constexpr (KIND == kDw) {
-        const int e = by_length(g, tm / g.tiles_m);
-        const int from = group_bound(g, e);
-        grp = {e, from, max(from, group_bound(g, e + 1)), tm % g.tiles_m};
-        c_row = grp.tile * TM, c_rows = g.m, k_total = grp.end - grp.first;
-    } else {
-        grp = find_group(g, tm, TM);
-        c_row = grp.first + grp.tile * TM, c_rows = grp.end, k_total = grp.expert < 0 ? 0 : g.k;
-    }
-    if (c_row >= c_rows) return;
-    const int64_t c_col = (int64_t)tn * TN;
+    if (c_row >= c_rows || c_col >= g.n) return;
 
     // where this lane's parts of a stage come from
     uint32_t a_off[LA], b_off[LB];
@@ -479,6 +473,55 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
     }
 }
 
+// id of `all` tiles, `tiles_n` to a row of them: in panels of g.panel rows
+__device__ __forceinline__ void panel_tile(const ExpertGemm& g, int id, int rows, int& tm, int& tn)
+{
+    const int panel = id / (g.panel * g.tiles_n), in_panel = id - panel * g.panel * g.tiles_n;
+    const int high = min(g.panel, rows - panel * g.panel);
+    tm = panel * g.panel + in_panel % high, tn = in_panel / high;
+}
+// Workgroups go round the XCDs in turn: of `at_once`, as many as are resident, each XCD takes a run
+__device__ __forceinline__ int xcd_run(int id, int all, int at_once)
+{
+    const int group = id / at_once * at_once;
+    return group + at_once <= all ? group + (id - group) % kXcds * (at_once / kXcds) + (id - group) / kXcds : id;
+}
+
+template <int KIND, bool GATHER, int WGM, int WGN, int IM, int JN, int STAGES, bool AHEAD>
+__global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm g)
+{
+    constexpr int TM = 16 * IM * WGM, TN = 16 * JN * WGN, LDS = STAGES * (TM + TN) * kRowBytes;
+    static_assert(LDS <= 160 * 1024, "LDS budget");
+    constexpr int AT_ONCE = kCus * (160 * 1024 / LDS);
+    __shared__ __attribute__((aligned(16))) char s_mem[LDS];
+    int tm, tn;
+    if constexpr (KIND == kDw) {
+        panel_tile(g, xcd_run((int)blockIdx.x, (int)gridDim.x, AT_ONCE), g.rows_of_tiles, tm, tn);
+        const int e = by_length(g, tm / g.tiles_m), from = group_bound(g, e);
+        const Group grp = {e, from, max(from, group_bound(g, e + 1)), tm % g.tiles_m};
+        gemm_tile<KIND, GATHER, WGM, WGN, IM, JN, STAGES, AHEAD>(g, grp, grp.tile * TM, g.m, (int64_t)tn * TN, grp.end - grp.first, s_mem);
+    } else {
+        const Groups groups(g, TM);
+        const int rows = AHEAD ? (int)min((int64_t)g.rows_of_tiles, groups.all) : g.rows_of_tiles, all = rows * g.tiles_n;
+        // What is left of the last round: up to a quarter of one in quarters of tiles, up to half in halves, so that it takes
+        // no whole round (16384 rows of 8 experts 768 -> 2048 gathered 75 -> 65 us, 32768 of 16 2048 -> 4096 494 -> 486).
+        const int left = AHEAD ? all % AT_ONCE : 0, parts = left == 0 || left > AT_ONCE / 2 ? 1 : left > AT_ONCE / 4 ? 2 : 4;
+        const int id = (int)blockIdx.x, whole = parts == 1 ? all : all - left;
+        const int tile = id < whole ? xcd_run(id, whole, AT_ONCE) : whole + (id - whole) / parts, part = id < whole ? 0 : (id - whole) % parts;
+        if (tile >= all) return;
+        panel_tile(g, tile, rows, tm, tn);
+        const Group grp = groups.find(g, tm, TM);
+        const int64_t c_row = grp.first + grp.tile * TM, c_col = (int64_t)tn * TN, k = grp.expert < 0 ? 0 : g.k;
+        if constexpr (AHEAD) {
+            if (id >= whole && parts == 4)
+                return gemm_tile<KIND, GATHER, WGM, WGN, IM / 2, JN / 2, STAGES, AHEAD>(g, grp, c_row + part / 2 * (TM / 2), grp.end, c_col + part % 2 * (TN / 2), k, s_mem);
+            if (id >= whole && parts == 2)
+                return gemm_tile<KIND, GATHER, WGM, WGN, IM, JN / 2, STAGES, AHEAD>(g, grp, c_row, grp.end, c_col + part * (TN / 2), k, s_mem);
+        }
+        gemm_tile<KIND, GATHER, WGM, WGN, IM, JN, STAGES, AHEAD>(g, grp, c_row, grp.end, c_col, k, s_mem);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Forward for few rows an expert: bound by reading the experts' weights.  A
 // workgroup has 16 columns and up to 32 rows, each of its eight waves an eighth
@@ -536,7 +579,7 @@ __global__ __launch_bounds__(512) void expert_few_kernel(ExpertGemm g)
 {
     __shared__ __attribute__((aligned(16))) f32x4 s_sum[8][2][64];
     const int tn = (int)blockIdx.x % g.tiles_n, tm = (int)blockIdx.x / g.tiles_n;
-    const Group grp = find_group(g, tm, kFewRows);
+    const Group grp = Groups(g, kFewRows).find(g, tm, kFewRows);
     const int64_t c_row = grp.first + grp.tile * kFewRows, c_rows = min(grp.end, c_row + kFewRows);
     if (c_row >= c_rows) return;
     if (c_rows - c_row <= 16)
@@ -556,8 +599,11 @@ static int launch_gemm(ExpertGemm g, const char* what, hipStream_t st)
     g.panel = 8;
     // (32768 rows of 16 experts 2048 -> 4096 510 us without, 489 with; dW of 64 experts 1024 -> 2048 147 and 110)
     g.stream = use_nontemporal((KIND == kDw ? (int64_t)g.experts * g.m : g.rows) * g.n * (KIND == kDx && g.c_f32 ? 4 : 2));
-    if (tiles_m * g.tiles_n >= (1ll << 32) / (64 * WGM * WGN)) return set_error(BS_ERR_INVALID, "%s: more tiles than a launch's 2^32 threads hold", what);
-    hipLaunchKernelGGL((expert_gemm_kernel<KIND, GATHER, WGM, WGN, IM, JN, STAGES, AHEAD>), dim3((uint32_t)(tiles_m * g.tiles_n)), dim3(64 * WGM * WGN), 0, st, g);
+    // (AHEAD: and the parts of the last round's tiles)
+    const int64_t blocks = tiles_m * g.tiles_n + (AHEAD && KIND != kDw ? 3 * kCus / 4 : 0);
+    g.rows_of_tiles = (int)tiles_m;
+    if (blocks >= (1ll << 32) / (64 * WGM * WGN)) return set_error(BS_ERR_INVALID, "%s: more tiles than a launch's 2^32 threads hold", what);
+    hipLaunchKernelGGL((expert_gemm_kernel<KIND, GATHER, WGM, WGN, IM, JN, STAGES, AHEAD>), dim3((uint32_t)blocks), dim3(64 * WGM * WGN), 0, st, g);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }
@@ -588,16 +634,19 @@ static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_on
     const double experts = (double)std::min<int64_t>(g.experts, g.rows), each = (double)g.rows / experts / tm;
     const double tiles = experts * columns * (experts == 1 ? std::ceil(each) : each <= 0.25 ? 1.0 : each < 0.75 ? 1.05 * std::max(1.0, each + 0.5) : each + 0.5);
     const double weights = experts * g.n * g.k * 2 / (tm == 64 ? 4.1e6 : 3.6e6);
-    return std::max(weights, std::ceil(tiles / at_once) * ((double)g.k / kBK * step + 5.0));
+    // (the last round in parts of the largest tiles: its steps take 0.35 and 0.65 of a tile's)
+    const double rounds = std::floor(tiles / at_once), left = tiles / at_once - rounds, steps = (double)g.k / kBK * step;
+    const double last = left == 0.0 ? 0.0 : steps * (tm < 256 || left > 0.5 ? 1.0 : left > 0.25 ? 0.65 : 0.35) + 5.0;
+    return std::max(weights, rounds * (steps + 5.0) + last);
 }
 
 // Forward for up to two rows an expert: expert_few_kernel (8 rows of 64 experts of 4096 -> 1024 13.2 us, on tiles of 64 x 64
 // 20.9; 64 rows 50 and 65; 32 rows of 8 experts of 4096 -> 2048 24.3 and 22.0).  Else the tile whose time is least by
 // tile_time (measured in us, forward / dx / dW, x gathered in forward):
 //   rows, experts, in -> out           64 x 64       128 x 128     192 x 128   256 x 256
-//   16384,  8,  768 -> 2048         119 / 91 / 95    78 / 65 / 72   73 / 72 / -   72 / 55 / 74
+//   16384,  8,  768 -> 2048         119 / 91 / 95    78 / 65 / 72   73 / 72 / -   65 / 55 / 74
 //   16384,  8, 2048 ->  768          92 / 102 / 93   68 / 66 / 68   73 / 59 / -   56 / 68 / 73
-//   32768, 16, 2048 -> 4096         976 / 929 / 996 621 / 570 / 572 559 / 532 / - 489 / 497 / 501
+//   32768, 16, 2048 -> 4096         976 / 929 / 996 621 / 570 / 572 559 / 532 / - 486 / 489 / 504
 //   16384,  4,  512 -> 1024          49 / 38 / 40    34 / 31 / 63   30 / 26 / -   36 / 27 / 116
 //     512,  8, 2048 -> 2048          22 / 22 / 41    27 / 24 / 21   31 / 30 / -   42 / 42 / 23
 //    2048, 64, 4096 -> 1024         132 / 116 / 278  171 / 122 / 124     -         138 / 127 / 126

@@ -296,6 +296,14 @@ def test_linear(T, k, E, D, N, gather):
 
 
 @pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("T,k,E,D,N", [
+    (4200, 1, 1, 136, 4104), (4360, 1, 1, 72, 4872), (4096, 2, 2, 200, 2312), (5000, 1, 1, 3912, 88), (9000, 2, 70, 520, 1032), (4700, 1, 1, 131, 4099)])
+def test_linear_of_last_rounds_in_parts(T, k, E, D, N, gather):
+    """A few tiles of 256 x 256 more than there are CUs: quarters and halves of them, some behind the last row and column."""
+    _check_linear(T, k, E, D, N, gather)
+
+
+@pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("T,k,E,D,N", [(1, 1, 1, 1, 1), (5, 2, 3, 7, 9), (130, 3, 5, 201, 133), (260, 2, 37, 501, 333), (33, 1, 2, 63, 65), (40, 2, 6, 130, 258)])
 def test_linear_odd(T, k, E, D, N, gather):
     _check_linear(T, k, E, D, N, gather, lost=0.2)
