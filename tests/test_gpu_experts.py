@@ -341,6 +341,25 @@ def test_linear_rows_behind_the_last_expert():
     assert torch.isfinite(y).all() and torch.isfinite(dt).all() and torch.isfinite(dW).all() and (dt[120:] == 0).all()
 
 
+@pytest.mark.parametrize("kept", [3052, 4355, 0])
+def test_rows_behind_among_the_last_rounds_parts(kept):
+    """Rows of no expert whose tiles are among those that go out in parts; results where a freed tensor of ones was."""
+    m, g = _mod(), _gen(kept)
+    T, D, N = 4360, 72, 4872
+    ids = torch.zeros(T, 1, dtype=torch.int32, device="cuda")
+    ids[torch.randperm(T, generator=g, device="cuda")[kept:]] = -1
+    plan = m.plan_experts(ids, 1)
+    order = plan.order[:kept].long()
+    x, W = _rn(g, T, D).to(BF), _rn(g, 1, N, D).to(BF)
+    x[ids[:, 0] < 0] = torch.nan
+    del_me = torch.ones(T, N, dtype=BF, device="cuda")
+    del del_me
+    y = m.expert_linear(x, W, plan, gather=True)
+    want = x[order].double() @ W[0].double().T
+    _close(y[:kept], want, x[order].double().abs() @ W[0].double().abs().T, D, "y")
+    assert (y[kept:] == 0).all()
+
+
 def test_linear_stays_inside_its_expert():
     """NaN weights and rows of one expert reach no other one's results."""
     m, g = _mod(), _gen(6)
