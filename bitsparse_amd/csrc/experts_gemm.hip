@@ -329,6 +329,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertGemm& g, const Group& grp,
     // all of the step's stage is in registers, so that it is loaded again, and the next step's stage has come, a whole
     // step after its loads.
     constexpr int MEET = IM / 4;
+    static_assert(!AHEAD || LOADS <= 2 * IM - MEET, "a place in the loop for each load");
     bf16x8 fa[IM], fb[2][JN];
     auto read_a = [&](int stage, int i, int k0) { fa[i] = read_fragment<TM, A_ALONG>(s_mem + stage * STAGE, wm * 16 * IM + 16 * i, k0, lane); };
     auto read_b = [&](int stage, int j, int k0) {
