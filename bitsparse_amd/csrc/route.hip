@@ -223,7 +223,7 @@ __device__ __forceinline__ void route_exact(const RouteArgs& a, double (&c)[V], 
     }
 }
 
-// The same between 32-bit values cut to 28 bits, the place in the lane in the
+// The same between 32-bit values, none of them -0, cut to 28 bits, the place in the lane in the
 // other four: their order as integers (0: none) is that of the values, and among equal ones
 // that of the places.  A lane's are sorted once, so that a choice is the largest of the lanes' first
 // ones.  True where what decides lies closer together than `near` and the cut (of values up to `size`):
@@ -364,7 +364,8 @@ __global__ __launch_bounds__(256) void route_forward_kernel(RouteArgs a)
     float most_bias = 0.f;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        c[i] = a.by_logit ? lg[i] : lg[i] == -INFINITY ? -INFINITY : c[i] + bias[i];
+        // (a logit of -0 becomes +0: they are equal, their bits are not; a score is never -0)
+        c[i] = a.by_logit ? lg[i] + 0.f : lg[i] == -INFINITY ? -INFINITY : c[i] + bias[i];
         c[i] = c[i] != c[i] ? INFINITY : c[i];
         most_bias = fmaxf(most_bias, bias[i] == -INFINITY ? 0.f : fabsf(bias[i]));
     }
