@@ -105,11 +105,12 @@ __device__ __forceinline__ void wave_order()
     __builtin_amdgcn_wave_barrier();
 }
 
-// A tile's expert: the tile'th tile of `size` rows in the order of the experts, or behind the last expert's
+// A tile's expert: the tile'th tile of `size` rows in the order of the experts, or of the rows of no expert, those before the
+// first one's and then those behind the last one's
 struct Group {
-    int expert;                 // -1: behind
-    int64_t first, end;         // the expert's rows
-    int64_t tile;               // of the expert, or of the rows behind
+    int expert;                 // -1: none
+    int64_t first, end;         // the expert's rows, or those before or behind all of them
+    int64_t tile;               // of these rows
 };
 __device__ __forceinline__ int group_bound(const ExpertGemm& g, int e)
 {
@@ -129,7 +130,8 @@ __device__ __forceinline__ int wave_scan(int v)
 // How `size` rows a tile lie over the experts
 struct Groups {
     int from, to, sum;          // of lane e's expert e < 64, and the tiles of those up to it
-    int64_t all;                // tiles, with those of the rows behind
+    int lead;                   // rows before the first expert's
+    int64_t all;                // tiles, with those of the rows of no expert
     __device__ __forceinline__ void load(const ExpertGemm& g, int e, int size)
     {
         from = group_bound(g, min(e, g.experts)), to = max(from, group_bound(g, min(e + 1, g.experts)));
@@ -144,7 +146,8 @@ struct Groups {
             all += __builtin_amdgcn_readlane(sum, 63);
         }
         load(g, lane, size);
-        all += __builtin_amdgcn_readlane(sum, 63);
+        lead = __builtin_amdgcn_readlane(from, 0);
+        all += __builtin_amdgcn_readlane(sum, 63) + (lead + (int64_t)size - 1) / size;
     }
     // (once)
     __device__ __forceinline__ Group find(const ExpertGemm& g, int tile, int size) const
@@ -161,7 +164,9 @@ struct Groups {
             }
             before += __builtin_amdgcn_readlane(now.sum, 63);
         }
-        return {-1, (int64_t)group_bound(g, g.experts), g.rows, tile - before};
+        const int64_t rest = tile - before, front = (lead + (int64_t)size - 1) / size;
+        if (rest < front) return {-1, 0, lead, rest};
+        return {-1, (int64_t)group_bound(g, g.experts), g.rows, rest - front};
     }
 };
 
@@ -595,8 +600,8 @@ static int launch_gemm(ExpertGemm g, const char* what, hipStream_t st)
     constexpr int TM = 16 * IM * WGM, TN = 16 * JN * WGN;
     g.tiles_n = (g.n + TN - 1) / TN;
     g.tiles_m = KIND == kDw ? (g.m + TM - 1) / TM : 0;
-    // (parts of tiles: one at most for each expert that has rows, and one of the rows behind them)
-    const int64_t tiles_m = KIND == kDw ? (int64_t)g.experts * g.tiles_m : g.rows / TM + std::min<int64_t>(g.experts + 1, g.rows);
+    // (parts of tiles: one at most for each expert that has rows, and one each of the rows before and behind them)
+    const int64_t tiles_m = KIND == kDw ? (int64_t)g.experts * g.tiles_m : g.rows / TM + std::min<int64_t>(g.experts + 2, g.rows);
     g.panel = 8;
     // (32768 rows of 16 experts 2048 -> 4096 510 us without, 489 with; dW of 64 experts 1024 -> 2048 147 and 110)
     g.stream = use_nontemporal((KIND == kDw ? (int64_t)g.experts * g.m : g.rows) * g.n * (KIND == kDx && g.c_f32 ? 4 : 2));
@@ -613,7 +618,7 @@ template <bool GATHER>
 static int launch_few(ExpertGemm g, const char* what, hipStream_t st)
 {
     g.tiles_n = (g.n + kFewCols - 1) / kFewCols;
-    const int64_t tiles_m = g.rows / kFewRows + std::min<int64_t>(g.experts + 1, g.rows);
+    const int64_t tiles_m = g.rows / kFewRows + std::min<int64_t>(g.experts + 2, g.rows);
     hipLaunchKernelGGL(expert_few_kernel<GATHER>, dim3((uint32_t)(tiles_m * g.tiles_n)), dim3(512), 0, st, g);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? BS_OK : set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));

@@ -36,7 +36,8 @@ class ExpertPlan(NamedTuple):
     """The routed (token, choice) pairs in the order of their experts, int32:
     rows offsets[e] up to offsets[e + 1] belong to expert e, order[row] is the
     pair token * top_k + choice, place[token, choice] its row, -1 where it has
-    none."""
+    none.  offsets[e0:e1 + 1] with W[e0:e1] is the plan of a part of the
+    experts: rows before the first offset and from the last on are of none."""
     offsets: Tensor
     order: Tensor
     place: Tensor
@@ -76,9 +77,9 @@ def expert_linear(x: Tensor, W: Tensor, plan: ExpertPlan, *, gather: bool = Fals
     """y[row] = x[row] @ W[expert of row].T, [rows, d_out], rows as in ``plan``.
 
     x: [rows, d_in], or with ``gather`` the tokens [..., d_in], each read where
-    its rows need it; W: [E, d_out, d_in]; both bfloat16.  Rows behind the last
-    expert's are 0, and the gradients of x (as x is given) and W take nothing
-    from them.  Sums in 32 bits, each result rounded once.  Differentiable once in x and W."""
+    its rows need it; W: [E, d_out, d_in]; both bfloat16.  Rows of no
+    expert, behind the last one's or before the first one's, are 0, and the
+    gradients of x (as x is given) and W take nothing from them.  Sums in 32 bits, each result rounded once.  Differentiable once in x and W."""
     return native().expert_linear(x, W, *plan, gather)
 
 

@@ -782,9 +782,10 @@ int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts, int32_t* o
  *   y[r] = act(x[src r] W[e]^T), dx[r] = dy[r] W[e], dW[e] = sum dy[r]^T x[src r]
  * src r = order[r] / top_k, a row of the `tokens` of x, or (order NULL) r; dx
  * and dW are of rows in the experts' order and take no order.
- * Rows that belong to no expert, or whose order is out of range, come out as
- * 0 (as act(0)); an expert without rows gets dW = 0.  Offsets out of range are
- * taken as the nearest in it.  Results are contiguous; dx is bf16 or, for the
+ * Rows that belong to no expert (before offsets[0], from offsets[experts] on),
+ * or whose order is out of range, come out as 0 (as act(0)); an expert without
+ * rows gets dW = 0.  Offsets do not fall; those out of range are taken as the
+ * nearest in it.  Results are contiguous; dx is bf16 or, for the
  * sum over a token's rows that follows where they were gathered, fp32 (dx_type).  Operands have rows at
  * 16-byte addresses, a multiple of 8 elements apart, and zeros from their
  * last column to the next multiple of 8 (bs_pad_rows makes such rows); of
