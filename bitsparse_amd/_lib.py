@@ -17,7 +17,7 @@ LIB_NAME = "libbitsparse_hip.so"
 # BITSPARSE_HIP_LIB points at another build of the same sources (tuning sweeps)
 LIB_PATH = os.environ.get("BITSPARSE_HIP_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 BS_OK = 0
 BS_ERR_INVALID = 1
@@ -108,6 +108,8 @@ _SIGNATURES = {
     "bs_pad_rows": [_vp, _i64, _i64, _i64, _vp, _i64, _vp],
     "bs_expert_combine": [_vp, _int, _i64, _vp, _vp, _i64, _int, _i64, _i64, _vp, _vp],
     "bs_expert_combine_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _int, _i64, _i64, _vp, _vp, _vp],
+    "bs_expert_combine_plan": [_vp, _vp, _int, _i64, _vp, _vp, _i64, _vp, _vp],
+    "bs_expert_combine_plan_backward": [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp],
     "bs_experts_act_grad": [_vp, _vp, _i64, _i64, _int, _f32, _vp, _vp, _vp, _i64, _vp, _vp],
     "bs_newton_schulz_workspace_bytes": [_i64, _i64, _i64, _int],
     "bs_newton_schulz": [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp],

@@ -4,6 +4,8 @@
 //   out[t] = sum over j of w[t, j] y[place[t, j]]        (32-bit sums in the order of j)
 //   dy[place[t, j]] = w[t, j] dout[t];  dw[t, j] = <dout[t], y[place[t, j]]>
 //
+// over the places that are rows of an expert; dy is 0 in all other rows.
+//
 // Bound by memory: y, dout and the results once.  A workgroup a token.  16384
 // tokens, 4 choices, 4096 wide: the sum 143 us, 4.7 TB/s; its gradients, with
 // dout held by the caches over a token's choices, 239 us, 5.1 TB/s (a copy
@@ -16,7 +18,7 @@
 namespace bs {
 
 constexpr int kMaxChoices = 64;
-constexpr int kTailBlocks = 64;     // workgroups that clear the rows behind the last expert's
+constexpr int kTailBlocks = 64;     // workgroups that clear the rows of no expert
 constexpr int64_t kSlice = 1 << 22; // workgroups of a launch, which has fewer than 2^32 threads
 
 struct CombineArgs {
@@ -25,7 +27,7 @@ struct CombineArgs {
     const void* y;
     int64_t y_stride;
     const float* weights;       // null: 1
-    const int32_t *place, *used;        // used: rows that belong to an expert
+    const int32_t *place, *first, *used;        // rows *first (null: 0) up to *used (null: all) belong to an expert
     bf16* out;
     // backward
     const bf16* g;
@@ -34,9 +36,31 @@ struct CombineArgs {
     float* dw;
 };
 
+// the rows that belong to an expert
+struct ExpertRows {
+    int from, to;
+    __device__ __forceinline__ explicit ExpertRows(const CombineArgs& a)
+        : from(a.first ? max(0, *a.first) : 0), to(a.used ? (int)min(a.rows, (int64_t)max(0, *a.used)) : (int)a.rows)
+    {
+    }
+    __device__ __forceinline__ bool have(int p) const { return p >= from && p < to; }
+};
+// 0 into dy's other rows, by kTailBlocks workgroups
+template <bool WHOLE>
+__device__ __forceinline__ void clear_others(const CombineArgs& a, const ExpertRows& of, int64_t block)
+{
+    const int64_t front = min((int64_t)of.from, a.rows);
+    for (int64_t i = block; i < front + (a.rows - of.to); i += kTailBlocks) {
+        const int64_t r = i < front ? i : of.to + (i - front);
+        for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048)
+            store_raw<WHOLE>(a.dy + r * a.cols + c, Raw<bf16>{}, (int)min((int64_t)8, a.cols - c));
+    }
+}
+
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
 {
+    const ExpertRows of(a);
     const int64_t t = blockIdx.x;
     const int32_t* place = a.place + t * a.top_k;
     for (int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8; c < a.cols; c += (int64_t)gridDim.y * 2048) {
@@ -44,7 +68,7 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a)
         float acc[8] = {};
         for (int j = 0; j < a.top_k; j++) {
             const int p = place[j];
-            if (p < 0 || p >= a.rows) continue;
+            if (!of.have(p)) continue;
             const float w = a.weights ? a.weights[t * a.top_k + j] : 1.f;
             const Raw<T> y = load_raw<WHOLE>(static_cast<const T*>(a.y) + p * a.y_stride + c, nv);
 #pragma unroll
@@ -59,18 +83,14 @@ template <bool WHOLE>
 __global__ __launch_bounds__(256) void spread_kernel(CombineArgs a)
 {
     const int64_t chunks = (a.cols + 7) / 8;
-    if ((int64_t)blockIdx.x >= a.tokens) {
-        for (int64_t r = max(0, *a.used) + (blockIdx.x - a.tokens); r < a.rows; r += kTailBlocks)
-            for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048)
-                store_raw<WHOLE>(a.dy + r * a.cols + c, Raw<bf16>{}, (int)min((int64_t)8, a.cols - c));
-        return;
-    }
+    const ExpertRows of(a);
+    if ((int64_t)blockIdx.x >= a.tokens) return clear_others<WHOLE>(a, of, blockIdx.x - a.tokens);
     const int64_t t = blockIdx.x;
     // (choices one after the other in a thread's chunks: a short row's threads are all at work)
     for (int64_t i = threadIdx.x; i < chunks * a.top_k; i += 256) {
         const int64_t j = i / chunks, c = (i - j * chunks) * 8;
         const int p = a.place[t * a.top_k + j];
-        if (p < 0 || p >= a.rows) continue;
+        if (!of.have(p)) continue;
         const int nv = (int)min((int64_t)8, a.cols - c);
         const Raw<bf16> g = load_raw<WHOLE>(a.g + t * a.g_stride + c, nv);
         if (a.weights == nullptr) {
@@ -91,17 +111,15 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(CombineArgs a)
 {
     __shared__ float s_dot[4][kMaxChoices];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const ExpertRows of(a);
     if ((int64_t)blockIdx.x >= a.tokens) {
-        if (a.dy == nullptr) return;
-        for (int64_t r = max(0, *a.used) + (blockIdx.x - a.tokens); r < a.rows; r += kTailBlocks)
-            for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048)
-                store_raw<WHOLE>(a.dy + r * a.cols + c, Raw<bf16>{}, (int)min((int64_t)8, a.cols - c));
+        if (a.dy) clear_others<WHOLE>(a, of, blockIdx.x - a.tokens);
         return;
     }
     const int64_t t = blockIdx.x;
     for (int j = 0; j < a.top_k; j++) {
         const int p = a.place[t * a.top_k + j];
-        const bool there = p >= 0 && p < a.rows;
+        const bool there = of.have(p);
         const float w = a.weights ? a.weights[t * a.top_k + j] : 1.f;
         float dot = 0.f;
         if (there)
@@ -181,15 +199,18 @@ static int combine_check(const char* what, int64_t tokens, int top_k, int64_t ro
     return BS_OK;
 }
 
-}  // namespace bs
-
-using namespace bs;
-
-extern "C" int bs_expert_combine(const void* y, int y_type, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
-                                 int64_t rows, int64_t cols, void* out, void* stream)
+// (the plan's tokens, choices and rows, as the two calls without a plan have them)
+static int combine_plan_check(const char* what, const bs_experts* x)
 {
-    clear_error();
-    const char* what = "bs_expert_combine";
+    if (x == nullptr) return set_error(BS_ERR_INVALID, "%s: null arguments", what);
+    if (x->experts < 1 || x->experts > 1024) return set_error(BS_ERR_INVALID, "%s: experts must be in 1..1024, got %d", what, x->experts);
+    if (x->offsets == nullptr || ((uintptr_t)x->offsets & 3u)) return set_error(BS_ERR_INVALID, "%s: null or misaligned offsets", what);
+    return BS_OK;
+}
+
+static int combine(const char* what, const void* y, int y_type, int64_t y_stride, const float* weights, const int32_t* place, const int32_t* first,
+                   const int32_t* used, int64_t tokens, int top_k, int64_t rows, int64_t cols, void* out, void* stream)
+{
     if (const int rc = combine_check(what, tokens, top_k, rows, cols); rc != BS_OK) return rc;
     if (tokens == 0 || cols == 0) return BS_OK;
     if ((rows && y == nullptr) || place == nullptr || out == nullptr) return set_error(BS_ERR_INVALID, "%s: null pointer", what);
@@ -198,7 +219,7 @@ extern "C" int bs_expert_combine(const void* y, int y_type, int64_t y_stride, co
     if (((uintptr_t)y & (y_type == BS_DT_F32 ? 3u : 1u)) || ((uintptr_t)out & 1u) || (((uintptr_t)weights | (uintptr_t)place) & 3u))
         return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
     CombineArgs a{};
-    a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride;
+    a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride, a.first = first, a.used = used;
     const bool whole = cols % 8 == 0;
     auto* kernel = y_type == BS_DT_F32 ? (whole ? combine_kernel<float, true> : combine_kernel<float, false>)
                                        : (whole ? combine_kernel<bf16, true> : combine_kernel<bf16, false>);
@@ -213,12 +234,10 @@ extern "C" int bs_expert_combine(const void* y, int y_type, int64_t y_stride, co
     return BS_OK;
 }
 
-extern "C" int bs_expert_combine_backward(const void* g, int64_t g_stride, const void* y, int64_t y_stride, const float* weights,
-                                          const int32_t* place, const int32_t* used, int64_t tokens, int top_k, int64_t rows, int64_t cols,
-                                          void* dy, float* dw, void* stream)
+static int combine_backward(const char* what, const void* g, int64_t g_stride, const void* y, int64_t y_stride, const float* weights,
+                            const int32_t* place, const int32_t* first, const int32_t* used, int64_t tokens, int top_k, int64_t rows, int64_t cols,
+                            void* dy, float* dw, void* stream)
 {
-    clear_error();
-    const char* what = "bs_expert_combine_backward";
     if (const int rc = combine_check(what, tokens, top_k, rows, cols); rc != BS_OK) return rc;
     if ((dy == nullptr && dw == nullptr) || (tokens == 0 && rows == 0)) return BS_OK;
     if ((tokens && cols && g == nullptr) || (tokens && place == nullptr) || (dy && used == nullptr) || (dw && rows && cols && y == nullptr))
@@ -228,10 +247,10 @@ extern "C" int bs_expert_combine_backward(const void* g, int64_t g_stride, const
         return set_error(BS_ERR_INVALID, "%s: misaligned pointer", what);
     CombineArgs a{};
     a.rows = rows, a.cols = cols, a.top_k = top_k, a.y = y, a.y_stride = y_stride;
-    a.used = used, a.g_stride = g_stride, a.dy = static_cast<bf16*>(dy);
+    a.first = first, a.used = used, a.g_stride = g_stride, a.dy = static_cast<bf16*>(dy);
     auto* kernel = dw ? (cols % 8 == 0 ? combine_backward_kernel<true> : combine_backward_kernel<false>)
                       : (cols % 8 == 0 ? spread_kernel<true> : spread_kernel<false>);
-    // (no tokens: the rows behind alone)
+    // (no tokens: the rows of no expert alone)
     for (int64_t t = 0; t == 0 || t < tokens; t += kSlice) {
         a.tokens = std::min(kSlice, tokens - t);
         const int64_t blocks = a.tokens + (dy && t + kSlice >= tokens ? kTailBlocks : 0);
@@ -243,6 +262,45 @@ extern "C" int bs_expert_combine_backward(const void* g, int64_t g_stride, const
         if (e != hipSuccess) return set_error(BS_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
     }
     return BS_OK;
+}
+
+}  // namespace bs
+
+using namespace bs;
+
+extern "C" int bs_expert_combine(const void* y, int y_type, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
+                                 int64_t rows, int64_t cols, void* out, void* stream)
+{
+    clear_error();
+    return combine("bs_expert_combine", y, y_type, y_stride, weights, place, nullptr, nullptr, tokens, top_k, rows, cols, out, stream);
+}
+
+extern "C" int bs_expert_combine_plan(const bs_experts* experts, const void* y, int y_type, int64_t y_stride, const float* weights, const int32_t* place,
+                                      int64_t cols, void* out, void* stream)
+{
+    clear_error();
+    const char* what = "bs_expert_combine_plan";
+    if (const int rc = combine_plan_check(what, experts); rc != BS_OK) return rc;
+    return combine(what, y, y_type, y_stride, weights, place, experts->offsets, experts->offsets + experts->experts, experts->tokens, experts->top_k,
+                   experts->rows, cols, out, stream);
+}
+
+extern "C" int bs_expert_combine_backward(const void* g, int64_t g_stride, const void* y, int64_t y_stride, const float* weights,
+                                          const int32_t* place, const int32_t* used, int64_t tokens, int top_k, int64_t rows, int64_t cols,
+                                          void* dy, float* dw, void* stream)
+{
+    clear_error();
+    return combine_backward("bs_expert_combine_backward", g, g_stride, y, y_stride, weights, place, nullptr, used, tokens, top_k, rows, cols, dy, dw, stream);
+}
+
+extern "C" int bs_expert_combine_plan_backward(const bs_experts* experts, const void* g, int64_t g_stride, const void* y, int64_t y_stride,
+                                               const float* weights, const int32_t* place, int64_t cols, void* dy, float* dw, void* stream)
+{
+    clear_error();
+    const char* what = "bs_expert_combine_plan_backward";
+    if (const int rc = combine_plan_check(what, experts); rc != BS_OK) return rc;
+    return combine_backward(what, g, g_stride, y, y_stride, weights, place, experts->offsets, experts->offsets + experts->experts, experts->tokens,
+                            experts->top_k, experts->rows, cols, dy, dw, stream);
 }
 
 extern "C" int bs_experts_act_grad(void* g, void* r, int64_t rows, int64_t cols, int square, float k, const float* weights,

@@ -40,8 +40,8 @@ using at::Tensor;
     F(bs_newton_schulz_workspace_bytes) F(bs_newton_schulz) F(bs_dropout) F(bs_join_drop_forward)                \
     F(bs_join_drop_backward) F(bs_route_forward) F(bs_route_backward) F(bs_expert_plan) F(bs_expert_linear)      \
     F(bs_expert_plan_workspace_bytes)                                                                             \
-    F(bs_expert_linear_dx) F(bs_expert_linear_dw) F(bs_pad_rows) F(bs_expert_combine)                            \
-    F(bs_expert_combine_backward) F(bs_experts_act_grad)
+    F(bs_expert_linear_dx) F(bs_expert_linear_dw) F(bs_pad_rows) F(bs_expert_combine_plan)                       \
+    F(bs_expert_combine_plan_backward) F(bs_experts_act_grad)
 struct Lib {
 #define F(name) decltype(&::name) name = nullptr;
     BS_FUNCS(F)

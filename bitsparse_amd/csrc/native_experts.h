@@ -307,9 +307,10 @@ struct Gathered {
     static Tensor written_out(const Tensor& x, const Plan& plan)
     {
         Tensor t = at::empty({plan.rows, x.size(1)}, x.options());
-        check(L.bs_expert_combine_backward(raw(x), row_stride(x), nullptr, 0, nullptr, ptr<int32_t>(plan.place), plan.used(), plan.tokens, plan.top_k,
-                                           plan.rows, x.size(1), raw(t), nullptr, stream_of(x)),
-              "bs_expert_combine_backward");
+        const bs_experts e = plan.args(false);
+        check(L.bs_expert_combine_plan_backward(&e, raw(x), row_stride(x), nullptr, 0, nullptr, ptr<int32_t>(plan.place), x.size(1), raw(t), nullptr,
+                                                stream_of(x)),
+              "bs_expert_combine_plan_backward");
         return t;
     }
 };
@@ -356,9 +357,10 @@ Tensor combined(const Tensor& y, const Tensor& weights, const Plan& plan)
     const c10::DeviceGuard guard(plan.offsets.device());
     Tensor out = at::empty(plan.token_shape(y.size(1)), y.options().dtype(at::kBFloat16));
     if (out.numel() == 0) return out;
-    check(L.bs_expert_combine(raw(y), y.scalar_type() == at::kFloat ? BS_DT_F32 : BS_DT_BF16, row_stride(y), ptr<float>(weights), ptr<int32_t>(plan.place), plan.tokens, plan.top_k, plan.rows, y.size(1),
-                              raw(out), stream_of(out)),
-          "bs_expert_combine");
+    const bs_experts e = plan.args(false);
+    check(L.bs_expert_combine_plan(&e, raw(y), y.scalar_type() == at::kFloat ? BS_DT_F32 : BS_DT_BF16, row_stride(y), ptr<float>(weights),
+                                   ptr<int32_t>(plan.place), y.size(1), raw(out), stream_of(out)),
+          "bs_expert_combine_plan");
     return out;
 }
 
@@ -510,9 +512,10 @@ struct ExpertCombine : torch::autograd::Function<ExpertCombine> {
             out[1] = at::empty(node.shape[1], grads[0].options().dtype(at::kFloat));
         }
         if (plan.rows == 0 || (!out[0].defined() && !out[1].defined())) return out;
-        check(L.bs_expert_combine_backward(raw(g), row_stride(g), raw(y), y.defined() ? row_stride(y) : 0, ptr<float>(w), ptr<int32_t>(plan.place),
-                                           plan.used(), plan.tokens, plan.top_k, plan.rows, D, raw(out[0]), ptr<float>(out[1]), stream_of(g)),
-              "bs_expert_combine_backward");
+        const bs_experts e = plan.args(false);
+        check(L.bs_expert_combine_plan_backward(&e, raw(g), row_stride(g), raw(y), y.defined() ? row_stride(y) : 0, ptr<float>(w),
+                                                ptr<int32_t>(plan.place), D, raw(out[0]), ptr<float>(out[1]), stream_of(g)),
+              "bs_expert_combine_plan_backward");
         return out;
     }
 };

@@ -85,7 +85,7 @@ def expert_linear(x: Tensor, W: Tensor, plan: ExpertPlan, *, gather: bool = Fals
 
 def expert_combine(y: Tensor, weights: Tensor, plan: ExpertPlan) -> Tensor:
     """out[token] = sum over its choices of weights[token, choice] * y[its
-    row], [..., d_out]; choices without a row add nothing.
+    row], [..., d_out]; choices without a row of an expert add nothing.
 
     y: bfloat16 [rows, d_out]; weights: float32 [..., top_k].  Sums in 32 bits
     in the order of the choices.  Differentiable once in y and weights."""

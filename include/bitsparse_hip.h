@@ -49,7 +49,7 @@ extern "C" {
 const char* bs_last_error(void);
 
 /* ABI version (bumped when an entry point changes): of this header, and of a built library. */
-#define BS_ABI_VERSION 21
+#define BS_ABI_VERSION 22
 int bs_abi_version(void);
 
 /*
@@ -816,13 +816,20 @@ int bs_pad_rows(const void* x, int64_t rows, int64_t cols, int64_t stride, void*
  * y bf16 or fp32; fp32 sums; weights NULL: 1); a place outside 0..rows-1 adds nothing.
  * Backward: dy[place[t, j]] = weights[t, j] g[t], 0 in the rows from *used
  * (a device address: offsets[experts]) on; dweights[t, j] = <g[t],
- * y[place[t, j]]>.  dy or dweights may be NULL.
+ * y[place[t, j]]>.  A place from *used on takes part in neither.  dy or dweights may be NULL (without dy used may be, for all rows).
+ * The calls of a plan: its tokens, top_k, rows and offsets (order is not
+ * read); a place takes part if it is among rows offsets[0] up to
+ * offsets[experts], dy is 0 in the rows outside them.
  */
 int bs_expert_combine(const void* y, int y_type, int64_t y_stride, const float* weights, const int32_t* place, int64_t tokens, int top_k,
                       int64_t rows, int64_t cols, void* out, void* stream);
 int bs_expert_combine_backward(const void* g, int64_t g_stride, const void* y, int64_t y_stride, const float* weights,
                                const int32_t* place, const int32_t* used, int64_t tokens, int top_k, int64_t rows, int64_t cols,
                                void* dy, float* dweights, void* stream);
+int bs_expert_combine_plan(const bs_experts* experts, const void* y, int y_type, int64_t y_stride, const float* weights, const int32_t* place,
+                           int64_t cols, void* out, void* stream);
+int bs_expert_combine_plan_backward(const bs_experts* experts, const void* g, int64_t g_stride, const void* y, int64_t y_stride,
+                                    const float* weights, const int32_t* place, int64_t cols, void* dy, float* dweights, void* stream);
 /*
  * Between the two products of a backward through y = sum of w act(z) W2^T: g
  * [rows, cols] holds the gradient of act(z) before its weight, r the saved

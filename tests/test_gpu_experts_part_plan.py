@@ -114,3 +114,37 @@ def test_block(T, k, E, e0, e1, D, H, O, square, own):
     assert (grads["w"][mine < 0] == 0).all()
     with torch.no_grad():
         assert torch.equal(layer.apply(*t.values(), plan), out)
+
+
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("T,k,E,e0,e1,D", [(1, 1, 3, 2, 3, 8), (40, 2, 4, 1, 3, 72), (130, 3, 5, 1, 3, 201), (300, 4, 8, 3, 6, 4104), (50, 1, 3, 1, 2, 64),
+                                           (2, 64, 64, 10, 40, 33)])
+def test_combine(T, k, E, e0, e1, D, own):
+    """Whatever y holds in rows of no expert is in no sum; the gradients there are 0, in every call the same."""
+    from bitsparse_amd.experts import expert_combine
+    g = _gen(T + D)
+    ids = _ids(T, k, E, g, lost=0.1)
+    if T == 50:
+        ids[:30], ids[30:] = 0, 2
+    _, plan, first, end = _part(ids, E, e0, e1, own)
+    R = T * k
+    y, w, go = _rn(g, R, D).to(BF), _rn(g, T, k).requires_grad_(), _rn(g, T, D).to(BF)
+    y[:first], y[end:] = torch.nan, torch.inf
+    y.requires_grad_()
+    mine = (ids >= e0) & (ids < e1)
+    at = plan.place.long().clamp(min=0)
+    rows = torch.where(mine[..., None], y.detach().double()[at], 0.0)
+    terms, dots = w.detach().double()[..., None] * rows, rows * go.double()[:, None]
+    want = torch.zeros(R, D, dtype=torch.float64, device="cuda")
+    want[at[mine]] = (w.detach().double()[..., None] * go.double()[:, None])[mine]
+    for _ in range(3):
+        _dirty(2 * R * D, 4 * R)
+        out = expert_combine(y, w, plan)
+        dy, dw = torch.autograd.grad(out, (y, w), go)
+        _close(out.detach(), terms.sum(1), terms.abs().sum(1), k, "out")
+        _close(dw, dots.sum(-1), dots.abs().sum(-1), D, "dw")
+        _close(dy, want, want.abs(), 1, "dy")
+        assert (dy[:first] == 0).all() and (dy[end:] == 0).all() and (dw[~mine] == 0).all()
+        _dirty(2 * R * D)
+        alone, = torch.autograd.grad(expert_combine(y, w.detach(), plan), y, go)
+        assert torch.equal(alone, dy)
