@@ -3,17 +3,18 @@
 // offsets[e + 1]:
 //   forward  y[r, n]     = sum over d of x[src r, d] W[e][n, d]
 //   dx       dx[r, d]    = sum over n of dy[r, n] W[e][n, d]
-//   dW       dW[e][n, d] = sum over the expert's r of dy[r, n] x[src r, d]
-// src r is r, or the row's token, so that gathered rows are never written.
+//   dW       dW[e][n, d] = sum over the expert's r of dy[r, n] x[r, d]
+// src r is r, or in forward the row's token: gathered rows are read where they are.  dW takes them written out in order.
 //
 // bf16 operands, fp32 sums, one rounding.  A workgroup a tile of results; the
 // tiles of ragged groups are found on the device, so the host knows nothing
 // of the routing and waits for nothing.
 //
-// Bound by the products: 32768 rows of 16 experts, 2048 -> 4096, 486 us
-// forward, 489 dx, 504 dW, 1.09 to 1.13 PFLOP/s; of one expert with 4096 rows, 16384 -> 4096, 1.28 to 1.39, the
-// library's 1.29.  The difference is the groups' part tiles, the last round's idle CUs and, of
-// shorter sums, the tiles' starts and ends: 16384 rows of 8 experts, 768 -> 2048, 0.79 to 0.94 PFLOP/s.
+// Bound by the products.  On several boxes: 32768 rows of 16 experts, 2048 -> 4096, 476 to 521 us forward, 465 to 504 dx, 469
+// to 504 dW, 1.06 to 1.18 PFLOP/s, the matrix pipes at work in 55 to 59% of the cycles; the library's dense product of that
+// size 385 to 394 us, 1.39 to 1.43.  One expert with 4096 rows, 16384 -> 4096: 390 to 439 us, 1.25 to 1.41, the library's 344 to 352,
+// 1.56 to 1.60.  16384 rows of 8 experts, 768 -> 2048, 55 to 73 us, 0.71 to 0.94, the library's 52 to 54.  The differences are the
+// loop's own (of one expert), the groups' part tiles, the last round's idle CUs and, of shorter sums, the tiles' starts and ends.
 #include <algorithm>
 #include <cmath>
 
@@ -510,7 +511,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
         const Groups groups(g, TM);
         const int rows = AHEAD ? (int)min((int64_t)g.rows_of_tiles, groups.all) : g.rows_of_tiles, all = rows * g.tiles_n;
         // What is left of the last round: up to a quarter of one in quarters of tiles, up to half in halves, so that it takes
-        // no whole round (16384 rows of 8 experts 768 -> 2048 gathered 75 -> 65 us, 32768 of 16 2048 -> 4096 494 -> 486).
+        // no whole round (16384 rows of 8 experts 768 -> 2048 gathered 73 -> 65 us on one box, 32768 of 16 2048 -> 4096 484 -> 476).
         const int left = AHEAD ? all % AT_ONCE : 0, parts = left == 0 || left > AT_ONCE / 2 ? 1 : left > AT_ONCE / 4 ? 2 : 4;
         const int id = (int)blockIdx.x, whole = parts == 1 ? all : all - left;
         const int tile = id < whole ? xcd_run(id, whole, AT_ONCE) : whole + (id - whole) / parts, part = id < whole ? 0 : (id - whole) % parts;
@@ -648,7 +649,7 @@ static double tile_time(const ExpertGemm& g, int kind, int tm, int tn, int at_on
 
 // Forward for up to two rows an expert: expert_few_kernel (8 rows of 64 experts of 4096 -> 1024 13.2 us, on tiles of 64 x 64
 // 20.9; 64 rows 50 and 65; 32 rows of 8 experts of 4096 -> 2048 24.3 and 22.0).  Else the tile whose time is least by
-// tile_time (measured in us, forward / dx / dW, x gathered in forward):
+// tile_time (measured on one box in us, forward / dx / dW, x gathered in forward):
 //   rows, experts, in -> out           64 x 64       128 x 128     192 x 128   256 x 256
 //   16384,  8,  768 -> 2048         119 / 91 / 95    78 / 65 / 72   73 / 72 / -   65 / 55 / 74
 //   16384,  8, 2048 ->  768          92 / 102 / 93   68 / 66 / 68   73 / 59 / -   56 / 68 / 73

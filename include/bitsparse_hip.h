@@ -745,7 +745,7 @@ int bs_join_drop_backward(const bs_join* args, const bs_join_grads* grads, const
  * of their experts the top_k largest c are chosen, the largest first.  The
  * choice is between 64-bit values (between the logits where the order is
  * theirs); of equal ones the lowest index goes first and a NaN before all.  weights = scale * s / sum(s of the chosen)
- * (renormalize; 0 where that sum is 0) or scale * s.  An expert whose logit or
+ * (renormalize; 0 where that sum, in 32 bits, is 0) or scale * s.  An expert whose logit or
  * c is -infinity is not chosen; a choice that is left without an expert is -1
  * with weight 0.  weights and chosen: [tokens, top_k], contiguous.
  * bs_route_backward: the gradient of the logits (their type, contiguous) from
@@ -779,7 +779,7 @@ int bs_expert_plan(const int32_t* chosen, int64_t pairs, int experts, int32_t* o
 /*
  * Products of the experts' rows with their bf16 weights [experts, out, in]
  * (w_stride elements from row to row), fp32 sums rounded once:
- *   y[r] = act(x[src r] W[e]^T), dx[r] = dy[r] W[e], dW[e] = sum dy[r]^T x[src r]
+ *   y[r] = act(x[src r] W[e]^T), dx[r] = dy[r] W[e], dW[e] = sum dy[r]^T x[r]
  * src r = order[r] / top_k, a row of the `tokens` of x, or (order NULL) r; dx
  * and dW are of rows in the experts' order and take no order.
  * Rows that belong to no expert (before offsets[0], from offsets[experts] on),
