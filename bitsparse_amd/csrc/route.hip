@@ -414,11 +414,12 @@ __global__ __launch_bounds__(256) void route_forward_kernel(RouteArgs a)
     for (int s = 0; s < SLOTS; s++) {
         w[s] = 0.f;
         if (s * L >= a.top_k) continue;
-        // the logit again; the difference's rounding, which the exponential turns into as much of its value, is put back
+        // the logit again; the difference's rounding, which the exponential turns into as much of its value, is put back (of none
+        // where it is 0: the difference may be past fp32's range)
         const int64_t at = row * a.stride + max(0, id[s]);
         const float of = a.f32 ? static_cast<const float*>(a.logits)[at] : (float)static_cast<const bf16*>(a.logits)[at];
         const float d = of - top, back = d - of, lost = (of - (d - back)) - (top + back), e = expf(a.sigmoid ? -of : d);
-        w[s] = id[s] < 0 ? 0.f : a.sigmoid ? 1.f / (1.f + e) : fmaf(e, lost, e) / sum;
+        w[s] = id[s] < 0 ? 0.f : a.sigmoid ? 1.f / (1.f + e) : fmaf(e, e == 0.f ? 0.f : lost, e) / sum;
         total += w[s];
     }
     if (a.renorm) total = Ln::all(total, sum_of);

@@ -104,3 +104,20 @@ def test_equal_scores_with_a_bias(E, k, score, dtype):
     gap = (c.gather(1, ids.long()) - c.gather(1, want.long())).abs()
     differ = ids != want
     assert ((gap[differ] > 0) & (gap[differ] < (E + 8) * 2.0 ** -52)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_logits_further_apart_than_their_type_holds(dtype, renormalize):
+    """Finite logits whose difference is not: the score is 0, as it is of any that far below the largest."""
+    from bitsparse_amd.experts import route
+    low = torch.finfo(dtype).min
+    l = torch.tensor([[1e38, low, 0.0], [low, 2e38, 1.0], [low, low, low], [0.0, low, 1.0]], dtype=dtype, device="cuda").requires_grad_()
+    w, ids = route(l, 3, renormalize=renormalize)
+    assert ids.tolist() == [[0, 2, 1], [1, 2, 0], [0, 1, 2], [2, 0, 1]]
+    e = torch.tensor(1.0, dtype=torch.float64).exp()
+    want = torch.tensor([[1, 0, 0], [1, 0, 0], [1 / 3] * 3, [e / (1 + e), 1 / (1 + e), 0]], dtype=torch.float64)
+    # an exponential to two roundings, a sum of three to three, a product and a quotient: eight of 2^-24 at most
+    assert ((w.detach().cpu().double() - want).abs() <= 8 * 2.0 ** -24 * want).all()
+    dl, = torch.autograd.grad(w, l, torch.tensor([[1.0, 2.0, 3.0]], device="cuda").expand(4, 3).contiguous())
+    assert torch.isfinite(dl).all() and (dl[:2] == 0).all() and dl[3, 1] == 0
